@@ -616,6 +616,84 @@ int zkv_sample_window(const float* logits, int64_t ld, int bs, int vocab, float 
                       int window, float top_p, const float* expo, int64_t expo_ld, int64_t* tokens,
                       int32_t* overflow, void* workspace, size_t workspace_bytes, zkv_stream_t stream);
 
+/* --------------------------------------------------------------------------
+ * The paged cache: one pool of pages per layer for K and one for V, read
+ * through a block table.  Pools are [num_pages, kv, page_size, d] with any
+ * (page, head, token) element strides whose rows start on 16 bytes (K and V
+ * alike) and d = 64, 128 or 256 contiguous channels; cells are bf16 or fp16
+ * (is_f16), or e4m3 codes (is_fp8) that stand for code * scale[head] (scale
+ * null: 1).  Page sizes are any number of tokens.  A slot is page * page_size
+ * + offset; a slot outside the pool (-1) is none.  No counterpart in the
+ * reference, whose cache is one contiguous run per sequence (S:519-611).
+ * ------------------------------------------------------------------------ */
+
+/* Status bits of zkv_page_advance (sticky in state[2]). */
+#define ZKV_PAGES_POOL_EMPTY 1 /* a request was not served: no free pages for it */
+#define ZKV_PAGES_TABLE_FULL 2 /* ... its tokens exceed the block table's width */
+#define ZKV_PAGES_SLOTS_FULL 4 /* ... its tokens exceed the slot map */
+#define ZKV_PAGES_BAD_LENGTH 8 /* ... its length is negative or beyond the table */
+#define ZKV_PAGES_RING_FULL 16 /* more pages given back than the ring holds */
+
+/* One step of the page tables of `requests` <= 8192 requests, one launch.
+ * Request i goes from seq_lens[i] to seq_lens[i] + new_tokens[i] tokens (not
+ * below 0).  Growing takes the pages it lacks from the ring of free page ids
+ * (free_pages int32 [num_pages], state[0] its head, state[1] how many are
+ * free) in request order and writes them into block_table int32 [requests,
+ * width] (row stride table_stride); shrinking gives pages back behind the
+ * ring's last, for later steps.  A request grows whole or not at all, and
+ * once the ring cannot serve one, only requests that need no page grow;
+ * state[2] collects ZKV_PAGES_* bits for those left as they were.
+ * slots int64 [capacity], positions int32 [capacity] (nullable): of the new
+ * tokens in request order, -1 for those of a request that was not served and
+ * behind the last token.  starts int32 [requests + 1] (nullable): running sum
+ * of the new tokens (max(new, 0)), at most capacity + 1.
+ * seq_lens_out / state_out may be seq_lens / state.  state int32 [4]: head,
+ * free, status, and an arrival count that is 0 between calls; calls that
+ * overlap on one state race. */
+int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_tokens, int requests, int32_t* block_table,
+                     int64_t table_stride, int width, int32_t* free_pages, int num_pages, int page_size,
+                     int32_t* state, int64_t* slots, int32_t* positions, int capacity, int32_t* starts,
+                     int32_t* seq_lens_out, int32_t* state_out, zkv_stream_t stream);
+
+/* K / V rows of `tokens` tokens (k, v: (token, head) element strides, 16-bit
+ * rows on 16 bytes) into slots int64 [tokens].  e4m3 pools take row / scale,
+ * values beyond 448 as 448.  Slots of one call are distinct (of two tokens
+ * with one slot either may end up there, K and V apart). */
+int zkv_paged_write(const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                    const int64_t* slots, int tokens, int kv, int d, int is_f16, void* k_pages, void* v_pages,
+                    int is_fp8, const float* k_scale, const float* v_scale, int num_pages, int page_size,
+                    int64_t page_stride, int64_t head_stride, int64_t token_stride, zkv_stream_t stream);
+
+/* zkv_qk_norm_rope for a paged cache and a batch whose rows have their own
+ * positions: qkv [rows, (hq + 2 kv) * d] (row stride qkv_stride), RMSNorm of
+ * the q and k heads, rotate-half RoPE with row positions[r] of cos / sin (fp32
+ * [max_positions, d / 2]), q to q_out [rows, hq, d], K and V to slots[r].
+ * fp32 from the input to the one rounding of the result.  A row whose position
+ * is outside [0, max_positions) writes nothing, one without a slot only q. */
+int zkv_paged_qk_norm_rope(const void* qkv, int64_t qkv_stride, int rows, int hq, int kv, int d, int is_f16,
+                           const void* q_norm, const void* k_norm, float eps, const float* cos, const float* sin,
+                           int max_positions, const int32_t* positions, const int64_t* slots, void* q_out,
+                           void* k_pages, void* v_pages, int is_fp8, const float* k_scale, const float* v_scale,
+                           int num_pages, int page_size, int64_t page_stride, int64_t head_stride,
+                           int64_t token_stride, zkv_stream_t stream);
+
+/* Attention of one query token per request over its pages, one launch:
+ * softmax(sm_scale q K^T) V over the last `window` tokens (0: all) of
+ * seq_lens[b] tokens, q [bs, hq, d] ((batch, head) strides, rows on 16 bytes),
+ * hq a multiple of kv, out [bs, hq, d] in q's type or fp32 (out_f32), lse
+ * (nullable) fp32 [bs, hq], natural log.  Lengths are read on the device and
+ * limited to [0, width * page_size]; tokens on a page id outside the pool are
+ * left out; a request without a token gives zeros and -inf.  At most 4096
+ * requests.  workspace: zkv_paged_attention_workspace_size(d) bytes, any
+ * content; calls that overlap on one workspace race. */
+size_t zkv_paged_attention_workspace_size(int d);
+int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, const void* k_pages,
+                        const void* v_pages, int is_fp8, const float* k_scale, const float* v_scale, int num_pages,
+                        int page_size, int64_t page_stride, int64_t head_stride, int64_t token_stride,
+                        const int32_t* block_table, int64_t table_stride, int width, const int32_t* seq_lens, int bs,
+                        int hq, int kv, int d, float sm_scale, int window, void* out, int out_f32, float* lse,
+                        void* workspace, size_t workspace_bytes, zkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

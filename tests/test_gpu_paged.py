@@ -1,0 +1,309 @@
+"""Page tables, paged writes and the paged norm + RoPE rows on the GPU, against
+oracle/paged.py and torch's casts: integers, copies and e4m3 codes exact,
+norm + RoPE rows within the rounding of their result."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as op
+from zoomkv_revision_amd import paged
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+# ---------------------------------------------------------------------------
+# page tables
+# ---------------------------------------------------------------------------
+def _new_tables(rng, requests, width, page, free, lens):
+    """Tables in the middle of their life: pages scattered, the ring wrapped."""
+    used = [-(-int(n) // page) for n in lens]
+    pages = sum(used) + free + 3                  # (three ids are nobody's)
+    ids = rng.permutation(pages).astype(np.int32)
+    table = np.full((requests, width), -7, np.int32)
+    at = 0
+    for i, u in enumerate(used):
+        table[i, :u] = ids[at:at + u]
+        at += u
+    ring = np.full(pages, -9, np.int32)
+    head = int(rng.integers(pages))
+    ring[(head + np.arange(free)) % pages] = ids[at:at + free]
+    return table, ring, np.array([head, free, 0, 0], np.int32)
+
+
+def _gpu(table, ring, state, lens, page):
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+    return paged.PageTables(t(table), t(np.asarray(lens, np.int32)), t(ring), t(state), page)
+
+
+def _same_step(rng, lens, new, width, page, free, cap):
+    requests = len(lens)
+    table, ring, state = _new_tables(rng, requests, width, page, free, lens)
+    want = op.advance(np.asarray(lens, np.int32), np.asarray(new, np.int32), table, ring, state, page, cap)
+    tables = _gpu(table, ring, state, lens, page)
+    slots = torch.full((cap,), -5, dtype=torch.int64, device=DEV)
+    positions = torch.full((cap,), -5, dtype=torch.int32, device=DEV)
+    starts = torch.full((requests + 1,), -5, dtype=torch.int32, device=DEV)
+    paged.page_advance(tables, torch.tensor(new, dtype=torch.int32, device=DEV), slots, positions, starts)
+    got = (tables.seq_lens, tables.block_table, tables.free_pages, tables.state, slots, positions, starts)
+    for name, a, b in zip(("lens", "table", "ring", "state", "slots", "positions", "starts"), got, want):
+        assert np.array_equal(a.cpu().numpy(), b), name
+    return want
+
+
+@pytest.mark.parametrize("requests,page,width,cap", [(1, 1, 40, 7), (1, 16, 3, 1), (3, 8, 6, 64), (64, 16, 20, 64),
+                                                     (65, 24, 7, 500), (257, 7, 9, 3000), (1000, 16, 40, 20000),
+                                                     (4097, 4, 5, 9000), (8192, 16, 4, 8192)])
+@pytest.mark.parametrize("free", ["enough", "some", "none"])
+def test_advance_equals_the_plain_form(requests, page, width, cap, free):
+    rng = np.random.default_rng(requests * 31 + cap)
+    lens = rng.integers(0, width * page + 1, requests)
+    new = rng.choice([0, 1, 1, 1, 2, page, 5 * page, -1, -page, -10 ** 6, 10 ** 6], requests)
+    n_free = {"enough": requests * width + 5, "some": requests // 3 + 1, "none": 0}[free]
+    _same_step(rng, lens, new, width, page, n_free, cap)
+
+
+def test_advance_extremes():
+    rng = np.random.default_rng(5)
+    big = 2 ** 31 - 1
+    # token counts whose sum passes 32 bits, lengths that are not lengths
+    _same_step(rng, [0, 5, 0, 3, 16], [1, big, big, 2, big], 4, 4, 40, 30)
+    _same_step(rng, [3, 9], [-big, -big - 1], 4, 4, 3, 4)
+    table, ring, state = _new_tables(rng, 4, 3, 8, 9, [0, 0, 0, 0])
+    lens = np.array([-1, 25, -big - 1, big], np.int32)
+    new = np.array([1, 1, -3, 2], np.int32)
+    want = op.advance(lens, new, table, ring, state, 8, 6)
+    t = _gpu(table, ring, state, lens, 8)
+    slots = torch.zeros(6, dtype=torch.int64, device=DEV)
+    paged.page_advance(t, torch.from_numpy(new).to(DEV), slots)
+    assert np.array_equal(t.seq_lens.cpu().numpy(), want[0]) and np.array_equal(slots.cpu().numpy(), want[4])
+    assert int(t.state[2]) == paged.BAD_LENGTH
+    with pytest.raises(RuntimeError, match="length"):
+        t.check()
+    # a ring that cannot take what comes back keeps what it held
+    t = _gpu(np.arange(6, dtype=np.int32).reshape(1, 6), np.arange(6, dtype=np.int32), np.array([2, 4, 0, 0], np.int32),
+             [12], 2)
+    paged.page_advance(t, torch.tensor([-12], dtype=torch.int32, device=DEV))
+    assert t.state.tolist() == [2, 6, paged.RING_FULL, 0] and t.free_pages.tolist() == [0, 1, 2, 3, 4, 5]
+
+
+def test_advance_strided_table_and_separate_outputs():
+    rng = np.random.default_rng(9)
+    lens = rng.integers(0, 60, 33)
+    table, ring, state = _new_tables(rng, 33, 6, 16, 40, lens)
+    new = rng.choice([1, 17, -4], 33)
+    want = op.advance(lens.astype(np.int32), new.astype(np.int32), table, ring, state, 16, 300)
+    wide = torch.full((33, 11), 77, dtype=torch.int32, device=DEV)
+    t = _gpu(table, ring, state, lens, 16)
+    wide[:, 2:8] = t.block_table
+    t.block_table = wide[:, 2:8]
+    slots = torch.empty(300, dtype=torch.int64, device=DEV)
+    lens_out, state_out = torch.empty_like(t.seq_lens), torch.full_like(t.state, 5)
+    for _ in range(2):        # the inputs are as they were: a second call gives the same
+        paged.page_advance(t, torch.tensor(new, dtype=torch.int32, device=DEV), slots, lens_out=lens_out,
+                           state_out=state_out)
+        assert np.array_equal(lens_out.cpu().numpy(), want[0]) and np.array_equal(state_out.cpu().numpy(), want[3])
+        assert np.array_equal(slots.cpu().numpy(), want[4]) and np.array_equal(t.block_table.cpu().numpy(), want[1])
+        assert np.array_equal(t.seq_lens.cpu().numpy(), lens) and np.array_equal(t.state.cpu().numpy(), state)
+    assert bool((wide[:, :2] == 77).all()) and bool((wide[:, 8:] == 77).all())
+
+
+def test_advance_without_a_slot_map():
+    t = paged.PageTables.allocate(2, 32, 8, 4, device=DEV)
+    t.seq_lens[0] = 3
+    paged.page_advance(t, torch.tensor([-2, 0], dtype=torch.int32, device=DEV))
+    assert t.seq_lens.tolist() == [1, 0]
+    paged.page_advance(t, torch.tensor([0, 1], dtype=torch.int32, device=DEV))
+    assert t.seq_lens.tolist() == [1, 0] and int(t.state[2]) == paged.SLOTS_FULL
+
+
+def test_captured_advance_replays_as_steps():
+    """A captured step reads the lengths that the replay before it left."""
+    tables = [paged.PageTables.allocate(5, 64, 30, 4, device=DEV) for _ in range(2)]
+    new = torch.tensor([1, 2, 0, 1, 3], dtype=torch.int32, device=DEV)
+    slots = [torch.empty(8, dtype=torch.int64, device=DEV) for _ in range(2)]
+    plans = [paged.PageAdvancePlan(t, new, s) for t, s in zip(tables, slots)]
+    plans[0].run()
+    plans[1].run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plans[0].run()
+    for step in range(12):
+        if step == 5:
+            new.copy_(torch.tensor([-3, 1, 1, 0, -1], dtype=torch.int32, device=DEV))
+        graph.replay()
+        plans[1].run()
+        torch.cuda.synchronize()
+        assert torch.equal(slots[0], slots[1]), step
+        for f in ("block_table", "seq_lens", "free_pages", "state"):
+            assert torch.equal(getattr(tables[0], f), getattr(tables[1], f)), (step, f)
+
+
+# ---------------------------------------------------------------------------
+# writes
+# ---------------------------------------------------------------------------
+def _pools(shape, dtype, nhd, fill):
+    """K and V pools [pages, kv, page, d] of known content."""
+    pages, kv, page, d = shape
+    out = []
+    for i in range(2):
+        t = torch.full((pages, page, kv, d) if nhd else shape, fill + i, device=DEV).to(dtype)
+        out.append(t.transpose(1, 2) if nhd else t)
+    return out
+
+
+def _slots(n, pages, page, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randperm(pages * page, generator=g)[:n].to(DEV)
+
+
+def _stored(pool, slots):
+    page = pool.shape[2]
+    raw = pool.view(torch.uint8) if pool.element_size() == 1 else pool
+    return raw[slots // page, :, slots % page]
+
+
+@pytest.mark.parametrize("n,kv,d,page,nhd", [(1, 1, 64, 1, False), (5, 8, 128, 16, False), (5, 8, 128, 16, True),
+                                             (333, 3, 128, 24, False), (40, 2, 256, 8, True), (1000, 5, 64, 64, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_write_rows(n, kv, d, page, nhd, dtype, fp8):
+    pages = -(-(n + 50) // page)
+    pools = _pools((pages, kv, page, d), torch.float8_e4m3fn if fp8 else dtype, nhd, 2.0)
+    before = [p.clone() for p in pools]
+    g = torch.Generator(device=DEV).manual_seed(n)
+    # the rows as a model's fused projection holds them: strided views
+    qkv = torch.randn(n, 4 * kv, d, generator=g, device=DEV).to(dtype)
+    k, v = qkv[:, kv:2 * kv], qkv[:, 3 * kv:]
+    scales = [0.5 + torch.rand(kv, generator=g, device=DEV) for _ in range(2)] if fp8 else [None, None]
+    slots = _slots(n, pages, page)
+    slots[n // 2] = -1
+    if n > 4:
+        slots[1], slots[2] = pages * page, 1 << 40
+    paged.paged_write(k, v, slots, *pools, *scales)
+    live = (slots >= 0) & (slots < pages * page)
+    for pool, old, rows, s in zip(pools, before, (k, v), scales):
+        want = rows[live] if not fp8 else \
+            (rows[live].float() / s[None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+        assert torch.equal(_stored(pool, slots[live]), want)
+        keep = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+        keep[slots[live]] = False
+        rest = torch.arange(pages * page, device=DEV)[keep]
+        assert torch.equal(_stored(pool, rest), _stored(old, rest))
+
+
+def test_every_16_bit_value_as_e4m3():
+    """All bf16 and fp16 values, infinities and NaN among them, against torch's
+    cast of the clamped value; the default scale is 1."""
+    bits = torch.arange(65536, dtype=torch.int32, device=DEV).to(torch.int16)
+    for dtype in (torch.bfloat16, torch.float16):
+        rows = bits.view(dtype).view(512, 1, 128)
+        pools = _pools((512, 1, 1, 128), torch.float8_e4m3fn, False, 0.0)
+        slots = torch.arange(512, device=DEV)
+        paged.paged_write(rows, rows, slots, *pools)
+        x = rows.float()
+        want = x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+        nan = torch.isnan(x)
+        for pool in pools:
+            got = _stored(pool, slots)
+            assert torch.equal(got[~nan], want[~nan])
+            assert bool(((got[nan] & 0x7F) == 0x7F).all())
+
+
+def test_write_of_unaligned_and_empty_rows():
+    pools = _pools((4, 2, 4, 128), torch.bfloat16, False, 0.0)
+    odd = torch.randn(3, 2, 129, device=DEV).to(torch.bfloat16)[..., 1:]
+    slots = torch.tensor([7, 0, 12], device=DEV)
+    paged.paged_write(odd, odd, slots, *pools)
+    assert torch.equal(_stored(pools[0], slots), odd) and torch.equal(_stored(pools[1], slots), odd)
+    empty = odd[:0]
+    paged.paged_write(empty, empty, slots[:0], *pools)
+    paged.PagedWritePlan(empty, empty, slots[:0], *pools).run()
+    # one head's row for all heads, one row for all tokens
+    one = torch.randn(1, 1, 128, device=DEV).to(torch.bfloat16).expand(3, 2, 128)
+    paged.paged_write(one, odd, slots, *pools)
+    assert torch.equal(_stored(pools[0], slots), one)
+
+
+# ---------------------------------------------------------------------------
+# norm + RoPE rows
+# ---------------------------------------------------------------------------
+def _rope_bound(ref, x, w, eps, half_step):
+    """The result's rounding, and fp32's on the way: the sum of squares (d
+    products and sums), the inverse root (1 unit), three products and a sum,
+    all relative to the rotated pair's magnitude."""
+    d = x.shape[-1]
+    y = np.abs(x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w)
+    pair = y + np.roll(y, d // 2, -1)
+    return half_step * np.abs(ref) + (d / 2 + 8) * 2.0 ** -24 * pair + 2.0 ** -25
+
+
+@pytest.mark.parametrize("rows,hq,kv,d,page,nhd", [(1, 1, 1, 64, 16, False), (8, 32, 8, 128, 16, False),
+                                                   (3, 5, 1, 128, 24, True), (77, 7, 7, 256, 8, False),
+                                                   (130, 16, 2, 64, 1, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_norm_rope_rows(rows, hq, kv, d, page, nhd, dtype, fp8):
+    pages = -(-(rows + 20) // page)
+    pools = _pools((pages, kv, page, d), torch.float8_e4m3fn if fp8 else dtype, nhd, 2.0)
+    before = [p.clone() for p in pools]
+    g = torch.Generator(device=DEV).manual_seed(rows + d)
+    wide = torch.randn(rows, (hq + 2 * kv) * d + 8, generator=g, device=DEV).to(dtype)
+    qkv = wide[:, 8:]                                    # rows with a stride of their own
+    w = [(1.0 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(dtype) for _ in range(2)]
+    ang = torch.arange(999, dtype=torch.float64)[:, None] / 1e4 ** (torch.arange(0, d, 2, dtype=torch.float64) / d)
+    cos, sin = ang.cos().float().to(DEV), ang.sin().float().to(DEV)
+    pos = torch.randint(0, 999, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    pos[0] = 998
+    slots = _slots(rows, pages, page)
+    if rows > 2:
+        pos[1], slots[2] = -1, -1                        # a row of padding, a row without a slot
+    if rows > 4:
+        pos[3], slots[4] = 999, pages * page
+    scales = [0.01 + 0.01 * torch.rand(kv, generator=g, device=DEV) for _ in range(2)] if fp8 else [None, None]
+    q_out = torch.full((rows, hq, d), 9.0, device=DEV).to(dtype)
+    eps = 1e-5
+    assert paged.paged_qk_norm_rope(qkv, hq, kv, *w, eps, cos, sin, pos, slots, q_out, *pools, *scales) is q_out
+    f64 = lambda t: t.double().cpu().numpy()
+    x = f64(qkv).reshape(rows, hq + 2 * kv, d)
+    live = ((pos >= 0) & (pos < 999)).cpu().numpy()
+    at = pos.clamp(0, 998).long().cpu().numpy()
+    cs, sn = f64(cos)[at][:, None], f64(sin)[at][:, None]
+    got = f64(q_out)
+    assert (got[~live] == 9.0).all()
+    ref = op.norm_rope(x[:, :hq], f64(w[0]), eps, cs, sn)
+    assert (np.abs(got - ref)[live] <= _rope_bound(ref, x[:, :hq], f64(w[0]), eps, HALF_STEP[dtype])[live]).all()
+    wrote = torch.from_numpy(live).to(DEV) & (slots >= 0) & (slots < pages * page)
+    sel, there = wrote.cpu().numpy(), slots[wrote]
+    k = op.norm_rope(x[:, hq:hq + kv], f64(w[1]), eps, cs, sn)
+    if not fp8:
+        assert (np.abs(f64(_stored(pools[0], there)) - k[sel]) <=
+                _rope_bound(k, x[:, hq:hq + kv], f64(w[1]), eps, HALF_STEP[dtype])[sel]).all()
+        assert torch.equal(_stored(pools[1], there), qkv[wrote].view(-1, hq + 2 * kv, d)[:, hq + kv:])
+    else:
+        # half a step of e4m3: 2^-4 of the value, 2^-10 below its smallest normal
+        s = f64(scales[0])[:, None]
+        want = np.clip(k / s, -448, 448)
+        code = f64(_stored(pools[0], there).view(torch.float8_e4m3fn))
+        slack = _rope_bound(k, x[:, hq:hq + kv], f64(w[1]), eps, 0.0) / s
+        assert (np.abs(code - want[sel]) <= (2.0 ** -4 * np.abs(want) + 2.0 ** -10 + slack * 1.07)[sel]).all()
+        v = qkv[wrote].view(-1, hq + 2 * kv, d)[:, hq + kv:].float()
+        assert torch.equal(_stored(pools[1], there), (v / scales[1][None, :, None]).clamp(-448, 448)
+                           .to(torch.float8_e4m3fn).view(torch.uint8))
+    keep = torch.ones(pages * page, dtype=torch.bool, device=DEV)
+    keep[there] = False
+    rest = torch.arange(pages * page, device=DEV)[keep]
+    for pool, old in zip(pools, before):
+        assert torch.equal(_stored(pool, rest), _stored(old, rest))
+
+
+def test_norm_rope_of_no_rows():
+    pools = _pools((2, 1, 4, 64), torch.bfloat16, False, 0.0)
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt, device=DEV)
+    args = (z(0, 3 * 64), 1, 1, z(64), z(64), 1e-6, z(4, 32, dt=torch.float32), z(4, 32, dt=torch.float32),
+            z(0, dt=torch.int32), z(0, dt=torch.int64), z(0, 1, 64), *pools)
+    paged.paged_qk_norm_rope(*args)
+    paged.PagedRopePlan(*args).run()

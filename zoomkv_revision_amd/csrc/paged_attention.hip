@@ -1,0 +1,771 @@
+// Attention of one new token per request over a paged K / V cache (gfx950).
+//
+// For request b, KV head h and each of its query heads, over the tokens t of
+// [first_b, len_b) (first_b = max(0, len_b - window) with a window, else 0):
+//
+//   s_t = scale * q . K[t],  m = max s_t,  l = sum exp(s_t - m),
+//   out = sum exp(s_t - m) V[t] / l,  lse = m + log l
+//
+// where token t lives in row t % page_size of page block_table[b, t / page_size].
+// One pass over the cache with the running maximum and sum of the softmax.
+//
+// Work.  A unit is one (b, KV head, group of up to 16 query heads); its tokens
+// are cut into tiles of 32.  The tiles of all units, in order, are one line of
+// T tiles: workgroup w takes tiles [w C, (w + 1) C), and inside it each wave an
+// equal run, whatever the lengths are (they are read on the device, so a
+// captured launch follows them).  A wave finishes the units that lie wholly in
+// its run by itself; the ends of its run go to LDS as partials (m, l, O) and
+// are joined there; the ends of the workgroup's run go to the workspace and
+// are joined by the last of the workgroups that share the unit.  Each
+// workgroup leaves at most two partials, whatever the batch is, and which
+// tiles are joined in which order depends on the lengths alone, so the result
+// is the same from run to run.
+//
+// Tile.  S^T = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32: K rows are the
+// A operand (lane 16 g + c: token c, channels 32 s + 8 g ..), q the B operand
+// (head c).  The scores come out with head c and tokens 4 g + i in lane
+// 16 g + c, which is where P has to be as the B operand of the second product
+// when its k-slice g is tokens 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3: no
+// value of S or P moves between lanes.  V rows are read whole by 16 lanes
+// (lane c: channels c D / 16 ..) and turned in registers, two tokens to a word,
+// by v_perm: row c of the j-th A operand is channel c D / 16 + j.  P enters as
+// two 16-bit parts (two products: the matrix cores wait for memory here
+// anyway): hi, cut towards zero, and lo, the rest, which together carry 15
+// bits (bf16) or 21 (fp16).  Neither part is negative and lo is never 0, so an
+// infinite V stays infinite (-lo * Inf or 0 * Inf would make it NaN).
+#include "paged_common.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace zkv {
+namespace {
+
+constexpr int kTile = 32;          // tokens of a tile: one k-step of the P V product
+constexpr int kHeads = 16;         // query heads of a unit: the columns of an MFMA
+constexpr int kMaxBatch = 4096;    // requests of a call: 4 bytes of LDS each
+constexpr int kMaxGroups = 256;    // workgroups: an arrival count is a byte
+constexpr float kInf = __builtin_inff();
+constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
+// The softmax's reference exponent m follows the scores' running maximum only
+// when that is more than this many powers of two above it: O is rescaled a few
+// times per run, not per tile.
+constexpr float kLazyBits = 8.0f;
+
+struct PagedAttnParams {
+  const uint16_t* q;
+  int64_t q_sb, q_sh;
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  PageLayout layout;
+  FastDiv page;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  float* part_o;   // [workgroup][2][kHeads][D]
+  float* part_ml;  // [workgroup][2][kHeads][2]
+  unsigned long long* arrivals;  // per workgroup: the unit that starts in it
+  unsigned long long epoch;
+  FastDiv units;   // units of one request: kv * groups
+  FastDiv groups;  // groups of up to 16 query heads of a KV head
+  float scale;     // softmax scale * log2 e
+  int bs, hq, kv, gqa, window, out_f32;
+  int max_len;     // width of the table * page size
+  int heads_lds;   // query heads kept per partial in LDS: min(gqa, 16)
+};
+
+template <int kType>
+struct Elem;
+template <>
+struct Elem<kBf16> {
+  typedef bf16x8_t x8;
+  // m is the maximum itself: P is at most 2^8
+  static constexpr float kUp = 0.0f;
+  // two values cut to the type, their parts beyond it (at least the smallest
+  // normal number)
+  static __device__ __forceinline__ uint32_t split(float a, float b, float& ra, float& rb) {
+    const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+    ra = fmaxf(a - __uint_as_float(ua & 0xFFFF0000u), 0x1p-126f);
+    rb = fmaxf(b - __uint_as_float(ub & 0xFFFF0000u), 0x1p-126f);
+    return __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+  }
+  static __device__ __forceinline__ float4_t mfma(x8 a, x8 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  typedef __bf16 one;
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t pair_of_fp8(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, kHigh));
+  }
+};
+template <>
+struct Elem<kF16> {
+  typedef half8_t x8;
+  // m is the maximum less 7: P is at most 2^15, and fp16's last place, 2^-24,
+  // is 2^-31 of the largest weight
+  static constexpr float kUp = 7.0f;
+  static __device__ __forceinline__ uint32_t split(float a, float b, float& ra, float& rb) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+    ra = fmaxf(a - static_cast<float>(h[0]), 0x1p-24f);
+    rb = fmaxf(b - static_cast<float>(h[1]), 0x1p-24f);
+    return __builtin_bit_cast(uint32_t, h);
+  }
+  static __device__ __forceinline__ float4_t mfma(x8 a, x8 b, float4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  typedef _Float16 one;
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t pair_of_fp8(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, kHigh));
+  }
+};
+
+// Maximum and sum over the four lanes 16 g + c of one c.
+__device__ __forceinline__ float across_max(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float across_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const float y = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ void store_dev(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_dev(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <int kWords>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t* w) {
+  if constexpr (kWords == 1) {
+    w[0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p));
+  } else if constexpr (kWords == 2) {
+    const u32x2_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
+    w[0] = x[0], w[1] = x[1];
+  } else {
+    const u32x4_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    w[0] = x[0], w[1] = x[1], w[2] = x[2], w[3] = x[3];
+  }
+}
+
+// Compile-time shape of a kernel.
+template <bool kFp8, int kD>
+struct Shape {
+  static constexpr int kCell = kFp8 ? 1 : 2;
+  static constexpr int kSteps = kD / 32;                 // k-steps of q K^T
+  static constexpr int kKLoads = kD * kCell / 64;        // 16-byte loads of a K row per lane
+  static constexpr int kJ = kD / 16;                     // channels of V per lane, A operands of P V
+  static constexpr int kChunk = std::min(kJ, 16 / kCell);  // of them in one load
+  static constexpr int kChunks = kJ / kChunk;
+  static constexpr int kChunkWords = kChunk * kCell / 4;
+  static constexpr int kVWords = kChunks * kChunkWords;
+  // 8 waves: 2 on a SIMD, 256 registers each.  Head dim 256 holds twice the
+  // tile and twice the output per wave: 4 waves with up to 512.
+  static constexpr int kWaves = kD == 256 ? 4 : 8;
+  // first channel of chunk n of output row r (r = 0 .. 15)
+  static __device__ __forceinline__ int channel(int r, int n) { return n * (16 * kChunk) + r * kChunk; }
+};
+
+template <bool kFp8, int kD>
+struct TileRegs {
+  u32x4_t k[2][Shape<kFp8, kD>::kKLoads];
+  uint32_t v[8][Shape<kFp8, kD>::kVWords];
+  uint32_t mask;  // bit t: token t is attended
+};
+
+// One segment's view: a request's table row, and the head's rows.
+struct SegView {
+  const int32_t* row;
+  const uint8_t* k;
+  const uint8_t* v;
+  int first, len;
+};
+
+template <int kType, bool kFp8, int kD>
+struct PagedAttn {
+  using S = Shape<kFp8, kD>;
+  using E = Elem<kType>;
+  using x8 = typename E::x8;
+  using Tile = TileRegs<kFp8, kD>;
+
+  float4_t o[S::kJ];
+  float m, l;
+  x8 q[S::kSteps];
+
+  // The page of token (lane & 31) of a tile (tokens past the end: the last).
+  static __device__ __forceinline__ int page_id(const PagedAttnParams& p, const SegView& s, int tile, int lane) {
+    const int t = min(tile * kTile + (lane & 31), s.len - 1);
+    return s.row[div_by(t, p.page)];
+  }
+
+  // Requests a tile's K and V.  The lane of each token forms its row's offset
+  // once; the lanes that read the row fetch it by ds_bpermute.
+  static __device__ __forceinline__ void request(const PagedAttnParams& p, const SegView& s, int tile, int page,
+                                                 int lane, Tile& x) {
+    const int t = tile * kTile + (lane & 31), tc = min(t, s.len - 1);
+    const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(p.layout.num_pages);
+    x.mask = static_cast<uint32_t>(__ballot(there && t < s.len && t >= s.first));
+    const uint32_t in_page = tc - div_by(tc, p.page) * p.page.d;
+    const int64_t off = there ? (page * p.layout.page_stride + in_page * p.layout.token_stride) * S::kCell : 0;
+    const int lo = static_cast<int>(off), hi = static_cast<int>(off >> 32);
+    const int c = lane & 15, g = lane >> 4;
+    const auto row_of = [&](int token) {
+      const uint32_t l32 = __builtin_amdgcn_ds_bpermute(4 * token, lo);
+      const uint32_t h32 = __builtin_amdgcn_ds_bpermute(4 * token, hi);
+      return static_cast<int64_t>((static_cast<uint64_t>(h32) << 32) | l32);
+    };
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      const uint8_t* r = s.k + row_of(16 * mt + c) + 16 * g;
+#pragma unroll
+      for (int i = 0; i < S::kKLoads; ++i)
+        x.k[mt][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + 64 * i));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint8_t* r = s.v + row_of((e & 4) * 4 + 4 * g + (e & 3)) + c * (S::kChunk * S::kCell);
+#pragma unroll
+      for (int n = 0; n < S::kChunks; ++n)
+        load_words<S::kChunkWords>(r + n * (16 * S::kChunk * S::kCell), x.v[e] + n * S::kChunkWords);
+    }
+  }
+
+  static __device__ __forceinline__ x8 words8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    const u32x4_t r = {a, b, c, d};
+    return __builtin_bit_cast(x8, r);
+  }
+
+  // K operand of k-step s: bf16 / fp16 as loaded; e4m3 two steps per load.
+  static __device__ __forceinline__ x8 k_operand(const Tile& x, int mt, int s) {
+    if constexpr (kFp8) {
+      const uint32_t a = x.k[mt][s >> 1][2 * (s & 1)], b = x.k[mt][s >> 1][2 * (s & 1) + 1];
+      return words8(E::template pair_of_fp8<false>(a), E::template pair_of_fp8<true>(a),
+                    E::template pair_of_fp8<false>(b), E::template pair_of_fp8<true>(b));
+    } else {
+      return __builtin_bit_cast(x8, x.k[mt][s]);
+    }
+  }
+
+  // Channels 2 w, 2 w + 1 of token e's part of V, as a pair of 16-bit values.
+  static __device__ __forceinline__ uint32_t v_pair(const Tile& x, int e, int w) {
+    if constexpr (kFp8) {
+      const uint32_t word = x.v[e][w >> 1];
+      return (w & 1) ? E::template pair_of_fp8<true>(word) : E::template pair_of_fp8<false>(word);
+    } else {
+      return x.v[e][w];
+    }
+  }
+
+  __device__ __forceinline__ void accumulate(Tile& x, float sc, int lane) {
+    const int g = lane >> 4;
+    float4_t s[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+      s[mt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i) s[mt] = E::mfma(k_operand(x, mt, i), q[i], s[mt]);
+      s[mt] *= sc;
+    }
+    if (x.mask != 0xFFFFFFFFu) {
+      // tokens that are not attended: score -inf (whatever their row holds),
+      // V 0, so that 0 * Inf and 0 * NaN never form
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (!((x.mask >> ((e & 4) * 4 + 4 * g + (e & 3))) & 1)) {
+          s[e >> 2][e & 3] = -kInf;
+#pragma unroll
+          for (int w = 0; w < S::kVWords; ++w) x.v[e][w] = 0;
+        }
+      }
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
+    top = across_max(top);
+    top -= E::kUp;
+    if (__any(top > m + kLazyBits)) {
+      const float now = fmaxf(m, top);
+      // (m = -inf: nothing summed yet; a lane that stays at -inf keeps its zeros)
+      const float a = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now;
+      l *= a;
+#pragma unroll
+      for (int j = 0; j < S::kJ; ++j) o[j] *= a;
+    }
+    const float base = m == -kInf ? 0.0f : m;
+    uint32_t hi[4];
+    typename E::one lo[8];
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - base);
+      const float p1 = __builtin_amdgcn_exp2f(s[e >> 2][(e & 3) + 1] - base);
+      l += p0 + p1;
+      float r0, r1;
+      hi[e >> 1] = E::split(p0, p1, r0, r1);
+      lo[e] = static_cast<typename E::one>(r0);
+      lo[e + 1] = static_cast<typename E::one>(r1);
+    }
+    const x8 ph = words8(hi[0], hi[1], hi[2], hi[3]);
+    const x8 pl = {lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]};
+#pragma unroll
+    for (int w = 0; w < S::kJ / 2; ++w) {
+      uint32_t r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = v_pair(x, e, w);
+      const x8 even = words8(__builtin_amdgcn_perm(r[1], r[0], 0x05040100u), __builtin_amdgcn_perm(r[3], r[2], 0x05040100u),
+                             __builtin_amdgcn_perm(r[5], r[4], 0x05040100u), __builtin_amdgcn_perm(r[7], r[6], 0x05040100u));
+      const x8 odd = words8(__builtin_amdgcn_perm(r[1], r[0], 0x07060302u), __builtin_amdgcn_perm(r[3], r[2], 0x07060302u),
+                            __builtin_amdgcn_perm(r[5], r[4], 0x07060302u), __builtin_amdgcn_perm(r[7], r[6], 0x07060302u));
+      o[2 * w] = E::mfma(even, ph, o[2 * w]);
+      o[2 * w + 1] = E::mfma(odd, ph, o[2 * w + 1]);
+      o[2 * w] = E::mfma(even, pl, o[2 * w]);
+      o[2 * w + 1] = E::mfma(odd, pl, o[2 * w + 1]);
+    }
+  }
+
+  // Tiles [t0, t1) of one unit: two register tiles, the next one requested
+  // before the present one is used; page ids one tile further ahead.  The
+  // tail is peeled so that no request in the loop is conditional (a request
+  // on one of two paths makes the compiler wait for all of them).
+  __device__ __forceinline__ void segment(const PagedAttnParams& p, const SegView& s, int b, int head0, int heads,
+                                          float sc, int t0, int t1, int lane) {
+    const int c = lane & 15, g = lane >> 4;
+    int page = page_id(p, s, t0, lane);
+    int next = page_id(p, s, min(t0 + 1, t1 - 1), lane);
+    // q as the B operand, in the channel order of the K operand's k-steps
+    const uint16_t* qr = p.q + b * p.q_sb + (head0 + min(c, heads - 1)) * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) {
+      const int ch = kFp8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+      u32x4_t w = *reinterpret_cast<const u32x4_t*>(qr + ch);
+      if (c >= heads) w = u32x4_t{0, 0, 0, 0};
+      q[i] = __builtin_bit_cast(x8, w);
+    }
+    m = -kInf;
+    l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < S::kJ; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    Tile a, z;
+    request(p, s, t0, page, lane, a);
+    int t = t0;
+    for (; t + 2 < t1; t += 2) {
+      page = page_id(p, s, t + 2, lane);
+      request(p, s, t + 1, next, lane, z);
+      accumulate(a, sc, lane);
+      next = page_id(p, s, min(t + 3, t1 - 1), lane);
+      request(p, s, t + 2, page, lane, a);
+      accumulate(z, sc, lane);
+    }
+    if (t + 1 < t1) {
+      request(p, s, t + 1, next, lane, z);
+      accumulate(a, sc, lane);
+      accumulate(z, sc, lane);
+    } else {
+      accumulate(a, sc, lane);
+    }
+    l = across_sum(l);
+  }
+};
+
+__device__ __forceinline__ void store_result(const PagedAttnParams& p, int type, int64_t at, float v) {
+  if (p.out_f32)
+    static_cast<float*>(p.out)[at] = v;
+  else
+    static_cast<uint16_t*>(p.out)[at] = type == kBf16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+}
+
+__device__ __forceinline__ float natural_lse(float m, float l) {
+  return l == 0.0f ? -kInf : (m + __log2f(l)) * kLn2v;
+}
+
+// One unit of the line of tiles.
+struct Unit {
+  int b, kvh, head0, heads;  // request, KV head, first query head, query heads
+  int start, tiles;          // first place on the line, tiles
+};
+
+template <int kType, bool kFp8, int kD>
+__global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attention_kernel(const PagedAttnParams p) {
+  using S = Shape<kFp8, kD>;
+  constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves;
+  constexpr int kRow = kD + 4;  // row stride of a partial in LDS: 4 banks of skew between heads
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem);                     // [2 waves][heads][kRow]
+  float* s_ml = s_o + 2 * kWaves * p.heads_lds * kRow;             // [2 waves][heads][2]
+  int* s_unit = reinterpret_cast<int*>(s_ml + 2 * kWaves * p.heads_lds * 2);  // [2 waves]: unit or -1
+  int* s_part = s_unit + 2 * kWaves;                               // [waves + 2]: scan, last-arrival flags
+  int* s_cum = s_part + kWaves + 2;                                // [bs + 1]: tiles of the requests before
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+
+  // --- tiles of every request, and their running sum -----------------------
+  const auto first_of = [&](int len) { return p.window > 0 ? max(0, len - p.window) : 0; };
+  const auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.max_len); };
+  const auto tiles_of = [&](int len) { return (len + kTile - 1) / kTile - first_of(len) / kTile; };
+  const int per = (p.bs + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, p.bs), b1 = min(b0 + per, p.bs);
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int n = tiles_of(len_of(b));
+    s_cum[b] = n;
+    mine += n;
+  }
+  int scan = mine;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const int u = __shfl_up(scan, i);
+    if (lane >= i) scan += u;
+  }
+  if (lane == 63) s_part[wave] = scan;
+  if (tid < 2 * kWaves) s_unit[tid] = -1;
+  __syncthreads();
+  int before = scan - mine, total = 0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) before += s_part[w];
+    total += s_part[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int n = s_cum[b];
+    s_cum[b] = before;
+    before += n;
+  }
+  if (tid == 0) s_cum[p.bs] = total;
+  __syncthreads();
+  total *= p.units.d;
+
+  // --- requests without a token: zeros -------------------------------------
+  for (int b = blockIdx.x; b < p.bs; b += gridDim.x) {
+    if (s_cum[b + 1] != s_cum[b]) continue;
+    const int64_t row = static_cast<int64_t>(b) * p.hq;
+    for (int i = tid; i < p.hq * kD; i += kThreads) store_result(p, kType, row * kD + i, 0.0f);
+    if (p.lse)
+      for (int i = tid; i < p.hq; i += kThreads) p.lse[row + i] = -kInf;
+  }
+
+  // --- this workgroup's run of tiles ---------------------------------------
+  const int chunk = max(kWaves, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+  const int64_t from = static_cast<int64_t>(blockIdx.x) * chunk;
+  if (from >= total) return;
+  const int wg0 = static_cast<int>(from), wg1 = static_cast<int>(min(from + chunk, static_cast<int64_t>(total)));
+  const auto unit_of = [&](int b, int rest) {
+    Unit u;
+    u.b = b;
+    const uint32_t kvh = div_by(rest, p.groups);
+    const int group = rest - static_cast<int>(kvh * p.groups.d);
+    u.kvh = static_cast<int>(kvh);
+    u.heads = min(kHeads, p.gqa - kHeads * group);
+    u.head0 = u.kvh * p.gqa + kHeads * group;
+    u.tiles = s_cum[b + 1] - s_cum[b];
+    u.start = s_cum[b] * static_cast<int>(p.units.d) + rest * u.tiles;
+    return u;
+  };
+
+  {
+    const int share = (wg1 - wg0 + kWaves - 1) / kWaves;
+    int x = wg0 + wave * share;
+    const int end = min(x + share, wg1);
+    int slot = 2 * wave;
+    PagedAttn<kType, kFp8, kD> attn;
+    while (x < end) {
+      // the request whose tiles hold place x
+      const int at = static_cast<int>(div_by(x, p.units));
+      int lo = 0, hi = p.bs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s_cum[mid + 1] > at)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      const int b = __builtin_amdgcn_readfirstlane(lo);
+      const int nt = s_cum[b + 1] - s_cum[b];
+      const int rest = (x - s_cum[b] * static_cast<int>(p.units.d)) / nt;
+      const Unit u = unit_of(b, rest);
+      const int t0 = x - u.start, t1 = min(nt, t0 + end - x);
+      const int len = len_of(b), first = first_of(len), tile0 = first / kTile;
+      const int64_t head_off = u.kvh * p.layout.head_stride * S::kCell;
+      const SegView view{p.table + b * p.table_stride, static_cast<const uint8_t*>(p.k) + head_off,
+                         static_cast<const uint8_t*>(p.v) + head_off, first, len};
+      float sc = p.scale;
+      if constexpr (kFp8) sc *= p.k_scale ? p.k_scale[u.kvh] : 1.0f;
+      attn.segment(p, view, b, u.head0, u.heads, sc, tile0 + t0, tile0 + t1, lane);
+      const int c = lane & 15, g = lane >> 4;
+      if (t0 == 0 && t1 == nt) {
+        // the whole unit: the result
+        if (c < u.heads) {
+          float inv = attn.l == 0.0f ? 0.0f : 1.0f / attn.l;
+          if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
+          const int64_t row = static_cast<int64_t>(b) * p.hq + u.head0 + c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < S::kChunks; ++n) {
+              const int64_t at0 = row * kD + S::channel(4 * g + i, n);
+#pragma unroll
+              for (int j = 0; j < S::kChunk; ++j)
+                store_result(p, kType, at0 + j, attn.o[n * S::kChunk + j][i] * inv);
+            }
+          if (p.lse && g == 0) p.lse[row] = natural_lse(attn.m, attn.l);
+        }
+      } else {
+        if (c < u.heads) {
+          float* dst = s_o + (slot * p.heads_lds + c) * kRow;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < S::kChunks; ++n)
+#pragma unroll
+              for (int j = 0; j < S::kChunk; j += 4) {
+                const float4_t y = {attn.o[n * S::kChunk + j][i], attn.o[n * S::kChunk + j + 1][i],
+                                    attn.o[n * S::kChunk + j + 2][i], attn.o[n * S::kChunk + j + 3][i]};
+                *reinterpret_cast<float4_t*>(dst + S::channel(4 * g + i, n) + j) = y;
+              }
+          if (g == 0) {
+            s_ml[(slot * p.heads_lds + c) * 2] = attn.m;
+            s_ml[(slot * p.heads_lds + c) * 2 + 1] = attn.l;
+          }
+        }
+        if (lane == 0) s_unit[slot] = b * static_cast<int>(p.units.d) + rest;
+        ++slot;  // at most the run's first and last unit are cut
+      }
+      x += t1 - t0;
+    }
+  }
+  __syncthreads();
+
+  // --- join the waves' partials, unit by unit ------------------------------
+  const auto unit_at = [&](int id) {
+    const int b = static_cast<int>(div_by(id, p.units));
+    return unit_of(b, id - b * static_cast<int>(p.units.d));
+  };
+  int cut[2] = {-1, -1};  // units shared with earlier / later workgroups
+  for (int i0 = 0; i0 < 2 * kWaves;) {
+    const int id = s_unit[i0];
+    if (id < 0) {
+      ++i0;
+      continue;
+    }
+    int i1 = i0 + 1;
+    while (i1 < 2 * kWaves && (s_unit[i1] == id || s_unit[i1] < 0)) ++i1;
+    const Unit u = unit_at(id);
+    const bool whole = u.start >= wg0 && u.start + u.tiles <= wg1;
+    const int side = u.start >= wg0 ? 1 : 0;
+    if (!whole) cut[side] = id;
+    for (int e = tid; e < u.heads * (kD / 4); e += kThreads) {
+      const int c = e / (kD / 4), d = 4 * (e % (kD / 4));
+      float top = -kInf;
+      for (int i = i0; i < i1; ++i)
+        if (s_unit[i] == id) top = fmaxf(top, s_ml[(i * p.heads_lds + c) * 2]);
+      const float base = top == -kInf ? 0.0f : top;
+      float den = 0.0f;
+      float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i = i0; i < i1; ++i) {
+        if (s_unit[i] != id) continue;
+        const float w = __builtin_amdgcn_exp2f(s_ml[(i * p.heads_lds + c) * 2] - base);
+        den += w * s_ml[(i * p.heads_lds + c) * 2 + 1];
+        num += w * *reinterpret_cast<const float4_t*>(s_o + (i * p.heads_lds + c) * kRow + d);
+      }
+      if (whole) {
+        float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
+        const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_result(p, kType, row * kD + d + j, num[j] * inv);
+        if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+      } else {
+        const int64_t row = (static_cast<int64_t>(blockIdx.x) * 2 + side) * kHeads + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_dev(p.part_o + row * kD + d + j, num[j]);
+        if (d == 0) {
+          store_dev(p.part_ml + row * 2, top);
+          store_dev(p.part_ml + row * 2 + 1, den);
+        }
+      }
+    }
+    i0 = i1;
+  }
+  if (cut[0] < 0 && cut[1] < 0) return;
+
+  // --- the last workgroup of a shared unit joins the workgroups' partials ---
+  // This lane's partial stores have reached the device's coherence point
+  // before the workgroup counts in (write-through stores, waited for), and the
+  // joining loads read there: no cache is written back or invalidated.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid < 2) {
+    const int id = cut[tid];
+    int last = 0;
+    if (id >= 0) {
+      const Unit u = unit_at(id);
+      const int w0 = u.start / chunk, w1 = (u.start + u.tiles - 1) / chunk;
+      last = arrive_last(p.arrivals + w0, p.epoch, w1 - w0 + 1);
+    }
+    s_part[tid] = last;
+  }
+  __syncthreads();
+  for (int side = 0; side < 2; ++side) {
+    if (cut[side] < 0 || !s_part[side]) continue;
+    const Unit u = unit_at(cut[side]);
+    const int w0 = u.start / chunk, n = (u.start + u.tiles - 1) / chunk - w0 + 1;
+    // partial i: the unit's first workgroup kept it as its later cut, the others as their earlier one
+    const auto row_of = [&](int i, int c) {
+      return ((static_cast<int64_t>(w0) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
+    };
+    constexpr int kBatch = 8;
+    for (int e = tid; e < u.heads * kD; e += kThreads) {
+      const int c = e / kD, d = e % kD;
+      float top = -kInf;
+      for (int i0 = 0; i0 < n; i0 += kBatch) {
+        float mv[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) mv[i] = load_dev(p.part_ml + row_of(min(i0 + i, n - 1), c) * 2);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top = fmaxf(top, mv[i]);
+      }
+      const float base = top == -kInf ? 0.0f : top;
+      float den = 0.0f, num = 0.0f;
+      for (int i0 = 0; i0 < n; i0 += kBatch) {
+        float mv[kBatch], lv[kBatch], ov[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int64_t row = row_of(min(i0 + i, n - 1), c);
+          mv[i] = load_dev(p.part_ml + row * 2);
+          lv[i] = load_dev(p.part_ml + row * 2 + 1);
+          ov[i] = load_dev(p.part_o + row * kD + d);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float w = __builtin_amdgcn_exp2f(mv[i] - base);
+          den = i0 + i < n ? den + w * lv[i] : den;
+          num = i0 + i < n ? num + w * ov[i] : num;
+        }
+      }
+      float inv = den == 0.0f ? 0.0f : 1.0f / den;
+      if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
+      const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
+      store_result(p, kType, row * kD + d, num * inv);
+      if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+    }
+  }
+}
+
+constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+size_t workspace_bytes_for(int d) {
+  return align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * d * 4) +
+         align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * 2 * 4) + kMaxGroups * 8;
+}
+
+template <int kType, bool kFp8, int kD>
+int launch_paged_attention(PagedAttnParams& p, int64_t most_tiles, hipStream_t s) {
+  using S = Shape<kFp8, kD>;
+  const auto kernel = paged_attention_kernel<kType, kFp8, kD>;
+  const size_t lds = static_cast<size_t>(2 * S::kWaves) * p.heads_lds * (kD + 6) * 4 +
+                     (2 * S::kWaves + S::kWaves + 2 + p.bs + 1) * 4;
+  if (lds > 60 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                          160 * 1024) != hipSuccess)
+    return fail(ZKV_ELAUNCH, "zkv_paged_attention: cannot raise the LDS limit to 160 KiB");
+  // one workgroup per CU, or as many as the longest lengths the table can
+  // hold give a tile for every wave
+  const int64_t want = (most_tiles + S::kWaves - 1) / S::kWaves;
+  const int grid = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kMaxGroups, want)));
+  kernel<<<grid, 64 * S::kWaves, lds, s>>>(p);
+  return check_launch("paged_attention_kernel");
+}
+
+template <int kType, bool kFp8>
+int launch_by_dim(PagedAttnParams& p, int d, int64_t most_tiles, hipStream_t s) {
+  if (d == 64) return launch_paged_attention<kType, kFp8, 64>(p, most_tiles, s);
+  if (d == 128) return launch_paged_attention<kType, kFp8, 128>(p, most_tiles, s);
+  return launch_paged_attention<kType, kFp8, 256>(p, most_tiles, s);
+}
+
+}  // namespace
+}  // namespace zkv
+
+using namespace zkv;
+
+extern "C" size_t zkv_paged_attention_workspace_size(int d) {
+  return d == 64 || d == 128 || d == 256 ? workspace_bytes_for(d) : 0;
+}
+
+extern "C" int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, const void* k_pages,
+                                   const void* v_pages, int is_fp8, const float* k_scale, const float* v_scale,
+                                   int num_pages, int page_size, int64_t page_stride, int64_t head_stride,
+                                   int64_t token_stride, const int32_t* block_table, int64_t table_stride, int width,
+                                   const int32_t* seq_lens, int bs, int hq, int kv, int d, float sm_scale, int window,
+                                   void* out, int out_f32, float* lse, void* workspace, size_t workspace_bytes,
+                                   zkv_stream_t stream) {
+  ZKV_REQUIRE(q && k_pages && v_pages && block_table && seq_lens && out && workspace,
+              "zkv_paged_attention: null pointer");
+  const PageLayout layout{page_stride, head_stride, token_stride, num_pages, page_size};
+  const char* why = check_pages(layout, kv, d, is_fp8 ? 1 : 2);
+  ZKV_REQUIRE(why == nullptr, "zkv_paged_attention: %s", why);
+  ZKV_REQUIRE(bs >= 1 && bs <= kMaxBatch, "zkv_paged_attention: %d requests outside [1, %d]", bs, kMaxBatch);
+  ZKV_REQUIRE(hq >= 1 && hq % kv == 0, "zkv_paged_attention: %d query heads over %d KV heads", hq, kv);
+  ZKV_REQUIRE(width >= 1 && table_stride >= 0 && window >= 0, "zkv_paged_attention: width %d, row stride %lld, window %d",
+              width, static_cast<long long>(table_stride), window);
+  ZKV_REQUIRE(static_cast<int64_t>(width) * page_size < (1ll << 31) - kTile,
+              "zkv_paged_attention: a request holds fewer than 2^31 - 32 tokens");
+  ZKV_REQUIRE(q_sb % 8 == 0 && q_sh % 8 == 0 &&
+                  ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) |
+                    reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0,
+              "zkv_paged_attention: rows start on 16 bytes");
+  ZKV_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "zkv_paged_attention: the workspace starts on 16 bytes");
+  const int gqa = hq / kv, groups = (gqa + kHeads - 1) / kHeads;
+  const int64_t most_tiles = static_cast<int64_t>(bs) * kv * groups *
+                             ((static_cast<int64_t>(width) * page_size + kTile - 1) / kTile + 1);
+  // (places on the line of tiles are 31-bit numbers)
+  ZKV_REQUIRE(most_tiles < (1ll << 31) - (1 << 20),
+              "zkv_paged_attention: %d requests of %d KV heads over %lld tokens are too many tiles for one call", bs, kv,
+              static_cast<long long>(width) * page_size);
+  if (workspace_bytes < workspace_bytes_for(d))
+    return fail(ZKV_ESPACE, "zkv_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
+                workspace_bytes_for(d));
+  PagedAttnParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_sb = q_sb;
+  p.q_sh = q_sh;
+  p.k = k_pages;
+  p.v = v_pages;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.layout = layout;
+  p.page = fast_div(static_cast<uint32_t>(page_size));
+  p.table = block_table;
+  p.table_stride = table_stride;
+  p.lens = seq_lens;
+  p.out = out;
+  p.lse = lse;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * d * 4);
+  p.part_ml = reinterpret_cast<float*>(ws);
+  ws += align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * 2 * 4);
+  p.arrivals = reinterpret_cast<unsigned long long*>(ws);
+  p.epoch = next_epoch();
+  p.units = fast_div(static_cast<uint32_t>(kv * groups));
+  p.groups = fast_div(static_cast<uint32_t>(groups));
+  p.scale = sm_scale * kLog2e;
+  p.bs = bs;
+  p.hq = hq;
+  p.kv = kv;
+  p.gqa = gqa;
+  p.window = window;
+  p.out_f32 = out_f32;
+  p.max_len = width * page_size;
+  p.heads_lds = std::min(gqa, kHeads);
+  auto s = reinterpret_cast<hipStream_t>(stream);
+  if (is_f16) return is_fp8 ? launch_by_dim<kF16, true>(p, d, most_tiles, s) : launch_by_dim<kF16, false>(p, d, most_tiles, s);
+  return is_fp8 ? launch_by_dim<kBf16, true>(p, d, most_tiles, s) : launch_by_dim<kBf16, false>(p, d, most_tiles, s);
+}
