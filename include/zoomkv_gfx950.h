@@ -684,8 +684,11 @@ int zkv_paged_qk_norm_rope(const void* qkv, int64_t qkv_stride, int rows, int hq
  * (nullable) fp32 [bs, hq], natural log.  Lengths are read on the device and
  * limited to [0, width * page_size]; tokens on a page id outside the pool are
  * left out; a request without a token gives zeros and -inf.  At most 4096
- * requests.  workspace: zkv_paged_attention_workspace_size(d) bytes, any
- * content; calls that overlap on one workspace race. */
+ * requests.  workspace: zkv_paged_attention_workspace_size(d) bytes, its first
+ * ZKV_PAGED_ARRIVAL_BYTES zero before the first call (every call leaves them
+ * zero; one workspace serves every d it is large enough for); calls that
+ * overlap on one workspace race. */
+#define ZKV_PAGED_ARRIVAL_BYTES 1024
 size_t zkv_paged_attention_workspace_size(int d);
 int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, const void* k_pages,
                         const void* v_pages, int is_fp8, const float* k_scale, const float* v_scale, int num_pages,

@@ -140,6 +140,32 @@ def test_lengths(lens):
     c.check(out, lse)
 
 
+@pytest.mark.parametrize("hq,kv,d,dtype", [(16, 16, 64, FP), (1, 1, 64, BF), (2, 1, 256, BF), (8, 8, 128, FP)])
+@pytest.mark.parametrize("n", [1500, 6000])
+def test_units_cut_on_both_sides(hq, kv, d, dtype, n):
+    """Few query heads, units longer than a workgroup's run: most workgroups
+    share a unit with the one before and another with the one after."""
+    c = Case([n + 37 * i for i in range(9)] + [40, 3, 0, 700], hq, kv, d, 24, dtype, seed=n)
+    for window in (0, n - 100):
+        out, lse = c.attend(window=window, return_softmax_lse=True)
+        c.check(out, lse, window=window, requests=[0, 4, 8, 9, 10, 11, 12])
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_calls(seed):
+    rng = np.random.default_rng(seed)
+    kv = int(rng.choice([1, 2, 3, 8]))
+    hq = kv * int(rng.choice([1, 2, 4, 5, 16, 24]))
+    top = int(rng.choice([20, 300, 5000]))
+    lens = [int(x) for x in rng.integers(0, top + 1, int(rng.integers(1, 40)))]
+    fp8 = bool(rng.integers(2))
+    c = Case(lens, hq, kv, int(rng.choice([64, 128, 256])), int(rng.choice([1, 8, 16, 24, 32, 100])),
+             [BF, FP][int(rng.integers(2))], fp8, bool(rng.integers(2)), seed=seed)
+    window = int(rng.choice([0, 0, 1, 33, 1000]))
+    out, lse = c.attend(window=window, return_softmax_lse=True)
+    c.check(out, lse, window=window, requests=sorted({0, len(lens) - 1, len(lens) // 2, int(np.argmax(lens))}))
+
+
 def test_long_sequence_of_one_head():
     """131072 tokens of one KV head: every workgroup holds a part of the unit."""
     c = Case([131072], 2, 1, 128, 128, seed=3)

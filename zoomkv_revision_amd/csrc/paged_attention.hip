@@ -10,16 +10,23 @@
 // One pass over the cache with the running maximum and sum of the softmax.
 //
 // Work.  A unit is one (b, KV head, group of up to 16 query heads); its tokens
-// are cut into tiles of 32.  The tiles of all units, in order, are one line of
-// T tiles: workgroup w takes tiles [w C, (w + 1) C), and inside it each wave an
-// equal run, whatever the lengths are (they are read on the device, so a
-// captured launch follows them).  A wave finishes the units that lie wholly in
-// its run by itself; the ends of its run go to LDS as partials (m, l, O) and
-// are joined there; the ends of the workgroup's run go to the workspace and
-// are joined by the last of the workgroups that share the unit.  Each
-// workgroup leaves at most two partials, whatever the batch is, and which
-// tiles are joined in which order depends on the lengths alone, so the result
-// is the same from run to run.
+// are cut into tiles of 32.  On a line, each unit takes a place per tile and
+// kUnitCost more for its start and end; workgroup w takes places [w C, (w + 1)
+// C), and inside it each wave an equal run, whatever the lengths are (they are
+// read on the device, so a captured launch follows them).  A wave finishes the
+// units that lie wholly in its run by itself; the ends of its run go to LDS as
+// partials (m, l, O) and are joined there; the ends of the workgroup's run go
+// to the workspace and are joined by the last of the workgroups that share the
+// unit.  Each workgroup leaves at most two partials, whatever the batch is, and
+// which tiles are joined in which order depends on the lengths alone, so the
+// result is the same from run to run.
+//
+// Stream.  A wave walks its run as one stream of tiles across the units: a
+// ring of kDepth tiles in registers, the request running kDepth - 1 tiles (and
+// the page ids one more) ahead of the use, so a unit's first tile does not
+// wait for memory any more than its others.  Of two waves on a SIMD the older
+// is served first and would end at 60% of the other's time; each publishes
+// its tiles done and raises its priority while it is behind.
 //
 // Tile.  S^T = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32: K rows are the
 // A operand (lane 16 g + c: token c, channels 32 s + 8 g ..), q the B operand
@@ -44,7 +51,12 @@ namespace {
 constexpr int kTile = 32;          // tokens of a tile: one k-step of the P V product
 constexpr int kHeads = 16;         // query heads of a unit: the columns of an MFMA
 constexpr int kMaxBatch = 4096;    // requests of a call: 4 bytes of LDS each
-constexpr int kMaxGroups = 256;    // workgroups: an arrival count is a byte
+constexpr int kMaxGroups = 256;    // workgroups
+constexpr int kUnitCost = 2;       // places of a unit beyond its tiles
+// Calls of at most this many places per workgroup are bound by latency: cuts
+// are then moved out of units of at most kWholeTiles tiles, whose joining
+// across workgroups would take longer than their tiles.
+constexpr int kShortRun = 32, kWholeTiles = 48;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
 // The softmax's reference exponent m follows the scores' running maximum only
@@ -68,8 +80,7 @@ struct PagedAttnParams {
   float* lse;
   float* part_o;   // [workgroup][2][kHeads][D]
   float* part_ml;  // [workgroup][2][kHeads][2]
-  unsigned long long* arrivals;  // per workgroup: the unit that starts in it
-  unsigned long long epoch;
+  unsigned int* arrivals;  // per workgroup: those of the unit that starts in it
   FastDiv units;   // units of one request: kv * groups
   FastDiv groups;  // groups of up to 16 query heads of a KV head
   float scale;     // softmax scale * log2 e
@@ -138,11 +149,15 @@ __device__ __forceinline__ float across_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-__device__ __forceinline__ void store_dev(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Device-coherent accesses of the partials (a pair of floats): the sharing
+// workgroups run on different XCDs, whose L2s are not coherent.
+__device__ __forceinline__ void store_dev(float* p, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, float2_t{a, b}),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float load_dev(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ float2_t load_dev(const float* p) {
+  return __builtin_bit_cast(float2_t, __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p),
+                                                        __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
 template <int kWords>
@@ -169,9 +184,13 @@ struct Shape {
   static constexpr int kChunks = kJ / kChunk;
   static constexpr int kChunkWords = kChunk * kCell / 4;
   static constexpr int kVWords = kChunks * kChunkWords;
+  static constexpr int kLoads = 2 * kKLoads + 8 * kChunks;  // of a tile
   // 8 waves: 2 on a SIMD, 256 registers each.  Head dim 256 holds twice the
   // tile and twice the output per wave: 4 waves with up to 512.
   static constexpr int kWaves = kD == 256 ? 4 : 8;
+  // tiles of the ring: 16 or 32 KiB per wave, in 64 to 256 registers
+  static constexpr int kTileRegs = kD * kCell / 4;
+  static constexpr int kDepth = kD == 256 ? (kFp8 ? 3 : 2) : (kTileRegs == 64 ? 2 : 4);
   // first channel of chunk n of output row r (r = 0 .. 15)
   static __device__ __forceinline__ int channel(int r, int n) { return n * (16 * kChunk) + r * kChunk; }
 };
@@ -181,14 +200,19 @@ struct TileRegs {
   u32x4_t k[2][Shape<kFp8, kD>::kKLoads];
   uint32_t v[8][Shape<kFp8, kD>::kVWords];
   uint32_t mask;  // bit t: token t is attended
+  int unit;       // the unit's number, -1: no tile
+  int flags;      // kFirst, kLast: of the wave's part of the unit; kWhole: the part is all of it
 };
+enum TileFlags : int { kFirst = 1, kLast = 2, kWhole = 4 };
 
-// One segment's view: a request's table row, and the head's rows.
-struct SegView {
-  const int32_t* row;
-  const uint8_t* k;
-  const uint8_t* v;
-  int first, len;
+// A place in a wave's stream of tiles.
+struct Cursor {
+  int b, rest;      // request, unit within it
+  int base, tiles;  // the unit's first place on the line, its tiles
+  int tile, left;   // the present tile of the request, the wave's tiles of the unit from it on (0: past the run)
+  int len;          // the request's length
+  int flags;        // kFirst, kWhole
+  int page;         // the page id of token (lane & 31) of the present tile
 };
 
 template <int kType, bool kFp8, int kD>
@@ -202,21 +226,19 @@ struct PagedAttn {
   float m, l;
   x8 q[S::kSteps];
 
-  // The page of token (lane & 31) of a tile (tokens past the end: the last).
-  static __device__ __forceinline__ int page_id(const PagedAttnParams& p, const SegView& s, int tile, int lane) {
-    const int t = min(tile * kTile + (lane & 31), s.len - 1);
-    return s.row[div_by(t, p.page)];
-  }
-
-  // Requests a tile's K and V.  The lane of each token forms its row's offset
-  // once; the lanes that read the row fetch it by ds_bpermute.
-  static __device__ __forceinline__ void request(const PagedAttnParams& p, const SegView& s, int tile, int page,
-                                                 int lane, Tile& x) {
-    const int t = tile * kTile + (lane & 31), tc = min(t, s.len - 1);
-    const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(p.layout.num_pages);
-    x.mask = static_cast<uint32_t>(__ballot(there && t < s.len && t >= s.first));
+  // Requests the K and V of a cursor's tile.  The lane of each token forms its
+  // row's offset once; the lanes that read the row fetch it by ds_bpermute.  A
+  // cursor past the run's end reads one row over and over.
+  static __device__ __forceinline__ void request(const PagedAttnParams& p, const Cursor& at, int lane, Tile& x) {
+    const int t = at.tile * kTile + (lane & 31), tc = min(t, at.len - 1);
+    const int first = p.window > 0 ? at.len - p.window : 0;
+    const bool there = at.left > 0 && static_cast<unsigned>(at.page) < static_cast<unsigned>(p.layout.num_pages);
+    x.mask = static_cast<uint32_t>(__ballot(there && t < at.len && t >= first));
+    x.unit = at.left > 0 ? at.b * static_cast<int>(p.units.d) + at.rest : -1;
+    x.flags = at.left > 0 ? at.flags | (at.left == 1 ? kLast : 0) : 0;
     const uint32_t in_page = tc - div_by(tc, p.page) * p.page.d;
-    const int64_t off = there ? (page * p.layout.page_stride + in_page * p.layout.token_stride) * S::kCell : 0;
+    const int64_t off =
+        there ? (at.page * p.layout.page_stride + in_page * p.layout.token_stride) * S::kCell : 0;
     const int lo = static_cast<int>(off), hi = static_cast<int>(off >> 32);
     const int c = lane & 15, g = lane >> 4;
     const auto row_of = [&](int token) {
@@ -224,20 +246,26 @@ struct PagedAttn {
       const uint32_t h32 = __builtin_amdgcn_ds_bpermute(4 * token, hi);
       return static_cast<int64_t>((static_cast<uint64_t>(h32) << 32) | l32);
     };
+    const int64_t head = div_by(at.rest, p.groups) * p.layout.head_stride * S::kCell;
+    const uint8_t* kp = static_cast<const uint8_t*>(p.k) + head + 16 * g;
+    const uint8_t* vp = static_cast<const uint8_t*>(p.v) + head + c * (S::kChunk * S::kCell);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      const uint8_t* r = s.k + row_of(16 * mt + c) + 16 * g;
+      const uint8_t* r = kp + row_of(16 * mt + c);
 #pragma unroll
       for (int i = 0; i < S::kKLoads; ++i)
         x.k[mt][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + 64 * i));
     }
+    __builtin_amdgcn_sched_barrier(0);  // K is used first: V behind it
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint8_t* r = s.v + row_of((e & 4) * 4 + 4 * g + (e & 3)) + c * (S::kChunk * S::kCell);
+      const uint8_t* r = vp + row_of((e & 4) * 4 + 4 * g + (e & 3));
 #pragma unroll
       for (int n = 0; n < S::kChunks; ++n)
         load_words<S::kChunkWords>(r + n * (16 * S::kChunk * S::kCell), x.v[e] + n * S::kChunkWords);
     }
+    // the use of an earlier tile stays behind these loads
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   static __device__ __forceinline__ x8 words8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -333,91 +361,90 @@ struct PagedAttn {
     }
   }
 
-  // Tiles [t0, t1) of one unit: two register tiles, the next one requested
-  // before the present one is used; page ids one tile further ahead.  The
-  // tail is peeled so that no request in the loop is conditional (a request
-  // on one of two paths makes the compiler wait for all of them).
-  __device__ __forceinline__ void segment(const PagedAttnParams& p, const SegView& s, int b, int head0, int heads,
-                                          float sc, int t0, int t1, int lane) {
+  // q of a unit as the B operand, in the channel order of the K operand's k-steps.
+  __device__ __forceinline__ void load_q(const PagedAttnParams& p, int b, int head0, int heads, int lane) {
     const int c = lane & 15, g = lane >> 4;
-    int page = page_id(p, s, t0, lane);
-    int next = page_id(p, s, min(t0 + 1, t1 - 1), lane);
-    // q as the B operand, in the channel order of the K operand's k-steps
     const uint16_t* qr = p.q + b * p.q_sb + (head0 + min(c, heads - 1)) * p.q_sh;
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
       const int ch = kFp8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
-      u32x4_t w = *reinterpret_cast<const u32x4_t*>(qr + ch);
-      if (c >= heads) w = u32x4_t{0, 0, 0, 0};
-      q[i] = __builtin_bit_cast(x8, w);
+      q[i] = __builtin_bit_cast(x8, *reinterpret_cast<const u32x4_t*>(qr + ch));
     }
+  }
+  // Uses, and so waits for, q: pending at every tile of the loop its loads
+  // would make each wait for the newest requests.
+  __device__ __forceinline__ void settle_q() {
+#pragma unroll
+    for (int i = 0; i < S::kSteps; ++i) asm volatile("" : "+v"(q[i]));
+  }
+
+  // output row r's (of this lane's four) channels j .. j + 3
+  __device__ __forceinline__ float4_t four(int j, int r) const {
+    return float4_t{o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]};
+  }
+
+  __device__ __forceinline__ void start() {
     m = -kInf;
     l = 0.0f;
 #pragma unroll
     for (int j = 0; j < S::kJ; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    Tile a, z;
-    request(p, s, t0, page, lane, a);
-    int t = t0;
-    for (; t + 2 < t1; t += 2) {
-      page = page_id(p, s, t + 2, lane);
-      request(p, s, t + 1, next, lane, z);
-      accumulate(a, sc, lane);
-      next = page_id(p, s, min(t + 3, t1 - 1), lane);
-      request(p, s, t + 2, page, lane, a);
-      accumulate(z, sc, lane);
-    }
-    if (t + 1 < t1) {
-      request(p, s, t + 1, next, lane, z);
-      accumulate(a, sc, lane);
-      accumulate(z, sc, lane);
-    } else {
-      accumulate(a, sc, lane);
-    }
-    l = across_sum(l);
   }
 };
 
-__device__ __forceinline__ void store_result(const PagedAttnParams& p, int type, int64_t at, float v) {
+// Four results (of one head, on 4 channels).
+template <int kType>
+__device__ __forceinline__ void store_result(const PagedAttnParams& p, int64_t at, const float4_t& v) {
   if (p.out_f32)
-    static_cast<float*>(p.out)[at] = v;
+    *reinterpret_cast<float4_t*>(static_cast<float*>(p.out) + at) = v;
   else
-    static_cast<uint16_t*>(p.out)[at] = type == kBf16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + at) =
+        u32x2_t{f32_to_elem<kType>(v[0]) | (f32_to_elem<kType>(v[1]) << 16),
+                f32_to_elem<kType>(v[2]) | (f32_to_elem<kType>(v[3]) << 16)};
 }
 
 __device__ __forceinline__ float natural_lse(float m, float l) {
   return l == 0.0f ? -kInf : (m + __log2f(l)) * kLn2v;
 }
 
-// One unit of the line of tiles.
+// LDS before the partials: the counters of a workgroup, and a place per request.
+__host__ __device__ constexpr size_t counter_bytes(int waves, int bs) {
+  return (static_cast<size_t>(4 * waves + 2 + bs + 1) * 4 + 15) / 16 * 16;
+}
+
+// One unit of the line.
 struct Unit {
   int b, kvh, head0, heads;  // request, KV head, first query head, query heads
-  int start, tiles;          // first place on the line, tiles
+  int base, tiles;           // first place on the line (its tiles start kUnitCost further), tiles
 };
 
 template <int kType, bool kFp8, int kD>
 __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attention_kernel(const PagedAttnParams p) {
   using S = Shape<kFp8, kD>;
-  constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves;
+  constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves, kSlots = 2 * kWaves;
   constexpr int kRow = kD + 4;  // row stride of a partial in LDS: 4 banks of skew between heads
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  float* s_o = reinterpret_cast<float*>(smem);                     // [2 waves][heads][kRow]
-  float* s_ml = s_o + 2 * kWaves * p.heads_lds * kRow;             // [2 waves][heads][2]
-  int* s_unit = reinterpret_cast<int*>(s_ml + 2 * kWaves * p.heads_lds * 2);  // [2 waves]: unit or -1
-  int* s_part = s_unit + 2 * kWaves;                               // [waves + 2]: scan, last-arrival flags
-  int* s_cum = s_part + kWaves + 2;                                // [bs + 1]: tiles of the requests before
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int* s_unit = reinterpret_cast<int*>(smem);  // [kSlots]: unit of a partial or -1
+  int* s_part = s_unit + kSlots;               // [kWaves + 2]: scan, last-arrival flags
+  int* s_done = s_part + kWaves + 2;           // [kWaves]: tiles done
+  int* s_cum = s_done + kWaves;                // [bs + 1]: places of the requests before, per unit
+  // (the last join uses the partials' space anew, beyond s_ml if it must: it comes last)
+  float* s_o = reinterpret_cast<float*>(smem + counter_bytes(kWaves, p.bs));  // [kSlots][heads][kRow]
+  float* s_ml = s_o + kSlots * p.heads_lds * kRow;                            // [kSlots][heads][2]
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int units = static_cast<int>(p.units.d);
 
-  // --- tiles of every request, and their running sum -----------------------
-  const auto first_of = [&](int len) { return p.window > 0 ? max(0, len - p.window) : 0; };
+  // --- places of every request, and their running sum -----------------------
   const auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.max_len); };
-  const auto tiles_of = [&](int len) { return (len + kTile - 1) / kTile - first_of(len) / kTile; };
+  const auto tile0_of = [&](int len) { return p.window > 0 ? max(0, len - p.window) / kTile : 0; };
+  const auto tiles_of = [&](int len) { return (len + kTile - 1) / kTile - tile0_of(len); };
   const int per = (p.bs + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.bs), b1 = min(b0 + per, p.bs);
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     const int n = tiles_of(len_of(b));
-    s_cum[b] = n;
-    mine += n;
+    s_cum[b] = n ? n + kUnitCost : 0;
+    mine += s_cum[b];
   }
   int scan = mine;
 #pragma unroll
@@ -426,7 +453,8 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     if (lane >= i) scan += u;
   }
   if (lane == 63) s_part[wave] = scan;
-  if (tid < 2 * kWaves) s_unit[tid] = -1;
+  if (tid < kSlots) s_unit[tid] = -1;
+  if (tid < kWaves) s_done[tid] = 0;
   __syncthreads();
   int before = scan - mine, total = 0;
   for (int w = 0; w < kWaves; ++w) {
@@ -440,158 +468,266 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   }
   if (tid == 0) s_cum[p.bs] = total;
   __syncthreads();
-  total *= p.units.d;
+  total = __builtin_amdgcn_readfirstlane(total) * units;
 
   // --- requests without a token: zeros -------------------------------------
   for (int b = blockIdx.x; b < p.bs; b += gridDim.x) {
     if (s_cum[b + 1] != s_cum[b]) continue;
     const int64_t row = static_cast<int64_t>(b) * p.hq;
-    for (int i = tid; i < p.hq * kD; i += kThreads) store_result(p, kType, row * kD + i, 0.0f);
+    for (int i = tid; i < p.hq * (kD / 4); i += kThreads)
+      store_result<kType>(p, row * kD + 4 * i, float4_t{0.0f, 0.0f, 0.0f, 0.0f});
     if (p.lse)
       for (int i = tid; i < p.hq; i += kThreads) p.lse[row + i] = -kInf;
   }
 
-  // --- this workgroup's run of tiles ---------------------------------------
-  const int chunk = max(kWaves, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
-  const int64_t from = static_cast<int64_t>(blockIdx.x) * chunk;
-  if (from >= total) return;
-  const int wg0 = static_cast<int>(from), wg1 = static_cast<int>(min(from + chunk, static_cast<int64_t>(total)));
-  const auto unit_of = [&](int b, int rest) {
+  // --- this workgroup's run of places --------------------------------------
+  const auto cum = [&](int b) { return __builtin_amdgcn_readfirstlane(s_cum[b]); };
+  // the request that place x belongs to
+  const auto request_at = [&](int x) {
+    const int at = static_cast<int>(div_by(x, p.units));
+    int lo = 0, hi = p.bs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (cum(mid + 1) > at)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    return lo;
+  };
+  const int grid = static_cast<int>(gridDim.x);
+  const int chunk = max(kWaves, (total + grid - 1) / grid);
+  const auto cut_at = [&](int w) {
+    const int64_t y64 = static_cast<int64_t>(w) * chunk;
+    if (y64 >= total) return total;
+    const int y = static_cast<int>(y64);
+    if (chunk > kShortRun) return y;
+    const int b = request_at(y), size = cum(b + 1) - cum(b), from = y - cum(b) * units, in = from % size;
+    return size - kUnitCost > kWholeTiles ? y : (2 * in < size ? y - in : y - in + size);
+  };
+  const int wg0 = cut_at(blockIdx.x), wg1 = cut_at(blockIdx.x + 1);
+  if (wg0 >= wg1) return;
+  const auto unit_at = [&](int id) {
     Unit u;
-    u.b = b;
-    const uint32_t kvh = div_by(rest, p.groups);
-    const int group = rest - static_cast<int>(kvh * p.groups.d);
-    u.kvh = static_cast<int>(kvh);
+    u.b = static_cast<int>(div_by(id, p.units));
+    const int rest = id - u.b * units;
+    u.kvh = static_cast<int>(div_by(rest, p.groups));
+    const int group = rest - u.kvh * static_cast<int>(p.groups.d);
     u.heads = min(kHeads, p.gqa - kHeads * group);
     u.head0 = u.kvh * p.gqa + kHeads * group;
-    u.tiles = s_cum[b + 1] - s_cum[b];
-    u.start = s_cum[b] * static_cast<int>(p.units.d) + rest * u.tiles;
+    const int size = cum(u.b + 1) - cum(u.b);
+    u.tiles = size - kUnitCost;
+    u.base = cum(u.b) * units + rest * size;
     return u;
   };
+  const auto v_scale_of = [&](int kvh) { return kFp8 && p.v_scale ? p.v_scale[kvh] : 1.0f; };
 
-  {
-    const int share = (wg1 - wg0 + kWaves - 1) / kWaves;
-    int x = wg0 + wave * share;
-    const int end = min(x + share, wg1);
-    int slot = 2 * wave;
-    PagedAttn<kType, kFp8, kD> attn;
-    while (x < end) {
-      // the request whose tiles hold place x
-      const int at = static_cast<int>(div_by(x, p.units));
-      int lo = 0, hi = p.bs - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s_cum[mid + 1] > at)
-          hi = mid;
-        else
-          lo = mid + 1;
+  // --- the wave's stream of tiles -------------------------------------------
+  const int share = (wg1 - wg0 + kWaves - 1) / kWaves;
+  const int x0 = wg0 + wave * share, x1 = min(x0 + share, wg1);
+  if (x0 < x1) {
+    Cursor at;
+    int tile0;
+    const auto enter = [&](int b) {  // a request's numbers
+      at.b = b;
+      at.len = len_of(b);
+      tile0 = tile0_of(at.len);
+      at.tiles = cum(b + 1) - cum(b) - kUnitCost;
+    };
+    const auto part = [&](int from) {  // the wave's part of the unit: its tiles from `from` on
+      const int end = min(at.tiles, x1 - at.base - kUnitCost);
+      at.tile = tile0 + from;
+      at.left = max(0, end - from);
+      at.flags = kFirst | (at.left == at.tiles ? kWhole : 0);
+    };
+    const auto next_unit = [&]() {
+      at.base += at.tiles + kUnitCost;
+      at.left = 0;
+      if (at.base + kUnitCost >= x1) return;  // (x1 is at most the line's end: there is a next unit)
+      if (++at.rest == units) {
+        at.rest = 0;
+        int b = at.b + 1;
+        while (cum(b + 1) == cum(b)) ++b;
+        enter(b);
       }
-      const int b = __builtin_amdgcn_readfirstlane(lo);
-      const int nt = s_cum[b + 1] - s_cum[b];
-      const int rest = (x - s_cum[b] * static_cast<int>(p.units.d)) / nt;
-      const Unit u = unit_of(b, rest);
-      const int t0 = x - u.start, t1 = min(nt, t0 + end - x);
-      const int len = len_of(b), first = first_of(len), tile0 = first / kTile;
-      const int64_t head_off = u.kvh * p.layout.head_stride * S::kCell;
-      const SegView view{p.table + b * p.table_stride, static_cast<const uint8_t*>(p.k) + head_off,
-                         static_cast<const uint8_t*>(p.v) + head_off, first, len};
-      float sc = p.scale;
-      if constexpr (kFp8) sc *= p.k_scale ? p.k_scale[u.kvh] : 1.0f;
-      attn.segment(p, view, b, u.head0, u.heads, sc, tile0 + t0, tile0 + t1, lane);
-      const int c = lane & 15, g = lane >> 4;
-      if (t0 == 0 && t1 == nt) {
-        // the whole unit: the result
-        if (c < u.heads) {
-          float inv = attn.l == 0.0f ? 0.0f : 1.0f / attn.l;
-          if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
-          const int64_t row = static_cast<int64_t>(b) * p.hq + u.head0 + c;
+      part(0);
+    };
+    // Page ids: 64 consecutive entries of the request's table row at a time,
+    // one a lane, handed out by ds_bpermute.  The load is waited for where it
+    // is made (the asm uses its value): a load that might be pending at every
+    // tile would make every tile wait for all but the newest request.
+    int window = 0, window0 = 0, window_of = -1;
+    const auto look_up = [&]() {
+      const int t = at.tile * kTile, t1 = min(t + kTile, at.len) - 1;
+      const int e0 = static_cast<int>(div_by(t, p.page)), e1 = static_cast<int>(div_by(t1, p.page));
+      if (at.b != window_of || e0 < window0 || e1 >= window0 + 64) {
+        window_of = at.b;
+        window0 = e0;
+        window = p.table[at.b * p.table_stride + min(e0 + lane, static_cast<int>(div_by(at.len - 1, p.page)))];
+        asm volatile("" : "+v"(window));
+      }
+      const int mine = static_cast<int>(div_by(min(t + (lane & 31), t1), p.page));
+      at.page = __builtin_amdgcn_ds_bpermute(4 * (mine - window0), window);
+    };
+    const auto advance = [&]() {
+      if (at.left > 1) {
+        --at.left;
+        ++at.tile;
+        at.flags &= ~kFirst;
+      } else if (at.left == 1) {
+        next_unit();
+      }
+      look_up();
+    };
+    enter(request_at(x0));
+    {
+      const int size = at.tiles + kUnitCost, from = x0 - cum(at.b) * units;
+      at.rest = from / size;
+      at.base = x0 - from + at.rest * size;
+      part(max(0, x0 - at.base - kUnitCost));
+      if (at.left == 0) next_unit();
+    }
+    PagedAttn<kType, kFp8, kD> attn;
+    float sc = 0.0f;
+    const auto begin_unit = [&](int id) {
+      const Unit u = unit_at(id);
+      attn.load_q(p, u.b, u.head0, u.heads, lane);
+      sc = p.scale * (kFp8 && p.k_scale ? p.k_scale[u.kvh] : 1.0f);
+      attn.start();
+    };
+    begin_unit(at.b * units + at.rest);  // (its q and the first page ids in one round trip)
+    look_up();
+    attn.settle_q();
+    TileRegs<kFp8, kD> ring[S::kDepth];
+    int slot = kSlots / kWaves * wave, done = 0;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < S::kDepth - 1; ++i) {
+      const Cursor now = at;
+      advance();
+      attn.request(p, now, lane, ring[i]);
+    }
+    ring[0].flags &= ~kFirst;
+    do {
 #pragma unroll
-            for (int n = 0; n < S::kChunks; ++n) {
-              const int64_t at0 = row * kD + S::channel(4 * g + i, n);
-#pragma unroll
-              for (int j = 0; j < S::kChunk; ++j)
-                store_result(p, kType, at0 + j, attn.o[n * S::kChunk + j][i] * inv);
-            }
-          if (p.lse && g == 0) p.lse[row] = natural_lse(attn.m, attn.l);
+      for (int i = 0; i < S::kDepth; ++i) {
+        TileRegs<kFp8, kD>& x = ring[i];
+        if (x.flags & kFirst) {
+          begin_unit(x.unit);
+          attn.settle_q();
         }
-      } else {
-        if (c < u.heads) {
-          float* dst = s_o + (slot * p.heads_lds + c) * kRow;
+        const Cursor now = at;
+        advance();
+        attn.request(p, now, lane, ring[(i + S::kDepth - 1) % S::kDepth]);
+        // The tile's loads are older than those of the kDepth - 1 requests
+        // behind it: waited for here by count, on every path, or a path that
+        // seems to pass them by would make the compiler wait for the newest.
+        wait_vmcnt<(S::kDepth - 1) * S::kLoads>();
+        if (x.unit < 0) continue;
+        attn.accumulate(x, sc, lane);
+        if constexpr (kWaves == 8) {
+          ++done;
+          __hip_atomic_store(&s_done[wave], done, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          const int other = __hip_atomic_load(&s_done[wave ^ 4], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          if (__builtin_amdgcn_readfirstlane(other) > done)
+            __builtin_amdgcn_s_setprio(1);
+          else
+            __builtin_amdgcn_s_setprio(0);
+        }
+        if (x.flags & kLast) {
+          const Unit u = unit_at(x.unit);
+          const int c = lane & 15, g = lane >> 4;
+          const float l = across_sum(attn.l);
+          if (x.flags & kWhole) {
+            if (c < u.heads) {
+              const float inv = (l == 0.0f ? 0.0f : 1.0f / l) * v_scale_of(u.kvh);
+              const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+              for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int n = 0; n < S::kChunks; ++n)
+                for (int n = 0; n < S::kChunks; ++n) {
+                  const int64_t at0 = row * kD + S::channel(4 * g + r, n);
 #pragma unroll
-              for (int j = 0; j < S::kChunk; j += 4) {
-                const float4_t y = {attn.o[n * S::kChunk + j][i], attn.o[n * S::kChunk + j + 1][i],
-                                    attn.o[n * S::kChunk + j + 2][i], attn.o[n * S::kChunk + j + 3][i]};
-                *reinterpret_cast<float4_t*>(dst + S::channel(4 * g + i, n) + j) = y;
+                  for (int j = 0; j < S::kChunk; j += 4)
+                    store_result<kType>(p, at0 + j, attn.four(n * S::kChunk + j, r) * inv);
+                }
+              if (p.lse && g == 0) p.lse[row] = natural_lse(attn.m, l);
+            }
+          } else {
+            // at most the run's first and last unit are cut
+            if (c < u.heads) {
+              float* dst = s_o + (slot * p.heads_lds + c) * kRow;
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int n = 0; n < S::kChunks; ++n)
+#pragma unroll
+                  for (int j = 0; j < S::kChunk; j += 4)
+                    *reinterpret_cast<float4_t*>(dst + S::channel(4 * g + r, n) + j) = attn.four(n * S::kChunk + j, r);
+              if (g == 0) {
+                s_ml[(slot * p.heads_lds + c) * 2] = attn.m;
+                s_ml[(slot * p.heads_lds + c) * 2 + 1] = l;
               }
-          if (g == 0) {
-            s_ml[(slot * p.heads_lds + c) * 2] = attn.m;
-            s_ml[(slot * p.heads_lds + c) * 2 + 1] = attn.l;
+            }
+            if (lane == 0) s_unit[slot] = x.unit;
+            ++slot;
           }
         }
-        if (lane == 0) s_unit[slot] = b * static_cast<int>(p.units.d) + rest;
-        ++slot;  // at most the run's first and last unit are cut
       }
-      x += t1 - t0;
-    }
+    } while (ring[0].unit >= 0);
+    __builtin_amdgcn_s_setprio(0);
   }
   __syncthreads();
 
   // --- join the waves' partials, unit by unit ------------------------------
-  const auto unit_at = [&](int id) {
-    const int b = static_cast<int>(div_by(id, p.units));
-    return unit_of(b, id - b * static_cast<int>(p.units.d));
-  };
+  int ids[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) ids[i] = __builtin_amdgcn_readfirstlane(s_unit[i]);
   int cut[2] = {-1, -1};  // units shared with earlier / later workgroups
-  for (int i0 = 0; i0 < 2 * kWaves;) {
-    const int id = s_unit[i0];
-    if (id < 0) {
-      ++i0;
-      continue;
-    }
-    int i1 = i0 + 1;
-    while (i1 < 2 * kWaves && (s_unit[i1] == id || s_unit[i1] < 0)) ++i1;
+  int id = -1;
+#pragma unroll 1
+  for (;;) {
+    // the next unit (they ascend through the slots)
+    int next = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) next = ids[i] > id ? min(next, ids[i]) : next;
+    if (next == 0x7FFFFFFF) break;
+    id = next;
     const Unit u = unit_at(id);
-    const bool whole = u.start >= wg0 && u.start + u.tiles <= wg1;
-    const int side = u.start >= wg0 ? 1 : 0;
-    if (!whole) cut[side] = id;
+    const bool starts = u.base + kUnitCost >= wg0;
+    const bool whole = starts && u.base + kUnitCost + u.tiles <= wg1;
+    if (!whole) cut[starts ? 1 : 0] = id;
     for (int e = tid; e < u.heads * (kD / 4); e += kThreads) {
       const int c = e / (kD / 4), d = 4 * (e % (kD / 4));
-      float top = -kInf;
-      for (int i = i0; i < i1; ++i)
-        if (s_unit[i] == id) top = fmaxf(top, s_ml[(i * p.heads_lds + c) * 2]);
+      float mv[kSlots], lv[kSlots], top = -kInf;
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        const float2_t ml = *reinterpret_cast<const float2_t*>(s_ml + (i * p.heads_lds + c) * 2);
+        mv[i] = ids[i] == id ? ml[0] : -kInf;
+        lv[i] = ids[i] == id ? ml[1] : 0.0f;
+        top = fmaxf(top, mv[i]);
+      }
       const float base = top == -kInf ? 0.0f : top;
       float den = 0.0f;
       float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int i = i0; i < i1; ++i) {
-        if (s_unit[i] != id) continue;
-        const float w = __builtin_amdgcn_exp2f(s_ml[(i * p.heads_lds + c) * 2] - base);
-        den += w * s_ml[(i * p.heads_lds + c) * 2 + 1];
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (ids[i] != id) continue;
+        const float w = __builtin_amdgcn_exp2f(mv[i] - base);
+        den += w * lv[i];
         num += w * *reinterpret_cast<const float4_t*>(s_o + (i * p.heads_lds + c) * kRow + d);
       }
       if (whole) {
-        float inv = den == 0.0f ? 0.0f : 1.0f / den;
-        if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
+        const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
         const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store_result(p, kType, row * kD + d + j, num[j] * inv);
+        store_result<kType>(p, row * kD + d, num * inv);
         if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
       } else {
-        const int64_t row = (static_cast<int64_t>(blockIdx.x) * 2 + side) * kHeads + c;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) store_dev(p.part_o + row * kD + d + j, num[j]);
-        if (d == 0) {
-          store_dev(p.part_ml + row * 2, top);
-          store_dev(p.part_ml + row * 2 + 1, den);
-        }
+        const int64_t row = (static_cast<int64_t>(blockIdx.x) * 2 + (starts ? 1 : 0)) * kHeads + c;
+        store_dev(p.part_o + row * kD + d, num[0], num[1]);
+        store_dev(p.part_o + row * kD + d + 2, num[2], num[3]);
+        if (d == 0) store_dev(p.part_ml + row * 2, top, den);
       }
     }
-    i0 = i1;
   }
   if (cut[0] < 0 && cut[1] < 0) return;
 
@@ -601,76 +737,106 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   // joining loads read there: no cache is written back or invalidated.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (tid < 2) {
-    const int id = cut[tid];
+  const auto first_group = [&](const Unit& u) { return (u.base + kUnitCost) / chunk; };
+  const auto groups_of = [&](const Unit& u) { return (u.base + kUnitCost + u.tiles - 1) / chunk - first_group(u) + 1; };
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
     int last = 0;
-    if (id >= 0) {
-      const Unit u = unit_at(id);
-      const int w0 = u.start / chunk, w1 = (u.start + u.tiles - 1) / chunk;
-      last = arrive_last(p.arrivals + w0, p.epoch, w1 - w0 + 1);
+    if (cut[side] >= 0) {
+      const Unit u = unit_at(cut[side]);
+      if (tid == side) last = arrive_last_count(p.arrivals + first_group(u), groups_of(u));
     }
-    s_part[tid] = last;
+    if (tid == side) s_part[side] = last;
   }
   __syncthreads();
+#pragma unroll 1
   for (int side = 0; side < 2; ++side) {
-    if (cut[side] < 0 || !s_part[side]) continue;
-    const Unit u = unit_at(cut[side]);
-    const int w0 = u.start / chunk, n = (u.start + u.tiles - 1) / chunk - w0 + 1;
-    // partial i: the unit's first workgroup kept it as its later cut, the others as their earlier one
+    const int id = side ? cut[1] : cut[0];
+    if (id < 0 || !__builtin_amdgcn_readfirstlane(s_part[side])) continue;
+    const Unit u = unit_at(id);
+    const int w0 = first_group(u), n = groups_of(u);
+    // partial i: the unit's first workgroup kept it as its later cut, the
+    // others as their earlier one
     const auto row_of = [&](int i, int c) {
       return ((static_cast<int64_t>(w0) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
     };
+    // four channels of a head per thread, and as many threads per such item
+    // as there are, each with its part of the partials, eight requested at
+    // once; the parts meet in LDS
+    const int items = u.heads * (kD / 4);
     constexpr int kBatch = 8;
-    for (int e = tid; e < u.heads * kD; e += kThreads) {
-      const int c = e / kD, d = e % kD;
-      float top = -kInf;
-      for (int i0 = 0; i0 < n; i0 += kBatch) {
-        float mv[kBatch];
+#pragma unroll 1
+    for (int e0 = 0; e0 < items; e0 += kThreads) {
+      const int here = min(kThreads, items - e0), parts = kThreads / here;
+      __syncthreads();  // (s_o of the join before is read)
+      const int part = tid / here, e = e0 + tid - part * here, c = e / (kD / 4), d = 4 * (e % (kD / 4));
+      if (part < parts) {
+        float top = -kInf, den = 0.0f;
+        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = part; i0 < n; i0 += kBatch * parts) {
+          float2_t ml[kBatch], lo[kBatch], hi[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) mv[i] = load_dev(p.part_ml + row_of(min(i0 + i, n - 1), c) * 2);
+          for (int i = 0; i < kBatch; ++i) {
+            const int64_t row = row_of(min(i0 + i * parts, n - 1), c);
+            ml[i] = load_dev(p.part_ml + row * 2);
+            lo[i] = load_dev(p.part_o + row * kD + d);
+            hi[i] = load_dev(p.part_o + row * kD + d + 2);
+          }
+          float now = top;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) top = fmaxf(top, mv[i]);
-      }
-      const float base = top == -kInf ? 0.0f : top;
-      float den = 0.0f, num = 0.0f;
-      for (int i0 = 0; i0 < n; i0 += kBatch) {
-        float mv[kBatch], lv[kBatch], ov[kBatch];
+          for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < n ? fmaxf(now, ml[i][0]) : now;
+          const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
+          top = now;
+          den *= a;
+          num *= a;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int64_t row = row_of(min(i0 + i, n - 1), c);
-          mv[i] = load_dev(p.part_ml + row * 2);
-          lv[i] = load_dev(p.part_ml + row * 2 + 1);
-          ov[i] = load_dev(p.part_o + row * kD + d);
+          for (int i = 0; i < kBatch; ++i) {
+            if (i0 + i * parts >= n) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
+            den += w * ml[i][1];
+            num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+          }
         }
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const float w = __builtin_amdgcn_exp2f(mv[i] - base);
-          den = i0 + i < n ? den + w * lv[i] : den;
-          num = i0 + i < n ? num + w * ov[i] : num;
-        }
+        float* dst = s_o + tid * 8;
+        *reinterpret_cast<float4_t*>(dst) = num;
+        dst[4] = top;
+        dst[5] = den;
       }
-      float inv = den == 0.0f ? 0.0f : 1.0f / den;
-      if constexpr (kFp8) inv *= p.v_scale ? p.v_scale[u.kvh] : 1.0f;
-      const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
-      store_result(p, kType, row * kD + d, num * inv);
-      if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+      __syncthreads();
+      if (tid < here) {
+        float top = -kInf;
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, s_o[(i * here + tid) * 8 + 4]);
+        const float base = top == -kInf ? 0.0f : top;
+        float den = 0.0f;
+        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < parts; ++i) {
+          const float* src = s_o + (i * here + tid) * 8;
+          const float w = __builtin_amdgcn_exp2f(src[4] - base);
+          den += w * src[5];
+          num += w * *reinterpret_cast<const float4_t*>(src);
+        }
+        const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
+        const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
+        store_result<kType>(p, row * kD + d, num * inv);
+        if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+      }
     }
   }
 }
 
-constexpr size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-
 size_t workspace_bytes_for(int d) {
-  return align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * d * 4) +
-         align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * 2 * 4) + kMaxGroups * 8;
+  static_assert(kMaxGroups * 4 == ZKV_PAGED_ARRIVAL_BYTES, "arrival counts");
+  return static_cast<size_t>(kMaxGroups) * 4 + static_cast<size_t>(kMaxGroups) * 2 * kHeads * (d + 2) * 4;
 }
 
 template <int kType, bool kFp8, int kD>
 int launch_paged_attention(PagedAttnParams& p, int64_t most_tiles, hipStream_t s) {
   using S = Shape<kFp8, kD>;
   const auto kernel = paged_attention_kernel<kType, kFp8, kD>;
-  const size_t lds = static_cast<size_t>(2 * S::kWaves) * p.heads_lds * (kD + 6) * 4 +
-                     (2 * S::kWaves + S::kWaves + 2 + p.bs + 1) * 4;
+  // the counters, then the partials (in the last join, 32 bytes a thread)
+  const size_t lds = std::max(static_cast<size_t>(2 * S::kWaves) * p.heads_lds * (kD + 6) * 4,
+                              static_cast<size_t>(64 * S::kWaves) * 32) +
+                     counter_bytes(S::kWaves, p.bs);
   if (lds > 60 * 1024 &&
       hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                           160 * 1024) != hipSuccess)
@@ -719,13 +885,13 @@ extern "C" int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, in
               "zkv_paged_attention: a request holds fewer than 2^31 - 32 tokens");
   ZKV_REQUIRE(q_sb % 8 == 0 && q_sh % 8 == 0 &&
                   ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) |
-                    reinterpret_cast<uintptr_t>(v_pages)) & 15) == 0,
+                    reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(out)) & 15) == 0,
               "zkv_paged_attention: rows start on 16 bytes");
   ZKV_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "zkv_paged_attention: the workspace starts on 16 bytes");
   const int gqa = hq / kv, groups = (gqa + kHeads - 1) / kHeads;
   const int64_t most_tiles = static_cast<int64_t>(bs) * kv * groups *
-                             ((static_cast<int64_t>(width) * page_size + kTile - 1) / kTile + 1);
-  // (places on the line of tiles are 31-bit numbers)
+                             ((static_cast<int64_t>(width) * page_size + kTile - 1) / kTile + 1 + kUnitCost);
+  // (places on the line are 31-bit numbers)
   ZKV_REQUIRE(most_tiles < (1ll << 31) - (1 << 20),
               "zkv_paged_attention: %d requests of %d KV heads over %lld tokens are too many tiles for one call", bs, kv,
               static_cast<long long>(width) * page_size);
@@ -748,12 +914,10 @@ extern "C" int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, in
   p.out = out;
   p.lse = lse;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  ws += align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * d * 4);
+  p.arrivals = reinterpret_cast<unsigned int*>(ws);
+  ws += kMaxGroups * 4;
   p.part_ml = reinterpret_cast<float*>(ws);
-  ws += align256(static_cast<size_t>(kMaxGroups) * 2 * kHeads * 2 * 4);
-  p.arrivals = reinterpret_cast<unsigned long long*>(ws);
-  p.epoch = next_epoch();
+  p.part_o = p.part_ml + static_cast<size_t>(kMaxGroups) * 2 * kHeads * 2;
   p.units = fast_div(static_cast<uint32_t>(kv * groups));
   p.groups = fast_div(static_cast<uint32_t>(groups));
   p.scale = sm_scale * kLog2e;

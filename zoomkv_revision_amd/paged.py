@@ -45,18 +45,28 @@ _STATUS_TEXT = {POOL_EMPTY: "no free pages for a request", TABLE_FULL: "a reques
                 RING_FULL: "more pages were given back than the ring holds"}
 
 _WS: dict = {}
+_ARRIVAL_BYTES = 1024        # of an attention workspace (ZKV_PAGED_ARRIVAL_BYTES)
 
 
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Partials and arrival slots per (device, stream); under graph capture a
-    buffer of the graph's own, so that two graphs never share one.  Its content
-    does not matter (the arrival slots carry each launch's epoch)."""
+    """Arrival counts and partials per (device, stream); under graph capture a
+    buffer of the graph's own, so that two graphs never share one (its counts
+    are then cleared in the graph, a launch more: a plan, or a workspace that
+    is passed in, saves it)."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return _new_workspace(device, nbytes)
     key = (device, device_stream(device))
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _WS[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        ws = _WS[key] = _new_workspace(device, nbytes)
+    return ws
+
+
+def _new_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """The arrival counts, at the front, are 0 between calls; the partials
+    behind them need no clearing."""
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws[:_ARRIVAL_BYTES].zero_()
     return ws
 
 
@@ -381,13 +391,14 @@ def _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, w
     if window < 0:
         raise ValueError(f"window must not be negative (0: the whole sequence); got {window}")
     groups = -(-(hq // kv) // 16)
-    if width * page >= (1 << 31) - 32 or bs * kv * groups * (-(-width * page // 32) + 1) >= (1 << 31) - (1 << 20):
+    if width * page >= (1 << 31) - 32 or bs * kv * groups * (-(-width * page // 32) + 2) >= (1 << 31) - (1 << 20):
         raise ValueError(f"{bs} requests of up to {width * page} tokens in one call")
     out_shape = tuple(q.shape)
     if out is None:
         out = torch.empty(out_shape, dtype=q.dtype, device=q.device)
-    elif out.dtype not in (q.dtype, torch.float32) or not out.is_contiguous() or out.numel() != bs * hq * d:
-        raise ValueError(f"out must be a contiguous {list(out_shape)} tensor of q's dtype or float32")
+    elif out.dtype not in (q.dtype, torch.float32) or not out.is_contiguous() or out.numel() != bs * hq * d or \
+            out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous {list(out_shape)} tensor of q's dtype or float32 on 16 bytes")
     _same_device(q, k_pages=k_pages, block_table=block_table, seq_lens=seq_lens, out=out, workspace=workspace)
     if not _check_rows("q", q3):
         if not copies:
@@ -419,8 +430,7 @@ class PagedAttentionPlan(_Plan):
     def __init__(self, q, k_pages, v_pages, block_table, seq_lens, softmax_scale=None, window=0, k_scale=None,
                  v_scale=None, return_softmax_lse=False, out=None, workspace=None):
         if workspace is None and q.is_cuda and q.shape[-1] in HEAD_DIMS:
-            workspace = torch.empty(lib().zkv_paged_attention_workspace_size(q.shape[-1]), dtype=torch.uint8,
-                                    device=q.device)
+            workspace = _new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
         args, result, keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                              v_scale, return_softmax_lse, out, workspace, copies=False)
         super().__init__(lib().zkv_paged_attention, q.device, args, result, keep)
