@@ -213,6 +213,21 @@ def test_every_16_bit_value_as_e4m3():
             assert bool(((got[nan] & 0x7F) == 0x7F).all())
 
 
+@pytest.mark.parametrize("scale", [1.0, 3.0, 0.007, 1e-3, 448.0, 2.0 ** -99, 2.0 ** -101, 2.0 ** -140, 1e30, 1e38, 0.0, -2.0])
+def test_quotients_of_every_bf16_value(scale):
+    """row / scale as torch divides and casts it, for every bf16 row value."""
+    rows = torch.arange(65536, dtype=torch.int32, device=DEV).to(torch.int16).view(torch.bfloat16).view(512, 1, 128)
+    pools = _pools((512, 1, 1, 128), torch.float8_e4m3fn, False, 0.0)
+    slots = torch.arange(512, device=DEV)
+    s = torch.full((1,), scale, device=DEV)
+    paged.paged_write(rows, rows, slots, *pools, s, s)
+    x = (rows.cpu().double() / s.cpu().double()).float()        # (the rounded quotient: 48 bits round to 24)
+    x = torch.where(rows.cpu().float().isinf() | (s.cpu() == 0), rows.cpu().float() / s.cpu(), x)
+    want, nan = x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8), torch.isnan(x)
+    got = _stored(pools[1], slots).cpu()
+    assert torch.equal(got[~nan], want[~nan]) and bool(((got[nan] & 0x7F) == 0x7F).all())
+
+
 def test_write_of_unaligned_and_empty_rows():
     pools = _pools((4, 2, 4, 128), torch.bfloat16, False, 0.0)
     odd = torch.randn(3, 2, 129, device=DEV).to(torch.bfloat16)[..., 1:]

@@ -9,13 +9,11 @@ the output's type; A = sum p |v| of the exact weights, n tokens, head dim d):
     2 e relative (numerator and denominator); exp2 of an fp32 argument x adds
     2^-24 |x| + 2^-23, below 2^-19 for |x| < 2^4.5, beyond which 131072 tokens
     together weigh less than one at x = 0;
-  * P enters the product as hi, cut to the type, and lo, its rest rounded: in
-    bf16 the rest is below 2^-7 P and lo is off by 2^-8 of that, 2^-15 P (fp16
-    less);
+  * P enters the product as three 8-bit or two 11-bit parts: 2^-21 relative;
   * sums of n fp32 terms, and the joining of partials: (n + 64) 2^-24, twice;
 
-so |out - ref| <= u |ref| + A (2 e + 2^-14 + (n + 64) 2^-23), as 2^-15 + 2 *
-2^-19 < 2^-14.  The log-sum-exp (of the unsplit P) moves by at most e + 2^-16 +
+so |out - ref| <= u |ref| + A (2 e + 2^-17 + (n + 64) 2^-23), as 2^-21 + 2 *
+2^-19 < 2^-17.  The log-sum-exp (of the unsplit P) moves by at most e + 2^-16 +
 (n + 64) 2^-23, plus its own fp32 rounding 2^-23 |lse|."""
 import numpy as np
 import pytest
@@ -97,7 +95,7 @@ class Case:
                     (np.abs(q[b, 0, heads]) @ np.abs(k).T).max(initial=0.0)
                 sums = (len(seen) + 64) * 2.0 ** -23
                 err = np.abs(got[b, heads] - ref)
-                tol = U[out.dtype] * np.abs(ref) + mass * (2 * e + 2.0 ** -14 + sums) + 2.0 ** -25
+                tol = U[out.dtype] * np.abs(ref) + mass * (2 * e + 2.0 ** -17 + sums) + 2.0 ** -25
                 assert (err <= tol).all(), (b, h, float((err - tol).max()))
                 if lse is not None:
                     gl = lse.double().cpu().numpy()[b, heads, 0]

@@ -21,7 +21,7 @@ namespace {
 // page tables
 // ---------------------------------------------------------------------------
 constexpr int kMaxRequests = 8192;      // the scans' LDS: 16 bytes a request
-constexpr int kAdvanceThreads = 256;
+constexpr int kFewRequests = 512;       // beyond: 1024 threads, so that one scans at most 8 requests
 constexpr uint32_t kGranted = 0x80000000u;
 
 struct AdvanceParams {
@@ -91,15 +91,18 @@ __device__ __forceinline__ int owner_of(const int* ends, int n, int x) {
 // writes.
 //
 // Bound by latency: one read of the batch, one LDS search and one dependent
-// read of a page id per token.
-__global__ __launch_bounds__(kAdvanceThreads) void page_advance_kernel(const AdvanceParams p) {
+// read of a page id per token.  5 us for 64 requests of one token; 1024 mixed
+// requests with 65536 slots 9.0 us (12.2 with 256 threads a workgroup, whose
+// scans are four requests a thread), 8192 requests 22 us.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvanceParams p) {
   extern __shared__ int smem[];
   const int R = p.requests, tid = threadIdx.x;
   uint32_t* s_len = reinterpret_cast<uint32_t*>(smem);  // length; kGranted: grows in this step
   int* s_tok = smem + R;                                // ends of the requests' tokens
   int* s_need = s_tok + R;                              // ends of the pages they take
   int* s_give = s_need + R;                             // ends of the pages they give back
-  __shared__ int part[kAdvanceThreads / 64];
+  __shared__ int part[kThreads / 64];
   __shared__ int s_status, s_taken, s_last;
   const int head = static_cast<int>(static_cast<uint32_t>(p.state[0]) % static_cast<uint32_t>(p.num_pages));
   const int count = min(max(p.state[1], 0), p.num_pages);
@@ -108,17 +111,24 @@ __global__ __launch_bounds__(kAdvanceThreads) void page_advance_kernel(const Adv
     s_status = 0;
     s_taken = 0;
   }
-  const int per = (R + kAdvanceThreads - 1) / kAdvanceThreads;
+  // the batch in one coalesced read (its lengths and new tokens as they are)
+#pragma unroll 4
+  for (int i = tid; i < R; i += kThreads) {
+    s_len[i] = static_cast<uint32_t>(p.lens[i]);
+    s_tok[i] = p.new_tokens[i];
+  }
+  __syncthreads();
+  const int per = (R + kThreads - 1) / kThreads;
   const int i0 = min(tid * per, R), i1 = min(i0 + per, R);
   const int tok_top = p.cap + 1, page_top = p.num_pages + 1;
   // tokens: every request's new ones count, whether or not it is served, so
   // that the rows of a packed batch keep their places
   int sum = 0;
-  for (int i = i0; i < i1; ++i) sum = limited(sum, min(max(p.new_tokens[i], 0), tok_top), tok_top);
+  for (int i = i0; i < i1; ++i) sum = limited(sum, min(max(s_tok[i], 0), tok_top), tok_top);
   sum = scan_before(sum, tok_top, part);
   int status = 0, need_sum = 0, give_sum = 0;
   for (int i = i0; i < i1; ++i) {
-    const int len = p.lens[i], n = p.new_tokens[i];
+    const int len = static_cast<int>(s_len[i]), n = s_tok[i];
     const int64_t after = static_cast<int64_t>(len) + n;
     sum = limited(sum, min(max(n, 0), tok_top), tok_top);
     int need = -1, give = 0;  // need < 0: not to be served
@@ -166,13 +176,13 @@ __global__ __launch_bounds__(kAdvanceThreads) void page_advance_kernel(const Adv
   if (tid == 0)
     s_last = gridDim.x == 1 || arrive_last_count(reinterpret_cast<unsigned*>(p.state + 3), static_cast<int>(gridDim.x));
   const int total = s_tok[R - 1], freed = s_give[R - 1];
-  const int page_size = static_cast<int>(p.page.d), stride = static_cast<int>(gridDim.x) * kAdvanceThreads;
+  const int page_size = static_cast<int>(p.page.d), stride = static_cast<int>(gridDim.x) * kThreads;
   const auto ring_at = [&](uint32_t rank) {  // (head + rank < 2 num_pages)
     const uint32_t w = static_cast<uint32_t>(head) + rank;
     return w >= static_cast<uint32_t>(p.num_pages) ? w - p.num_pages : w;
   };
   // slots and positions; the token that opens a new page writes its table entry
-  for (int t = blockIdx.x * kAdvanceThreads + tid; t < p.cap; t += stride) {
+  for (int t = blockIdx.x * kThreads + tid; t < p.cap; t += stride) {
     int64_t slot = -1;
     int pos = -1;
     if (t < total) {
@@ -200,14 +210,14 @@ __global__ __launch_bounds__(kAdvanceThreads) void page_advance_kernel(const Adv
   // pages given back, in request order and table order, behind the ring's
   // last; never beyond the ring (an inconsistent state would overrun it)
   const int room = min(freed, p.num_pages - count);
-  for (int j = blockIdx.x * kAdvanceThreads + tid; j < room; j += stride) {
+  for (int j = blockIdx.x * kThreads + tid; j < room; j += stride) {
     const int r = owner_of(s_give, R, j);
     const int held = pages_of(s_len[r], p.page);
     p.ring[ring_at(count + j)] = p.table[r * p.table_stride + held - (s_give[r] - j)];
   }
   __syncthreads();  // s_last
   if (!s_last) return;
-  for (int i = tid; i < R; i += kAdvanceThreads) {
+  for (int i = tid; i < R; i += kThreads) {
     const int len = p.lens[i], n = p.new_tokens[i];
     int now = len;
     if (s_len[i] & kGranted)
@@ -248,11 +258,35 @@ __device__ __forceinline__ u32x4_t pack8(const float (&y)[8]) {
   return r;
 }
 
-// y / scale as e4m3, the quotient rounded once to fp32 (an IEEE division) and
-// once to the code.
-__device__ __forceinline__ u32x2_t quant8(const float (&y)[8], float scale) {
-  return u32x2_t{e4m3x4(y[0] / scale, y[1] / scale, y[2] / scale, y[3] / scale),
-                 e4m3x4(y[4] / scale, y[5] / scale, y[6] / scale, y[7] / scale)};
+// y / scale as e4m3: the quotient as an IEEE division rounds it, clamped, and
+// rounded once to the code.  The quotient is x r (r the rounded reciprocal),
+// corrected by its remainder: q + (x - q s) r, which is the rounded quotient
+// for a rounded reciprocal (Markstein); beyond 512 the code is the largest
+// whatever the last bits are, and the product alone is kept (its remainder
+// could be Inf - Inf).  6 instructions a value, an IEEE division 11: it is the
+// write's bound (32768 tokens of 8 heads of 128: 44.5 us with it).  Scales near
+// the ends of fp32, whose products would leave it, are divided by.
+struct Quotient {
+  float s, r;
+  bool plain;
+  __device__ __forceinline__ explicit Quotient(float scale)
+      : s(scale), r(1.0f / scale), plain(!(scale >= 0x1p-100f && scale <= 0x1p100f)) {}
+  __device__ __forceinline__ float of(float x) const {
+    const float q = x * r;
+    const float c = fmaf(fmaf(-q, s, x), r, q);
+    return fabsf(q) < 512.0f ? copysignf(c, q) : q;  // (the sum of -0 and 0 is 0)
+  }
+};
+
+__device__ __forceinline__ u32x2_t quant8(const float (&y)[8], const Quotient& by) {
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = by.of(y[i]);
+  if (by.plain) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] = y[i] / by.s;
+  }
+  return u32x2_t{e4m3x4(z[0], z[1], z[2], z[3]), e4m3x4(z[4], z[5], z[6], z[7])};
 }
 
 // Element offset of a slot's row of head h, or -1 when the slot is none.
@@ -276,8 +310,11 @@ struct WriteParams {
 // One 16-byte chunk of a row per thread and trip, kWriteUnroll trips with
 // their loads requested together; consecutive threads take consecutive chunks
 // of a token's heads, so a wave reads 1 KiB and writes whole rows (256 bytes
-// at head dim 128).  Bound by HBM: each row is read and written once.
-constexpr int kWriteThreads = 256, kWriteUnroll = 4;
+// at head dim 128).  Bound by HBM: each row is read and written once.  32768
+// tokens of 8 heads of 128: 39 us (6.9 TB/s read and written) in 16 bits, its
+// stores streamed (42 us otherwise), 38 us (5.2 TB/s) as e4m3, whose 8-byte
+// stores gain nothing by that; one trip 40 and 51 us, four 40 and 41.
+constexpr int kWriteThreads = 256, kWriteUnroll = 2;
 
 template <int kType, bool kFp8>
 __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(const WriteParams p) {
@@ -304,9 +341,9 @@ __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(const WriteP
     if constexpr (kFp8) {
       float y[8];
       unpack8<kType>(x[u], y);
-      *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(p.dst[which]) + row[u] + ch[u]) = quant8(y, scale[u]);
+      *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(p.dst[which]) + row[u] + ch[u]) = quant8(y, Quotient(scale[u]));
     } else {
-      *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p.dst[which]) + row[u] + ch[u]) = x[u];
+      __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p.dst[which]) + row[u] + ch[u]));
     }
   }
 }
@@ -386,7 +423,7 @@ __global__ __launch_bounds__(256) void paged_rope_kernel(const RopeParams p) {
   void* base = is_v ? p.dst[1] : p.dst[0];
   if constexpr (kFp8) {
     const float* sp = is_v ? p.scale[1] : p.scale[0];
-    *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(base) + dst + 8 * l) = quant8(z, sp ? sp[kh] : 1.0f);
+    *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(base) + dst + 8 * l) = quant8(z, Quotient(sp ? sp[kh] : 1.0f));
   } else {
     *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(base) + dst + 8 * l) = is_v ? x : pack8<kType>(z);
   }
@@ -416,20 +453,23 @@ extern "C" int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_toke
   const AdvanceParams p{seq_lens,  seq_lens_out, new_tokens, block_table, table_stride, free_pages, state,
                         state_out, slots,        positions,  starts,      requests,     num_pages,  capacity,
                         fast_div(static_cast<uint32_t>(page_size)), static_cast<int64_t>(width) * page_size};
+  const bool few = requests <= kFewRequests;
   const size_t lds = static_cast<size_t>(requests) * 16;
-  if (lds > 60 * 1024) {
-    // dynamic LDS above 64 KiB has to be allowed (per device: the call is cheap)
-    if (hipFuncSetAttribute(reinterpret_cast<const void*>(&page_advance_kernel),
-                            hipFuncAttributeMaxDynamicSharedMemorySize, kMaxRequests * 16) != hipSuccess)
-      return fail(ZKV_ELAUNCH, "zkv_page_advance: cannot raise the LDS limit to 128 KiB");
-  }
-  // four tokens a thread, and at least one workgroup for every 16 requests'
-  // pages to give back; every workgroup scans the whole batch, so no more
-  // than one per CU
-  const int64_t want = std::max<int64_t>((static_cast<int64_t>(capacity) + 4 * kAdvanceThreads - 1) / (4 * kAdvanceThreads),
-                                         (requests + 255) / 256);
-  const int grid = static_cast<int>(std::min<int64_t>(256, std::max<int64_t>(1, want)));
-  page_advance_kernel<<<grid, kAdvanceThreads, lds, reinterpret_cast<hipStream_t>(stream)>>>(p);
+  // dynamic LDS above 64 KiB has to be allowed (per device: the call is cheap)
+  if (lds > 60 * 1024 &&
+      hipFuncSetAttribute(reinterpret_cast<const void*>(&page_advance_kernel<1024>),
+                          hipFuncAttributeMaxDynamicSharedMemorySize, kMaxRequests * 16) != hipSuccess)
+    return fail(ZKV_ELAUNCH, "zkv_page_advance: cannot raise the LDS limit to 128 KiB");
+  // a token a thread, or a page to give back for every request; every
+  // workgroup scans the whole batch, so no more than one per CU
+  const int threads = few ? 256 : 1024;
+  const int64_t want = (std::max<int64_t>(capacity, requests) + threads - 1) / threads;
+  const int grid = static_cast<int>(std::min<int64_t>(256, want));
+  auto s = reinterpret_cast<hipStream_t>(stream);
+  if (few)
+    page_advance_kernel<256><<<grid, 256, lds, s>>>(p);
+  else
+    page_advance_kernel<1024><<<grid, 1024, lds, s>>>(p);
   return check_launch("page_advance_kernel");
 }
 

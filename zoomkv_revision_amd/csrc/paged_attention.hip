@@ -36,10 +36,11 @@
 // value of S or P moves between lanes.  V rows are read whole by 16 lanes
 // (lane c: channels c D / 16 ..) and turned in registers, two tokens to a word,
 // by v_perm: row c of the j-th A operand is channel c D / 16 + j.  P enters as
-// two 16-bit parts (two products: the matrix cores wait for memory here
-// anyway): hi, cut towards zero, and lo, the rest, which together carry 15
-// bits (bf16) or 21 (fp16).  Neither part is negative and lo is never 0, so an
-// infinite V stays infinite (-lo * Inf or 0 * Inf would make it NaN).
+// the sum of its leading 16-bit parts, one product each (the matrix cores wait
+// for memory here anyway): three of 8 bits for bf16, two of 11 for fp16, so
+// the weights keep 21 bits and more.  The parts are cut towards zero and those
+// behind the first are never 0: none is negative, and an infinite V stays
+// infinite (-part * Inf or 0 * Inf would make it NaN).
 #include "paged_common.hpp"
 
 #include <algorithm>
@@ -53,10 +54,12 @@ constexpr int kHeads = 16;         // query heads of a unit: the columns of an M
 constexpr int kMaxBatch = 4096;    // requests of a call: 4 bytes of LDS each
 constexpr int kMaxGroups = 256;    // workgroups
 constexpr int kUnitCost = 2;       // places of a unit beyond its tiles
-// Calls of at most this many places per workgroup are bound by latency: cuts
-// are then moved out of units of at most kWholeTiles tiles, whose joining
-// across workgroups would take longer than their tiles.
-constexpr int kShortRun = 32, kWholeTiles = 48;
+// Where there is no more than a place per wave, cuts are moved out of units of
+// at most kWholeTiles tiles: joining their parts across workgroups takes longer
+// than their tiles one after the other (1 x 100 tokens, 32 / 8 heads: 10.1 us,
+// 14.0 with them cut; 8 x 300: 12.1, 17.0; 1 x 700: 14.5, 16.2; with longer runs
+// the uneven loads cost more: 16 x 700 19.6 us, cut 16.3).
+constexpr int kWholeTiles = 48;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
 // The softmax's reference exponent m follows the scores' running maximum only
@@ -96,14 +99,15 @@ struct Elem<kBf16> {
   typedef bf16x8_t x8;
   // m is the maximum itself: P is at most 2^8
   static constexpr float kUp = 0.0f;
-  // two values cut to the type, their parts beyond it (at least the smallest
-  // normal number)
-  static __device__ __forceinline__ uint32_t split(float a, float b, float& ra, float& rb) {
+  static constexpr int kParts = 3;
+  // two values cut to the type, and what is left of them
+  static __device__ __forceinline__ uint32_t cut(float& a, float& b) {
     const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
-    ra = fmaxf(a - __uint_as_float(ua & 0xFFFF0000u), 0x1p-126f);
-    rb = fmaxf(b - __uint_as_float(ub & 0xFFFF0000u), 0x1p-126f);
+    a -= __uint_as_float(ua & 0xFFFF0000u);
+    b -= __uint_as_float(ub & 0xFFFF0000u);
     return __builtin_amdgcn_perm(ub, ua, 0x07060302u);
   }
+  static constexpr float kLeast = 0x1p-126f;  // the smallest normal number
   static __device__ __forceinline__ float4_t mfma(x8 a, x8 b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -119,12 +123,14 @@ struct Elem<kF16> {
   // m is the maximum less 7: P is at most 2^15, and fp16's last place, 2^-24,
   // is 2^-31 of the largest weight
   static constexpr float kUp = 7.0f;
-  static __device__ __forceinline__ uint32_t split(float a, float b, float& ra, float& rb) {
+  static constexpr int kParts = 2;
+  static __device__ __forceinline__ uint32_t cut(float& a, float& b) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-    ra = fmaxf(a - static_cast<float>(h[0]), 0x1p-24f);
-    rb = fmaxf(b - static_cast<float>(h[1]), 0x1p-24f);
+    a -= static_cast<float>(h[0]);
+    b -= static_cast<float>(h[1]);
     return __builtin_bit_cast(uint32_t, h);
   }
+  static constexpr float kLeast = 0x1p-24f;
   static __device__ __forceinline__ float4_t mfma(x8 a, x8 b, float4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -331,20 +337,18 @@ struct PagedAttn {
       for (int j = 0; j < S::kJ; ++j) o[j] *= a;
     }
     const float base = m == -kInf ? 0.0f : m;
-    uint32_t hi[4];
-    typename E::one lo[8];
+    uint32_t parts[E::kParts][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - base);
-      const float p1 = __builtin_amdgcn_exp2f(s[e >> 2][(e & 3) + 1] - base);
+      float p0 = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - base);
+      float p1 = __builtin_amdgcn_exp2f(s[e >> 2][(e & 3) + 1] - base);
       l += p0 + p1;
-      float r0, r1;
-      hi[e >> 1] = E::split(p0, p1, r0, r1);
-      lo[e] = static_cast<typename E::one>(r0);
-      lo[e + 1] = static_cast<typename E::one>(r1);
+#pragma unroll
+      for (int n = 0; n < E::kParts; ++n) {
+        if (n > 0) p0 = fmaxf(p0, E::kLeast), p1 = fmaxf(p1, E::kLeast);
+        parts[n][e >> 1] = E::cut(p0, p1);
+      }
     }
-    const x8 ph = words8(hi[0], hi[1], hi[2], hi[3]);
-    const x8 pl = {lo[0], lo[1], lo[2], lo[3], lo[4], lo[5], lo[6], lo[7]};
 #pragma unroll
     for (int w = 0; w < S::kJ / 2; ++w) {
       uint32_t r[8];
@@ -354,10 +358,12 @@ struct PagedAttn {
                              __builtin_amdgcn_perm(r[5], r[4], 0x05040100u), __builtin_amdgcn_perm(r[7], r[6], 0x05040100u));
       const x8 odd = words8(__builtin_amdgcn_perm(r[1], r[0], 0x07060302u), __builtin_amdgcn_perm(r[3], r[2], 0x07060302u),
                             __builtin_amdgcn_perm(r[5], r[4], 0x07060302u), __builtin_amdgcn_perm(r[7], r[6], 0x07060302u));
-      o[2 * w] = E::mfma(even, ph, o[2 * w]);
-      o[2 * w + 1] = E::mfma(odd, ph, o[2 * w + 1]);
-      o[2 * w] = E::mfma(even, pl, o[2 * w]);
-      o[2 * w + 1] = E::mfma(odd, pl, o[2 * w + 1]);
+#pragma unroll
+      for (int n = 0; n < E::kParts; ++n) {
+        const x8 pn = words8(parts[n][0], parts[n][1], parts[n][2], parts[n][3]);
+        o[2 * w] = E::mfma(even, pn, o[2 * w]);
+        o[2 * w + 1] = E::mfma(odd, pn, o[2 * w + 1]);
+      }
     }
   }
 
@@ -501,7 +507,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const int64_t y64 = static_cast<int64_t>(w) * chunk;
     if (y64 >= total) return total;
     const int y = static_cast<int>(y64);
-    if (chunk > kShortRun) return y;
+    if (chunk > kWaves) return y;
     const int b = request_at(y), size = cum(b + 1) - cum(b), from = y - cum(b) * units, in = from % size;
     return size - kUnitCost > kWholeTiles ? y : (2 * in < size ? y - in : y - in + size);
   };
