@@ -644,15 +644,17 @@ int zkv_sample_window(const float* logits, int64_t ld, int bs, int vocab, float 
  * once the ring cannot serve one, only requests that need no page grow;
  * state[2] collects ZKV_PAGES_* bits for those left as they were.
  * slots int64 [capacity], positions int32 [capacity] (nullable): of the new
- * tokens in request order, -1 for those of a request that was not served and
- * behind the last token.  starts int32 [requests + 1] (nullable): running sum
- * of the new tokens (max(new, 0)), at most capacity + 1.
+ * tokens, packed in request order (row 0), or each request's at the end of a
+ * row of `row` places (capacity = requests * row: the rows of a left-padded
+ * batch); -1 for those of a request that was not served and where there is no
+ * token.  starts int32 [requests + 1] (nullable; packed only): running sum of
+ * the new tokens (max(new, 0)), at most capacity + 1.
  * seq_lens_out / state_out may be seq_lens / state.  state int32 [4]: head,
  * free, status, and an arrival count that is 0 between calls; calls that
  * overlap on one state race. */
 int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_tokens, int requests, int32_t* block_table,
                      int64_t table_stride, int width, int32_t* free_pages, int num_pages, int page_size,
-                     int32_t* state, int64_t* slots, int32_t* positions, int capacity, int32_t* starts,
+                     int32_t* state, int64_t* slots, int32_t* positions, int capacity, int row, int32_t* starts,
                      int32_t* seq_lens_out, int32_t* state_out, zkv_stream_t stream);
 
 /* K / V rows of `tokens` tokens (k, v: (token, head) element strides, 16-bit

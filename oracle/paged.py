@@ -9,10 +9,10 @@ import numpy as np
 POOL_EMPTY, TABLE_FULL, SLOTS_FULL, BAD_LENGTH, RING_FULL = 1, 2, 4, 8, 16
 
 
-def advance(seq_lens, new_tokens, table, free_pages, state, page, cap):
+def advance(seq_lens, new_tokens, table, free_pages, state, page, cap, row=0):
     """One step of the page tables, one request after the other.  Arrays are
     not changed; returns (lens, table, free_pages, state, slots, positions,
-    starts)."""
+    starts).  row > 0: the tokens of request i end at place (i + 1) * row."""
     lens, table, ring = seq_lens.astype(np.int64), table.copy(), free_pages.copy()
     head, count, status = int(state[0]), int(state[1]), int(state[2])
     pages, width = len(ring), table.shape[1]
@@ -34,7 +34,7 @@ def advance(seq_lens, new_tokens, table, free_pages, state, page, cap):
             lens[i] = kept
         elif n > 0 and have + n > width * page:
             status |= TABLE_FULL
-        elif n > 0 and at + n > cap:
+        elif n > 0 and (n > row if row else at + n > cap):
             status |= SLOTS_FULL
         elif n > 0:
             first, last = -(-have // page), -(-(have + n) // page)
@@ -45,6 +45,7 @@ def advance(seq_lens, new_tokens, table, free_pages, state, page, cap):
             for j in range(first, last):
                 table[i, j] = free_pages[(head + taken + j - first) % pages]
             taken += last - first
+            at = (i + 1) * row - n if row else at
             for t in range(n):
                 positions[at + t] = have + t
                 slots[at + t] = int(table[i, (have + t) // page]) * page + (have + t) % page

@@ -38,18 +38,18 @@ def _gpu(table, ring, state, lens, page):
     return paged.PageTables(t(table), t(np.asarray(lens, np.int32)), t(ring), t(state), page)
 
 
-def _same_step(rng, lens, new, width, page, free, cap):
+def _same_step(rng, lens, new, width, page, free, cap, row=0):
     requests = len(lens)
     table, ring, state = _new_tables(rng, requests, width, page, free, lens)
-    want = op.advance(np.asarray(lens, np.int32), np.asarray(new, np.int32), table, ring, state, page, cap)
+    want = op.advance(np.asarray(lens, np.int32), np.asarray(new, np.int32), table, ring, state, page, cap, row)
     tables = _gpu(table, ring, state, lens, page)
     slots = torch.full((cap,), -5, dtype=torch.int64, device=DEV)
     positions = torch.full((cap,), -5, dtype=torch.int32, device=DEV)
-    starts = torch.full((requests + 1,), -5, dtype=torch.int32, device=DEV)
-    paged.page_advance(tables, torch.tensor(new, dtype=torch.int32, device=DEV), slots, positions, starts)
+    starts = None if row else torch.full((requests + 1,), -5, dtype=torch.int32, device=DEV)
+    paged.page_advance(tables, torch.tensor(new, dtype=torch.int32, device=DEV), slots, positions, starts, row=row)
     got = (tables.seq_lens, tables.block_table, tables.free_pages, tables.state, slots, positions, starts)
     for name, a, b in zip(("lens", "table", "ring", "state", "slots", "positions", "starts"), got, want):
-        assert np.array_equal(a.cpu().numpy(), b), name
+        assert a is None or np.array_equal(a.cpu().numpy(), b), name
     return want
 
 
@@ -63,6 +63,15 @@ def test_advance_equals_the_plain_form(requests, page, width, cap, free):
     new = rng.choice([0, 1, 1, 1, 2, page, 5 * page, -1, -page, -10 ** 6, 10 ** 6], requests)
     n_free = {"enough": requests * width + 5, "some": requests // 3 + 1, "none": 0}[free]
     _same_step(rng, lens, new, width, page, n_free, cap)
+
+
+@pytest.mark.parametrize("requests,row", [(1, 1), (5, 1), (64, 1), (9, 33), (700, 5), (8192, 1)])
+@pytest.mark.parametrize("free", [10 ** 4, 7])
+def test_advance_in_rows(requests, row, free):
+    rng = np.random.default_rng(requests + row)
+    lens = rng.integers(0, 60, requests)
+    new = rng.choice([0, 1, row, row, row + 1, -2, 2 ** 31 - 1], requests)
+    _same_step(rng, lens, new, 12, 8, free, requests * row, row)
 
 
 def test_advance_extremes():

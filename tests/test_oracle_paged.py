@@ -37,6 +37,13 @@ def test_pages_given_back_are_handed_out_later():
     assert out[0].tolist() == [0, 3] and out[1][1, :2].tolist() == [6, 7] and out[3].tolist() == [1, 2, op.POOL_EMPTY, 0]
 
 
+def test_rows_end_with_their_tokens():
+    out = op.advance(_i32(0, 3, 0), _i32(2, 0, 4), np.full((3, 2), -1, np.int32), np.arange(4, dtype=np.int32),
+                     _i32(0, 4, 0, 0), 2, 9, row=3)
+    assert out[4].tolist() == [-1, 0, 1, -1, -1, -1, -1, -1, -1] and out[5].tolist() == [-1, 0, 1] + [-1] * 6
+    assert out[0].tolist() == [2, 3, 0] and out[3][2] == op.SLOTS_FULL
+
+
 def test_every_status_bit():
     t = np.zeros((1, 2), np.int32)
     one = lambda have, n, count=4, cap=8: op.advance(_i32(have), _i32(n), t, np.arange(4, dtype=np.int32),

@@ -178,7 +178,8 @@ def test_tables_refusals():
     for changed in (dict(new_tokens=new.long()), dict(new_tokens=new[:2]), dict(slots=slots.int()),
                     dict(slots=torch.zeros(8, dtype=torch.int64)[::2]), dict(positions=torch.zeros(3, **i32)),
                     dict(starts=torch.zeros(BS, **i32)), dict(lens_out=torch.zeros(BS + 1, **i32)),
-                    dict(state_out=torch.zeros(5, **i32))):
+                    dict(state_out=torch.zeros(5, **i32)), dict(row=-1), dict(row=1),
+                    dict(slots=torch.zeros(BS, dtype=torch.int64), row=1, starts=torch.zeros(BS + 1, **i32))):
         with pytest.raises(ValueError):
             paged.page_advance(**{**dict(tables=_tables(), new_tokens=new, slots=slots), **changed})
     big = paged.MAX_TABLE_REQUESTS + 1
@@ -227,9 +228,10 @@ def _c_refusals():
     assert write(n=0) == 0
     advance = lambda **c: L.zkv_page_advance(*{**dict(
         lens=x, new=x, n=4, table=x, tstride=8, width=8, ring=x, pages=4, page=16, state=x, slots=x, pos=None, cap=4,
-        starts=None, lo=x, so=x, stream=None), **c}.values())
+        row=0, starts=None, lo=x, so=x, stream=None), **c}.values())
     for c in (dict(n=0), dict(n=8193), dict(width=0), dict(tstride=7), dict(page=0), dict(pages=0), dict(cap=-1),
-              dict(slots=None), dict(state=None), dict(page=1 << 30)):
+              dict(slots=None), dict(state=None), dict(page=1 << 30), dict(row=-1), dict(row=2),
+              dict(row=1, starts=x)):
         assert advance(**c) == 1, c
     rope = lambda **c: L.zkv_paged_qk_norm_rope(*{**dict(
         qkv=x, stride=1536, n=4, hq=8, kv=2, d=128, f16=0, qn=x, kn=x, eps=1e-6, cos=x, sin=x, maxp=4, pos=x, slots=x,

@@ -92,7 +92,7 @@ SIGNATURES = {
     "zkv_qk_norm_rope": (I32, [P, I64, I32, I32, I32, P, P, F32, P, P, P, P, I64, I64, P, I64, I64, P]),
     "zkv_sample_window_workspace_size": (SZ, [I32, I32, I32]),
     "zkv_sample_window": (I32, [P, I64, I32, I32, F32, I32, I32, F32, P, I64, P, P, P, SZ, P]),
-    "zkv_page_advance": (I32, [P, P, I32, P, I64, I32, P, I32, I32, P, P, P, I32, P, P, P, P]),
+    "zkv_page_advance": (I32, [P, P, I32, P, I64, I32, P, I32, I32, P, P, P, I32, I32, P, P, P, P]),
     "zkv_paged_write": (I32, [P, I64, I64, P, I64, I64, P, I32, I32, I32, I32, P, P, I32, P, P, I32, I32, I64, I64,
                               I64, P]),
     "zkv_paged_qk_norm_rope": (I32, [P, I64, I32, I32, I32, I32, I32, P, P, F32, P, P, I32, P, P, P, P, P, I32, P, P,

@@ -5,8 +5,10 @@
   v_cache [bs, n, kv, 128] bf16 (any strides with a contiguous last dim, e.g.
   the ``concat.transpose(1, 2)`` views of S:1740-1747), GQA, non-causal (for one
   query token, causal and non-causal agree).  ``softmax_scale`` and
-  ``return_softmax_lse`` follow flash_attn_with_kvcache; other keyword
-  arguments of that function are not supported and raise.
+  ``return_softmax_lse`` follow flash_attn_with_kvcache, and so do
+  ``block_table`` with ``cache_seqlens`` (a paged cache [pages, page_size, kv,
+  d]: ``paged.paged_attention``); its other keyword arguments are not supported
+  and raise.
 * ``lse_merge`` / ``lse_merge_torch`` / ``lse_merge_cuda`` mirror
   ``Z/cache_hub/lse_merge/lse_merge.py:79-149``: two outputs [bs, 1, heads, dim]
   with LSEs in [bs, heads, 1], [bs, 1, heads] or [bs, heads].
@@ -49,16 +51,30 @@ def _check_out(out: torch.Tensor | None, q: torch.Tensor, bs: int, hq: int) -> t
 def flash_attn_with_kvcache_compat(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                                    causal: bool = False, softmax_scale: float | None = None,
                                    return_softmax_lse: bool = False, out: torch.Tensor | None = None,
-                                   n_splits: int = 0, **kwargs):
+                                   n_splits: int = 0, cache_seqlens: torch.Tensor | None = None,
+                                   block_table: torch.Tensor | None = None, **kwargs):
     """softmax(q K^T * scale) V for one query token per sequence.
+
+    With ``block_table`` (int32 [bs, width]) and ``cache_seqlens`` (int32 [bs])
+    k_cache / v_cache are the pages [pages, page_size, kv, d] of a paged cache,
+    d 64, 128 or 256, bf16 or fp16 (``paged.paged_attention``).
 
     Returns out [bs, 1, hq, 128] in q's dtype (bf16; a float32 ``out`` buffer
     receives the unrounded result), and with ``return_softmax_lse`` also the
     fp32 LSE [bs, hq, 1].  K and V enter the matrix cores as stored (bf16),
     so every finite bf16 value is supported.
     """
+    if block_table is None and cache_seqlens is not None:
+        kwargs["cache_seqlens"] = cache_seqlens
     if kwargs:
         raise NotImplementedError(f"flash_attn_with_kvcache_compat: unsupported arguments {sorted(kwargs)}")
+    if block_table is not None:
+        if not isinstance(cache_seqlens, torch.Tensor) or k_cache.dim() != 4 or v_cache.dim() != 4 or n_splits:
+            raise ValueError("block_table goes with cache_seqlens (a tensor), pages [pages, page_size, kv, d] and "
+                             "n_splits 0")
+        from .paged import paged_attention
+        return paged_attention(q, k_cache.transpose(1, 2), v_cache.transpose(1, 2), block_table, cache_seqlens,
+                               softmax_scale, return_softmax_lse=return_softmax_lse, out=out)
     require_gpu(q, k_cache, v_cache)
     if q.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
         raise TypeError("q, k_cache and v_cache must be bfloat16")

@@ -38,6 +38,7 @@ struct AdvanceParams {
   int32_t* starts;     // or null
   int requests, num_pages, cap;
   FastDiv page;
+  FastDiv row;         // d > 0: request i's tokens end row i of d places; else packed in request order
   int64_t max_len;     // width * page size
 };
 
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
   extern __shared__ int smem[];
   const int R = p.requests, tid = threadIdx.x;
   uint32_t* s_len = reinterpret_cast<uint32_t*>(smem);  // length; kGranted: grows in this step
-  int* s_tok = smem + R;                                // ends of the requests' tokens
+  int* s_tok = smem + R;                                // ends of the requests' tokens (rows: how many)
   int* s_need = s_tok + R;                              // ends of the pages they take
   int* s_give = s_need + R;                             // ends of the pages they give back
   __shared__ int part[kThreads / 64];
@@ -123,6 +124,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
   const int tok_top = p.cap + 1, page_top = p.num_pages + 1;
   // tokens: every request's new ones count, whether or not it is served, so
   // that the rows of a packed batch keep their places
+  const int row = static_cast<int>(p.row.d);
   int sum = 0;
   for (int i = i0; i < i1; ++i) sum = limited(sum, min(max(s_tok[i], 0), tok_top), tok_top);
   sum = scan_before(sum, tok_top, part);
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
     } else if (n > 0) {
       if (after > p.max_len)
         status |= ZKV_PAGES_TABLE_FULL;
-      else if (sum > p.cap)
+      else if (row ? n > row : sum > p.cap)
         status |= ZKV_PAGES_SLOTS_FULL;
       else
         need = pages_of(static_cast<uint32_t>(after), p.page) - pages_of(len, p.page);
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
       give = pages_of(len, p.page) - pages_of(static_cast<uint32_t>(max(after, int64_t{0})), p.page);
     }
     s_len[i] = static_cast<uint32_t>(max(len, 0));
-    s_tok[i] = sum;
+    s_tok[i] = row ? n : sum;
     s_need[i] = need;
     s_give[i] = give;
     need_sum = limited(need_sum, max(need, 0), page_top);
@@ -185,12 +187,14 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
   for (int t = blockIdx.x * kThreads + tid; t < p.cap; t += stride) {
     int64_t slot = -1;
     int pos = -1;
-    if (t < total) {
-      const int r = owner_of(s_tok, R, t);
+    const int r = row ? static_cast<int>(div_by(t, p.row)) : owner_of(s_tok, R, t);
+    // the token's number among its request's
+    const int j = row ? t - (r + 1) * row + s_tok[r] : t - (r ? s_tok[r - 1] : 0);
+    if (row ? j >= 0 : t < total) {
       const uint32_t lg = s_len[r];
       if (lg & kGranted) {
         const int len = static_cast<int>(lg & ~kGranted);
-        pos = len + t - (r ? s_tok[r - 1] : 0);
+        pos = len + j;
         const int at = static_cast<int>(div_by(pos, p.page)), off = pos - at * page_size;
         const int held = pages_of(len, p.page);
         int32_t* entry = p.table + r * p.table_stride + at;
@@ -436,8 +440,8 @@ using namespace zkv;
 
 extern "C" int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_tokens, int requests, int32_t* block_table,
                                 int64_t table_stride, int width, int32_t* free_pages, int num_pages, int page_size,
-                                int32_t* state, int64_t* slots, int32_t* positions, int capacity, int32_t* starts,
-                                int32_t* seq_lens_out, int32_t* state_out, zkv_stream_t stream) {
+                                int32_t* state, int64_t* slots, int32_t* positions, int capacity, int row,
+                                int32_t* starts, int32_t* seq_lens_out, int32_t* state_out, zkv_stream_t stream) {
   ZKV_REQUIRE(seq_lens && new_tokens && block_table && free_pages && state && seq_lens_out && state_out,
               "zkv_page_advance: null pointer");
   ZKV_REQUIRE(requests >= 1 && requests <= kMaxRequests, "zkv_page_advance: %d requests outside [1, %d]", requests,
@@ -450,9 +454,14 @@ extern "C" int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_toke
               "zkv_page_advance: a request and the pool hold fewer than 2^31 tokens");
   ZKV_REQUIRE(capacity >= 0 && capacity <= (1 << 30) && (capacity == 0 || slots),
               "zkv_page_advance: a slot map of %d", capacity);
+  ZKV_REQUIRE(row >= 0 && (row == 0 || (static_cast<int64_t>(row) * requests == capacity && starts == nullptr)),
+              "zkv_page_advance: %d requests in rows of %d make a slot map of that many, without starts (%d)", requests,
+              row, capacity);
   const AdvanceParams p{seq_lens,  seq_lens_out, new_tokens, block_table, table_stride, free_pages, state,
                         state_out, slots,        positions,  starts,      requests,     num_pages,  capacity,
-                        fast_div(static_cast<uint32_t>(page_size)), static_cast<int64_t>(width) * page_size};
+                        fast_div(static_cast<uint32_t>(page_size)),
+                        row ? fast_div(static_cast<uint32_t>(row)) : FastDiv{0, 0, 0},
+                        static_cast<int64_t>(width) * page_size};
   const bool few = requests <= kFewRequests;
   const size_t lds = static_cast<size_t>(requests) * 16;
   // dynamic LDS above 64 KiB has to be allowed (per device: the call is cheap)

@@ -23,6 +23,11 @@ projection with the residual add.  The torch ops of ``layer_decode_torch``
 (the reference's flashinfer rmsnorm / rope / silu have no ROCm build) are
 the same layer written out op by op: the CPU path, and the check the fused
 kernels are tested against.
+
+Over a ``paged_cache.paged_cache`` (requests of lengths of their own, full
+attention) the same step runs with each row's own position: the norm + RoPE
+launch writes the K / V rows into their page slots
+(``paged.paged_qk_norm_rope``), and ``cache.compute`` attends the pages.
 """
 from __future__ import annotations
 
@@ -117,6 +122,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     return (xf * weight.float()).to(x.dtype)
 
 
+def _is_paged(cache) -> bool:
+    """Whether the rows of the batch have positions of their own (paged_cache)."""
+    return hasattr(cache, "decode_norm_rope")
+
+
 class RandomQwen3:
     """Random-init bf16 weights of a Qwen3 decoder (std 0.02, norms at 1), on one GPU."""
 
@@ -160,11 +170,14 @@ class RandomQwen3:
             n += sum(t.numel() for t in L.values())
         return 2 * n
 
-    def _rope(self, x: torch.Tensor, pos: int) -> torch.Tensor:
-        """x [bs, 1, heads, 128] rotated at position pos (rotate-half, as the
-        reference's fp32 path and flashinfer's is_neox=True)."""
+    def _rope(self, x: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+        """x [bs, 1, heads, 128] rotated at position pos, or row b at pos[b]
+        (rotate-half, as the reference's fp32 path and flashinfer's
+        is_neox=True)."""
         h = self.geo.head_dim // 2
         cos, sin = self.cos[pos], self.sin[pos]
+        if cos.dim() == 2:
+            cos, sin = cos[:, None, None], sin[:, None, None]
         xf = x.float()
         x1, x2 = xf[..., :h], xf[..., h:]
         return torch.cat((x1 * cos - x2 * sin, x2 * cos + x1 * sin), dim=-1).to(x.dtype)
@@ -183,11 +196,15 @@ class RandomQwen3:
         x = hidden.reshape(bs, geo.hidden)
         qkv = torch.empty(bs, qd + 2 * kd, dtype=torch.bfloat16, device=hidden.device)
         decode_linear(x, L["wqkv"], qkv, norm_w=L["input_ln"], eps=geo.eps)
-        pos = cache.context
-        row = cache.decode_reserve_row(ldx)
-        q = torch.empty(bs, 1, geo.heads, geo.head_dim, dtype=torch.bfloat16, device=hidden.device)
-        qk_norm_rope(qkv, geo.heads, geo.kv_heads, L["q_norm"], L["k_norm"], geo.eps, self.cos[pos],
-                     self.sin[pos], q, cache.unified_keys[ldx][:, :, row], cache.unified_values[ldx][:, :, row])
+        if _is_paged(cache):
+            cache.decode_begin(ldx)
+            q = cache.decode_norm_rope(qkv, L["q_norm"], L["k_norm"], geo.eps, self.cos, self.sin, ldx)
+        else:
+            pos = cache.context
+            row = cache.decode_reserve_row(ldx)
+            q = torch.empty(bs, 1, geo.heads, geo.head_dim, dtype=torch.bfloat16, device=hidden.device)
+            qk_norm_rope(qkv, geo.heads, geo.kv_heads, L["q_norm"], L["k_norm"], geo.eps, self.cos[pos],
+                         self.sin[pos], q, cache.unified_keys[ldx][:, :, row], cache.unified_values[ldx][:, :, row])
         attn = cache.compute(q, ldx)                                   # [bs, 1, heads, 128]
         h1 = torch.empty(bs, geo.hidden, dtype=torch.bfloat16, device=hidden.device)
         decode_linear(attn.reshape(bs, qd), L["wo"], h1, residual=x)
@@ -209,9 +226,15 @@ class RandomQwen3:
         q = rms_norm(q.reshape(bs, 1, geo.heads, geo.head_dim), L["q_norm"], geo.eps)
         k = rms_norm(k.reshape(bs, 1, geo.kv_heads, geo.head_dim), L["k_norm"], geo.eps)
         pos = cache.context
+        if _is_paged(cache):
+            cache.decode_begin(ldx)
+            pos = cache.positions.clamp(min=0).long()      # (idle rows: any)
         q, k = self._rope(q, pos), self._rope(k, pos)
         v = v.reshape(bs, 1, geo.kv_heads, geo.head_dim)
-        cache.decode_update_kv_cache(k, v, ldx)
+        if _is_paged(cache):
+            cache.decode_write(k, v, ldx)
+        else:
+            cache.decode_update_kv_cache(k, v, ldx)
         attn = cache.compute(q, ldx)                                   # [bs, 1, heads, 128]
         hidden = residual + F.linear(attn.reshape(bs, 1, qd), L["wo"])
         residual = hidden
@@ -401,6 +424,18 @@ def build_cache(geo: Qwen3Geometry, batch: int, context: int, max_new: int, inte
         max_new_length=max_new, core=22, nprobe=150, cache_unit_size=8, cache_cluster_num=450,
         num_gpus=1, model_size=4, dynamic_update_interval=interval, full_attention_threshold=full_threshold,
         **knobs)
+
+
+def build_paged_cache(geo: Qwen3Geometry, batch: int, max_tokens: int, device, page_size: int = 16,
+                      num_pages: int | None = None, kv_dtype: torch.dtype | None = None):
+    """paged_cache for `batch` requests of up to max_tokens tokens each, over a
+    pool of num_pages pages (default: enough for all of them at once); kv_dtype
+    torch.float8_e4m3fn keeps K and V in 8 bits."""
+    from .paged_cache import paged_cache
+    return paged_cache(valid_start=[0] * batch, layer_num=geo.layers, batch_size=batch, max_length=max_tokens,
+                       num_key_value_heads=geo.kv_heads, num_heads=geo.heads, head_dim=geo.head_dim,
+                       dtype=torch.bfloat16, layer_mapping={str(i): str(device) for i in range(geo.layers)},
+                       max_new_length=0, page_size=page_size, num_pages=num_pages, kv_dtype=kv_dtype)
 
 
 def fill_cache(cache, geo: Qwen3Geometry, batch: int, context: int, seed: int, device) -> None:

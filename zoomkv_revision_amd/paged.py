@@ -54,16 +54,17 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     are then cleared in the graph, a launch more: a plan, or a workspace that
     is passed in, saves it)."""
     if torch.cuda.is_current_stream_capturing():
-        return _new_workspace(device, nbytes)
+        return new_workspace(device, nbytes)
     key = (device, device_stream(device))
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _WS[key] = _new_workspace(device, nbytes)
+        ws = _WS[key] = new_workspace(device, nbytes)
     return ws
 
 
-def _new_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
-    """The arrival counts, at the front, are 0 between calls; the partials
+def new_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """A workspace for paged_attention (zkv_paged_attention_workspace_size(d)
+    bytes).  The arrival counts, at the front, are 0 between calls; the partials
     behind them need no clearing."""
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     ws[:_ARRIVAL_BYTES].zero_()
@@ -178,7 +179,7 @@ class PageTables:
             raise RuntimeError("page tables: " + "; ".join(t for b, t in _STATUS_TEXT.items() if bits & b))
 
 
-def _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_out):
+def _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_out, row):
     t = tables
     requests = t.seq_lens.numel()
     if t.block_table.dtype != torch.int32 or t.block_table.dim() != 2 or t.block_table.shape[0] != requests or \
@@ -195,8 +196,9 @@ def _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_
     if t.page_size < 1 or pages < 1 or pages > 1 << 30 or pages * t.page_size >= 1 << 31 or \
             width * t.page_size >= 1 << 31:
         raise ValueError(f"{pages} pages of {t.page_size} tokens, {width} a request")
-    if cap > 1 << 30:
-        raise ValueError(f"a slot map of {cap}")
+    row = int(row)
+    if cap > 1 << 30 or row < 0 or (row and (row * requests != cap or starts is not None)):
+        raise ValueError(f"a slot map of {cap} for {requests} requests" + (f" in rows of {row}" if row else ""))
     if slots is not None:
         _check_ints("slots", slots, torch.int64, (cap,))
     if positions is not None:
@@ -213,7 +215,7 @@ def _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_
     require_gpu(t.seq_lens)
     args = (ptr(t.seq_lens), ptr(new_tokens), requests, ptr(t.block_table),
             t.block_table.stride(0) if requests > 1 else width, width, ptr(t.free_pages), pages, t.page_size,
-            ptr(t.state), ptr(slots) if cap else None, ptr(positions) if cap else None, cap, ptr(starts),
+            ptr(t.state), ptr(slots) if cap else None, ptr(positions) if cap else None, cap, row, ptr(starts),
             ptr(lens_out), ptr(state_out))
     return args, (slots, positions), (t, new_tokens, slots, positions, starts, lens_out, state_out)
 
@@ -222,14 +224,14 @@ class PageAdvancePlan(_Plan):
     """``page_advance`` with its checks done once for fixed buffers."""
 
     def __init__(self, tables: PageTables, new_tokens, slots=None, positions=None, starts=None, lens_out=None,
-                 state_out=None):
-        args, out, keep = _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_out)
+                 state_out=None, row=0):
+        args, out, keep = _advance_args(tables, new_tokens, slots, positions, starts, lens_out, state_out, row)
         super().__init__(lib().zkv_page_advance, new_tokens.device, args, out, keep)
 
 
 def page_advance(tables: PageTables, new_tokens: torch.Tensor, slots: torch.Tensor | None = None,
                  positions: torch.Tensor | None = None, starts: torch.Tensor | None = None,
-                 lens_out: torch.Tensor | None = None, state_out: torch.Tensor | None = None):
+                 lens_out: torch.Tensor | None = None, state_out: torch.Tensor | None = None, row: int = 0):
     """One step of the page tables, one launch: request i goes from
     seq_lens[i] to seq_lens[i] + new_tokens[i] tokens (int32; 0: stays; negative:
     drops that many, at most all, which ends the request).
@@ -241,12 +243,14 @@ def page_advance(tables: PageTables, new_tokens: torch.Tensor, slots: torch.Tens
     the slot map, keeps its length and sets a status bit (``tables.check()``),
     and from the first that the ring cannot serve on, only requests that need
     no page grow.  slots int64 [capacity] and positions int32 [capacity] get the
-    slot and position of each new token, packed in request order, -1 for those
-    of a request that was not served and behind the last; starts int32
-    [requests + 1] the running sum of the new tokens.  seq_lens and state are
-    updated in place unless lens_out / state_out are given.  Returns (slots,
-    positions)."""
-    return PageAdvancePlan(tables, new_tokens, slots, positions, starts, lens_out, state_out).run()
+    slot and position of each new token, packed in request order, or with
+    row > 0 each request's at the end of its row of that many (capacity =
+    requests * row: a left-padded batch; 1: a decode batch with idle rows), -1
+    for those of a request that was not served and where there is no token;
+    starts int32 [requests + 1] (packed only) the running sum of the new tokens.
+    seq_lens and state are updated in place unless lens_out / state_out are
+    given.  Returns (slots, positions)."""
+    return PageAdvancePlan(tables, new_tokens, slots, positions, starts, lens_out, state_out, row).run()
 
 
 # ---------------------------------------------------------------------------
@@ -430,7 +434,7 @@ class PagedAttentionPlan(_Plan):
     def __init__(self, q, k_pages, v_pages, block_table, seq_lens, softmax_scale=None, window=0, k_scale=None,
                  v_scale=None, return_softmax_lse=False, out=None, workspace=None):
         if workspace is None and q.is_cuda and q.shape[-1] in HEAD_DIMS:
-            workspace = _new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
+            workspace = new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
         args, result, keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                              v_scale, return_softmax_lse, out, workspace, copies=False)
         super().__init__(lib().zkv_paged_attention, q.device, args, result, keep)
