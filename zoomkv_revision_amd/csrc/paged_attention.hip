@@ -743,89 +743,100 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   // joining loads read there: no cache is written back or invalidated.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  const auto first_group = [&](const Unit& u) { return (u.base + kUnitCost) / chunk; };
-  const auto groups_of = [&](const Unit& u) { return (u.base + kUnitCost + u.tiles - 1) / chunk - first_group(u) + 1; };
+  int w0[2], n[2] = {0, 0};  // first of the workgroups that share the cut unit, how many
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
-    int last = 0;
-    if (cut[side] >= 0) {
-      const Unit u = unit_at(cut[side]);
-      if (tid == side) last = arrive_last_count(p.arrivals + first_group(u), groups_of(u));
-    }
-    if (tid == side) s_part[side] = last;
+    w0[side] = 0;
+    if (cut[side] < 0) continue;
+    const Unit u = unit_at(cut[side]);
+    w0[side] = (u.base + kUnitCost) / chunk;
+    n[side] = (u.base + kUnitCost + u.tiles - 1) / chunk - w0[side] + 1;
+  }
+  if (tid < 2) {  // (both arrivals in one round trip)
+    const int of = tid ? n[1] : n[0];
+    s_part[tid] = of && arrive_last_count(p.arrivals + (tid ? w0[1] : w0[0]), of);
   }
   __syncthreads();
+  const bool last0 = __builtin_amdgcn_readfirstlane(s_part[0]), last1 = __builtin_amdgcn_readfirstlane(s_part[1]);
+  if (!last0 && !last1) return;
+  // Four channels of a head per thread, and for each such item as many threads
+  // as there are partials, or threads, each with its part of the partials,
+  // eight requested at once; the parts meet in LDS.  With two units to join,
+  // each takes half of the workgroup.
+  const bool both = last0 && last1;
+  const int width = both ? kThreads / 2 : kThreads;
+  const int side = both ? (wave >= kWaves / 2 ? 1 : 0) : (last1 ? 1 : 0);
+  const int me = both ? tid % (kThreads / 2) : tid;
+  const Unit u = unit_at(side ? cut[1] : cut[0]);
+  const int from = side ? w0[1] : w0[0], count = side ? n[1] : n[0];
+  // partial i: the unit's first workgroup kept it as its later cut, the others
+  // as their earlier one
+  const auto row_of = [&](int i, int c) {
+    return ((static_cast<int64_t>(from) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
+  };
+  const int items = u.heads * (kD / 4);
+  float* s_mine = s_o + (tid - me) * 8;  // 8 floats a thread
+  constexpr int kBatch = 8;
+  // (as many passes for both units: the barriers are the workgroup's)
+  const int passes = (p.heads_lds * (kD / 4) + width - 1) / width;
 #pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    const int id = side ? cut[1] : cut[0];
-    if (id < 0 || !__builtin_amdgcn_readfirstlane(s_part[side])) continue;
-    const Unit u = unit_at(id);
-    const int w0 = first_group(u), n = groups_of(u);
-    // partial i: the unit's first workgroup kept it as its later cut, the
-    // others as their earlier one
-    const auto row_of = [&](int i, int c) {
-      return ((static_cast<int64_t>(w0) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
-    };
-    // four channels of a head per thread, and as many threads per such item
-    // as there are, each with its part of the partials, eight requested at
-    // once; the parts meet in LDS
-    const int items = u.heads * (kD / 4);
-    constexpr int kBatch = 8;
-#pragma unroll 1
-    for (int e0 = 0; e0 < items; e0 += kThreads) {
-      const int here = min(kThreads, items - e0), parts = kThreads / here;
-      __syncthreads();  // (s_o of the join before is read)
-      const int part = tid / here, e = e0 + tid - part * here, c = e / (kD / 4), d = 4 * (e % (kD / 4));
-      if (part < parts) {
-        float top = -kInf, den = 0.0f;
-        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i0 = part; i0 < n; i0 += kBatch * parts) {
-          float2_t ml[kBatch], lo[kBatch], hi[kBatch];
+  for (int pass = 0; pass < passes; ++pass) {
+    const int e0 = pass * width, here = max(1, min(width, items - e0));
+    const int parts = min(width / here, count);
+    const int part = me / here, e = e0 + me - part * here, c = e / (kD / 4), d = 4 * (e % (kD / 4));
+    const bool mine = e0 < items && part < parts;
+    __syncthreads();  // (s_o of the join before is read)
+    if (mine) {
+      float top = -kInf, den = 0.0f;
+      float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i0 = part; i0 < count; i0 += kBatch * parts) {
+        float2_t ml[kBatch], lo[kBatch], hi[kBatch];
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int64_t row = row_of(min(i0 + i * parts, n - 1), c);
-            ml[i] = load_dev(p.part_ml + row * 2);
-            lo[i] = load_dev(p.part_o + row * kD + d);
-            hi[i] = load_dev(p.part_o + row * kD + d + 2);
-          }
-          float now = top;
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < n ? fmaxf(now, ml[i][0]) : now;
-          const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
-          top = now;
-          den *= a;
-          num *= a;
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            if (i0 + i * parts >= n) continue;
-            const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
-            den += w * ml[i][1];
-            num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
-          }
+        for (int i = 0; i < kBatch; ++i) {
+          const int64_t row = row_of(min(i0 + i * parts, count - 1), c);
+          ml[i] = load_dev(p.part_ml + row * 2);
+          lo[i] = load_dev(p.part_o + row * kD + d);
+          hi[i] = load_dev(p.part_o + row * kD + d + 2);
         }
-        float* dst = s_o + tid * 8;
-        *reinterpret_cast<float4_t*>(dst) = num;
-        dst[4] = top;
-        dst[5] = den;
-      }
-      __syncthreads();
-      if (tid < here) {
-        float top = -kInf;
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, s_o[(i * here + tid) * 8 + 4]);
-        const float base = top == -kInf ? 0.0f : top;
-        float den = 0.0f;
-        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i = 0; i < parts; ++i) {
-          const float* src = s_o + (i * here + tid) * 8;
-          const float w = __builtin_amdgcn_exp2f(src[4] - base);
-          den += w * src[5];
-          num += w * *reinterpret_cast<const float4_t*>(src);
+        float now = top;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < count ? fmaxf(now, ml[i][0]) : now;
+        const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
+        top = now;
+        den *= a;
+        num *= a;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          if (i0 + i * parts >= count) continue;
+          const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
+          den += w * ml[i][1];
+          num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
         }
-        const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
-        const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
-        store_result<kType>(p, row * kD + d, num * inv);
-        if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
       }
+      float* dst = s_mine + me * 8;
+      *reinterpret_cast<float4_t*>(dst) = num;
+      dst[4] = top;
+      dst[5] = den;
+    }
+    __syncthreads();
+    if (mine && part == 0) {
+      float top = -kInf;
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) top = fmaxf(top, s_mine[(i * here + me) * 8 + 4]);
+      const float base = top == -kInf ? 0.0f : top;
+      float den = 0.0f;
+      float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) {
+        const float* src = s_mine + (i * here + me) * 8;
+        const float w = __builtin_amdgcn_exp2f(src[4] - base);
+        den += w * src[5];
+        num += w * *reinterpret_cast<const float4_t*>(src);
+      }
+      const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
+      const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
+      store_result<kType>(p, row * kD + d, num * inv);
+      if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
     }
   }
 }
