@@ -368,6 +368,44 @@ def test_two_captured_graphs_at_once():
             assert torch.equal(wo, o) and torch.equal(wl, l), step
 
 
+@pytest.mark.parametrize("hq,kv,d", [(16, 1, 128), (64, 4, 256), (40, 1, 64)])
+def test_captured_with_the_largest_partials(hq, kv, d):
+    """16 query heads a unit: the launch asks for the most LDS, also inside a
+    capture."""
+    c = Case([9000, 40, 3000], hq, kv, d, 16, seed=40)
+    plan = paged.PagedAttentionPlan(c.q, c.k, c.v, c.table, c.lens, return_softmax_lse=True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plan.run()
+    for n in (9000, 100, 7777):
+        c.lens[0] = n
+        g.replay()
+        out, lse = (x.clone() for x in plan.out)
+        c.check(out, lse, requests=[0, 2])
+        again, _ = c.attend(return_softmax_lse=True)
+        assert torch.equal(again, out)
+
+
+def test_a_plan_on_another_stream():
+    c = Case([2000, 7], 8, 2, 128, 16, seed=41)
+    want = c.attend()
+    plan = paged.PagedAttentionPlan(c.q, c.k, c.v, c.table, c.lens)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(4):
+            got = plan.run().clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_out_in_place_of_q():
+    c = Case([2000, 7, 0, 300], 8, 2, 128, 16, seed=42)
+    want = c.attend()
+    q = c.q.clone()
+    assert paged.paged_attention(q, c.k, c.v, c.table, c.lens, out=q) is q and torch.equal(q, want)
+
+
 def test_a_workspace_too_small_is_refused():
     c = Case([10], 2, 1, 64, 16, seed=30)
     with pytest.raises(ValueError, match="workspace"):

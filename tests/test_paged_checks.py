@@ -114,6 +114,8 @@ def test_pools_the_kernels_cannot_read_are_refused(call, args, i):
     dict(seq_lens=torch.ones(BS + 1, dtype=torch.int32)),
     dict(seq_lens=torch.ones(2 * BS, dtype=torch.int32)[::2]),
     dict(window=-1),
+    dict(k_pages=_pool(shape=(1, KV, PAGE, D)).expand(1 << 20, KV, PAGE, D).as_strided(
+        (1 << 20, KV, PAGE, D), (0, PAGE * D, D, 1)), v_pages=_pool(), q=torch.zeros(BS, 1, HQ, D, dtype=BF)),
     dict(out=torch.zeros(BS, 1, HQ, D, dtype=torch.float16)),
     dict(out=torch.zeros(BS, 1, HQ, 2 * D, dtype=BF)[..., :D]),
     dict(out=torch.zeros(BS, 1, HQ - 1, D, dtype=BF)),
@@ -216,7 +218,7 @@ def _c_refusals():
         ws=x, wsb=1 << 30, stream=None), **c}.values())
     for c in (dict(q=None), dict(d=96), dict(bs=0), dict(bs=4097), dict(hq=7), dict(kv=0), dict(width=0),
               dict(pages=0), dict(page=0), dict(ts=4), dict(ps=-8), dict(q_sb=4), dict(q=x + 2), dict(window=-1),
-              dict(width=1 << 27), dict(pages=1 << 28), dict(bs=4096, width=1 << 20), dict(ws=x + 8)):
+              dict(width=1 << 27), dict(pages=1 << 28), dict(pages=1 << 20, ps=1 << 16), dict(bs=4096, width=1 << 20), dict(ws=x + 8)):
         assert attend(**c) == 1, c
     assert attend(wsb=1000) == 3
     assert L.zkv_paged_attention_workspace_size(96) == 0

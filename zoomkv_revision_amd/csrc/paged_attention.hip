@@ -141,12 +141,20 @@ struct Elem<kF16> {
   }
 };
 
+// One instruction where fmaxf first quiets both operands.  Not for the results
+// of a matrix product: the wait states they need are not inserted before asm.
+__device__ __forceinline__ float vmax(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
+
 // Maximum and sum over the four lanes 16 g + c of one c.
 __device__ __forceinline__ float across_max(float x) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const float y = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float across_sum(float x) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -194,9 +202,12 @@ struct Shape {
   // 8 waves: 2 on a SIMD, 256 registers each.  Head dim 256 holds twice the
   // tile and twice the output per wave: 4 waves with up to 512.
   static constexpr int kWaves = kD == 256 ? 4 : 8;
-  // tiles of the ring: 16 or 32 KiB per wave, in 64 to 256 registers
-  static constexpr int kTileRegs = kD * kCell / 4;
-  static constexpr int kDepth = kD == 256 ? (kFp8 ? 3 : 2) : (kTileRegs == 64 ? 2 : 4);
+  // Tiles of the ring: two, one in use and one on its way, also where more
+  // registers are left (32 requests of up to 32768 tokens in e4m3, head dim
+  // 128: 69 us; with three 72, four 73, five 87: the longer unrolled loop costs
+  // more than the loads in flight gain); three for e4m3 at head dim 256 (176
+  // us for 16 requests of 32768 tokens, 189 with two).
+  static constexpr int kDepth = kD == 256 && kFp8 ? 3 : 2;
   // first channel of chunk n of output row r (r = 0 .. 15)
   static __device__ __forceinline__ int channel(int r, int n) { return n * (16 * kChunk) + r * kChunk; }
 };
@@ -218,7 +229,7 @@ struct Cursor {
   int tile, left;   // the present tile of the request, the wave's tiles of the unit from it on (0: past the run)
   int len;          // the request's length
   int flags;        // kFirst, kWhole
-  int page;         // the page id of token (lane & 31) of the present tile
+  uint32_t mask;    // the present tile's tokens that are attended
 };
 
 template <int kType, bool kFp8, int kD>
@@ -232,32 +243,24 @@ struct PagedAttn {
   float m, l;
   x8 q[S::kSteps];
 
-  // Requests the K and V of a cursor's tile.  The lane of each token forms its
-  // row's offset once; the lanes that read the row fetch it by ds_bpermute.  A
-  // cursor past the run's end reads one row over and over.
-  static __device__ __forceinline__ void request(const PagedAttnParams& p, const Cursor& at, int lane, Tile& x) {
-    const int t = at.tile * kTile + (lane & 31), tc = min(t, at.len - 1);
-    const int first = p.window > 0 ? at.len - p.window : 0;
-    const bool there = at.left > 0 && static_cast<unsigned>(at.page) < static_cast<unsigned>(p.layout.num_pages);
-    x.mask = static_cast<uint32_t>(__ballot(there && t < at.len && t >= first));
+  // Requests the K and V of a cursor's tile, whose rows' places (in 16 bytes
+  // from the pool's start) are in LDS.  A cursor past the run's end reads one
+  // row over and over.
+  static __device__ __forceinline__ void request(const PagedAttnParams& p, const Cursor& at, const uint32_t* rows,
+                                                 int lane, Tile& x) {
+    x.mask = at.mask;
     x.unit = at.left > 0 ? at.b * static_cast<int>(p.units.d) + at.rest : -1;
     x.flags = at.left > 0 ? at.flags | (at.left == 1 ? kLast : 0) : 0;
-    const uint32_t in_page = tc - div_by(tc, p.page) * p.page.d;
-    const int64_t off =
-        there ? (at.page * p.layout.page_stride + in_page * p.layout.token_stride) * S::kCell : 0;
-    const int lo = static_cast<int>(off), hi = static_cast<int>(off >> 32);
     const int c = lane & 15, g = lane >> 4;
-    const auto row_of = [&](int token) {
-      const uint32_t l32 = __builtin_amdgcn_ds_bpermute(4 * token, lo);
-      const uint32_t h32 = __builtin_amdgcn_ds_bpermute(4 * token, hi);
-      return static_cast<int64_t>((static_cast<uint64_t>(h32) << 32) | l32);
-    };
+    const uint32_t krow[2] = {rows[c], rows[16 + c]};
+    const u32x4_t vrow[2] = {*reinterpret_cast<const u32x4_t*>(rows + 4 * g),
+                             *reinterpret_cast<const u32x4_t*>(rows + 16 + 4 * g)};
     const int64_t head = div_by(at.rest, p.groups) * p.layout.head_stride * S::kCell;
     const uint8_t* kp = static_cast<const uint8_t*>(p.k) + head + 16 * g;
     const uint8_t* vp = static_cast<const uint8_t*>(p.v) + head + c * (S::kChunk * S::kCell);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      const uint8_t* r = kp + row_of(16 * mt + c);
+      const uint8_t* r = kp + (static_cast<uint64_t>(krow[mt]) << 4);
 #pragma unroll
       for (int i = 0; i < S::kKLoads; ++i)
         x.k[mt][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + 64 * i));
@@ -265,7 +268,7 @@ struct PagedAttn {
     __builtin_amdgcn_sched_barrier(0);  // K is used first: V behind it
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint8_t* r = vp + row_of((e & 4) * 4 + 4 * g + (e & 3));
+      const uint8_t* r = vp + (static_cast<uint64_t>(vrow[e >> 2][e & 3]) << 4);
 #pragma unroll
       for (int n = 0; n < S::kChunks; ++n)
         load_words<S::kChunkWords>(r + n * (16 * S::kChunk * S::kCell), x.v[e] + n * S::kChunkWords);
@@ -308,7 +311,6 @@ struct PagedAttn {
       s[mt] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < S::kSteps; ++i) s[mt] = E::mfma(k_operand(x, mt, i), q[i], s[mt]);
-      s[mt] *= sc;
     }
     if (x.mask != 0xFFFFFFFFu) {
       // tokens that are not attended: score -inf (whatever their row holds),
@@ -322,13 +324,13 @@ struct PagedAttn {
         }
       }
     }
+    // (sc is positive: the largest score is the largest product)
     float top = s[0][0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) top = fmaxf(top, s[e >> 2][e & 3]);
-    top = across_max(top);
-    top -= E::kUp;
+    top = across_max(top) * sc - E::kUp;
     if (__any(top > m + kLazyBits)) {
-      const float now = fmaxf(m, top);
+      const float now = vmax(m, top);
       // (m = -inf: nothing summed yet; a lane that stays at -inf keeps its zeros)
       const float a = now == -kInf ? 1.0f : __builtin_amdgcn_exp2f(m - now);
       m = now;
@@ -340,8 +342,8 @@ struct PagedAttn {
     uint32_t parts[E::kParts][4];
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      float p0 = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - base);
-      float p1 = __builtin_amdgcn_exp2f(s[e >> 2][(e & 3) + 1] - base);
+      float p0 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], sc, -base));
+      float p1 = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][(e & 3) + 1], sc, -base));
       l += p0 + p1;
 #pragma unroll
       for (int n = 0; n < E::kParts; ++n) {
@@ -368,13 +370,19 @@ struct PagedAttn {
   }
 
   // q of a unit as the B operand, in the channel order of the K operand's k-steps.
-  __device__ __forceinline__ void load_q(const PagedAttnParams& p, int b, int head0, int heads, int lane) {
+  // A negative scale is taken as its magnitude and the negated q.
+  __device__ __forceinline__ void load_q(const PagedAttnParams& p, int b, int head0, int heads, bool negate, int lane) {
     const int c = lane & 15, g = lane >> 4;
     const uint16_t* qr = p.q + b * p.q_sb + (head0 + min(c, heads - 1)) * p.q_sh;
 #pragma unroll
     for (int i = 0; i < S::kSteps; ++i) {
       const int ch = kFp8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
       q[i] = __builtin_bit_cast(x8, *reinterpret_cast<const u32x4_t*>(qr + ch));
+    }
+    if (negate) {
+#pragma unroll
+      for (int i = 0; i < S::kSteps; ++i)
+        q[i] = __builtin_bit_cast(x8, __builtin_bit_cast(u32x4_t, q[i]) ^ 0x80008000u);
     }
   }
   // Uses, and so waits for, q: pending at every tile of the loop its loads
@@ -412,9 +420,10 @@ __device__ __forceinline__ float natural_lse(float m, float l) {
   return l == 0.0f ? -kInf : (m + __log2f(l)) * kLn2v;
 }
 
-// LDS before the partials: the counters of a workgroup, and a place per request.
+// LDS before the partials: the counters of a workgroup, the rows of each wave's
+// next tile, and a place per request.
 __host__ __device__ constexpr size_t counter_bytes(int waves, int bs) {
-  return (static_cast<size_t>(4 * waves + 2 + bs + 1) * 4 + 15) / 16 * 16;
+  return static_cast<size_t>((4 * waves + 2 + 3) / 4 + kTile * waves / 4 + (bs + 1 + 3) / 4) * 16;
 }
 
 // One unit of the line.
@@ -432,7 +441,8 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   int* s_unit = reinterpret_cast<int*>(smem);  // [kSlots]: unit of a partial or -1
   int* s_part = s_unit + kSlots;               // [kWaves + 2]: scan, last-arrival flags
   int* s_done = s_part + kWaves + 2;           // [kWaves]: tiles done
-  int* s_cum = s_done + kWaves;                // [bs + 1]: places of the requests before, per unit
+  uint32_t* s_rows = reinterpret_cast<uint32_t*>(smem + 16 * ((4 * kWaves + 2 + 3) / 4));  // [kWaves][kTile]
+  int* s_cum = reinterpret_cast<int*>(s_rows + kTile * kWaves);  // [bs + 1]: places of the requests before, per unit
   // (the last join uses the partials' space anew, beyond s_ml if it must: it comes last)
   float* s_o = reinterpret_cast<float*>(smem + counter_bytes(kWaves, p.bs));  // [kSlots][heads][kRow]
   float* s_ml = s_o + kSlots * p.heads_lds * kRow;                            // [kSlots][heads][2]
@@ -533,11 +543,15 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   const int x0 = wg0 + wave * share, x1 = min(x0 + share, wg1);
   if (x0 < x1) {
     Cursor at;
-    int tile0;
+    uint32_t* rows = s_rows + kTile * wave;
+    int tile0, first;  // the request's first tile and first token
+    const uint32_t page16 = static_cast<uint32_t>(p.layout.page_stride * S::kCell / 16);
+    const uint32_t token16 = static_cast<uint32_t>(p.layout.token_stride * S::kCell / 16);
     const auto enter = [&](int b) {  // a request's numbers
       at.b = b;
       at.len = len_of(b);
       tile0 = tile0_of(at.len);
+      first = p.window > 0 ? at.len - p.window : 0;
       at.tiles = cum(b + 1) - cum(b) - kUnitCost;
     };
     const auto part = [&](int from) {  // the wave's part of the unit: its tiles from `from` on
@@ -563,17 +577,23 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     // is made (the asm uses its value): a load that might be pending at every
     // tile would make every tile wait for all but the newest request.
     int window = 0, window0 = 0, window_of = -1;
+    // places of the present tile's tokens (past the end: of the last), and
+    // which of them are attended
     const auto look_up = [&]() {
-      const int t = at.tile * kTile, t1 = min(t + kTile, at.len) - 1;
-      const int e0 = static_cast<int>(div_by(t, p.page)), e1 = static_cast<int>(div_by(t1, p.page));
+      const int t0 = at.tile * kTile, t1 = min(t0 + kTile, at.len) - 1;
+      const int e0 = static_cast<int>(div_by(t0, p.page)), e1 = static_cast<int>(div_by(t1, p.page));
       if (at.b != window_of || e0 < window0 || e1 >= window0 + 64) {
         window_of = at.b;
         window0 = e0;
         window = p.table[at.b * p.table_stride + min(e0 + lane, static_cast<int>(div_by(at.len - 1, p.page)))];
         asm volatile("" : "+v"(window));
       }
-      const int mine = static_cast<int>(div_by(min(t + (lane & 31), t1), p.page));
-      at.page = __builtin_amdgcn_ds_bpermute(4 * (mine - window0), window);
+      const int t = t0 + (lane & 31), tc = min(t, t1);
+      const uint32_t entry = div_by(tc, p.page), in_page = tc - entry * p.page.d;
+      const uint32_t page = __builtin_amdgcn_ds_bpermute(4 * (static_cast<int>(entry) - window0), window);
+      const bool there = at.left > 0 && page < static_cast<uint32_t>(p.layout.num_pages);
+      rows[lane & 31] = (there ? page : 0) * page16 + (there ? in_page : 0) * token16;
+      at.mask = static_cast<uint32_t>(__ballot(there && t <= t1 && t >= first));
     };
     const auto advance = [&]() {
       if (at.left > 1) {
@@ -597,8 +617,10 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     float sc = 0.0f;
     const auto begin_unit = [&](int id) {
       const Unit u = unit_at(id);
-      attn.load_q(p, u.b, u.head0, u.heads, lane);
       sc = p.scale * (kFp8 && p.k_scale ? p.k_scale[u.kvh] : 1.0f);
+      attn.load_q(p, u.b, u.head0, u.heads, sc < 0.0f, lane);
+      // (positive also for a scale of 0, whose product with -Inf would be NaN)
+      sc = sc != sc ? sc : fmaxf(fabsf(sc), 0x1p-120f);
       attn.start();
     };
     begin_unit(at.b * units + at.rest);  // (its q and the first page ids in one round trip)
@@ -608,9 +630,8 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     int slot = kSlots / kWaves * wave, done = 0;
 #pragma unroll
     for (int i = 0; i < S::kDepth - 1; ++i) {
-      const Cursor now = at;
+      attn.request(p, at, rows, lane, ring[i]);
       advance();
-      attn.request(p, now, lane, ring[i]);
     }
     ring[0].flags &= ~kFirst;
     do {
@@ -621,9 +642,8 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
           begin_unit(x.unit);
           attn.settle_q();
         }
-        const Cursor now = at;
+        attn.request(p, at, rows, lane, ring[(i + S::kDepth - 1) % S::kDepth]);
         advance();
-        attn.request(p, now, lane, ring[(i + S::kDepth - 1) % S::kDepth]);
         // The tile's loads are older than those of the kDepth - 1 requests
         // behind it: waited for here by count, on every path, or a path that
         // seems to pass them by would make the compiler wait for the newest.
@@ -912,6 +932,9 @@ extern "C" int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, in
   ZKV_REQUIRE(most_tiles < (1ll << 31) - (1 << 20),
               "zkv_paged_attention: %d requests of %d KV heads over %lld tokens are too many tiles for one call", bs, kv,
               static_cast<long long>(width) * page_size);
+  // (rows are found by 32-bit numbers of 16 bytes)
+  ZKV_REQUIRE(((num_pages - 1) * page_stride + (page_size - 1) * token_stride) * (is_fp8 ? 1 : 2) < (1ll << 36),
+              "zkv_paged_attention: the rows of a pool start within 64 GiB");
   if (workspace_bytes < workspace_bytes_for(d))
     return fail(ZKV_ESPACE, "zkv_paged_attention: workspace of %zu bytes, %zu needed", workspace_bytes,
                 workspace_bytes_for(d));

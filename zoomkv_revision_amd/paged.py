@@ -394,6 +394,9 @@ def _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, w
     width, window = block_table.shape[1], int(window)
     if window < 0:
         raise ValueError(f"window must not be negative (0: the whole sequence); got {window}")
+    window = min(window, (1 << 31) - 1)
+    if ((pages - 1) * strides[0] + (page - 1) * strides[2]) * k_pages.element_size() >= 1 << 36:
+        raise ValueError("the rows of a pool must start within 64 GiB")
     groups = -(-(hq // kv) // 16)
     if width * page >= (1 << 31) - 32 or bs * kv * groups * (-(-width * page // 32) + 2) >= (1 << 31) - (1 << 20):
         raise ValueError(f"{bs} requests of up to {width * page} tokens in one call")
@@ -435,6 +438,8 @@ class PagedAttentionPlan(_Plan):
                  v_scale=None, return_softmax_lse=False, out=None, workspace=None):
         if workspace is None and q.is_cuda and q.shape[-1] in HEAD_DIMS:
             workspace = new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(q.device).synchronize()   # cleared, whichever stream the plan runs on
         args, result, keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                              v_scale, return_softmax_lse, out, workspace, copies=False)
         super().__init__(lib().zkv_paged_attention, q.device, args, result, keep)
