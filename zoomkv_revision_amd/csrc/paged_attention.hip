@@ -498,8 +498,9 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
 
   // --- this workgroup's run of places --------------------------------------
   const auto cum = [&](int b) { return __builtin_amdgcn_readfirstlane(s_cum[b]); };
-  // the request that place x belongs to
-  const auto request_at = [&](int x) {
+  // the request that place x belongs to (`cum` for a place of the whole wave,
+  // plain reads where each lane has its own)
+  const auto request_at = [&](int x, auto cum) {
     const int at = static_cast<int>(div_by(x, p.units));
     int lo = 0, hi = p.bs - 1;
     while (lo < hi) {
@@ -513,15 +514,15 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   };
   const int grid = static_cast<int>(gridDim.x);
   const int chunk = max(kWaves, (total + grid - 1) / grid);
-  const auto cut_at = [&](int w) {
-    const int64_t y64 = static_cast<int64_t>(w) * chunk;
-    if (y64 >= total) return total;
-    const int y = static_cast<int>(y64);
-    if (chunk > kWaves) return y;
-    const int b = request_at(y), size = cum(b + 1) - cum(b), from = y - cum(b) * units, in = from % size;
-    return size - kUnitCost > kWholeTiles ? y : (2 * in < size ? y - in : y - in + size);
-  };
-  const int wg0 = cut_at(blockIdx.x), wg1 = cut_at(blockIdx.x + 1);
+  // both ends of the run, one a lane
+  const int64_t y64 = (static_cast<int64_t>(blockIdx.x) + (lane & 1)) * chunk;
+  int end = static_cast<int>(min(y64, static_cast<int64_t>(total)));
+  if (chunk == kWaves && y64 < total) {
+    const int b = request_at(end, [&](int i) { return s_cum[i]; });
+    const int size = s_cum[b + 1] - s_cum[b], in = (end - s_cum[b] * units) % size;
+    if (size - kUnitCost <= kWholeTiles) end += 2 * in < size ? -in : size - in;
+  }
+  const int wg0 = __builtin_amdgcn_readlane(end, 0), wg1 = __builtin_amdgcn_readlane(end, 1);
   if (wg0 >= wg1) return;
   const auto unit_at = [&](int id) {
     Unit u;
@@ -605,7 +606,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
       }
       look_up();
     };
-    enter(request_at(x0));
+    enter(request_at(x0, cum));
     {
       const int size = at.tiles + kUnitCost, from = x0 - cum(at.b) * units;
       at.rest = from / size;
