@@ -32,7 +32,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._lib import check, device_stream, lib, ptr, require_gpu, stream_of
+from ._lib import check, device_stream, lib, ptr, require_gpu
 
 HEAD_DIMS = (64, 128, 256)
 MAX_REQUESTS = 4096          # of one attention call
@@ -71,6 +71,16 @@ def new_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     return ws
 
 
+def _launch(fn, device: torch.device, args) -> None:
+    """One C-ABI call on the current stream of `device`, which need not be the
+    current device."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, device_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, device_stream(device)))
+
+
 class _Plan:
     """A checked call over fixed buffers: ``run()`` is one C-ABI call on the
     current stream of their device.  The tensors must stay alive and keep their
@@ -80,31 +90,33 @@ class _Plan:
         self._fn, self._device, self._args, self.out, self._keep = fn, device, args, result, keep
 
     def run(self):
-        if torch.cuda.current_device() != self._device.index:
-            with torch.cuda.device(self._device):
-                check(self._fn(*self._args, device_stream(self._device)))
-        else:
-            check(self._fn(*self._args, device_stream(self._device)))
+        _launch(self._fn, self._device, self._args)
         return self.out
 
 
 def _same_device(first: torch.Tensor, **others) -> None:
+    device = first.device
     for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, not on {first.device}")
-
-
-def _check_rows(name: str, t: torch.Tensor, align: int = 16) -> bool:
-    """Whether t's rows are contiguous and start on `align` bytes."""
-    item = t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % align == 0 and \
-        all(t.stride(i) * item % align == 0 for i in range(t.dim() - 1) if t.shape[i] > 1)
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, not on {device}")
 
 
 def _strides(t: torch.Tensor) -> tuple[int, ...]:
     """Strides in elements; those of single-entry dims (any number in torch)
     as 0."""
-    return tuple(0 if t.shape[i] == 1 else t.stride(i) for i in range(t.dim()))
+    strides, shape = t.stride(), t.shape
+    return tuple([0 if n == 1 else s for n, s in zip(shape, strides)]) if 1 in shape else strides
+
+
+def _check_rows(t: torch.Tensor, strides: tuple[int, ...]) -> bool:
+    """Whether t's rows are contiguous and start on 16 bytes (strides: t's)."""
+    cells = 16 // t.element_size()
+    if strides[-1] != 1 or t.data_ptr() % 16:
+        return False
+    for s in strides[:-1]:
+        if s % cells:
+            return False
+    return True
 
 
 def _check_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, k_scale, v_scale):
@@ -121,9 +133,10 @@ def _check_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtyp
         raise ValueError(f"the head dim must be one of {HEAD_DIMS}; got {d}")
     if min(pages, kv, page) < 1 or pages * page >= 1 << 31:
         raise ValueError(f"a pool of {pages} pages of {page} tokens, {kv} heads")
-    if _strides(k_pages) != _strides(v_pages):
+    strides = _strides(k_pages)
+    if strides != _strides(v_pages):
         raise ValueError(f"K and V pages must have the same strides; got {k_pages.stride()}, {v_pages.stride()}")
-    if not (_check_rows("k_pages", k_pages) and _check_rows("v_pages", v_pages)):
+    if not (_check_rows(k_pages, strides) and _check_rows(v_pages, strides)):
         raise ValueError("the rows of a pool must be contiguous and start on 16 bytes")
     fp8 = k_pages.dtype == torch.float8_e4m3fn
     for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
@@ -134,7 +147,7 @@ def _check_pools(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtyp
         if s.dtype != torch.float32 or tuple(s.shape) != (kv,) or (kv > 1 and s.stride(0) != 1):
             raise ValueError(f"{name} must be contiguous float32 [{kv}]")
     _same_device(k_pages, v_pages=v_pages, k_scale=k_scale, v_scale=v_scale)
-    return int(fp8), pages, kv, page, d, _strides(k_pages)[:3]
+    return int(fp8), pages, kv, page, d, strides[:3]
 
 
 def _check_ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> None:
@@ -257,7 +270,7 @@ def page_advance(tables: PageTables, new_tokens: torch.Tensor, slots: torch.Tens
 # writes
 # ---------------------------------------------------------------------------
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    return t if _check_rows("", t) else t.contiguous()
+    return t if _check_rows(t, _strides(t)) else t.contiguous()
 
 
 def _write_args(k, v, slots, k_pages, v_pages, k_scale, v_scale, copies: bool):
@@ -271,7 +284,7 @@ def _write_args(k, v, slots, k_pages, v_pages, k_scale, v_scale, copies: bool):
     _same_device(k_pages, k=k, v=v, slots=slots)
     if n * kv * (d // 8) >= (1 << 31) - 1024:
         raise ValueError(f"{n} tokens of {kv} heads in one call")
-    if n and not (_check_rows("k", k) and _check_rows("v", v)):
+    if n and not (_check_rows(k, _strides(k)) and _check_rows(v, _strides(v))):
         if not copies:
             raise ValueError("a write plan reads k and v in place: their rows must be contiguous and start on 16 bytes")
         k, v = _aligned(k), _aligned(v)
@@ -302,8 +315,7 @@ def paged_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     1), rounded to nearest even, magnitudes above 448 as 448, NaN kept."""
     args, keep = _write_args(k, v, slots, k_pages, v_pages, k_scale, v_scale, copies=True)
     if keep[0].shape[0]:
-        with torch.cuda.device(k_pages.device):
-            check(lib().zkv_paged_write(*args, stream_of(k_pages)))
+        _launch(lib().zkv_paged_write, k_pages.device, args)
 
 
 def _rope_args(qkv, heads, kv_heads, q_norm, k_norm, eps, cos, sin, positions, slots, q_out, k_pages, v_pages,
@@ -331,7 +343,7 @@ def _rope_args(qkv, heads, kv_heads, q_norm, k_norm, eps, cos, sin, positions, s
         raise ValueError(f"{n} rows of {heads + 2 * kv} heads in one call")
     _same_device(k_pages, qkv=qkv, q_norm=q_norm, k_norm=k_norm, cos=cos, sin=sin, positions=positions, slots=slots,
                  q_out=q_out)
-    if n and not _check_rows("qkv", qkv):
+    if n and not _check_rows(qkv, _strides(qkv)):
         if not copies:
             raise ValueError("a rope plan reads qkv in place: its rows must be contiguous and start on 16 bytes")
         qkv = qkv.contiguous()
@@ -367,8 +379,7 @@ def paged_qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm: tor
     args, keep = _rope_args(qkv, heads, kv_heads, q_norm, k_norm, eps, cos, sin, positions, slots, q_out, k_pages,
                             v_pages, k_scale, v_scale, copies=True)
     if keep[0].shape[0]:
-        with torch.cuda.device(k_pages.device):
-            check(lib().zkv_paged_qk_norm_rope(*args, stream_of(k_pages)))
+        _launch(lib().zkv_paged_qk_norm_rope, k_pages.device, args)
     return q_out
 
 
@@ -407,7 +418,7 @@ def _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, w
             out.data_ptr() % 16:
         raise ValueError(f"out must be a contiguous {list(out_shape)} tensor of q's dtype or float32 on 16 bytes")
     _same_device(q, k_pages=k_pages, block_table=block_table, seq_lens=seq_lens, out=out, workspace=workspace)
-    if not _check_rows("q", q3):
+    if not _check_rows(q3, _strides(q3)):
         if not copies:
             raise ValueError("an attention plan reads q in place: its rows must be contiguous and start on 16 bytes")
         q3 = q3.contiguous()
@@ -465,6 +476,5 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     to run."""
     args, result, _keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                           v_scale, return_softmax_lse, out, workspace, copies=True)
-    with torch.cuda.device(q.device):
-        check(lib().zkv_paged_attention(*args, stream_of(q)))
+    _launch(lib().zkv_paged_attention, q.device, args)
     return result
