@@ -447,13 +447,25 @@ class PagedAttentionPlan(_Plan):
 
     def __init__(self, q, k_pages, v_pages, block_table, seq_lens, softmax_scale=None, window=0, k_scale=None,
                  v_scale=None, return_softmax_lse=False, out=None, workspace=None):
+        self._cleared = None
         if workspace is None and q.is_cuda and q.shape[-1] in HEAD_DIMS:
             workspace = new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
             if not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream(q.device).synchronize()   # cleared, whichever stream the plan runs on
+                stream = torch.cuda.current_stream(q.device)
+                self._cleared = (stream.cuda_stream, stream.record_event())
         args, result, keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                              v_scale, return_softmax_lse, out, workspace, copies=False)
         super().__init__(lib().zkv_paged_attention, q.device, args, result, keep)
+
+    def run(self):
+        if self._cleared is not None:
+            # the plan's own workspace was cleared on the stream it was made on
+            # (a capture starts after a synchronisation)
+            made_on, event = self._cleared
+            if device_stream(self._device) != made_on and not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(self._device).wait_event(event)
+            self._cleared = None
+        return super().run()
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
