@@ -322,6 +322,20 @@ def test_the_same_bits_every_time():
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
 
 
+@pytest.mark.parametrize("lens,hq,kv,dtype,fp8", [([32926] * 4 + [0], 4, 1, BF, True), ([2268] * 79, 4, 1, BF, False),
+                                                  ([6017] * 6 + [3], 8, 4, FP, True), ([4613, 800, 77, 3000], 64, 8, BF, False),
+                                                  ([20126, 700, 15000], 20, 4, FP, False), ([3578] * 75, 8, 2, BF, False)])
+def test_the_same_bits_whoever_ends_last(lens, hq, kv, dtype, fp8):
+    """Workgroups that share units on both sides, whose last arrivals change
+    from run to run."""
+    c = Case(lens, hq, kv, 128, 16, dtype, fp8, seed=16)
+    out = torch.empty(len(lens), 1, hq, 128, dtype=torch.float32, device=DEV)
+    first = [x.clone() for x in c.attend(out=out, return_softmax_lse=True)]
+    for _ in range(60):
+        again = c.attend(out=out, return_softmax_lse=True)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_two_streams_at_once():
     """Two calls that overlap on the device, each on its stream's workspace."""
     cs = [Case([6000, 3000, 40], 8, 2, 128, 16, seed=15 + i) for i in range(2)]

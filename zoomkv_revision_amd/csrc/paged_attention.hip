@@ -785,15 +785,15 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   __syncthreads();
   const bool last0 = __builtin_amdgcn_readfirstlane(s_part[0]), last1 = __builtin_amdgcn_readfirstlane(s_part[1]);
   if (!last0 && !last1) return;
-  // Four channels of a head per thread, and for each such item as many threads
-  // as there are partials, or threads, each with its part of the partials,
-  // eight requested at once; the parts meet in LDS.  With two units to join,
-  // each takes half of the workgroup.
-  const bool both = last0 && last1;
-  const int width = both ? kThreads / 2 : kThreads;
-  const int side = both ? (wave >= kWaves / 2 ? 1 : 0) : (last1 ? 1 : 0);
-  const int me = both ? tid % (kThreads / 2) : tid;
-  const Unit u = unit_at(side ? cut[1] : cut[0]);
+  // Four channels of a head per item; an item's partials in as many parts as
+  // half of the workgroup has threads for, eight partials requested at once;
+  // the parts meet in LDS.  Each side has its half of the threads, also where
+  // only one unit ends here: which of the two do is a matter of time, and the
+  // order of the sums must not follow it.
+  constexpr int kHalf = kThreads / 2;
+  const int side = wave >= kWaves / 2 ? 1 : 0, me = tid % kHalf;
+  const bool join = side ? last1 : last0;
+  const Unit u = unit_at(join ? (side ? cut[1] : cut[0]) : (last0 ? cut[0] : cut[1]));
   const int from = side ? w0[1] : w0[0], count = side ? n[1] : n[0];
   // partial i: the unit's first workgroup kept it as its later cut, the others
   // as their earlier one
@@ -801,16 +801,16 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     return ((static_cast<int64_t>(from) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
   };
   const int items = u.heads * (kD / 4);
-  float* s_mine = s_o + (tid - me) * 8;  // 8 floats a thread
+  float* s_mine = s_o + side * (kHalf * 8);  // [part][item][8]
   constexpr int kBatch = 8;
-  // (as many passes for both units: the barriers are the workgroup's)
-  const int passes = (p.heads_lds * (kD / 4) + width - 1) / width;
+  // (as many passes for both sides: the barriers are the workgroup's)
+  const int passes = (p.heads_lds * (kD / 4) + kHalf - 1) / kHalf;
 #pragma unroll 1
   for (int pass = 0; pass < passes; ++pass) {
-    const int e0 = pass * width, here = max(1, min(width, items - e0));
-    const int parts = min(width / here, count);
-    const int part = me / here, e = e0 + me - part * here, c = e / (kD / 4), d = 4 * (e % (kD / 4));
-    const bool mine = e0 < items && part < parts;
+    const int e0 = pass * kHalf, here = max(1, min(kHalf, items - e0));
+    const int parts = min(kHalf / here, max(count, 1)), part = me / here, item = me - part * here;
+    const int e = e0 + item, c = e / (kD / 4), d = 4 * (e % (kD / 4));
+    const bool mine = join && e0 < items && part < parts;
     __syncthreads();  // (s_o of the join before is read)
     if (mine) {
       float top = -kInf, den = 0.0f;
