@@ -21,7 +21,7 @@ import torch
 
 from oracle import paged as op
 from zoomkv_revision_amd import paged
-from zoomkv_revision_amd._lib import ZkvError
+from zoomkv_revision_amd._lib import ZkvError, lib
 
 pytestmark = pytest.mark.gpu
 
@@ -170,6 +170,30 @@ def test_long_sequence_of_one_head():
     out = torch.empty(1, 1, 2, 128, dtype=torch.float32, device=DEV)
     _, lse = c.attend(out=out, return_softmax_lse=True)
     c.check(out, lse)
+
+
+@pytest.mark.parametrize("lens,hq,kv,d,dtype,fp8", [
+    ([4200], 16, 1, 128, BF, False),                 # 17 workgroups and a few more
+    ([4400, 0, 3], 16, 1, 128, FP, True),
+    ([20000], 24, 1, 128, BF, False),                # 16 heads in two steps, 8 in one or two
+    ([66000], 8, 1, 128, BF, False),                 # 256 workgroups
+    ([30000, 31000], 40, 1, 64, FP, False),
+    ([33333, 1, 700, 20011], 16, 1, 128, BF, False),  # long units that meet inside a workgroup
+    ([9000, 9000, 9000], 16, 1, 256, BF, False),
+    ([12000, 50], 20, 2, 256, FP, True)])
+def test_units_of_many_workgroups(lens, hq, kv, d, dtype, fp8):
+    """Partials joined in two steps; the counts are ready for the next call,
+    and the bits are the same from call to call."""
+    c = Case(lens, hq, kv, d, 16, dtype, fp8, seed=hq + d)
+    out, lse = c.attend(return_softmax_lse=True)
+    c.check(out, lse)
+    workspace = paged.new_workspace(torch.device(DEV), lib().zkv_paged_attention_workspace_size(d))
+    for window in (0, 0, lens[0] - 77, 0):
+        got, gl = c.attend(return_softmax_lse=True, workspace=workspace, window=window)
+        if window:
+            c.check(got, gl, window=window)
+        else:
+            assert torch.equal(got, out) and torch.equal(gl, lse)
 
 
 @pytest.mark.parametrize("window", [1, 5, 32, 100, 512, 100000])

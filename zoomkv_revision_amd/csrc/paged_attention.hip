@@ -17,7 +17,7 @@
 // units that lie wholly in its run by itself; the ends of its run go to LDS as
 // partials (m, l, O) and are joined there; the ends of the workgroup's run go
 // to the workspace and are joined by the last of the workgroups that share the
-// unit.  Each workgroup leaves at most two partials, whatever the batch is, and
+// unit (where these are many, by the last of each few first).  Each workgroup leaves at most two partials, whatever the batch is, and
 // which tiles are joined in which order depends on the lengths alone, so the
 // result is the same from run to run.
 //
@@ -69,6 +69,13 @@ constexpr int kUnitCost = 2;       // places of a unit beyond its tiles
 constexpr int kWholeTiles = 48;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
+// Partials of the last join that a thread requests at once, and the batches of
+// them one after the other, at half of the workgroup, above which it is done in
+// two steps (131072 tokens of one KV head with 8 query heads, 256 partials: 26
+// us, 50 in one step; 32768 tokens with 16 heads of 256, four requests: 38, 84.
+// At 4 batches and below the second step costs what it saves: 131072 tokens of
+// 8 KV heads, 32 query heads, 103.6 us in one step, 104.8 in two).
+constexpr int kBatch = 8, kRounds = 4;
 // The softmax's reference exponent m follows the scores' running maximum only
 // when that is more than this many powers of two above it: O is rescaled a few
 // times per run, not per tile.
@@ -441,6 +448,7 @@ template <int kType, bool kFp8, int kD>
 __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attention_kernel(const PagedAttnParams p) {
   using S = Shape<kFp8, kD>;
   constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves, kSlots = 2 * kWaves;
+  constexpr int kFan = 2 * kWaves;  // partials of a first step of the last join, where it has two
   constexpr int kRow = kD + 4;  // row stride of a partial in LDS: 4 banks of skew between heads
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   int* s_unit = reinterpret_cast<int*>(smem);  // [kSlots]: unit of a partial or -1
@@ -767,9 +775,11 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   // This lane's partial stores have reached the device's coherence point
   // before the workgroup counts in (write-through stores, waited for), and the
   // joining loads read there: no cache is written back or invalidated.
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  int w0[2], n[2] = {0, 0};  // first of the workgroups that share the cut unit, how many
+  // A unit of many workgroups is joined in two steps: the last of each kFan
+  // neighbours joins theirs, in the place of the first one's, and the last of
+  // those joins what they left.  The counts of a unit's fans are those of the
+  // workgroups behind its first one: no unit starts in these.
+  int w0[2], n[2] = {0, 0}, fans[2] = {0, 0};  // first of the workgroups that share the cut unit, how many, fans
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     w0[side] = 0;
@@ -777,93 +787,120 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const Unit u = unit_at(cut[side]);
     w0[side] = (u.base + kUnitCost) / chunk;
     n[side] = (u.base + kUnitCost + u.tiles - 1) / chunk - w0[side] + 1;
+    if (n[side] > kFan && n[side] * u.heads * (kD / 4) > kRounds * kBatch * (kThreads / 2))
+      fans[side] = (n[side] + kFan - 1) / kFan;
   }
-  if (tid < 2) {  // (both arrivals in one round trip)
-    const int of = tid ? n[1] : n[0];
-    s_part[tid] = of && arrive_last_count(p.arrivals + (tid ? w0[1] : w0[0]), of);
-  }
-  __syncthreads();
-  const bool last0 = __builtin_amdgcn_readfirstlane(s_part[0]), last1 = __builtin_amdgcn_readfirstlane(s_part[1]);
-  if (!last0 && !last1) return;
   // Four channels of a head per item; an item's partials in as many parts as
   // half of the workgroup has threads for, eight partials requested at once;
-  // the parts meet in LDS.  Each side has its half of the threads, also where
-  // only one unit ends here: which of the two do is a matter of time, and the
-  // order of the sums must not follow it.
-  constexpr int kHalf = kThreads / 2;
-  const int side = wave >= kWaves / 2 ? 1 : 0, me = tid % kHalf;
-  const bool join = side ? last1 : last0;
-  const Unit u = unit_at(join ? (side ? cut[1] : cut[0]) : (last0 ? cut[0] : cut[1]));
-  const int from = side ? w0[1] : w0[0], count = side ? n[1] : n[0];
-  // partial i: the unit's first workgroup kept it as its later cut, the others
-  // as their earlier one
-  const auto row_of = [&](int i, int c) {
-    return ((static_cast<int64_t>(from) + i) * 2 + (i == 0 ? 1 : 0)) * kHeads + c;
-  };
-  const int items = u.heads * (kD / 4);
-  float* s_mine = s_o + side * (kHalf * 8);  // [part][item][8]
-  constexpr int kBatch = 8;
-  // (as many passes for both sides: the barriers are the workgroup's)
-  const int passes = (p.heads_lds * (kD / 4) + kHalf - 1) / kHalf;
+  // the parts meet in LDS.  Where two units end here, each has half of the
+  // threads, where one does, more items at a time, but not more parts: which
+  // of the two end here is a matter of time, and the order of the sums must
+  // not follow it.
+  bool in0 = cut[0] >= 0, in1 = cut[1] >= 0;  // the sides still to be joined
 #pragma unroll 1
-  for (int pass = 0; pass < passes; ++pass) {
-    const int e0 = pass * kHalf, here = max(1, min(kHalf, items - e0));
-    const int parts = min(kHalf / here, max(count, 1)), part = me / here, item = me - part * here;
-    const int e = e0 + item, c = e / (kD / 4), d = 4 * (e % (kD / 4));
-    const bool mine = join && e0 < items && part < parts;
-    __syncthreads();  // (s_o of the join before is read)
-    if (mine) {
-      float top = -kInf, den = 0.0f;
-      float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int i0 = part; i0 < count; i0 += kBatch * parts) {
-        float2_t ml[kBatch], lo[kBatch], hi[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int64_t row = row_of(min(i0 + i * parts, count - 1), c);
-          ml[i] = load_dev(p.part_ml + row * 2);
-          lo[i] = load_dev(p.part_o + row * kD + d);
-          hi[i] = load_dev(p.part_o + row * kD + d + 2);
-        }
-        float now = top;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < count ? fmaxf(now, ml[i][0]) : now;
-        const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
-        top = now;
-        den *= a;
-        num *= a;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          if (i0 + i * parts >= count) continue;
-          const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
-          den += w * ml[i][1];
-          num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
-        }
-      }
-      float* dst = s_mine + me * 8;
-      *reinterpret_cast<float4_t*>(dst) = num;
-      dst[4] = top;
-      dst[5] = den;
+  for (int step = 0; step < 2; ++step) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid < 2) {  // (both arrivals in one round trip)
+      const int first = tid ? w0[1] : w0[0], count = tid ? n[1] : n[0], fans_of = tid ? fans[1] : fans[0];
+      const int mine = (static_cast<int>(blockIdx.x) - first) / kFan;
+      const bool by_fan = fans_of && step == 0;
+      s_part[tid] = (tid ? in1 : in0) &&
+                    arrive_last_count(p.arrivals + first + (by_fan ? 1 + mine : 0),
+                                      by_fan ? min(kFan, count - kFan * mine) : fans_of ? fans_of : count);
     }
     __syncthreads();
-    if (mine && part == 0) {
-      float top = -kInf;
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i) top = fmaxf(top, s_mine[(i * here + me) * 8 + 4]);
-      const float base = top == -kInf ? 0.0f : top;
-      float den = 0.0f;
-      float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-      for (int i = 0; i < parts; ++i) {
-        const float* src = s_mine + (i * here + me) * 8;
-        const float w = __builtin_amdgcn_exp2f(src[4] - base);
-        den += w * src[5];
-        num += w * *reinterpret_cast<const float4_t*>(src);
+    const bool last0 = __builtin_amdgcn_readfirstlane(s_part[0]), last1 = __builtin_amdgcn_readfirstlane(s_part[1]);
+    if (!last0 && !last1) return;
+    const bool both = last0 && last1;
+    const int side = both ? (wave >= kWaves / 2 ? 1 : 0) : (last1 ? 1 : 0);
+    const int width = both ? kThreads / 2 : kThreads, me = both ? tid % (kThreads / 2) : tid;
+    const int from = side ? w0[1] : w0[0], all = side ? n[1] : n[0], fanned = side ? fans[1] : fans[0];
+    const int fan = fanned ? (static_cast<int>(blockIdx.x) - from) / kFan : 0;
+    float* s_mine = s_o + (both ? side * (kThreads / 2 * 8) : 0);  // [part][item][8]
+    // (as many passes for both sides: the barriers are the workgroup's)
+    const int passes = (p.heads_lds * (kD / 4) + width - 1) / width;
+    const bool ends = !fanned || step == 1;  // this step gives the unit's result
+    const Unit u = unit_at(side ? cut[1] : cut[0]);
+    const int count = !fanned ? all : step ? fanned : min(kFan, all - kFan * fan);
+    // partial i of the step: the unit's first workgroup kept it as its later
+    // cut, the others as their earlier one
+    const int begin = fanned && step == 0 ? kFan * fan : 0, stride = fanned && step ? kFan : 1;
+    const auto row_of = [&](int i, int c) {
+      const int at = begin + i * stride;
+      return ((static_cast<int64_t>(from) + at) * 2 + (at == 0 ? 1 : 0)) * kHeads + c;
+    };
+    const int items = u.heads * (kD / 4), parts = max(1, min(kThreads / 2 / items, count));
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {  // (of whole heads)
+      const int e0 = pass * width, here = max(1, min(width, items - e0));
+      const int part = me / here, item = me - part * here;
+      const int e = e0 + item, c = e / (kD / 4), d = 4 * (e % (kD / 4));
+      const bool mine = e0 < items && part < parts;
+      __syncthreads();  // (s_o of the join before is read)
+      if (mine) {
+        float top = -kInf, den = 0.0f;
+        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i0 = part; i0 < count; i0 += kBatch * parts) {
+          float2_t ml[kBatch], lo[kBatch], hi[kBatch];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const int64_t row = row_of(min(i0 + i * parts, count - 1), c);
+            ml[i] = load_dev(p.part_ml + row * 2);
+            lo[i] = load_dev(p.part_o + row * kD + d);
+            hi[i] = load_dev(p.part_o + row * kD + d + 2);
+          }
+          float now = top;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < count ? fmaxf(now, ml[i][0]) : now;
+          const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
+          top = now;
+          den *= a;
+          num *= a;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (i0 + i * parts >= count) continue;
+            const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
+            den += w * ml[i][1];
+            num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+          }
+        }
+        float* dst = s_mine + me * 8;
+        *reinterpret_cast<float4_t*>(dst) = num;
+        dst[4] = top;
+        dst[5] = den;
       }
-      const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
-      const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
-      store_result<kType>(p, row * kD + d, num * inv);
-      if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+      __syncthreads();
+      if (mine && part == 0) {
+        float top = -kInf;
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) top = fmaxf(top, s_mine[(i * here + me) * 8 + 4]);
+        const float base = top == -kInf ? 0.0f : top;
+        float den = 0.0f;
+        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+          const float* src = s_mine + (i * here + me) * 8;
+          const float w = __builtin_amdgcn_exp2f(src[4] - base);
+          den += w * src[5];
+          num += w * *reinterpret_cast<const float4_t*>(src);
+        }
+        if (ends) {
+          const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
+          const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
+          store_result<kType>(p, row * kD + d, num * inv);
+          if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+        } else {
+          const int64_t row = row_of(0, c);
+          store_dev(p.part_o + row * kD + d, num[0], num[1]);
+          store_dev(p.part_o + row * kD + d + 2, num[2], num[3]);
+          if (d == 0) store_dev(p.part_ml + row * 2, top, den);
+        }
+      }
     }
+    in0 = last0 && fans[0] && step == 0;
+    in1 = last1 && fans[1] && step == 0;
+    if (!in0 && !in1) return;
   }
 }
 
