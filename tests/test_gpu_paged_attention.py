@@ -196,6 +196,27 @@ def test_units_of_many_workgroups(lens, hq, kv, d, dtype, fp8):
             assert torch.equal(got, out) and torch.equal(gl, lse)
 
 
+@pytest.mark.parametrize("lens,hq,kv,d,dtype,fp8", [
+    ([70000], 16, 4, 128, BF, False),                      # sets of four heads
+    ([40000, 0, 31, 9000, 1], 64, 8, 128, BF, False),      # of two
+    ([5000] * 20 + [3, 0, 700], 10, 2, 64, FP, False),     # of two, five query heads each
+    ([3000 + 7 * i for i in range(15)], 8, 8, 128, BF, True),   # of eight
+    ([33000, 2000], 8, 4, 256, FP, True),
+    ([4100] * 9 + [60, 8000], 6, 6, 64, BF, False),        # of two: three sets
+    ([60000, 20000], 48, 2, 64, FP, False)])               # more than 16 query heads a KV head: none
+def test_heads_of_a_token_together(lens, hq, kv, d, dtype, fp8):
+    """Pools [page, token, head] over enough tokens that neighbouring waves take
+    the heads of a set: the same results, with a window, and every time."""
+    c = Case(lens, hq, kv, d, 16, dtype, fp8, nhd=True, seed=hq + d)
+    some = sorted({0, len(lens) // 2, len(lens) - 2, len(lens) - 1})
+    out, lse = c.attend(return_softmax_lse=True)
+    c.check(out, lse, requests=some)
+    again, lse2 = c.attend(return_softmax_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    window = max(lens) - 500
+    c.check(*c.attend(return_softmax_lse=True, window=window), window=window, requests=some)
+
+
 @pytest.mark.parametrize("window", [1, 5, 32, 100, 512, 100000])
 @pytest.mark.parametrize("page", [16, 24])
 def test_windows(window, page):

@@ -32,9 +32,8 @@
 // Bound by HBM: 16 requests of 32768 tokens, 32 / 8 heads of 128, bf16 (2.1 GB):
 // 328 us, 6.5 TB/s; 64 requests of 1 to 8192 tokens 64 us (5.5 TB/s, behind
 // about 10 us of launch, first round trips and joins); 1 x 700 tokens 14.3 us,
-// a chain of round trips (lengths, page ids and q, three tiles a wave).  A pool
-// laid out [page, token, head] gives each head a part of the memory channels
-// only: 1 x 131072 tokens 103 us, 91 as [page, head, token].
+// a chain of round trips (lengths, page ids and q, three tiles a wave).
+// 1 x 131072 tokens: 91 us, 97 where the pool is laid out [page, token, head].
 //
 // Tile.  S^T = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32: K rows are the
 // A operand (lane 16 g + c: token c, channels 32 s + 8 g ..), q the B operand
@@ -69,6 +68,17 @@ constexpr int kUnitCost = 2;       // places of a unit beyond its tiles
 constexpr int kWholeTiles = 48;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
+// Rows of one head at a stride of 512 bytes or a multiple (pools [page, token,
+// head]) share few of the first cache's sets, which holds the lines on their
+// way: fewer loads of a CU are in flight.  There a unit is a set of KV heads
+// (two to eight, up to 16 query heads) that neighbouring waves take, from
+// kSetPlaces places per wave on: 16 requests of 32768 tokens, 32 / 8 heads of
+// 128, bf16 372 -> 328 us (322 as [page, head, token]); 64 of 4096 in e4m3, heads
+// of 64, 79 -> 66; 1 x 131072 103.3 -> 96.5, its join having four times the
+// partials per unit; below, 64 requests of 1 to 8192 tokens, 7 tiles a wave,
+// would take 54.2 for 52.6.  Head dim 256, whose rows are two and four sets wide,
+// does not gain (64 x 4096: 174 us, 180 with sets).
+constexpr int kSetPlaces = 12;
 // Partials of the last join that a thread requests at once, and the batches of
 // them one after the other, at half of the workgroup, above which it is done in
 // two steps (131072 tokens of one KV head with 8 query heads, 256 partials: 26
@@ -99,6 +109,8 @@ struct PagedAttnParams {
   float* part_ml;  // [workgroup][2][kHeads][2]
   unsigned int* arrivals;  // per workgroup: those of the unit that starts in it
   FastDiv units;   // units of one request: kv * groups
+  FastDiv sets;    // where a unit is a set of KV heads: kv / set
+  int set;         // KV heads of a set (a power of two)
   FastDiv groups;  // groups of up to 16 query heads of a KV head
   float scale;     // softmax scale * log2 e
   int bs, hq, kv, gqa, window, out_f32;
@@ -258,16 +270,16 @@ struct PagedAttn {
   // Requests the K and V of a cursor's tile, whose rows' places (in 16 bytes
   // from the pool's start) are in LDS.  A cursor past the run's end reads one
   // row over and over.
-  static __device__ __forceinline__ void request(const PagedAttnParams& p, const Cursor& at, const uint32_t* rows,
-                                                 int lane, Tile& x) {
+  static __device__ __forceinline__ void request(const PagedAttnParams& p, const Cursor& at, int units, int set,
+                                                 int member, const uint32_t* rows, int lane, Tile& x) {
     x.mask = at.mask;
-    x.unit = at.left > 0 ? at.b * static_cast<int>(p.units.d) + at.rest : -1;
+    x.unit = at.left > 0 ? at.b * units + at.rest : -1;
     x.flags = at.left > 0 ? at.flags | (at.left == 1 ? kLast : 0) : 0;
     const int c = lane & 15, g = lane >> 4;
     const uint32_t krow[2] = {rows[c], rows[16 + c]};
     const u32x4_t vrow[2] = {*reinterpret_cast<const u32x4_t*>(rows + 4 * g),
                              *reinterpret_cast<const u32x4_t*>(rows + 16 + 4 * g)};
-    const int64_t head = div_by(at.rest, p.groups) * p.layout.head_stride * S::kCell;
+    const int64_t head = (static_cast<int>(div_by(at.rest, p.groups)) * set + member) * p.layout.head_stride * S::kCell;
     const uint8_t* kp = static_cast<const uint8_t*>(p.k) + head + 16 * g;
     const uint8_t* vp = static_cast<const uint8_t*>(p.v) + head + c * (S::kChunk * S::kCell);
 #pragma unroll
@@ -440,11 +452,11 @@ __host__ __device__ constexpr size_t counter_bytes(int waves, int bs) {
 
 // One unit of the line.
 struct Unit {
-  int b, kvh, head0, heads;  // request, KV head, first query head, query heads
+  int b, head0, heads;       // request, first query head, query heads (of a set: of all of its KV heads)
   int base, tiles;           // first place on the line (its tiles start kUnitCost further), tiles
 };
 
-template <int kType, bool kFp8, int kD>
+template <int kType, bool kFp8, int kD, bool kSets>
 __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attention_kernel(const PagedAttnParams p) {
   using S = Shape<kFp8, kD>;
   constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves, kSlots = 2 * kWaves;
@@ -461,7 +473,6 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   float* s_ml = s_o + kSlots * p.heads_lds * kRow;                            // [kSlots][heads][2]
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int units = static_cast<int>(p.units.d);
 
   // --- places of every request, and their running sum -----------------------
   const auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.max_len); };
@@ -497,7 +508,13 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   }
   if (tid == 0) s_cum[p.bs] = total;
   __syncthreads();
-  total = __builtin_amdgcn_readfirstlane(total) * units;
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int grid = static_cast<int>(gridDim.x);
+  const bool sets = kSets && total * static_cast<int>(p.units.d) >= kSetPlaces * kWaves * grid;
+  const FastDiv units_div = sets ? p.sets : p.units;
+  const int units = static_cast<int>(units_div.d), set = sets ? p.set : 1, member = wave & (set - 1);
+  const int runs = kWaves / set;  // the workgroup's run is cut into
+  total *= units;
 
   // --- requests without a token: zeros -------------------------------------
   for (int b = blockIdx.x; b < p.bs; b += gridDim.x) {
@@ -514,7 +531,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   // the request that place x belongs to (`cum` for a place of the whole wave,
   // plain reads where each lane has its own)
   const auto request_at = [&](int x, auto cum) {
-    const int at = static_cast<int>(div_by(x, p.units));
+    const int at = static_cast<int>(div_by(x, units_div));
     int lo = 0, hi = p.bs - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -525,12 +542,11 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     }
     return lo;
   };
-  const int grid = static_cast<int>(gridDim.x);
-  const int chunk = max(kWaves, (total + grid - 1) / grid);
+  const int chunk = max(runs, (total + grid - 1) / grid);
   // both ends of the run, one a lane
   const int64_t y64 = (static_cast<int64_t>(blockIdx.x) + (lane & 1)) * chunk;
   int end = static_cast<int>(min(y64, static_cast<int64_t>(total)));
-  if (chunk == kWaves && y64 < total) {
+  if (!sets && chunk == kWaves && y64 < total) {
     const int b = request_at(end, [&](int i) { return s_cum[i]; });
     const int size = s_cum[b + 1] - s_cum[b], in = (end - s_cum[b] * units) % size;
     if (size - kUnitCost <= kWholeTiles) end += 2 * in < size ? -in : size - in;
@@ -539,22 +555,21 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   if (wg0 >= wg1) return;
   const auto unit_at = [&](int id) {
     Unit u;
-    u.b = static_cast<int>(div_by(id, p.units));
+    u.b = static_cast<int>(div_by(id, units_div));
     const int rest = id - u.b * units;
-    u.kvh = static_cast<int>(div_by(rest, p.groups));
-    const int group = rest - u.kvh * static_cast<int>(p.groups.d);
-    u.heads = min(kHeads, p.gqa - kHeads * group);
-    u.head0 = u.kvh * p.gqa + kHeads * group;
+    const int kvh = static_cast<int>(div_by(rest, p.groups)), group = rest - kvh * static_cast<int>(p.groups.d);
+    u.heads = min(kHeads, set * p.gqa - kHeads * group);
+    u.head0 = kvh * set * p.gqa + kHeads * group;
     const int size = cum(u.b + 1) - cum(u.b);
     u.tiles = size - kUnitCost;
     u.base = cum(u.b) * units + rest * size;
     return u;
   };
-  const auto v_scale_of = [&](int kvh) { return kFp8 && p.v_scale ? p.v_scale[kvh] : 1.0f; };
+  const auto v_scale_of = [&](int head) { return kFp8 && p.v_scale ? p.v_scale[head / p.gqa] : 1.0f; };
 
   // --- the wave's stream of tiles -------------------------------------------
-  const int share = (wg1 - wg0 + kWaves - 1) / kWaves;
-  const int x0 = wg0 + wave * share, x1 = min(x0 + share, wg1);
+  const int share = (wg1 - wg0 + runs - 1) / runs;
+  const int x0 = wg0 + wave / set * share, x1 = min(x0 + share, wg1);
   if (x0 < x1) {
     Cursor at;
     uint32_t* rows = s_rows + kTile * wave;
@@ -629,9 +644,13 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     }
     PagedAttn<kType, kFp8, kD> attn;
     float sc = 0.0f;
+    const auto mine_of = [&](Unit u) {  // the wave's KV head of a set
+      if (sets) u.heads = p.gqa, u.head0 += member * p.gqa;
+      return u;
+    };
     const auto begin_unit = [&](int id) {
-      const Unit u = unit_at(id);
-      sc = p.scale * (kFp8 && p.k_scale ? p.k_scale[u.kvh] : 1.0f);
+      const Unit u = mine_of(unit_at(id));
+      sc = p.scale * (kFp8 && p.k_scale ? p.k_scale[u.head0 / p.gqa] : 1.0f);
       attn.load_q(p, u.b, u.head0, u.heads, sc < 0.0f, lane);
       // (positive also for a scale of 0, whose product with -Inf would be NaN)
       sc = sc != sc ? sc : fmaxf(fabsf(sc), 0x1p-120f);
@@ -644,7 +663,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     int slot = kSlots / kWaves * wave, done = 0;
 #pragma unroll
     for (int i = 0; i < S::kDepth - 1; ++i) {
-      attn.request(p, at, rows, lane, ring[i]);
+      attn.request(p, at, units, set, member, rows, lane, ring[i]);
       advance();
     }
     ring[0].flags &= ~kFirst;
@@ -656,7 +675,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
           begin_unit(x.unit);
           attn.settle_q();
         }
-        attn.request(p, at, rows, lane, ring[(i + S::kDepth - 1) % S::kDepth]);
+        attn.request(p, at, units, set, member, rows, lane, ring[(i + S::kDepth - 1) % S::kDepth]);
         advance();
         // The tile's loads are older than those of the kDepth - 1 requests
         // behind it: waited for here by count, on every path, or a path that
@@ -674,12 +693,12 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
             __builtin_amdgcn_s_setprio(0);
         }
         if (x.flags & kLast) {
-          const Unit u = unit_at(x.unit);
+          const Unit u = mine_of(unit_at(x.unit));
           const int c = lane & 15, g = lane >> 4;
           const float l = across_sum(attn.l);
           if (x.flags & kWhole) {
             if (c < u.heads) {
-              const float inv = (l == 0.0f ? 0.0f : 1.0f / l) * v_scale_of(u.kvh);
+              const float inv = (l == 0.0f ? 0.0f : 1.0f / l) * v_scale_of(u.head0);
               const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
 #pragma unroll
               for (int r = 0; r < 4; ++r)
@@ -738,12 +757,15 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     if (!whole) cut[starts ? 1 : 0] = id;
     for (int e = tid; e < u.heads * (kD / 4); e += kThreads) {
       const int c = e / (kD / 4), d = 4 * (e % (kD / 4));
+      // (a set's KV heads are the neighbouring waves')
+      const int of = sets ? c / p.gqa : 0, at = c - of * p.gqa;
+      const auto has = [&](int i) { return ids[i] == id && (i / (kSlots / kWaves) & (set - 1)) == of; };
       float mv[kSlots], lv[kSlots], top = -kInf;
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
-        const float2_t ml = *reinterpret_cast<const float2_t*>(s_ml + (i * p.heads_lds + c) * 2);
-        mv[i] = ids[i] == id ? ml[0] : -kInf;
-        lv[i] = ids[i] == id ? ml[1] : 0.0f;
+        const float2_t ml = *reinterpret_cast<const float2_t*>(s_ml + (i * p.heads_lds + at) * 2);
+        mv[i] = has(i) ? ml[0] : -kInf;
+        lv[i] = has(i) ? ml[1] : 0.0f;
         top = fmaxf(top, mv[i]);
       }
       const float base = top == -kInf ? 0.0f : top;
@@ -751,13 +773,13 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
       float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < kSlots; ++i) {
-        if (ids[i] != id) continue;
+        if (!has(i)) continue;
         const float w = __builtin_amdgcn_exp2f(mv[i] - base);
         den += w * lv[i];
-        num += w * *reinterpret_cast<const float4_t*>(s_o + (i * p.heads_lds + c) * kRow + d);
+        num += w * *reinterpret_cast<const float4_t*>(s_o + (i * p.heads_lds + at) * kRow + d);
       }
       if (whole) {
-        const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
+        const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.head0 + c);
         const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
         store_result<kType>(p, row * kD + d, num * inv);
         if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
@@ -819,7 +841,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const int fan = fanned ? (static_cast<int>(blockIdx.x) - from) / kFan : 0;
     float* s_mine = s_o + (both ? side * (kThreads / 2 * 8) : 0);  // [part][item][8]
     // (as many passes for both sides: the barriers are the workgroup's)
-    const int passes = (p.heads_lds * (kD / 4) + width - 1) / width;
+    const int passes = (set * p.heads_lds * (kD / 4) + width - 1) / width;
     const bool ends = !fanned || step == 1;  // this step gives the unit's result
     const Unit u = unit_at(side ? cut[1] : cut[0]);
     const int count = !fanned ? all : step ? fanned : min(kFan, all - kFan * fan);
@@ -886,7 +908,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
           num += w * *reinterpret_cast<const float4_t*>(src);
         }
         if (ends) {
-          const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.kvh);
+          const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.head0 + c);
           const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
           store_result<kType>(p, row * kD + d, num * inv);
           if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
@@ -912,7 +934,14 @@ size_t workspace_bytes_for(int d) {
 template <int kType, bool kFp8, int kD>
 int launch_paged_attention(PagedAttnParams& p, int64_t most_tiles, hipStream_t s) {
   using S = Shape<kFp8, kD>;
-  const auto kernel = paged_attention_kernel<kType, kFp8, kD>;
+  auto kernel = paged_attention_kernel<kType, kFp8, kD, false>;
+  p.set = 1;
+  if constexpr (kD < 256) {
+    if (p.layout.head_stride < p.layout.token_stride && p.layout.token_stride * S::kCell % 512 == 0)
+      while (2 * p.set <= S::kWaves && 2 * p.set * p.gqa <= kHeads && p.kv % (2 * p.set) == 0) p.set *= 2;
+    if (p.set > 1) kernel = paged_attention_kernel<kType, kFp8, kD, true>;
+  }
+  p.sets = fast_div(static_cast<uint32_t>(p.kv / p.set));
   // the counters, then the partials (in the last join, 32 bytes a thread)
   const size_t lds = std::max(static_cast<size_t>(2 * S::kWaves) * p.heads_lds * (kD + 6) * 4,
                               static_cast<size_t>(64 * S::kWaves) * 32) +
