@@ -60,12 +60,6 @@ constexpr int kHeads = 16;         // query heads of a unit: the columns of an M
 constexpr int kMaxBatch = 4096;    // requests of a call: 4 bytes of LDS each
 constexpr int kMaxGroups = 256;    // workgroups
 constexpr int kUnitCost = 2;       // places of a unit beyond its tiles
-// Where there is no more than a place per wave, cuts are moved out of units of
-// at most kWholeTiles tiles: joining their parts across workgroups takes longer
-// than their tiles one after the other (1 x 100 tokens, 32 / 8 heads: 10.1 us,
-// 14.0 with them cut; 8 x 300: 12.1, 17.0; 1 x 700: 14.5, 16.2; with longer runs
-// the uneven loads cost more: 16 x 700 19.6 us, cut 16.3).
-constexpr int kWholeTiles = 48;
 constexpr float kInf = __builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
 // Rows of one head at a stride of 512 bytes or a multiple (pools [page, token,
@@ -226,6 +220,15 @@ struct Shape {
   // 8 waves: 2 on a SIMD, 256 registers each.  Head dim 256 holds twice the
   // tile and twice the output per wave: 4 waves with up to 512.
   static constexpr int kWaves = kD == 256 ? 4 : 8;
+  // Where there is no more than a place per wave, cuts are moved out of units of
+  // at most kWholeTiles tiles: joining their parts across workgroups takes
+  // longer than two or three tiles of a wave one after the other.  Us whole, cut
+  // (one request, 32 / 8 heads): head dim 128, 8 tiles 9.1, 13.7; 16 12.6, 13.5;
+  // 24 14.2, 13.5; 48 23.3, 13.7 (seven requests with 16 query heads of one KV
+  // head: 24 15.2, 17.9; 32 19.2, 17.5); head dim 64, 24 10.7, 12.6; 32 12.4,
+  // 12.5; 48 15.3, 12.6; head dim 256, 4 tiles 10.3 both, 8 14.0, 13.5 (16 query
+  // heads 17.6, 21.4); 16 19.8, 13.7.
+  static constexpr int kWholeTiles = kD == 64 ? 28 : 5 * kWaves / 2;
   // Tiles of the ring: two, one in use and one on its way, also where more
   // registers are left (32 requests of up to 32768 tokens in e4m3, head dim
   // 128: 69 us; with three 72, four 73, five 87: the longer unrolled loop costs
@@ -549,7 +552,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   if (!sets && chunk == kWaves && y64 < total) {
     const int b = request_at(end, [&](int i) { return s_cum[i]; });
     const int size = s_cum[b + 1] - s_cum[b], in = (end - s_cum[b] * units) % size;
-    if (size - kUnitCost <= kWholeTiles) end += 2 * in < size ? -in : size - in;
+    if (size - kUnitCost <= S::kWholeTiles) end += 2 * in < size ? -in : size - in;
   }
   const int wg0 = __builtin_amdgcn_readlane(end, 0), wg1 = __builtin_amdgcn_readlane(end, 1);
   if (wg0 >= wg1) return;
