@@ -74,12 +74,9 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2v = 0.6931471805599453f;
 // does not gain (64 x 4096: 174 us, 180 with sets).
 constexpr int kSetPlaces = 12;
 // Partials of the last join that a thread requests at once, and the batches of
-// them one after the other, at half of the workgroup, above which it is done in
-// two steps (131072 tokens of one KV head with 8 query heads, 256 partials: 26
-// us, 50 in one step; 32768 tokens with 16 heads of 256, four requests: 38, 84.
-// At 4 batches and below the second step costs what it saves: 131072 tokens of
-// 8 KV heads, 32 query heads, 103.6 us in one step, 104.8 in two).
-constexpr int kBatch = 8, kRounds = 4;
+// them one after the other that a second step costs (131072 tokens of one KV
+// head with 8 query heads, 256 partials: 26 us, 50 in one step).
+constexpr int kBatch = 8, kStepRounds = 2;
 // The softmax's reference exponent m follows the scores' running maximum only
 // when that is more than this many powers of two above it: O is rescaled a few
 // times per run, not per tile.
@@ -464,6 +461,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   using S = Shape<kFp8, kD>;
   constexpr int kWaves = S::kWaves, kThreads = 64 * kWaves, kSlots = 2 * kWaves;
   constexpr int kFan = 2 * kWaves;  // partials of a first step of the last join, where it has two
+  constexpr int kItems = std::max(1, kHeads * (kD / 4) / kThreads);  // of the last join, of a thread
   constexpr int kRow = kD + 4;  // row stride of a partial in LDS: 4 banks of skew between heads
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   int* s_unit = reinterpret_cast<int*>(smem);  // [kSlots]: unit of a partial or -1
@@ -812,8 +810,12 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const Unit u = unit_at(cut[side]);
     w0[side] = (u.base + kUnitCost) / chunk;
     n[side] = (u.base + kUnitCost + u.tiles - 1) / chunk - w0[side] + 1;
-    if (n[side] > kFan && n[side] * u.heads * (kD / 4) > kRounds * kBatch * (kThreads / 2))
-      fans[side] = (n[side] + kFan - 1) / kFan;
+    const auto rounds = [&](int count) {  // of loads, one after the other
+      const int at_once = kBatch * max(1, min(kThreads / 2 / (u.heads * (kD / 4)), count));
+      return (count + at_once - 1) / at_once;
+    };
+    const int of = (n[side] + kFan - 1) / kFan;
+    if (n[side] > kFan && rounds(n[side]) > rounds(kFan) + rounds(of) + kStepRounds) fans[side] = of;
   }
   // Four channels of a head per item; an item's partials in as many parts as
   // half of the workgroup has threads for, eight partials requested at once;
@@ -844,7 +846,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const int fan = fanned ? (static_cast<int>(blockIdx.x) - from) / kFan : 0;
     float* s_mine = s_o + (both ? side * (kThreads / 2 * 8) : 0);  // [part][item][8]
     // (as many passes for both sides: the barriers are the workgroup's)
-    const int passes = (set * p.heads_lds * (kD / 4) + width - 1) / width;
+    const int passes = (set * p.heads_lds * (kD / 4) + kItems * width - 1) / (kItems * width);
     const bool ends = !fanned || step == 1;  // this step gives the unit's result
     const Unit u = unit_at(side ? cut[1] : cut[0]);
     const int count = !fanned ? all : step ? fanned : min(kFan, all - kFan * fan);
@@ -858,68 +860,90 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
     const int items = u.heads * (kD / 4), parts = max(1, min(kThreads / 2 / items, count));
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {  // (of whole heads)
-      const int e0 = pass * width, here = max(1, min(width, items - e0));
+      const int e0 = pass * kItems * width, here = max(1, min(width, items - e0));
       const int part = me / here, item = me - part * here;
-      const int e = e0 + item, c = e / (kD / 4), d = 4 * (e % (kD / 4));
-      const bool mine = e0 < items && part < parts;
-      __syncthreads();  // (s_o of the join before is read)
-      if (mine) {
-        float top = -kInf, den = 0.0f;
-        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int i0 = part; i0 < count; i0 += kBatch * parts) {
-          float2_t ml[kBatch], lo[kBatch], hi[kBatch];
+      float top[kItems], den[kItems];
+      float4_t num[kItems];
+      int head[kItems], d[kItems];
+      bool mine[kItems];
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        const int e = e0 + j * width + item;
+        mine[j] = e < items && part < parts;
+        head[j] = mine[j] ? e / (kD / 4) : 0;
+        d[j] = 4 * (e % (kD / 4));
+        top[j] = -kInf;
+        den[j] = 0.0f;
+        num[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+      for (int i0 = part; i0 < count && mine[0]; i0 += kBatch * parts) {
+        float2_t ml[kItems][kBatch], lo[kItems][kBatch], hi[kItems][kBatch];
+#pragma unroll
+        for (int j = 0; j < kItems; ++j) {
+          if (e0 + j * width >= items) continue;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
-            const int64_t row = row_of(min(i0 + i * parts, count - 1), c);
-            ml[i] = load_dev(p.part_ml + row * 2);
-            lo[i] = load_dev(p.part_o + row * kD + d);
-            hi[i] = load_dev(p.part_o + row * kD + d + 2);
+            const int64_t row = row_of(min(i0 + i * parts, count - 1), head[j]);
+            ml[j][i] = load_dev(p.part_ml + row * 2);
+            lo[j][i] = load_dev(p.part_o + row * kD + d[j]);
+            hi[j][i] = load_dev(p.part_o + row * kD + d[j] + 2);
           }
-          float now = top;
+        }
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < count ? fmaxf(now, ml[i][0]) : now;
-          const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top - base);
-          top = now;
-          den *= a;
-          num *= a;
+        for (int j = 0; j < kItems; ++j) {
+          if (e0 + j * width >= items) continue;
+          float now = top[j];
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) now = i0 + i * parts < count ? fmaxf(now, ml[j][i][0]) : now;
+          const float base = now == -kInf ? 0.0f : now, a = __builtin_amdgcn_exp2f(top[j] - base);
+          top[j] = now;
+          den[j] *= a;
+          num[j] *= a;
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
             if (i0 + i * parts >= count) continue;
-            const float w = __builtin_amdgcn_exp2f(ml[i][0] - base);
-            den += w * ml[i][1];
-            num += w * float4_t{lo[i][0], lo[i][1], hi[i][0], hi[i][1]};
+            const float w = __builtin_amdgcn_exp2f(ml[j][i][0] - base);
+            den[j] += w * ml[j][i][1];
+            num[j] += w * float4_t{lo[j][i][0], lo[j][i][1], hi[j][i][0], hi[j][i][1]};
           }
         }
+      }
+      __syncthreads();  // (s_o of the join before is read)
+      if (parts > 1 && mine[0]) {  // (one item a thread then)
         float* dst = s_mine + me * 8;
-        *reinterpret_cast<float4_t*>(dst) = num;
-        dst[4] = top;
-        dst[5] = den;
+        *reinterpret_cast<float4_t*>(dst) = num[0];
+        dst[4] = top[0];
+        dst[5] = den[0];
       }
       __syncthreads();
-      if (mine && part == 0) {
-        float top = -kInf;
+      if (parts > 1 && mine[0] && part == 0) {
 #pragma unroll 4
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, s_mine[(i * here + me) * 8 + 4]);
-        const float base = top == -kInf ? 0.0f : top;
-        float den = 0.0f;
-        float4_t num = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < parts; ++i) top[0] = fmaxf(top[0], s_mine[(i * here + me) * 8 + 4]);
+        const float base = top[0] == -kInf ? 0.0f : top[0];
+        den[0] = 0.0f;
+        num[0] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int i = 0; i < parts; ++i) {
           const float* src = s_mine + (i * here + me) * 8;
           const float w = __builtin_amdgcn_exp2f(src[4] - base);
-          den += w * src[5];
-          num += w * *reinterpret_cast<const float4_t*>(src);
+          den[0] += w * src[5];
+          num[0] += w * *reinterpret_cast<const float4_t*>(src);
         }
+      }
+#pragma unroll
+      for (int j = 0; j < kItems; ++j) {
+        if (!mine[j] || part != 0) continue;
+        const int c = head[j];
         if (ends) {
-          const float inv = (den == 0.0f ? 0.0f : 1.0f / den) * v_scale_of(u.head0 + c);
+          const float inv = (den[j] == 0.0f ? 0.0f : 1.0f / den[j]) * v_scale_of(u.head0 + c);
           const int64_t row = static_cast<int64_t>(u.b) * p.hq + u.head0 + c;
-          store_result<kType>(p, row * kD + d, num * inv);
-          if (p.lse && d == 0) p.lse[row] = natural_lse(top, den);
+          store_result<kType>(p, row * kD + d[j], num[j] * inv);
+          if (p.lse && d[j] == 0) p.lse[row] = natural_lse(top[j], den[j]);
         } else {
           const int64_t row = row_of(0, c);
-          store_dev(p.part_o + row * kD + d, num[0], num[1]);
-          store_dev(p.part_o + row * kD + d + 2, num[2], num[3]);
-          if (d == 0) store_dev(p.part_ml + row * 2, top, den);
+          store_dev(p.part_o + row * kD + d[j], num[j][0], num[j][1]);
+          store_dev(p.part_o + row * kD + d[j] + 2, num[j][2], num[j][3]);
+          if (d[j] == 0) store_dev(p.part_ml + row * 2, top[j], den[j]);
         }
       }
     }
