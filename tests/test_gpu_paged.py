@@ -65,6 +65,15 @@ def test_advance_equals_the_plain_form(requests, page, width, cap, free):
     _same_step(rng, lens, new, width, page, n_free, cap)
 
 
+@pytest.mark.parametrize("requests,cap", [(3, 70001), (500, 32769), (60, 300000)])
+def test_advance_of_long_prompts(requests, cap):
+    """Few requests, many slots, more than one a thread."""
+    rng = np.random.default_rng(cap)
+    lens = rng.integers(0, 400, requests)
+    new = rng.choice([2 * cap // requests, cap // requests, 1, 0, -90], requests)
+    _same_step(rng, lens, new, 5000, 16, 30000, cap)
+
+
 @pytest.mark.parametrize("requests,row", [(1, 1), (5, 1), (64, 1), (9, 33), (700, 5), (8192, 1)])
 @pytest.mark.parametrize("free", [10 ** 4, 7])
 def test_advance_in_rows(requests, row, free):

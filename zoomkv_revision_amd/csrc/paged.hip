@@ -21,7 +21,10 @@ namespace {
 // page tables
 // ---------------------------------------------------------------------------
 constexpr int kMaxRequests = 8192;      // the scans' LDS: 16 bytes a request
-constexpr int kFewRequests = 512;       // beyond: 1024 threads, so that one scans at most 8 requests
+// Beyond either: 1024 threads, so that one scans at most 8 requests, and fewer
+// workgroups that scan (500 mixed requests, 16384 slots 7.9 us, 8.0 with 1024;
+// 65536 slots 10.0, 8.4; 128 requests 6.6, 7.5 and 8.8, 8.0).
+constexpr int kFewRequests = 512, kFewSlots = 32768;
 constexpr uint32_t kGranted = 0x80000000u;
 
 struct AdvanceParams {
@@ -462,7 +465,7 @@ extern "C" int zkv_page_advance(const int32_t* seq_lens, const int32_t* new_toke
                         fast_div(static_cast<uint32_t>(page_size)),
                         row ? fast_div(static_cast<uint32_t>(row)) : FastDiv{0, 0, 0},
                         static_cast<int64_t>(width) * page_size};
-  const bool few = requests <= kFewRequests;
+  const bool few = requests <= kFewRequests && capacity <= kFewSlots;
   const size_t lds = static_cast<size_t>(requests) * 16;
   // dynamic LDS above 64 KiB has to be allowed (per device: the call is cheap)
   if (lds > 60 * 1024 &&
