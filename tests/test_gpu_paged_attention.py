@@ -217,6 +217,16 @@ def test_heads_of_a_token_together(lens, hq, kv, d, dtype, fp8):
     c.check(*c.attend(return_softmax_lse=True, window=window), window=window, requests=some)
 
 
+@pytest.mark.parametrize("hq,kv,d,dtype,fp8", [(64, 8, 64, BF, True), (8, 8, 128, BF, False), (96, 4, 256, FP, False)])
+@pytest.mark.parametrize("lens", [[66] * 235, [1 + 37 * i % 160 for i in range(250)],
+                                  [0, 1, 2, 33] * 40 + [4000] + [5, 0, 96] * 60])
+def test_many_short_units(hq, kv, d, dtype, fp8, lens):
+    """Several units a wave, long ones among them."""
+    c = Case(lens, hq, kv, d, 16, dtype, fp8, seed=len(lens) + d)
+    out, lse = c.attend(return_softmax_lse=True)
+    c.check(out, lse, requests=sorted({*range(0, len(lens), 9), *range(150, 170), len(lens) - 1}))
+
+
 @pytest.mark.parametrize("window", [1, 5, 32, 100, 512, 100000])
 @pytest.mark.parametrize("page", [16, 24])
 def test_windows(window, page):
