@@ -17,9 +17,10 @@
 // units that lie wholly in its run by itself; the ends of its run go to LDS as
 // partials (m, l, O) and are joined there; the ends of the workgroup's run go
 // to the workspace and are joined by the last of the workgroups that share the
-// unit (where these are many, by the last of each few first).  Each workgroup leaves at most two partials, whatever the batch is, and
-// which tiles are joined in which order depends on the lengths alone, so the
-// result is the same from run to run.
+// unit (where these are many, by the last of each few first).  Each workgroup
+// leaves at most two partials, whatever the batch is, and which tiles are joined
+// in which order depends on the lengths alone, so the result is the same from
+// run to run.
 //
 // Stream.  A wave walks its run as one stream of tiles across the units: a
 // ring of kDepth tiles in registers, the request running kDepth - 1 tiles (and
@@ -31,9 +32,10 @@
 //
 // Bound by HBM: 16 requests of 32768 tokens, 32 / 8 heads of 128, bf16 (2.1 GB):
 // 328 us, 6.5 TB/s; 64 requests of 1 to 8192 tokens 64 us (5.5 TB/s, behind
-// about 10 us of launch, first round trips and joins); 1 x 700 tokens 14.3 us,
-// a chain of round trips (lengths, page ids and q, three tiles a wave).
-// 1 x 131072 tokens: 91 us, 97 where the pool is laid out [page, token, head].
+// about 9 us of launch, first round trips and joins); 1 x 700 tokens 12.9 us, a
+// chain of round trips (lengths, page ids and q, a tile, the partials out and
+// back).  1 x 131072 tokens: 91 us, 96 where the pool is laid out [page, token,
+// head].
 //
 // Tile.  S^T = K q^T and O^T = V^T P^T on v_mfma_f32_16x16x32: K rows are the
 // A operand (lane 16 g + c: token c, channels 32 s + 8 g ..), q the B operand
