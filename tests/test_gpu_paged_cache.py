@@ -237,3 +237,21 @@ def test_flash_attn_compat_takes_a_block_table():
         flash_attn_with_kvcache_compat(q, k, v, block_table=table)
     with pytest.raises(ValueError):
         flash_attn_with_kvcache_compat(q, k, v, cache_seqlens=lens, block_table=table, n_splits=2)
+
+
+def test_the_capture_counts_as_the_first_replay():
+    lens = [40, 15, 31]
+    model, cache = _prompted(lens)
+    tok = torch.tensor([1, 2, 3], device=DEV)
+    model.decode_step(tok, cache)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        model.decode_step(tok, cache)
+    graph.replay()
+    assert cache.tables.seq_lens.tolist() == cache.lengths == [n + 2 for n in lens]
+    for _ in range(5):
+        graph.replay()
+    cache.replayed(5)
+    cache.check()
+    assert cache.tables.seq_lens.tolist() == cache.lengths == [n + 7 for n in lens] and cache.context == 47

@@ -563,7 +563,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   // both ends of the run, one a lane
   const int64_t y64 = (static_cast<int64_t>(blockIdx.x) + (lane & 1)) * chunk;
   int end = static_cast<int>(min(y64, static_cast<int64_t>(total)));
-  const bool small = 2 * kSmallUnit <= chunk && total <= kSmallUnit * p.bs * units;
+  const bool small = 2 * kSmallUnit <= chunk && total / kSmallUnit < p.bs * units;
   if (!sets && (chunk == kWaves || small) && y64 < total) {
     const int b = request_at(end, [&](int i) { return s_cum[i]; });
     const int size = s_cum[b + 1] - s_cum[b], in = (end - s_cum[b] * units) % size;

@@ -110,8 +110,8 @@ class paged_cache:
         self.tables.check()
 
     def replayed(self, steps: int = 1) -> None:
-        """Count `steps` replays of a captured decode step, each one more token
-        of every active row."""
+        """Count `steps` replays of a captured decode step beyond the first
+        (which the capture counted), each one more token of every active row."""
         for _ in range(steps):
             self._grow([1 if n else 0 for n in self.lengths])
             self.context += 1
