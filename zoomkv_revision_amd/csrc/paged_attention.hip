@@ -184,6 +184,17 @@ __device__ __forceinline__ float across_sum(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Running sum over the wave's lanes, this one's included.
+__device__ __forceinline__ int scan64(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // from 1, 2, 4, 8 lanes before, in a row of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // the last of the row before, to rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // the last of lane 31, to rows 2 and 3
+  return x;
+}
+
 // Device-coherent accesses of the partials: the sharing workgroups run on
 // different XCDs, whose L2s are not coherent.  16 bytes a lane go through a
 // buffer descriptor, whose accesses take the same coherence bit as an atomic of
@@ -495,36 +506,44 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
   const auto len_of = [&](int b) { return min(max(p.lens[b], 0), p.max_len); };
   const auto tile0_of = [&](int len) { return p.window > 0 ? max(0, len - p.window) / kTile : 0; };
   const auto tiles_of = [&](int len) { return (len + kTile - 1) / kTile - tile0_of(len); };
-  const int per = (p.bs + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.bs), b1 = min(b0 + per, p.bs);
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int n = tiles_of(len_of(b));
-    s_cum[b] = n ? n + kUnitCost : 0;
-    mine += s_cum[b];
+  const bool few = p.bs <= 64;
+  int ends = 0, total = 0;  // few requests: the places up to the lane's one's end
+  if (few) {
+    // every wave for itself, without a barrier (all write the same)
+    const int n = lane < p.bs ? tiles_of(len_of(lane)) : 0;
+    ends = scan64(n ? n + kUnitCost : 0);
+    if (lane < p.bs) s_cum[lane + 1] = ends;
+    if (lane == 0) s_cum[0] = 0, s_done[wave] = 0;
+    if (lane < kSlots / kWaves) s_unit[kSlots / kWaves * wave + lane] = -1;
+    total = __builtin_amdgcn_readlane(ends, 63);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  } else {
+    const int per = (p.bs + kThreads - 1) / kThreads;
+    const int b0 = min(tid * per, p.bs), b1 = min(b0 + per, p.bs);
+    int mine = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int n = tiles_of(len_of(b));
+      s_cum[b] = n ? n + kUnitCost : 0;
+      mine += s_cum[b];
+    }
+    const int scan = scan64(mine);
+    if (lane == 63) s_part[wave] = scan;
+    if (tid < kSlots) s_unit[tid] = -1;
+    if (tid < kWaves) s_done[tid] = 0;
+    __syncthreads();
+    int sum = scan - mine;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) sum += s_part[w];
+      total += s_part[w];
+    }
+    for (int b = b0; b < b1; ++b) {
+      const int n = s_cum[b];
+      s_cum[b] = sum;
+      sum += n;
+    }
+    if (tid == 0) s_cum[p.bs] = total;
+    __syncthreads();
   }
-  int scan = mine;
-#pragma unroll
-  for (int i = 1; i < 64; i <<= 1) {
-    const int u = __shfl_up(scan, i);
-    if (lane >= i) scan += u;
-  }
-  if (lane == 63) s_part[wave] = scan;
-  if (tid < kSlots) s_unit[tid] = -1;
-  if (tid < kWaves) s_done[tid] = 0;
-  __syncthreads();
-  int sum = scan - mine, total = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) sum += s_part[w];
-    total += s_part[w];
-  }
-  for (int b = b0; b < b1; ++b) {
-    const int n = s_cum[b];
-    s_cum[b] = sum;
-    sum += n;
-  }
-  if (tid == 0) s_cum[p.bs] = total;
-  __syncthreads();
   total = __builtin_amdgcn_readfirstlane(total);
   const int grid = static_cast<int>(gridDim.x);
   const bool sets = kSets && total * static_cast<int>(p.units.d) >= kSetPlaces * kWaves * grid;
@@ -652,7 +671,7 @@ __global__ __launch_bounds__((64 * Shape<kFp8, kD>::kWaves)) void paged_attentio
       }
       look_up();
     };
-    enter(request_at(x0, cum));
+    enter(few ? __builtin_popcountll(__ballot(ends <= static_cast<int>(div_by(x0, units_div)))) : request_at(x0, cum));
     {
       const int size = at.tiles + kUnitCost, from = x0 - cum(at.b) * units;
       at.rest = from / size;
