@@ -47,23 +47,44 @@ struct AdvanceParams {
 
 // Sum of two non-negative numbers up to a limit (associative, so a scan of
 // such sums is one of the true sums, limited).
-__device__ __forceinline__ int limited(int a, int b, int top) { return min(a + b, top); }
+__device__ __forceinline__ int limited(int a, int b, int top) {  // (two limits may pass 31 bits)
+  return static_cast<int>(min(static_cast<unsigned>(a) + static_cast<unsigned>(b), static_cast<unsigned>(top)));
+}
 
-// The limited sum of v over the threads before this one.
-__device__ __forceinline__ int scan_before(int v, int top, int* part) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o);
-    if (lane >= o) v = limited(v, u, top);
+// Running limited sum over the wave's lanes, this one's included (over rows of
+// 16 lanes only if !kAll).
+template <bool kAll>
+__device__ __forceinline__ int scan_lanes(int v, int top) {
+  v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false), top);  // from 1, 2, 4, 8 lanes before
+  v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false), top);
+  v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false), top);
+  v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false), top);
+  if constexpr (kAll) {
+    v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false), top);  // the last of the row before
+    v = limited(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false), top);  // the last of lane 31
   }
-  const int up = __shfl_up(v, 1);
-  if (lane == 63) part[wave] = v;
+  return v;
+}
+
+// The limited sums of kN values over the threads before this one, in one pass
+// (part: kN x 16, no two calls the same).
+template <int kN>
+__device__ __forceinline__ void scan_before(int (&v)[kN], int top, int (*part)[16]) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int up[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int sum = scan_lanes<true>(v[i], top);
+    up[i] = __builtin_amdgcn_update_dpp(0, sum, 0x138, 0xF, 0xF, false);  // of the lane before
+    if (lane == 63) part[i][wave] = sum;
+  }
   __syncthreads();
-  int before = lane ? up : 0;
-  for (int w = 0; w < wave; ++w) before = limited(before, part[w], top);
-  __syncthreads();  // part may be written again
-  return before;
+  const int waves = blockDim.x >> 6;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const int sums = scan_lanes<false>((lane & 15) < waves ? part[i][lane & 15] : 0, top);
+    v[i] = limited(up[i], wave ? __builtin_amdgcn_readlane(sums, wave - 1) : 0, top);
+  }
 }
 
 __device__ __forceinline__ int pages_of(uint32_t n, const FastDiv& page) {
@@ -106,7 +127,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
   int* s_tok = smem + R;                                // ends of the requests' tokens (rows: how many)
   int* s_need = s_tok + R;                              // ends of the pages they take
   int* s_give = s_need + R;                             // ends of the pages they give back
-  __shared__ int part[kThreads / 64];
+  __shared__ int part[3][16];
   __shared__ int s_status, s_taken, s_last;
   const int head = static_cast<int>(static_cast<uint32_t>(p.state[0]) % static_cast<uint32_t>(p.num_pages));
   const int count = min(max(p.state[1], 0), p.num_pages);
@@ -130,7 +151,11 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
   const int row = static_cast<int>(p.row.d);
   int sum = 0;
   for (int i = i0; i < i1; ++i) sum = limited(sum, min(max(s_tok[i], 0), tok_top), tok_top);
-  sum = scan_before(sum, tok_top, part);
+  {
+    int v[1] = {sum};
+    scan_before<1>(v, tok_top, part);
+    sum = v[0];
+  }
   int status = 0, need_sum = 0, give_sum = 0;
   for (int i = i0; i < i1; ++i) {
     const int len = static_cast<int>(s_len[i]), n = s_tok[i];
@@ -156,8 +181,11 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvancePar
     need_sum = limited(need_sum, max(need, 0), page_top);
     give_sum = limited(give_sum, give, page_top);
   }
-  need_sum = scan_before(need_sum, page_top, part);
-  give_sum = scan_before(give_sum, page_top, part);
+  {
+    int v[2] = {need_sum, give_sum};
+    scan_before<2>(v, page_top, part + 1);
+    need_sum = v[0], give_sum = v[1];
+  }
   int taken = 0;
   for (int i = i0; i < i1; ++i) {
     const int need = s_need[i];
