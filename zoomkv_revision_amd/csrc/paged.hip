@@ -21,10 +21,10 @@ namespace {
 // page tables
 // ---------------------------------------------------------------------------
 constexpr int kMaxRequests = 8192;      // the scans' LDS: 16 bytes a request
-// Beyond either: 1024 threads, so that one scans at most 8 requests, and fewer
-// workgroups that scan (500 mixed requests, 16384 slots 7.9 us, 8.0 with 1024;
-// 65536 slots 10.0, 8.4; 128 requests 6.6, 7.5 and 8.8, 8.0).
-constexpr int kFewRequests = 512, kFewSlots = 32768;
+// Beyond either: 1024 threads, so that one scans at most 8 requests and fewer
+// workgroups scan (decode steps of 100 requests 4.4 us, 4.9 with 1024 threads;
+// of 300 6.0, 5.1; 128 requests with 65536 slots 8.0, 5.9).
+constexpr int kFewRequests = 256, kFewSlots = 8192;
 constexpr uint32_t kGranted = 0x80000000u;
 
 struct AdvanceParams {
@@ -116,9 +116,8 @@ __device__ __forceinline__ int owner_of(const int* ends, int n, int x) {
 // writes.
 //
 // Bound by latency: one read of the batch, one LDS search and one dependent
-// read of a page id per token.  5 us for 64 requests of one token; 1024 mixed
-// requests with 65536 slots 9.0 us (12.2 with 256 threads a workgroup, whose
-// scans are four requests a thread), 8192 requests 22 us.
+// read of a page id per token.  4.9 us for 64 requests of one token; 1024 mixed
+// requests with 65536 slots 7.1 us, 8192 requests 20 us.
 template <int kThreads>
 __global__ __launch_bounds__(kThreads) void page_advance_kernel(const AdvanceParams p) {
   extern __shared__ int smem[];
