@@ -337,17 +337,19 @@ struct WriteParams {
   void* dst[2];
   const float* scale[2];   // one per head, or null for 1
   PageLayout layout;
-  FastDiv page, row_chunks;  // row_chunks: 16-byte chunks of a token's kv heads
+  FastDiv page, row_chunks;  // row_chunks: chunks (16-byte stores) of a token's kv heads
   int tokens, chunk_shift;   // 1 << chunk_shift chunks of one head's row
 };
 
-// One 16-byte chunk of a row per thread and trip, kWriteUnroll trips with
-// their loads requested together; consecutive threads take consecutive chunks
-// of a token's heads, so a wave reads 1 KiB and writes whole rows (256 bytes
-// at head dim 128).  Bound by HBM: each row is read and written once.  32768
-// tokens of 8 heads of 128: 39 us (6.9 TB/s read and written) in 16 bits, its
-// stores streamed (42 us otherwise), 38 us (5.2 TB/s) as e4m3, whose 8-byte
-// stores gain nothing by that; one trip 40 and 51 us, four 40 and 41.
+// A chunk of a row per thread and trip, the 8 or, as e4m3, 16 channels of a
+// 16-byte store; kWriteUnroll trips with their loads requested together;
+// consecutive threads take consecutive chunks of a token's heads, so a wave
+// writes 1 KiB of whole rows (256 bytes at head dim 128).  Bound by HBM: each
+// row is read and written once, the stores streamed.  32768 tokens of 8 heads
+// of 128: 39 us (6.9 TB/s read and written) in 16 bits (42 with stores that stay
+// in the cache, 40 with one trip or four), 34.6 us (5.7 TB/s; 38.7 where the
+// inputs change from call to call) as e4m3 (36.0 with plain stores, 36.6 with
+// one trip, 36.8 with four, 35.9 with 8 channels and 8-byte stores).
 constexpr int kWriteThreads = 256, kWriteUnroll = 2;
 
 template <int kType, bool kFp8>
@@ -355,7 +357,8 @@ __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(const WriteP
   const int which = blockIdx.y;
   const uint32_t n = static_cast<uint32_t>(p.tokens) * p.row_chunks.d;  // (< 2^31)
   const uint32_t first = blockIdx.x * (kWriteThreads * kWriteUnroll) + threadIdx.x;
-  u32x4_t x[kWriteUnroll];
+  constexpr int kLoads = kFp8 ? 2 : 1;  // 16-byte loads of a chunk
+  u32x4_t x[kWriteUnroll][kLoads];
   int64_t row[kWriteUnroll];
   float scale[kWriteUnroll];
   uint32_t ch[kWriteUnroll];
@@ -364,8 +367,10 @@ __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(const WriteP
     const uint32_t i = min(first + u * kWriteThreads, n - 1);
     const uint32_t t = div_by(i, p.row_chunks), c = i - t * p.row_chunks.d;
     const uint32_t h = c >> p.chunk_shift;
-    ch[u] = 8 * (c & ((1u << p.chunk_shift) - 1));
-    x[u] = *reinterpret_cast<const u32x4_t*>(p.src[which] + t * p.src_token[which] + h * p.src_head[which] + ch[u]);
+    ch[u] = 8 * kLoads * (c & ((1u << p.chunk_shift) - 1));
+    const uint16_t* src = p.src[which] + t * p.src_token[which] + h * p.src_head[which] + ch[u];
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) x[u][k] = reinterpret_cast<const u32x4_t*>(src)[k];
     row[u] = first + u * kWriteThreads < n ? slot_row(p.slots[t], p.layout, p.page, h) : -1;
     if constexpr (kFp8) scale[u] = p.scale[which] ? p.scale[which][h] : 1.0f;
   }
@@ -373,11 +378,18 @@ __global__ __launch_bounds__(kWriteThreads) void paged_write_kernel(const WriteP
   for (int u = 0; u < kWriteUnroll; ++u) {
     if (row[u] < 0) continue;
     if constexpr (kFp8) {
-      float y[8];
-      unpack8<kType>(x[u], y);
-      *reinterpret_cast<u32x2_t*>(static_cast<uint8_t*>(p.dst[which]) + row[u] + ch[u]) = quant8(y, Quotient(scale[u]));
+      const Quotient by(scale[u]);
+      u32x2_t r[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float y[8];
+        unpack8<kType>(x[u][k], y);
+        r[k] = quant8(y, by);
+      }
+      __builtin_nontemporal_store(u32x4_t{r[0][0], r[0][1], r[1][0], r[1][1]},
+                                  reinterpret_cast<u32x4_t*>(static_cast<uint8_t*>(p.dst[which]) + row[u] + ch[u]));
     } else {
-      __builtin_nontemporal_store(x[u], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p.dst[which]) + row[u] + ch[u]));
+      __builtin_nontemporal_store(x[u][0], reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(p.dst[which]) + row[u] + ch[u]));
     }
   }
 }
@@ -529,7 +541,8 @@ extern "C" int zkv_paged_write(const void* k, int64_t k_token, int64_t k_head, c
   ZKV_REQUIRE(static_cast<int64_t>(tokens) * kv * (d / 8) < (1ll << 31) - kWriteThreads * kWriteUnroll,
               "zkv_paged_write: %d tokens of %d heads in one call", tokens, kv);
   if (tokens == 0) return ZKV_OK;
-  const uint32_t chunks = static_cast<uint32_t>(kv) * (d / 8);
+  const int chunk = is_fp8 ? 16 : 8;  // channels that a thread takes
+  const uint32_t chunks = static_cast<uint32_t>(kv) * (d / chunk);
   const WriteParams p{{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v)},
                       {k_token, v_token},
                       {k_head, v_head},
@@ -540,7 +553,7 @@ extern "C" int zkv_paged_write(const void* k, int64_t k_token, int64_t k_head, c
                       fast_div(static_cast<uint32_t>(page_size)),
                       fast_div(chunks),
                       tokens,
-                      d == 64 ? 3 : (d == 128 ? 4 : 5)};
+                      (d == 64 ? 3 : (d == 128 ? 4 : 5)) - (is_fp8 ? 1 : 0)};
   const uint32_t n = static_cast<uint32_t>(tokens) * chunks;
   const dim3 grid((n + kWriteThreads * kWriteUnroll - 1) / (kWriteThreads * kWriteUnroll), 2);
   auto s = reinterpret_cast<hipStream_t>(stream);
