@@ -255,3 +255,26 @@ def test_the_capture_counts_as_the_first_replay():
     cache.replayed(5)
     cache.check()
     assert cache.tables.seq_lens.tolist() == cache.lengths == [n + 7 for n in lens] and cache.context == 47
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_a_step_beyond_the_rope_table_is_refused(fused):
+    """The model's RoPE table ends before the cache does: the step that would
+    need a row beyond is refused with the cache as it was, and goes on once the
+    long request has ended."""
+    model = ds.RandomQwen3(GEO, DEV, seed=7, max_position=66, fused=fused)
+    cache = ds.build_paged_cache(GEO, 2, 100, DEV)
+    zeros = torch.zeros(1, 64, 2, 128, dtype=BF, device=DEV)
+    for r, n in enumerate((64, 20)):
+        for layer in range(GEO.layers):
+            cache.prefill_update_kv_cache(None, zeros[:, :n], zeros[:, :n], layer, r)
+    tok = torch.tensor([1, 2], device=DEV)
+    for _ in range(2):
+        assert bool(torch.isfinite(model.decode_step(tok, cache)).all())
+    with pytest.raises(RuntimeError, match="position 66"):
+        model.decode_step(tok, cache)
+    assert cache.lengths == [66, 22] == cache.tables.seq_lens.tolist() and cache.context == 66
+    cache.release(0)
+    model.decode_step(tok, cache)
+    assert cache.lengths == [0, 23] == cache.tables.seq_lens.tolist()
+    cache.check()

@@ -197,7 +197,7 @@ class RandomQwen3:
         qkv = torch.empty(bs, qd + 2 * kd, dtype=torch.bfloat16, device=hidden.device)
         decode_linear(x, L["wqkv"], qkv, norm_w=L["input_ln"], eps=geo.eps)
         if _is_paged(cache):
-            cache.decode_begin(ldx)
+            cache.decode_begin(ldx, self.cos.shape[0])
             q = cache.decode_norm_rope(qkv, L["q_norm"], L["k_norm"], geo.eps, self.cos, self.sin, ldx)
         else:
             pos = cache.context
@@ -227,7 +227,7 @@ class RandomQwen3:
         k = rms_norm(k.reshape(bs, 1, geo.kv_heads, geo.head_dim), L["k_norm"], geo.eps)
         pos = cache.context
         if _is_paged(cache):
-            cache.decode_begin(ldx)
+            cache.decode_begin(ldx, self.cos.shape[0])
             pos = cache.positions.clamp(min=0).long()      # (idle rows: any)
         q, k = self._rope(q, pos), self._rope(k, pos)
         v = v.reshape(bs, 1, geo.kv_heads, geo.head_dim)

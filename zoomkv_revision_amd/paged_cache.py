@@ -73,6 +73,7 @@ class paged_cache:
         self.v_scale: list = [None] * layer_num
         self.context = 0
         self.lengths = [0] * batch_size          # tokens of each row, as the host has ordered them
+        self._max_positions: int | None = None   # rows of the RoPE table that the last decode step was given
         # one decode step: which rows get a token, and where it goes
         self.active = torch.zeros(batch_size, dtype=torch.int32, device=self.device)
         self.slots = torch.full((batch_size,), -1, dtype=torch.int64, device=self.device)
@@ -100,6 +101,12 @@ class paged_cache:
             raise RuntimeError(f"{held} pages needed, the pool has {self.num_pages}")
         self.lengths = after
 
+    def _refuse_positions(self, max_positions: int | None, length: int) -> None:
+        """A step whose longest row ends at `length` tokens rotates it at
+        position length - 1: that is to be a row of the RoPE table."""
+        if max_positions is not None and length > max_positions:
+            raise RuntimeError(f"position {length - 1} is beyond the RoPE table's {max_positions} rows")
+
     def _rows_tensor(self, values: list[int]) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32).to(self.device)
 
@@ -111,8 +118,11 @@ class paged_cache:
 
     def replayed(self, steps: int = 1) -> None:
         """Count `steps` replays of a captured decode step beyond the first
-        (which the capture counted), each one more token of every active row."""
+        (which the capture counted), each one more token of every active row;
+        refuses what the host can count, the pool and the captured step's RoPE
+        table among it: call it before the replays where they may run out."""
         for _ in range(steps):
+            self._refuse_positions(self._max_positions, max(n + 1 if n else 0 for n in self.lengths))
             self._grow([1 if n else 0 for n in self.lengths])
             self.context += 1
 
@@ -183,12 +193,17 @@ class paged_cache:
     # ------------------------------------------------------------------
     # decode
     # ------------------------------------------------------------------
-    def decode_begin(self, layer_idx) -> None:
+    def decode_begin(self, layer_idx, max_positions: int | None = None) -> None:
         """The bookkeeping of a decode step, without the write: at layer 0 every
         active row gets its next place (``positions`` int32 [bs], ``slots``
-        int64 [bs], -1 for idle rows), which serve all layers."""
+        int64 [bs], -1 for idle rows), which serve all layers.  max_positions:
+        the rows of the RoPE table that the step goes on with; a step (or a
+        replay of it) that needs a row beyond is refused before anything is
+        launched."""
         if layer_idx == 0:
+            self._refuse_positions(max_positions, max(n + 1 if n else 0 for n in self.lengths))
             self._grow([1 if n else 0 for n in self.lengths])
+            self._max_positions = max_positions
             self._step.run()
         if layer_idx == self.layer_num - 1:
             self.context += 1
@@ -209,7 +224,10 @@ class paged_cache:
     def decode_norm_rope(self, qkv, q_norm, k_norm, eps, cos, sin, layer_idx) -> torch.Tensor:
         """decode_write from the fused projection qkv [bs, (heads + 2 kv) d],
         with the q / k norms and RoPE at each row's position; the query heads
-        [bs, 1, heads, d] (idle rows 0)."""
+        [bs, 1, heads, d] (idle rows 0).  Refuses tables cos / sin that a row's
+        position lies beyond (its token would not be written)."""
+        self._refuse_positions(cos.shape[0], max(self.lengths))
+        self._max_positions = cos.shape[0]
         q = torch.zeros(self.batch_size, 1, self.num_heads, self.head_dim, dtype=self.dtype, device=self.device)
         return paged.paged_qk_norm_rope(qkv, self.num_heads, self.kv_head, q_norm, k_norm, eps, cos, sin,
                                         self.positions, self.slots, q, self.k_pages[layer_idx],
