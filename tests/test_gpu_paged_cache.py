@@ -278,3 +278,23 @@ def test_a_step_beyond_the_rope_table_is_refused(fused):
     model.decode_step(tok, cache)
     assert cache.lengths == [0, 23] == cache.tables.seq_lens.tolist()
     cache.check()
+
+
+def test_a_refused_prompt_leaves_the_running_request():
+    """A prompt for a row that holds a request, too long for the pool or for
+    max_length: the request goes on, its attention bit for bit."""
+    c = _cache(layers=1, num_pages=12, max_length=80)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    new = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF)
+    for r, n in ((0, 40), (2, 33)):
+        c.prefill_update_kv_cache(None, new(1, n, 2, 128), new(1, n, 2, 128), 0, r)
+    q = new(3, 1, 4, 128)
+    before = [x.clone() for x in (c.compute(q, 0), c.tables.seq_lens, c.tables.block_table, c.tables.state, c.active)]
+    for n, why in ((81, "max_length"), (64, "pages")):
+        with pytest.raises(RuntimeError, match=why):
+            c.prefill_update_kv_cache(None, new(1, n, 2, 128), new(1, n, 2, 128), 0, 0)
+    after = c.compute(q, 0), c.tables.seq_lens, c.tables.block_table, c.tables.state, c.active
+    assert all(torch.equal(a, b) for a, b in zip(after, before)) and c.lengths == [40, 0, 33]
+    c.prefill_update_kv_cache(None, new(1, 56, 2, 128), new(1, 56, 2, 128), 0, 0)    # all the pages the other leaves
+    assert c.lengths == [56, 0, 33] == c.tables.seq_lens.tolist()
+    c.check()

@@ -126,3 +126,33 @@ def test_replays_beyond_the_rope_table_are_refused(make):
     other.decode_begin(0)             # rotated by the caller: no table to run out of
     other.replayed(20)
     assert other.lengths == [0, 24, 0]
+
+
+# ---------------------------------------------------------------------------
+# prompts that are refused
+# ---------------------------------------------------------------------------
+def test_a_refused_prompt_leaves_the_running_request(make):
+    c = make(pages=12, max_length=40)
+    _prefill(c, 0, 20)                # 5 pages
+    _prefill(c, 1, 17)                # 5 pages
+    before = _state(c)
+    c.launched.clear()
+    rows = lambda n, b=1: [torch.zeros(b, n, 1, 64, dtype=BF) for _ in range(2)]
+    with pytest.raises(RuntimeError, match="max_length"):
+        c.prefill_update_kv_cache(None, *rows(41), 0, 0)
+    with pytest.raises(RuntimeError, match="pages"):
+        c.prefill_update_kv_cache(None, *rows(29), 0, 0)          # 8 pages with 5 held by the other row
+    with pytest.raises(RuntimeError, match="pages"):
+        c.prefill_update_kv_cache(None, *rows(20, 3), 0, 0)
+    with pytest.raises(ValueError, match="not on cpu"):
+        c.prefill_update_kv_cache(None, *(x.to("meta") for x in rows(4)), 0, 0)
+    with pytest.raises(IndexError):
+        c.prefill_update_kv_cache(None, *rows(4), 0, 3)
+    assert _state(c) == before and not c.launched
+    _prefill(c, 0, 28)                # 7 pages: the row's own 5 and the 2 that were free
+    assert c.lengths == [28, 17, 0] == c.tables.seq_lens.tolist() and int(c.tables.state[1]) == 0
+    assert int(c.tables.state[2]) == 0
+    c.release([0, 1])
+    for layer in range(2):
+        c.prefill_update_kv_cache(None, *rows(16, 3), layer, 0)
+    assert c.lengths == [16, 16, 16] == c.tables.seq_lens.tolist()

@@ -88,18 +88,22 @@ class paged_cache:
     def _pages(self, n: int) -> int:
         return -(-n // self.page_size)
 
-    def _grow(self, new: list[int]) -> None:
-        """The host's count of the rows after a step; refuses one that does
-        not fit before anything is launched (tables.check() has the device's
-        word, for steps that were replayed)."""
-        after = [n + max(x, -n) for n, x in zip(self.lengths, new)]
+    def _fitted(self, lengths: list[int], new: list[int]) -> list[int]:
+        """Rows of these lengths after a step; refuses one that does not fit."""
+        after = [n + max(x, -n) for n, x in zip(lengths, new)]
         # pages that this step gives back serve later steps
-        held = sum(self._pages(max(a, b)) for a, b in zip(after, self.lengths))
+        held = sum(self._pages(max(a, b)) for a, b in zip(after, lengths))
         if max(after) > self.max_length:
             raise RuntimeError(f"a request of {max(after)} tokens exceeds max_length {self.max_length}")
         if held > self.num_pages:
             raise RuntimeError(f"{held} pages needed, the pool has {self.num_pages}")
-        self.lengths = after
+        return after
+
+    def _grow(self, new: list[int]) -> None:
+        """The host's count of the rows after a step; refuses one that does
+        not fit before anything is launched (tables.check() has the device's
+        word, for steps that were replayed)."""
+        self.lengths = self._fitted(self.lengths, new)
 
     def _refuse_positions(self, max_positions: int | None, length: int) -> None:
         """A step whose longest row ends at `length` tokens rotates it at
@@ -144,17 +148,20 @@ class paged_cache:
         """key_states / value_states [bsz, seq_len, kv, d], left-padded by
         valid_start; bsz == 1 writes row batch_idx, bsz == batch_size writes
         all rows (on batch_idx 0), each with its own valid_start.  Layer 0 comes
-        first and makes the pages (a row that holds a request is released).
-        Returns the inputs without the padding that all rows share."""
+        first and makes the pages (a row that holds a request is released; a
+        prompt that is refused leaves it running).  Returns the inputs without
+        the padding that all rows share."""
         del query_states
         bsz, seq = key_states.shape[:2]
         if key_states.shape != value_states.shape or tuple(key_states.shape[2:]) != (self.kv_head, self.head_dim):
             raise ValueError(f"keys / values must be [bsz, seq, {self.kv_head}, {self.head_dim}]; got "
                              f"{tuple(key_states.shape)}, {tuple(value_states.shape)}")
+        if key_states.device != self.device or value_states.device != self.device:
+            raise ValueError(f"keys / values are on {key_states.device}, {value_states.device}, not on {self.device}")
         if bsz != 1 and bsz != self.batch_size:
             raise ValueError(f"bsz ({bsz}) must be 1 or the cache batch_size ({self.batch_size})")
         start = lambda r: int(self.valid_start[r]) if hasattr(self.valid_start, "__len__") else int(self.valid_start)
-        rows = [batch_idx] if bsz == 1 else list(range(bsz))
+        rows = [range(self.batch_size)[batch_idx]] if bsz == 1 else list(range(bsz))
         starts = [start(r) for r in rows]
         if any(not 0 <= s <= seq for s in starts):
             raise ValueError(f"valid_start {starts} outside [0, {seq}]")
@@ -163,13 +170,14 @@ class paged_cache:
             return key_states[:, shared:], value_states[:, shared:]
         key = (bsz, rows[0])
         if layer_idx == 0:
-            if any(self.lengths[r] for r in rows):
-                self.release([r for r in rows if self.lengths[r]])
             new = [0] * self.batch_size
             for r, s in zip(rows, starts):
                 new[r] = seq - s
-            self._grow(new)
+            self._fitted([0 if r in rows else n for r, n in enumerate(self.lengths)], new)
             slots = torch.empty(self.batch_size * seq if bsz > 1 else seq, dtype=torch.int64, device=self.device)
+            if any(self.lengths[r] for r in rows):
+                self.release([r for r in rows if self.lengths[r]])
+            self._grow(new)
             paged.page_advance(self.tables, self._rows_tensor(new), slots, row=seq if bsz > 1 else 0)
             if bsz == 1:          # (packed: the row's tokens from place 0 on; its padding has no slot)
                 slots = torch.cat((slots.new_full((starts[0],), -1), slots[:seq - starts[0]]))
