@@ -541,3 +541,41 @@ def test_a_serving_loop(dtype, fp8):
                 ref, _, mass = op.attention(q[r, 0, 3 * h:3 * h + 3].double().cpu().numpy(), *rows, d ** -0.5)
                 err = np.abs(out[r, 0, 3 * h:3 * h + 3].double().cpu().numpy() - ref)
                 assert (err <= U[dtype] * np.abs(ref) + mass * 2.0 ** -12).all()
+
+
+def test_plans_and_captures_in_any_order():
+    """Captures begun on a side stream right behind the making of the plan, a
+    plan made inside a capture, eager runs of either before and after replays."""
+    c = Case([9000, 7, 0, 1500], 8, 2, 128, 16, seed=43)
+    want, want_lse = c.attend(return_softmax_lse=True)
+    nbytes = lib().zkv_paged_attention_workspace_size(128)
+    torch.full((nbytes,), 255, dtype=torch.uint8, device=DEV)       # (freed: what torch.empty may find)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs, plans = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    plans.append(paged.PagedAttentionPlan(c.q, c.k, c.v, c.table, c.lens, return_softmax_lse=True))
+    for i, g in enumerate(graphs):
+        with torch.cuda.stream(side):
+            g.capture_begin()
+            if i == 1:
+                plans.append(paged.PagedAttentionPlan(c.q, c.k, c.v, c.table, c.lens, return_softmax_lse=True))
+            plans[i].run()
+            g.capture_end()
+
+    def same(plan):
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(plan.out[0], want) and torch.equal(plan.out[1], want_lse)
+        for x in plan.out:
+            x.fill_(9.0)
+        torch.cuda.synchronize()
+
+    plans[1].run()                                # eager, before the graph it was made in has run
+    same(plans[1])
+    for _ in range(3):
+        for g, plan in zip(graphs, plans):
+            with torch.cuda.stream(side):
+                g.replay()
+            same(plan)
+            plan.run()
+            same(plan)

@@ -48,12 +48,21 @@ _WS: dict = {}
 _ARRIVAL_BYTES = 1024        # of an attention workspace (ZKV_PAGED_ARRIVAL_BYTES)
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the current stream of `device`, which need not be the current
+    device, is being captured."""
+    if torch.cuda.current_device() == device.index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Arrival counts and partials per (device, stream); under graph capture a
     buffer of the graph's own, so that two graphs never share one (its counts
     are then cleared in the graph, a launch more: a plan, or a workspace that
     is passed in, saves it)."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(device):
         return new_workspace(device, nbytes)
     key = (device, device_stream(device))
     ws = _WS.get(key)
@@ -65,7 +74,8 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
 def new_workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """A workspace for paged_attention (zkv_paged_attention_workspace_size(d)
     bytes).  The arrival counts, at the front, are 0 between calls; the partials
-    behind them need no clearing."""
+    behind them need no clearing.  It is cleared on the current stream: order
+    the calls of another stream behind it."""
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     ws[:_ARRIVAL_BYTES].zero_()
     return ws
@@ -442,29 +452,32 @@ def _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, w
 class PagedAttentionPlan(_Plan):
     """``paged_attention`` with its checks done once for fixed buffers (a
     decode loop: new query, lengths, table entries and pages in the same
-    tensors).  A plan has a workspace of its own unless one is given; runs of
-    one plan must not overlap on the device."""
+    tensors).  A plan has a workspace of its own unless one is given, ready for
+    any stream and any capture once the plan is made (which waits for its
+    clearing); runs of one plan must not overlap on the device."""
 
     def __init__(self, q, k_pages, v_pages, block_table, seq_lens, softmax_scale=None, window=0, k_scale=None,
                  v_scale=None, return_softmax_lse=False, out=None, workspace=None):
-        self._cleared = None
+        self._counts = None       # arrival counts that no run has cleared yet
         if workspace is None and q.is_cuda and q.shape[-1] in HEAD_DIMS:
-            workspace = new_workspace(q.device, lib().zkv_paged_attention_workspace_size(q.shape[-1]))
-            if not torch.cuda.is_current_stream_capturing():
-                stream = torch.cuda.current_stream(q.device)
-                self._cleared = (stream.cuda_stream, stream.record_event())
+            nbytes = lib().zkv_paged_attention_workspace_size(q.shape[-1])
+            if _capturing(q.device):
+                # nothing runs here: each captured run clears the counts in its
+                # graph, and so does the first eager one, whichever comes first
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+                self._counts = workspace[:_ARRIVAL_BYTES]
+            else:
+                workspace = new_workspace(q.device, nbytes)
+                torch.cuda.current_stream(q.device).synchronize()
         args, result, keep = _attention_args(q, k_pages, v_pages, block_table, seq_lens, softmax_scale, window, k_scale,
                                              v_scale, return_softmax_lse, out, workspace, copies=False)
         super().__init__(lib().zkv_paged_attention, q.device, args, result, keep)
 
     def run(self):
-        if self._cleared is not None:
-            # the plan's own workspace was cleared on the stream it was made on
-            # (a capture starts after a synchronisation)
-            made_on, event = self._cleared
-            if device_stream(self._device) != made_on and not torch.cuda.is_current_stream_capturing():
-                torch.cuda.current_stream(self._device).wait_event(event)
-            self._cleared = None
+        if self._counts is not None:
+            self._counts.zero_()
+            if not _capturing(self._device):
+                self._counts = None
         return super().run()
 
 
