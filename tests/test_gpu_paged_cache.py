@@ -298,3 +298,22 @@ def test_a_refused_prompt_leaves_the_running_request():
     c.prefill_update_kv_cache(None, new(1, 56, 2, 128), new(1, 56, 2, 128), 0, 0)    # all the pages the other leaves
     assert c.lengths == [56, 0, 33] == c.tables.seq_lens.tolist()
     c.check()
+
+
+def test_a_new_cache_is_ready_for_any_stream():
+    """Made behind a queue of work on one stream and used on another at once."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    k, v, q = (torch.randn(*s, generator=g, device=DEV).to(BF) for s in ((1, 5000, 2, 128), (1, 5000, 2, 128), (3, 1, 4, 128)))
+    outs = []
+    side, busy = torch.cuda.Stream(), torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    for stream in (torch.cuda.current_stream(), side):
+        for _ in range(20):
+            busy = busy @ busy * 1e-3
+        c = _cache(layers=1, max_length=5100)
+        with torch.cuda.stream(stream):
+            c.prefill_update_kv_cache(None, k, v, 0, 1)
+            outs.append(c.compute(q, 0))
+        torch.cuda.synchronize()
+        c.check()
+    assert torch.equal(*outs) and not outs[0][[0, 2]].any() and bool(outs[0][1].any())

@@ -32,7 +32,12 @@ class paged_cache:
     ``page_size`` tokens a page, ``num_pages`` pages a layer (default: enough
     for every row at ``max_length``), ``kv_dtype`` the cells' type (default
     ``dtype``; torch.float8_e4m3fn stores 8 bits, with ``k_scale[layer]`` /
-    ``v_scale[layer]`` float32 [kv] once they are set, else 1)."""
+    ``v_scale[layer]`` float32 [kv] once they are set, else 1).
+
+    Its calls share one set of tables, slots and positions and one workspace:
+    calls on several streams, and replays beside eager calls, are to be ordered
+    one behind the other by the caller.  A cache is ready for any stream once it
+    is made."""
 
     def __init__(self, valid_start, layer_num: int, batch_size: int, max_length: int, num_key_value_heads: int,
                  num_heads: int, head_dim: int, dtype: torch.dtype, layer_mapping: dict, max_new_length: int,
@@ -81,6 +86,7 @@ class paged_cache:
         self._step = paged.PageAdvancePlan(self.tables, self.active, self.slots, self.positions, row=1)
         self._prompt_slots: dict = {}
         self._workspace = paged.new_workspace(self.device, lib().zkv_paged_attention_workspace_size(head_dim))
+        torch.cuda.current_stream(self.device).synchronize()    # the buffers are filled, whatever stream comes first
 
     # ------------------------------------------------------------------
     # bookkeeping
