@@ -144,3 +144,21 @@ def test_production_env_matches_reference_runner(monkeypatch):
     assert os.environ["POLAR_QUEST_DYNAMIC_CAND_RATIOS"] == "0.7,0.5,0.4"
     assert os.environ["POLAR_CDS_DENSE_RATIO"] == "0.3"
     assert ds.PRODUCTION_CACHE_KNOBS["final_topk"] == 100
+
+
+@pytest.mark.parametrize("rows", [17, 40])
+def test_projections_of_more_rows_than_the_kernel_takes(rows):
+    g = torch.Generator().manual_seed(rows)
+    new = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)
+    x, w, norm_w, res = new(rows, 64), new(96, 64) * 0.1, new(64), new(rows, 96)
+    f = lambda t: t.double()
+    normed = f(ds.rms_norm(x, norm_w, 1e-6))
+    plain, wide = f(x) @ f(w).T, normed @ f(w).T
+    near = lambda got, ref, steps: bool(((f(got) - ref).abs() <= steps * 2.0 ** -8 * ref.abs() + 2.0 ** -6).all())
+    out = torch.empty(rows, 96, dtype=torch.bfloat16)
+    assert ds._layer_linear(x, w, out) is out and near(out, plain, 2)
+    assert near(ds._layer_linear(x, w, torch.empty(rows, 96, dtype=torch.float32), norm_w=norm_w, eps=1e-6), wide, 2)
+    assert near(ds._layer_linear(x, w, out, residual=res), plain + f(res), 2)
+    half = torch.empty(rows, 48, dtype=torch.bfloat16)
+    gate, up = wide[:, :48], wide[:, 48:]
+    assert near(ds._layer_linear(x, w, half, norm_w=norm_w, eps=1e-6, silu_mul=True), gate * torch.sigmoid(gate) * up, 8)

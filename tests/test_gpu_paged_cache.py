@@ -317,3 +317,36 @@ def test_a_new_cache_is_ready_for_any_stream():
         torch.cuda.synchronize()
         c.check()
     assert torch.equal(*outs) and not outs[0][[0, 2]].any() and bool(outs[0][1].any())
+
+
+@pytest.mark.parametrize("rows", [16, 17, 70])
+def test_wide_batches_decode(rows):
+    """The most rows that decode_linear takes and more: the fused step against the
+    torch layer, within the bound of test_decode_step_equals_the_torch_layer, and
+    replayed from a graph bit for bit."""
+    lens = [1 + 37 * r % 300 for r in range(rows)]
+    model, fused = _prompted(lens, idle=(3,))
+    _, plain = _prompted(lens, idle=(3,))
+    _, replayed = _prompted(lens, idle=(3,))
+    tok = torch.arange(rows, device=DEV) * 13 % GEO.vocab
+    keep = [r for r in range(rows) if r != 3]
+    model.decode_step(tok, replayed)                   # warm-up: a step of its own
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = model.decode_step(tok, replayed)
+    steps = []
+    for step in range(5):
+        model.fused = True
+        steps.append(model.decode_step(tok, fused))
+        model.fused = False
+        want = model.decode_step(tok, plain)
+        unit = want.abs().amax(-1, keepdim=True) * 2.0 ** -7
+        assert bool(((steps[-1] - want).abs() <= 8 * unit)[keep].all()), step
+        if step:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(logits[keep], steps[-1][keep]), step
+    assert fused.lengths == plain.lengths == [0 if r == 3 else n + 5 for r, n in enumerate(lens)]
+    assert torch.equal(fused.tables.seq_lens, replayed.tables.seq_lens)
+    fused.check()

@@ -75,6 +75,9 @@ class Qwen3Geometry:
     eps: float = 1.0e-6
 
 
+LINEAR_ROWS = 16    # of a decode batch that decode_linear takes
+
+
 def decode_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, norm_w: torch.Tensor | None = None,
                   eps: float = 0.0, residual: torch.Tensor | None = None, silu_mul: bool = False) -> torch.Tensor:
     """out = [silu * up of] [rmsnorm(x) of] x @ w.T [+ residual] on the GPU
@@ -95,6 +98,22 @@ def decode_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, norm_w: t
                                   0 if residual is None else residual.stride(0), out.data_ptr(), out.stride(0),
                                   int(out.dtype == torch.float32), epi, stream_of(out)))
     return out
+
+
+def _layer_linear(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor, norm_w: torch.Tensor | None = None,
+                  eps: float = 0.0, residual: torch.Tensor | None = None, silu_mul: bool = False) -> torch.Tensor:
+    """decode_linear, and for batches of more rows than it takes the same step
+    around the library's matrix product, each result rounded to bf16 as in
+    layer_decode_torch."""
+    if x.shape[0] <= LINEAR_ROWS:
+        return decode_linear(x, w, out, norm_w, eps, residual, silu_mul)
+    y = F.linear(x if norm_w is None else rms_norm(x, norm_w, eps), w)
+    if silu_mul:
+        gate, up = y.chunk(2, dim=-1)
+        y = F.silu(gate) * up
+    elif residual is not None:
+        y = residual + y
+    return out.copy_(y)
 
 
 def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor,
@@ -189,13 +208,14 @@ class RandomQwen3:
         return self.layer_decode_torch(ldx, hidden, cache)
 
     def layer_decode_fused(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
-        """layer_decode in five kernels around cache.compute (see the module docstring)."""
+        """layer_decode in five kernels around cache.compute (see the module
+        docstring); beyond 16 rows the projections are the library's."""
         geo, L = self.geo, self.layers[ldx]
         bs = hidden.shape[0]
         qd, kd = geo.heads * geo.head_dim, geo.kv_heads * geo.head_dim
         x = hidden.reshape(bs, geo.hidden)
         qkv = torch.empty(bs, qd + 2 * kd, dtype=torch.bfloat16, device=hidden.device)
-        decode_linear(x, L["wqkv"], qkv, norm_w=L["input_ln"], eps=geo.eps)
+        _layer_linear(x, L["wqkv"], qkv, norm_w=L["input_ln"], eps=geo.eps)
         if _is_paged(cache):
             cache.decode_begin(ldx, self.cos.shape[0])
             q = cache.decode_norm_rope(qkv, L["q_norm"], L["k_norm"], geo.eps, self.cos, self.sin, ldx)
@@ -207,11 +227,11 @@ class RandomQwen3:
                          self.sin[pos], q, cache.unified_keys[ldx][:, :, row], cache.unified_values[ldx][:, :, row])
         attn = cache.compute(q, ldx)                                   # [bs, 1, heads, 128]
         h1 = torch.empty(bs, geo.hidden, dtype=torch.bfloat16, device=hidden.device)
-        decode_linear(attn.reshape(bs, qd), L["wo"], h1, residual=x)
+        _layer_linear(attn.reshape(bs, qd), L["wo"], h1, residual=x)
         act = torch.empty(bs, geo.ffn, dtype=torch.bfloat16, device=hidden.device)
-        decode_linear(h1, L["gate_up"], act, norm_w=L["post_ln"], eps=geo.eps, silu_mul=True)
+        _layer_linear(h1, L["gate_up"], act, norm_w=L["post_ln"], eps=geo.eps, silu_mul=True)
         h2 = torch.empty(bs, geo.hidden, dtype=torch.bfloat16, device=hidden.device)
-        decode_linear(act, L["down"], h2, residual=h1)
+        _layer_linear(act, L["down"], h2, residual=h1)
         return h2.view(bs, 1, geo.hidden)
 
     def layer_decode_torch(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
@@ -251,7 +271,7 @@ class RandomQwen3:
         if hidden.is_cuda and self.fused:
             bs = hidden.shape[0]
             logits = torch.empty(bs, self.geo.vocab, dtype=torch.float32, device=hidden.device)
-            return decode_linear(hidden.reshape(bs, self.geo.hidden), self.embed, logits, norm_w=self.final_norm,
+            return _layer_linear(hidden.reshape(bs, self.geo.hidden), self.embed, logits, norm_w=self.final_norm,
                                  eps=self.geo.eps)
         hidden = rms_norm(hidden, self.final_norm, self.geo.eps)
         return F.linear(hidden[:, 0], self.embed).float()
@@ -430,7 +450,9 @@ def build_paged_cache(geo: Qwen3Geometry, batch: int, max_tokens: int, device, p
                       num_pages: int | None = None, kv_dtype: torch.dtype | None = None):
     """paged_cache for `batch` requests of up to max_tokens tokens each, over a
     pool of num_pages pages (default: enough for all of them at once); kv_dtype
-    torch.float8_e4m3fn keeps K and V in 8 bits."""
+    torch.float8_e4m3fn keeps K and V in 8 bits.  Batches of any size decode:
+    up to LINEAR_ROWS rows the projections are decode_linear's, beyond the
+    library's."""
     from .paged_cache import paged_cache
     return paged_cache(valid_start=[0] * batch, layer_num=geo.layers, batch_size=batch, max_length=max_tokens,
                        num_key_value_heads=geo.kv_heads, num_heads=geo.heads, head_dim=geo.head_dim,
