@@ -156,3 +156,32 @@ def test_a_refused_prompt_leaves_the_running_request(make):
     for layer in range(2):
         c.prefill_update_kv_cache(None, *rows(16, 3), layer, 0)
     assert c.lengths == [16, 16, 16] == c.tables.seq_lens.tolist()
+
+
+# ---------------------------------------------------------------------------
+# prompts on their way
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("batch", [False, True])
+def test_a_prompt_whose_row_is_released_writes_no_more(make, batch):
+    """Its pages may be another request's by the time of its next layer."""
+    c = make(pages=12)
+    rows = lambda n: [torch.zeros(3 if batch else 1, n, 1, 64, dtype=BF) for _ in range(2)]
+    at = 0 if batch else 1
+    c.prefill_update_kv_cache(None, *rows(8), 0, at)
+    c.release(1)
+    _prefill(c, 1 if batch else 2, 16)  # a request that takes the row, or another that takes the pages
+    c.launched.clear()
+    with pytest.raises(RuntimeError, match="without layer 0"):
+        c.prefill_update_kv_cache(None, *rows(8), 1, at)
+    assert not c.launched
+
+
+def test_a_prompt_on_its_way_does_not_mind_another_row(make):
+    c = make(pages=12)
+    rows = lambda n: [torch.zeros(1, n, 1, 64, dtype=BF) for _ in range(2)]
+    _prefill(c, 0, 5)
+    c.prefill_update_kv_cache(None, *rows(8), 0, 1)
+    c.release(0)
+    _prefill(c, 2, 16)
+    c.prefill_update_kv_cache(None, *rows(8), 1, 1)
+    assert c.lengths == [0, 8, 16] and not c._prompt_slots

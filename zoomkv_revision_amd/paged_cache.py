@@ -138,12 +138,16 @@ class paged_cache:
 
     def release(self, rows) -> None:
         """End the requests of these rows: their pages serve later steps, the
-        rows are idle until a prefill gives them a request."""
+        rows are idle until a prefill gives them a request (one that has not
+        reached its last layer ends with them)."""
         rows = [int(r) for r in ([rows] if isinstance(rows, int) else rows)]
         if any(not 0 <= r < self.batch_size for r in rows):
             raise ValueError(f"rows {rows} outside [0, {self.batch_size})")
         new = [-n if r in rows else 0 for r, n in enumerate(self.lengths)]
         self._grow(new)
+        # the slots of a prompt on its way may be another request's from now on
+        self._prompt_slots = {(bsz, r): slots for (bsz, r), slots in self._prompt_slots.items()
+                              if not any(r <= x < r + bsz for x in rows)}
         paged.page_advance(self.tables, self._rows_tensor(new))
         self.active.copy_(self._rows_tensor([int(n > 0) for n in self.lengths]))
 
