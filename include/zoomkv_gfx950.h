@@ -686,7 +686,8 @@ int zkv_paged_qk_norm_rope(const void* qkv, int64_t qkv_stride, int rows, int hq
  * (nullable) fp32 [bs, hq], natural log.  Lengths are read on the device and
  * limited to [0, width * page_size]; tokens on a page id outside the pool are
  * left out; a request without a token gives zeros and -inf.  At most 4096
- * requests; the rows of a pool start within 64 GiB.  workspace: zkv_paged_attention_workspace_size(d) bytes, its first
+ * requests; the rows of a pool start within 64 GiB.  workspace:
+ * zkv_paged_attention_workspace_size(d) bytes, its first
  * ZKV_PAGED_ARRIVAL_BYTES zero before the first call (every call leaves them
  * zero; one workspace serves every d it is large enough for); calls that
  * overlap on one workspace race. */

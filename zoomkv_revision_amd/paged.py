@@ -270,7 +270,8 @@ def page_advance(tables: PageTables, new_tokens: torch.Tensor, slots: torch.Tens
     row > 0 each request's at the end of its row of that many (capacity =
     requests * row: a left-padded batch; 1: a decode batch with idle rows), -1
     for those of a request that was not served and where there is no token;
-    starts int32 [requests + 1] (packed only) the running sum of the new tokens.
+    starts int32 [requests + 1] (packed only) the running sum of the new tokens,
+    at most capacity + 1.
     seq_lens and state are updated in place unless lens_out / state_out are
     given.  Returns (slots, positions)."""
     return PageAdvancePlan(tables, new_tokens, slots, positions, starts, lens_out, state_out, row).run()
