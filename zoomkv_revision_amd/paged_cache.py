@@ -143,7 +143,9 @@ class paged_cache:
         rows = [int(r) for r in ([rows] if isinstance(rows, int) else rows)]
         if any(not 0 <= r < self.batch_size for r in rows):
             raise ValueError(f"rows {rows} outside [0, {self.batch_size})")
-        new = [-n if r in rows else 0 for r, n in enumerate(self.lengths)]
+        new = [0] * self.batch_size
+        for r in rows:
+            new[r] = -self.lengths[r]
         self._grow(new)
         # the slots of a prompt on its way may be another request's from now on
         self._prompt_slots = {(bsz, r): slots for (bsz, r), slots in self._prompt_slots.items()
@@ -180,10 +182,10 @@ class paged_cache:
             return key_states[:, shared:], value_states[:, shared:]
         key = (bsz, rows[0])
         if layer_idx == 0:
-            new = [0] * self.batch_size
+            new, others = [0] * self.batch_size, self.lengths[:]
             for r, s in zip(rows, starts):
-                new[r] = seq - s
-            self._fitted([0 if r in rows else n for r, n in enumerate(self.lengths)], new)
+                new[r], others[r] = seq - s, 0
+            self._fitted(others, new)
             slots = torch.empty(self.batch_size * seq if bsz > 1 else seq, dtype=torch.int64, device=self.device)
             if any(self.lengths[r] for r in rows):
                 self.release([r for r in rows if self.lengths[r]])
@@ -244,8 +246,9 @@ class paged_cache:
         with the q / k norms and RoPE at each row's position; the query heads
         [bs, 1, heads, d] (idle rows 0).  Refuses tables cos / sin that a row's
         position lies beyond (its token would not be written)."""
-        self._refuse_positions(cos.shape[0], max(self.lengths))
-        self._max_positions = cos.shape[0]
+        if cos.shape[0] != self._max_positions:      # (else decode_begin or the layer before has looked)
+            self._refuse_positions(cos.shape[0], max(self.lengths))
+            self._max_positions = cos.shape[0]
         q = torch.zeros(self.batch_size, 1, self.num_heads, self.head_dim, dtype=self.dtype, device=self.device)
         return paged.paged_qk_norm_rope(qkv, self.num_heads, self.kv_head, q_norm, k_norm, eps, cos, sin,
                                         self.positions, self.slots, q, self.k_pages[layer_idx],
