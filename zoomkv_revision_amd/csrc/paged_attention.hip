@@ -55,7 +55,9 @@
 // at least its last place, and where the first may be 0 such V are taken out and
 // multiplied apart.  The second part's own product takes 0 to 1.5% of a call
 // in fp16 against one sum for both parts, which held 2^-31 of the largest weight,
-// 3% at head dim 256 (16 requests of 8192 tokens, 16 / 4 heads: 91.7 us, 88.9).
+// 3% at head dim 256 (16 requests of 8192 tokens, 16 / 4 heads: 91.7 us, 88.9);
+// with scores so far apart that V is looked through in every tile 0.3 to 3.5%, 9%
+// at head dim 256.
 #include "paged_common.hpp"
 
 #include <algorithm>
