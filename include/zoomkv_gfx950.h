@@ -700,6 +700,47 @@ int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, c
                         int hq, int kv, int d, float sm_scale, int window, void* out, int out_f32, float* lse,
                         void* workspace, size_t workspace_bytes, zkv_stream_t stream);
 
+/* --------------------------------------------------------------------------
+ * Linear layers in 8 bits: rows of e4m3 codes [M, 128 B] with an fp32 scale per
+ * 128 channels, weights of codes [rows, 128 B] with a scale per 128 x 128; a code
+ * stands for code * scale.  B = ceil(K / 128); codes behind K are 0.  The scale
+ * of a block is its largest magnitude / 448, at least 2^-100 (NaN, as its codes,
+ * where it holds an infinity or a NaN).  Scales of rows lie at m * s_m + b * s_b,
+ * those of a weight [blocks of rows, B] contiguous.  Types: 0 bf16, 1 fp16, 2
+ * fp32.  The reference's projections are bf16 (Z/model_hub/qwen.py:439-604).
+ * ------------------------------------------------------------------------ */
+
+/* Rows x [M, K] of `type` (row strides in elements) as codes (rows of whole
+ * blocks, on 8 bytes) and scales.  norm_w [K] (nullable): of h * rsqrt(mean(h^2)
+ * + eps) * norm_w, h = x [+ residual], K <= 65536; sum_out (nullable) takes h
+ * rounded to `type`, and may be x or residual. */
+int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type, const void* norm_w, float eps,
+                 const void* residual, int64_t res_ld, void* sum_out, int64_t sum_ld, uint8_t* codes,
+                 int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, zkv_stream_t stream);
+
+/* A weight w [N, K] of `type`, `parts` matrices of N / parts rows one behind the
+ * other, each with blocks of its own: scales [parts * ceil(N / parts / 128), B]. */
+int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int parts, uint8_t* codes, int64_t codes_ld,
+                   float* scales, zkv_stream_t stream);
+
+/* out[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in b} x[m, k] w[n, k]
+ * [+ residual[m, n]], fp32 sums rounded once to `type` (out and residual; out may
+ * be residual).  K is a multiple of 128, at most 16384; rows of codes start on 16
+ * bytes. */
+int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b, const uint8_t* w,
+                   int64_t w_ld, const float* ws, int M, int N, int K, const void* residual, int64_t res_ld,
+                   void* out, int64_t out_ld, int type, zkv_stream_t stream);
+
+/* The same for a weight of 2 F rows in two parts, gate and up: codes and scales
+ * of silu(gate) * up [M, F] (codes: rows of whole blocks of F, on 8 bytes).
+ * workspace: zkv_fp8_gated_workspace_size(M, F) bytes on 16, of any content;
+ * calls that overlap on one race. */
+size_t zkv_fp8_gated_workspace_size(int M, int F);
+int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
+                         const uint8_t* w, int64_t w_ld, const float* ws, int M, int F, int K, uint8_t* codes,
+                         int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, void* workspace,
+                         size_t workspace_bytes, zkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

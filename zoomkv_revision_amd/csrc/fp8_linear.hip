@@ -1,0 +1,593 @@
+// Products of rows and weights held as e4m3 codes with a scale per block of 128:
+//
+//   y[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
+//
+// The codes go into the bf16 matrix instructions, which they enter exactly (one
+// v_cvt_scalef32_pk_bf16_fp8 per two): their sums are those of fp32 (1e-8 to 4e-8 of
+// the sum of magnitudes over a block, measured).  The 8-bit instructions run at
+// twice the rate but add each 8 products with 14 bits below the largest (1.5e-5 to
+// 2.3e-5): a small term next to two large ones that cancel would be gone.  A
+// block's sum times its two scales is added to the running sums in fp32, one
+// multiply-add per value.  An element sits in the same place of A (weight rows) and
+// B (x rows), so which k a lane holds does not matter: a lane takes whole runs of 16
+// bytes.
+//
+//  * linear: y [+ residual], rounded once to the output's type.
+//  * gated: the weight's first half of rows is gate, the second up; y =
+//    silu(gate) * up, never rounded to 16 bits, comes out as codes and scales.
+#include "fp8_common.hpp"
+
+#include <algorithm>
+
+namespace zkv {
+namespace {
+
+struct LinearArgs {
+  const uint8_t* x;  // [M, 128 nkb]
+  int64_t x_ld;
+  const float* xs;  // element (m, b) at m * xs_m + b * xs_b
+  int64_t xs_m, xs_b;
+  const uint8_t* w;  // [N, 128 nkb], or [2 N, ...] where gated
+  int64_t w_ld;
+  const float* ws;  // [blocks of N (twice where gated), nkb]
+  int M, N, nkb;    // N: rows of the weight, of its gate half where gated
+  // linear
+  const void* res;
+  int64_t res_ld;
+  void* out;
+  int64_t out_ld;
+  int type;
+  // gated
+  uint8_t* codes;
+  int64_t codes_ld;
+  float* scales;
+  int64_t s_m, s_b;
+  float* act;                 // [blocks of N][M][128]
+  unsigned long long* slots;  // arrivals per (block of N, group of x rows)
+  unsigned long long epoch;
+};
+
+// 16 codes as two operands of 8 bf16 values.
+__device__ __forceinline__ void codes_to_bf16(const u32x4_t c, bf16x8_t& lo, bf16x8_t& hi) {
+  u32x4_t a, b;
+#define ZKV_PAIR(w, half) __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, half))
+  a[0] = ZKV_PAIR(c[0], false), a[1] = ZKV_PAIR(c[0], true);
+  a[2] = ZKV_PAIR(c[1], false), a[3] = ZKV_PAIR(c[1], true);
+  b[0] = ZKV_PAIR(c[2], false), b[1] = ZKV_PAIR(c[2], true);
+  b[2] = ZKV_PAIR(c[3], false), b[3] = ZKV_PAIR(c[3], true);
+#undef ZKV_PAIR
+  lo = __builtin_bit_cast(bf16x8_t, a), hi = __builtin_bit_cast(bf16x8_t, b);
+}
+
+// A lane's 32 codes of a row's block, for the 16 x 16 products.
+struct Operand16 {
+  bf16x8_t v[4];
+  __device__ __forceinline__ void set(const u32x4_t a, const u32x4_t b) {
+    codes_to_bf16(a, v[0], v[1]);
+    codes_to_bf16(b, v[2], v[3]);
+  }
+};
+
+__device__ __forceinline__ float4_t block_sum(const Operand16& a, const Operand16& b) {
+  float4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], s, 0, 0, 0);
+  return s;
+}
+
+__device__ __forceinline__ void add_scaled(float4_t& acc, float4_t v, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(v[i], s, acc[i]);
+}
+
+__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+__device__ __forceinline__ void store_out(const LinearArgs& p, int m, int n, float y) {
+  const int64_t o = m * p.out_ld + n, r = m * p.res_ld + n;
+  if (p.type == kRowBf16) {
+    if (p.res) y += elem_to_f32<kBf16>(static_cast<const uint16_t*>(p.res)[r]);
+    static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(f32_to_elem<kBf16>(y));
+  } else if (p.type == kRowF16) {
+    if (p.res) y += elem_to_f32<kF16>(static_cast<const uint16_t*>(p.res)[r]);
+    static_cast<uint16_t*>(p.out)[o] = static_cast<uint16_t>(f32_to_elem<kF16>(y));
+  } else {
+    if (p.res) y += static_cast<const float*>(p.res)[r];
+    static_cast<float*>(p.out)[o] = y;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows of x: the weights stream from memory into registers.  A unit is R
+// (16, 8 or 4) weight rows (gated: R gate rows and the matching up rows) of 16 kMT rows
+// of x; the waves of a workgroup split its blocks of k (wave w takes blocks w, w +
+// nw, ...), so nothing is staged and every wave reads its own part of x.  Lanes
+// whose A row is past R, or whose B column is past M, repeat the last: no more
+// memory moves.  The waves' sums meet in LDS and are added in wave order.
+// ---------------------------------------------------------------------------
+template <int kTiles, int kMT>
+struct StreamWave {
+  float4_t acc[kTiles][kMT];
+
+  // kCnt blocks, three in flight
+  template <int kCnt>
+  __device__ __forceinline__ void run(const uint8_t* const (&wr)[kTiles], const float* const (&wsr)[kTiles],
+                                      const uint8_t* const (&xr)[kMT], const float* const (&xsr)[kMT], int64_t xs_b,
+                                      int wave, int nw) {
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int j = 0; j < kMT; ++j) acc[t][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (kCnt > 0) {
+      constexpr int kDepth = kCnt < 3 ? kCnt : 3;
+      u32x4_t a[kDepth][kTiles][2], b[kDepth][kMT][2];
+      float xs[kDepth][kMT], ws[kDepth][kTiles];
+      auto load = [&](int i) {
+        const int kb = wave + i * nw, d = i % kDepth;
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+          a[d][t][0] = *reinterpret_cast<const u32x4_t*>(wr[t] + kb * kFp8Block);
+          a[d][t][1] = *reinterpret_cast<const u32x4_t*>(wr[t] + kb * kFp8Block + 64);
+          ws[d][t] = wsr[t][kb];
+        }
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) {
+          b[d][j][0] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block);
+          b[d][j][1] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block + 64);
+          xs[d][j] = xsr[j][kb * xs_b];
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < kDepth; ++i) load(i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kCnt; ++i) {
+        const int d = i % kDepth;
+        Operand16 A[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) A[t].set(a[d][t][0], a[d][t][1]);
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) {
+          Operand16 B;
+          B.set(b[d][j][0], b[d][j][1]);
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) add_scaled(acc[t][j], block_sum(A[t], B), xs[d][j] * ws[d][t]);
+        }
+        if (i + kDepth < kCnt) load(i + kDepth);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+};
+
+// The quantised output of one block of 128 gated values for rows [m0, m1): by the
+// workgroup that arrives last there.
+__device__ __forceinline__ void quantise_act(const LinearArgs& p, int jb, int m0, int m1) {
+  const int q = threadIdx.x & 15;
+  for (int m = m0 + (threadIdx.x >> 4); m < m1; m += blockDim.x >> 4) {
+    const unsigned long long* src =
+        reinterpret_cast<const unsigned long long*>(p.act + (static_cast<int64_t>(jb) * p.M + m) * kFp8Block + 8 * q);
+    float y[8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned long long v = __hip_atomic_load(src + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      y[2 * i] = __uint_as_float(static_cast<uint32_t>(v));
+      y[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(v >> 32));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (jb * kFp8Block + 8 * q + i >= p.N) y[i] = 0.0f;
+      amax = max(amax, abs_bits(y[i]));
+    }
+    const float s = fp8_scale(row_max(amax)), r = 1.0f / s;
+    *reinterpret_cast<u32x2_t*>(p.codes + m * p.codes_ld + jb * kFp8Block + 8 * q) =
+        u32x2_t{fp8_codes4(y, s, r), fp8_codes4(y + 4, s, r)};
+    if (q == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
+  }
+}
+
+template <bool kGated, int kMT, int kCnt>
+__global__ __launch_bounds__(1024) void fp8_stream_kernel(const LinearArgs p, int R) {
+  constexpr int kTiles = kGated ? 2 : 1;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][tile][x rows][lane]
+  const int nw = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * R, m0 = blockIdx.y * 16 * kMT;
+  const int row = min(n0 + min(c, R - 1), p.N - 1);
+  const uint8_t *wr[kTiles], *xr[kMT];
+  const float *wsr[kTiles], *xsr[kMT];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    wr[t] = p.w + (static_cast<int64_t>(t) * p.N + row) * p.w_ld + 16 * g;
+    // (R divides 128: a unit lies in one block of rows)
+    wsr[t] = p.ws + static_cast<int64_t>(t * ((p.N + kFp8Block - 1) / kFp8Block) + n0 / kFp8Block) * p.nkb;
+  }
+#pragma unroll
+  for (int j = 0; j < kMT; ++j) {
+    const int m = min(m0 + 16 * j + c, p.M - 1);
+    xr[j] = p.x + m * p.x_ld + 16 * g;
+    xsr[j] = p.xs + m * p.xs_m;
+  }
+  // a wave's blocks are all there but for the last: one without it takes a
+  // straight line of its own
+  const bool full = wave + (kCnt - 1) * nw < p.nkb;
+  StreamWave<kTiles, kMT> s;
+  if (full) {
+    asm volatile("; all blocks");
+    s.template run<kCnt>(wr, wsr, xr, xsr, p.xs_b, wave, nw);
+  } else {
+    asm volatile("; one fewer");
+    s.template run<kCnt - 1>(wr, wsr, xr, xsr, p.xs_b, wave, nw);
+  }
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) red[((wave * kTiles + t) * kMT + j) * 64 + lane] = s.acc[t][j];
+  __syncthreads();
+  // lane (c, g) holds rows 4 g + i of the unit for row c of x
+  for (int j = wave; j < kMT; j += nw) {
+    float4_t v[kTiles];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+      v[t] = red[(t * kMT + j) * 64 + lane];
+      for (int w = 1; w < nw; ++w) v[t] += red[((w * kTiles + t) * kMT + j) * 64 + lane];
+    }
+    const int m = m0 + 16 * j + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * g + i, n = n0 + r;
+      if (m >= p.M || r >= R || n >= p.N) continue;
+      if constexpr (kGated)
+        __hip_atomic_store(p.act + (static_cast<int64_t>(n / kFp8Block) * p.M + m) * kFp8Block + n % kFp8Block,
+                           silu_mul(v[0][i], v[kTiles - 1][i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      else
+        store_out(p, m, n, v[0][i]);
+    }
+  }
+  if constexpr (kGated) {
+    // the units of a block of 128 outputs: the last one quantises it.  Values go
+    // out and come back past the L2s, which the XCDs do not share; each lane's
+    // stores have been acknowledged before the workgroup counts itself in
+    __shared__ bool last;
+    const int jb = n0 / kFp8Block;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last = arrive_last(p.slots + static_cast<int64_t>(jb) * gridDim.y + blockIdx.y, p.epoch,
+                         (min(kFp8Block, p.N - jb * kFp8Block) + R - 1) / R);
+    __syncthreads();
+    if (last) quantise_act(p, jb, m0, min(p.M, m0 + 16 * kMT));
+  }
+}
+
+template <bool kGated>
+int launch_stream(const LinearArgs& p, hipStream_t s) {
+  constexpr int kMT = 1;
+  const int R = 8;
+  const int cnt = std::max(std::min(8, (p.nkb + 7) / 8), (p.nkb + 15) / 16);
+  const int nw = (p.nkb + cnt - 1) / cnt;
+  const dim3 grid((p.N + R - 1) / R, (p.M + 16 * kMT - 1) / (16 * kMT));
+  const size_t lds = static_cast<size_t>(nw) * (kGated ? 2 : 1) * kMT * 1024;
+#define ZKV_CNT(C)                                                         \
+  case C:                                                                  \
+    fp8_stream_kernel<kGated, kMT, C><<<grid, 64 * nw, lds, s>>>(p, R);    \
+    break;
+  switch (cnt) {
+    ZKV_CNT(1) ZKV_CNT(2) ZKV_CNT(3) ZKV_CNT(4) ZKV_CNT(5) ZKV_CNT(6) ZKV_CNT(7) ZKV_CNT(8)
+    default:
+      return fail(ZKV_EINVAL, "fp8 linear: %d blocks per wave", cnt);
+  }
+#undef ZKV_CNT
+  return check_launch("fp8_stream_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// Many rows of x: a workgroup of kWN x kWM waves computes 64 kWN weight rows (gated: 32
+// kWN gate rows and the matching up rows) for 64 kWM rows of x, a wave 64 x 64 of
+// it as 2 x 2 products of 32 x 32.  A block of 128 k of the tile's rows goes from
+// memory straight into one of two LDS stages while the other is computed on.
+//
+// LDS: a row is 8 chunks of 16 bytes, chunk c in slot c ^ ((row >> 1) & 7): the 16
+// lanes of a read phase, each with the same chunk of its own row, hit every bank
+// once.  A lane converts its codes after reading them (64 conversions per wave, block
+// and 32 rows): the LDS moves bytes, not bf16.
+// ---------------------------------------------------------------------------
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
+}
+
+// 64 lanes x 16 bytes into LDS at dst + 16 lane (dst wave-uniform), not seen by the
+// compiler's wait counts: with the builtin every LDS read waits for all of them.
+__device__ __forceinline__ void dma16_tile(const void* src, uint32_t dst) {
+  asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(dst) : "memory");
+}
+
+// A lane's 64 codes of a row's block.
+struct Operand32 {
+  bf16x8_t v[8];
+  __device__ __forceinline__ void read(const uint8_t* row, uint32_t first) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      codes_to_bf16(*reinterpret_cast<const u32x4_t*>(row + (first ^ (16 * t))), v[2 * t], v[2 * t + 1]);
+  }
+};
+
+__device__ __forceinline__ float16_t block_sum(const Operand32& a, const Operand32& b) {
+  float16_t s = {};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[q], b.v[q], s, 0, 0, 0);
+  return s;
+}
+
+// Four neighbouring columns of a row of the output.
+__device__ __forceinline__ void store_out4(const LinearArgs& p, int m, int n, const float (&y)[4], bool vec) {
+  if (!vec || n + 4 > p.N) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) store_out(p, m, n + i, y[i]);
+    return;
+  }
+  const int64_t o = m * p.out_ld + n, r = m * p.res_ld + n;
+  if (p.type == kRowF32) {
+    float4_t v = {y[0], y[1], y[2], y[3]};
+    if (p.res) v += *reinterpret_cast<const float4_t*>(static_cast<const float*>(p.res) + r);
+    *reinterpret_cast<float4_t*>(static_cast<float*>(p.out) + o) = v;
+  } else {
+    float v[4] = {y[0], y[1], y[2], y[3]};
+    const bool bf = p.type == kRowBf16;
+    if (p.res) {
+      const u32x2_t h = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.res) + r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = i & 1 ? h[i >> 1] >> 16 : h[i >> 1] & 0xFFFFu;
+        v[i] += bf ? elem_to_f32<kBf16>(e) : elem_to_f32<kF16>(e);
+      }
+    }
+    u32x2_t q;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      q[i] = bf ? f32_to_elem<kBf16>(v[2 * i]) | (f32_to_elem<kBf16>(v[2 * i + 1]) << 16)
+                : f32_to_elem<kF16>(v[2 * i]) | (f32_to_elem<kF16>(v[2 * i + 1]) << 16);
+    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + o) = q;
+  }
+}
+
+template <bool kGated, int kWN, int kWM>
+struct TileShape {
+  static constexpr int kRowsN = 64 * kWN, kRowsM = 64 * kWM;
+  static constexpr int kCols = kGated ? kRowsN / 2 : kRowsN;  // output columns
+  static constexpr int kStage = (kRowsN + kRowsM) * kFp8Block;
+};
+
+template <bool kGated, int kWN, int kWM>
+__global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const LinearArgs p, int tiles_n, int tiles_m,
+                                                                    int vec) {
+  using Shape = TileShape<kGated, kWN, kWM>;
+  constexpr int kWaves = kWN * kWM;
+  constexpr int kDmas = Shape::kStage / 1024 / kWaves;  // per wave and block
+  static_assert(Shape::kStage % (1024 * kWaves) == 0, "whole DMAs");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Shape::kStage];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = lane & 31, h = lane >> 5;
+  const int wn = wave % kWN, wm = wave / kWN;
+
+  // Workgroups go to the eight XCDs in turn: each takes a run of tiles, in bands of
+  // four tiles of weight rows, so that those at work at one time share rows in its L2
+  const int T = tiles_n * tiles_m, per = (T + 7) / 8;
+  const int t = static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3);
+  if (t >= T || static_cast<int>(blockIdx.x >> 3) >= per) return;
+  const int band = t / (4 * tiles_m), in_band = t - band * 4 * tiles_m, width = min(4, tiles_n - 4 * band);
+  const int tn = 4 * band + in_band % width, tm = in_band / width;
+  const int n0 = tn * Shape::kCols, m0 = tm * Shape::kRowsM;
+
+  // where this lane's DMAs read: eight rows of 128 bytes each, slots permuted
+  const uint8_t* src[kDmas];
+#pragma unroll
+  for (int i = 0; i < kDmas; ++i) {
+    const int row = 8 * (wave * kDmas + i) + (lane >> 3);
+    const int chunk = (lane & 7) ^ ((row >> 1) & 7);
+    if (row < Shape::kRowsN) {
+      int n;
+      if constexpr (kGated)  // 32 gate rows and the 32 matching up rows in turn
+        n = min(n0 + (row >> 6) * 32 + (row & 31), p.N - 1) + (row & 32 ? p.N : 0);
+      else
+        n = min(n0 + row, p.N - 1);
+      src[i] = p.w + static_cast<int64_t>(n) * p.w_ld + 16 * chunk;
+    } else {
+      src[i] = p.x + static_cast<int64_t>(min(m0 + row - Shape::kRowsN, p.M - 1)) * p.x_ld + 16 * chunk;
+    }
+  }
+  const uint32_t dst = lds_offset(lds) + wave * kDmas * 1024;
+  auto request = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kDmas; ++i) {
+      dma16_tile(src[i], __builtin_amdgcn_readfirstlane(dst + stage * Shape::kStage + i * 1024));
+      src[i] += kFp8Block;
+    }
+  };
+  // scales: of this lane's two x rows, and of the wave's weight rows (one block; gate and up: two)
+  const float *xsp[2], *wsp[2];
+  int zero = 0;
+  asm("" : "+v"(zero));  // keeps the weight's scales out of scalar loads, whose waits are for all of them
+#pragma unroll
+  for (int j = 0; j < 2; ++j) xsp[j] = p.xs + min(m0 + 64 * wm + 32 * j + r, p.M - 1) * p.xs_m;
+  const int nb = (p.N + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int b = kGated ? i * nb + min(n0 + 32 * wn, p.N - 1) / kFp8Block : min(n0 + 64 * wn, p.N - 1) / kFp8Block;
+    wsp[i] = p.ws + static_cast<int64_t>(b) * p.nkb + zero;
+  }
+  float xs[2], ws[2];
+  auto request_scales = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) xs[j] = xsp[j][kb * p.xs_b];
+#pragma unroll
+    for (int i = 0; i < (kGated ? 2 : 1); ++i) ws[i] = wsp[i][kb];
+  };
+
+  float16_t acc[2][2] = {};
+  const uint32_t first = 16 * ((4 * h) ^ ((r >> 1) & 7));
+  const uint8_t* rows_n = lds + (64 * wn + r) * kFp8Block;
+  const uint8_t* rows_m = lds + (Shape::kRowsN + 64 * wm + r) * kFp8Block;
+  request(0);
+  request_scales(0);
+  for (int kb = 0; kb < p.nkb; ++kb) {
+    wait_vmcnt<0>();
+    __syncthreads();
+    float s[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[i][j] = xs[j] * ws[kGated ? i : 0];
+    if (kb + 1 < p.nkb) {
+      request((kb + 1) & 1);
+      request_scales(kb + 1);
+    }
+    const int at = (kb & 1) * Shape::kStage;
+    Operand32 B[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) B[j].read(rows_m + at + 32 * j * kFp8Block, first);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      Operand32 A;
+      A.read(rows_n + at + 32 * i * kFp8Block, first);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float16_t v = block_sum(A, B[j]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(v[e], s[i][j], acc[i][j][e]);
+      }
+    }
+  }
+
+  // lane (r, h) holds columns 8 q + 4 h + 0..3 of row r of each product
+  if constexpr (!kGated) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int m = m0 + 64 * wm + 32 * j + r;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float y[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          store_out4(p, m, n0 + 64 * wn + 32 * i + 8 * q + 4 * h, y, vec);
+        }
+    }
+  } else {
+    // 128 columns, one block: its largest magnitudes meet in LDS, [wn][row]
+    static_assert(Shape::kCols == kFp8Block, "one block of outputs");
+    __syncthreads();
+    uint32_t* amax = reinterpret_cast<uint32_t*>(lds);
+    float y[2][16];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int n = n0 + 32 * wn + 8 * (e >> 2) + 4 * h + (e & 3);
+        y[j][e] = n < p.N ? silu_mul(acc[0][j][e], acc[1][j][e]) : 0.0f;
+        a = max(a, abs_bits(y[j][e]));
+      }
+      a = max(a, static_cast<uint32_t>(__shfl_xor(static_cast<int>(a), 32)));
+      if (h == 0) amax[wn * Shape::kRowsM + 64 * wm + 32 * j + r] = a;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = 64 * wm + 32 * j + r, m = m0 + row;
+      uint32_t a = amax[row];
+#pragma unroll
+      for (int w = 1; w < kWN; ++w) a = max(a, amax[w * Shape::kRowsM + row]);
+      const float sc = fp8_scale(a), rc = 1.0f / sc;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint32_t*>(p.codes + m * p.codes_ld + n0 + 32 * wn + 8 * q + 4 * h) =
+            fp8_codes4(y[j] + 4 * q, sc, rc);
+      if (wn == 0 && h == 0) p.scales[m * p.s_m + tn * p.s_b] = sc;
+    }
+  }
+}
+
+template <bool kGated, int kWN, int kWM>
+int launch_tile(const LinearArgs& p, hipStream_t s) {
+  using Shape = TileShape<kGated, kWN, kWM>;
+  const int tiles_n = (p.N + Shape::kCols - 1) / Shape::kCols, tiles_m = (p.M + Shape::kRowsM - 1) / Shape::kRowsM;
+  const int item = p.type == kRowF32 ? 4 : 2;
+  const int vec = !kGated && reinterpret_cast<uintptr_t>(p.out) % (4 * item) == 0 && p.out_ld % 4 == 0 &&
+                  (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
+  const unsigned grid = (static_cast<unsigned>(tiles_n) * tiles_m + 7) / 8 * 8;
+  fp8_tile_kernel<kGated, kWN, kWM><<<grid, 64 * kWN * kWM, 0, s>>>(p, tiles_n, tiles_m, vec);
+  return check_launch("fp8_tile_kernel");
+}
+
+int blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+// Checks what both entry points take; null or what is wrong.
+const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, const uint8_t* w, int64_t w_ld,
+                           const float* ws, int M, int N, int K) {
+  if (!x || !xs || !w || !ws) return "null pointer";
+  if (M < 1 || N < 1 || K < 1) return "empty product";
+  if (K % kFp8Block || K > 128 * kFp8Block) return "K is a multiple of 128, at most 16384";
+  if (x_ld < K || w_ld < K || !rows_on_16(x, x_ld, 1) || !rows_on_16(w, w_ld, 1))
+    return "rows of codes hold K bytes and start on 16";
+  return nullptr;
+}
+
+}  // namespace
+}  // namespace zkv
+
+using namespace zkv;
+
+extern "C" int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
+                              const uint8_t* w, int64_t w_ld, const float* ws, int M, int N, int K,
+                              const void* residual, int64_t res_ld, void* out, int64_t out_ld, int type,
+                              zkv_stream_t stream) {
+  const char* bad = check_operands(x, x_ld, xs, w, w_ld, ws, M, N, K);
+  ZKV_REQUIRE(!bad, "zkv_fp8_linear: %s (M=%d N=%d K=%d)", bad, M, N, K);
+  ZKV_REQUIRE(out && type >= kRowBf16 && type <= kRowF32, "zkv_fp8_linear: bad output");
+  LinearArgs p{};
+  p.x = x, p.x_ld = x_ld, p.xs = xs, p.xs_m = xs_m, p.xs_b = xs_b, p.w = w, p.w_ld = w_ld, p.ws = ws;
+  p.M = M, p.N = N, p.nkb = K / kFp8Block;
+  p.res = residual, p.res_ld = res_ld, p.out = out, p.out_ld = out_ld, p.type = type;
+  auto s = reinterpret_cast<hipStream_t>(stream);
+  if (M <= 64) return launch_stream<false>(p, s);
+  return launch_tile<false, 4, 2>(p, s);
+}
+
+extern "C" size_t zkv_fp8_gated_workspace_size(int M, int F) {
+  if (M < 1 || F < 1) return 0;
+  const size_t nb = blocks_of(F);
+  return (nb * ((M + 15) / 16) * 8 + 255) / 256 * 256 + nb * M * kFp8Block * 4;
+}
+
+extern "C" int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
+                                    const uint8_t* w, int64_t w_ld, const float* ws, int M, int F, int K,
+                                    uint8_t* codes, int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b,
+                                    void* workspace, size_t workspace_bytes, zkv_stream_t stream) {
+  const char* bad = check_operands(x, x_ld, xs, w, w_ld, ws, M, F, K);
+  ZKV_REQUIRE(!bad, "zkv_fp8_gated_linear: %s (M=%d F=%d K=%d)", bad, M, F, K);
+  ZKV_REQUIRE(codes && scales && codes_ld >= static_cast<int64_t>(blocks_of(F)) * kFp8Block && codes_ld % 8 == 0 &&
+                  (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
+              "zkv_fp8_gated_linear: rows of codes hold whole blocks of 128 and start on 8 bytes");
+  const size_t need = zkv_fp8_gated_workspace_size(M, F);
+  if (workspace_bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(ZKV_ESPACE, "zkv_fp8_gated_linear: %zu bytes of workspace on 16 bytes, %zu needed", workspace_bytes,
+                need);
+  LinearArgs p{};
+  p.x = x, p.x_ld = x_ld, p.xs = xs, p.xs_m = xs_m, p.xs_b = xs_b, p.w = w, p.w_ld = w_ld, p.ws = ws;
+  p.M = M, p.N = F, p.nkb = K / kFp8Block;
+  p.codes = codes, p.codes_ld = codes_ld, p.scales = scales, p.s_m = s_m, p.s_b = s_b;
+  p.slots = static_cast<unsigned long long*>(workspace);
+  p.act = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
+                                   (static_cast<size_t>(blocks_of(F)) * ((M + 15) / 16) * 8 + 255) / 256 * 256);
+  p.epoch = next_epoch();
+  auto s = reinterpret_cast<hipStream_t>(stream);
+  if (M <= 64) return launch_stream<true>(p, s);
+  return launch_tile<true, 4, 2>(p, s);
+}

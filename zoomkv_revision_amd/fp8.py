@@ -1,0 +1,338 @@
+"""Linear layers in 8 bits: e4m3 codes with a scale per block of 128 (gfx950).
+
+A row of a hidden state is e4m3 codes (``torch.float8_e4m3fn``) with an fp32
+scale per 128 channels, a weight codes with a scale per 128 x 128: a code stands
+for code * scale.  Rows of codes are as long as whole blocks, zeros behind the
+last channel, so ``codes`` is [M, ceil(K / 128) * 128].
+
+  * ``rms_norm_quant``: the residual's addition, RMS norm and the codes of the
+    normed rows in one launch; ``quantize_rows`` the codes alone (an attention's
+    output on its way into the o-projection).
+  * ``quantize_weight``: a weight, once, when it is loaded.
+  * ``linear``: rows times weight, with a residual added on the way out where
+    there is one, for any number of rows (``decode_step.decode_linear`` is the
+    bf16 counterpart, for at most 16).
+  * ``gated_linear``: both projections of a gated feed-forward block, silu(gate)
+    * up, and the result as codes and scales for the down projection.
+
+The scale of a block is its largest magnitude / 448 (the largest e4m3 value) and
+not below 2^-100; the code is value / scale rounded to nearest even.  A block
+that holds an infinity or a NaN has a NaN scale and NaN codes.  Sums, norms and
+activations are fp32, and nothing is rounded to 16 bits between the codes of the
+inputs and the one rounding of the result.  (The product of a row's and a
+weight's scale is formed first: it should stay within fp32's range.)
+
+Each function checks its arguments on every call; the ``*Plan`` classes check
+once for fixed buffers and then make one C-ABI call per ``run()``.
+
+The reference's projections are bf16 (Z/model_hub/qwen.py:439-604).
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._lib import lib, ptr, require_gpu
+from .paged import _launch, _nothing, _Plan, _same_device, _strides
+
+BLOCK = 128
+MAX_K = 16384          # of a product
+MAX_NORM_K = 65536     # of a normed row
+E4M3 = torch.float8_e4m3fn
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _check_type(name: str, dtype: torch.dtype) -> int:
+    if dtype not in _TYPES:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32; got {dtype}")
+    return _TYPES[dtype]
+
+
+def _row_stride(name: str, t: torch.Tensor, shape: tuple) -> int:
+    """The row stride of a 2-D tensor with contiguous rows that do not overlap
+    (0 where there is one row)."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
+    ld, one = _strides(t)
+    if (shape[1] > 1 and one != 1) or (shape[0] > 1 and ld < shape[1]):
+        raise ValueError(f"the rows of {name} must be contiguous and apart; got strides {t.stride()}")
+    return ld if shape[0] > 1 else shape[1]
+
+
+def _check_codes(name: str, codes: torch.Tensor, rows: int, K: int, align: int) -> int:
+    if codes.dtype != E4M3:
+        raise TypeError(f"{name} must be float8_e4m3fn; got {codes.dtype}")
+    ld = _row_stride(name, codes, (rows, blocks(K) * BLOCK))
+    if codes.data_ptr() % align or ld % align:
+        raise ValueError(f"the rows of {name} must start on {align} bytes")
+    return ld
+
+
+def _check_scales(name: str, scales: torch.Tensor, rows: int, K: int, apart: bool) -> tuple[int, int]:
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (rows, blocks(K)):
+        raise ValueError(f"{name} must be float32 [{rows}, {blocks(K)}]; got {scales.dtype} {list(scales.shape)}")
+    s = _strides(scales)
+    if apart and any(x < 1 for x, n in zip(s, scales.shape) if n > 1):
+        raise ValueError(f"{name} must have a place for every scale; got strides {scales.stride()}")
+    return s
+
+
+def _new_codes(rows: int, K: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(rows, blocks(K) * BLOCK, dtype=E4M3, device=like.device)
+
+
+def _new_scales(rows: int, K: int, like: torch.Tensor) -> torch.Tensor:
+    """Scales as columns of `rows` (neighbouring rows' scales of one block lie
+    together, as a product reads them)."""
+    return torch.empty(blocks(K), rows, dtype=torch.float32, device=like.device).t()
+
+
+# ---------------------------------------------------------------------------
+# rows
+# ---------------------------------------------------------------------------
+def _rows_args(x, weight, eps, residual, sum_out, codes, scales):
+    kind = _check_type("x", x.dtype)
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be [rows, channels]; got {list(x.shape)}")
+    M, K = x.shape
+    if M >= 1 << 27 or K >= 1 << 30:
+        raise ValueError(f"{M} rows of {K} channels in one call")
+    x_ld = _row_stride("x", x, (M, K))
+    res_ld = sum_ld = 0
+    if weight is not None:
+        if weight.dtype != x.dtype or tuple(weight.shape) != (K,) or (K > 1 and weight.stride(0) != 1):
+            raise ValueError(f"the norm's weight must be contiguous {x.dtype} [{K}]; got {weight.dtype} "
+                             f"{list(weight.shape)}")
+        if K > MAX_NORM_K:
+            raise ValueError(f"normed rows have at most {MAX_NORM_K} channels; got {K}")
+    if residual is not None:
+        if residual.dtype != x.dtype:
+            raise TypeError(f"the residual must be {x.dtype}; got {residual.dtype}")
+        res_ld = _row_stride("residual", residual, (M, K))
+        sum_out = torch.empty(M, K, dtype=x.dtype, device=x.device) if sum_out is None else sum_out
+        if sum_out.dtype != x.dtype:
+            raise TypeError(f"sum_out must be {x.dtype}; got {sum_out.dtype}")
+        sum_ld = _row_stride("sum_out", sum_out, (M, K))
+        for name, t in (("x", x), ("residual", residual)):
+            if sum_out.data_ptr() != t.data_ptr() and _overlap(sum_out, t) or \
+                    sum_out.data_ptr() == t.data_ptr() and _strides(sum_out) != _strides(t):
+                raise ValueError(f"sum_out must be {name} itself or lie apart from it")
+    elif sum_out is not None:
+        raise ValueError("sum_out goes with a residual")
+    codes = _new_codes(M, K, x) if codes is None else codes
+    scales = _new_scales(M, K, x) if scales is None else scales
+    codes_ld = _check_codes("codes", codes, M, K, 8)
+    s_m, s_b = _check_scales("scales", scales, M, K, apart=True)
+    _same_device(x, weight=weight, residual=residual, sum_out=sum_out, codes=codes, scales=scales)
+    require_gpu(x)
+    args = (ptr(x), x_ld, M, K, kind, ptr(weight), float(eps), ptr(residual), res_ld, ptr(sum_out), sum_ld,
+            ptr(codes), codes_ld, ptr(scales), s_m, s_b)
+    result = (codes, scales) if residual is None else (codes, scales, sum_out)
+    return args, result, (x, weight, residual, sum_out, codes, scales)
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes that a tensor's elements lie in."""
+    if not t.numel():
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a0 < b1 and b0 < a1
+
+
+class RmsNormQuantPlan(_Plan):
+    """``rms_norm_quant`` with its checks done once for fixed buffers."""
+
+    def __init__(self, x, weight, eps, residual=None, sum_out=None, codes=None, scales=None):
+        if weight is None:
+            raise ValueError("the norm needs its weight")
+        args, result, keep = _rows_args(x, weight, eps, residual, sum_out, codes, scales)
+        super().__init__(lib().zkv_fp8_rows if x.shape[0] else _nothing, x.device, args, result, keep)
+
+
+class QuantizeRowsPlan(_Plan):
+    """``quantize_rows`` with its checks done once for fixed buffers."""
+
+    def __init__(self, x, codes=None, scales=None):
+        args, result, keep = _rows_args(x, None, 0.0, None, None, codes, scales)
+        super().__init__(lib().zkv_fp8_rows if x.shape[0] else _nothing, x.device, args, result, keep)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
+                   sum_out: torch.Tensor | None = None, codes: torch.Tensor | None = None,
+                   scales: torch.Tensor | None = None):
+    """h = x [+ residual]; h * rsqrt(mean(h^2) + eps) * weight per row of x [M,
+    K] (bf16, fp16 or fp32; residual and weight [K] alike), as codes [M,
+    ceil(K / 128) * 128] and scales float32 [M, ceil(K / 128)].
+
+    fp32 throughout; the norm goes by the unrounded sum, which is rounded to x's
+    type where it is stored.  Returns (codes, scales), and with a residual (codes,
+    scales, sum_out); sum_out may be x or residual.  New scales are laid out as
+    columns of M."""
+    return RmsNormQuantPlan(x, weight, eps, residual, sum_out, codes, scales).run()
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """The rows of x [M, K] (bf16, fp16 or fp32) as codes [M, ceil(K / 128) *
+    128] and scales float32 [M, ceil(K / 128)]."""
+    return QuantizeRowsPlan(x, codes, scales).run()
+
+
+# ---------------------------------------------------------------------------
+# weights
+# ---------------------------------------------------------------------------
+@dataclass
+class Fp8Weight:
+    """A weight of codes [rows, ceil(K / 128) * 128] (zeros behind K) and scales
+    float32 [blocks of rows, ceil(K / 128)], contiguous.  parts: the rows are
+    that many matrices, one behind the other, with blocks of their own (a gate /
+    up weight has 2)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    parts: int = 1
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    def dequantize(self) -> torch.Tensor:
+        """float32 [rows, ceil(K / 128) * 128]."""
+        n = self.rows // self.parts
+        s = self.scales.view(self.parts, blocks(n), -1).repeat_interleave(BLOCK, 1)[:, :n].reshape(self.rows, -1, 1)
+        return (self.codes.float().view(self.rows, -1, BLOCK) * s).view(self.rows, -1)
+
+
+def quantize_weight(w: torch.Tensor, parts: int = 1) -> Fp8Weight:
+    """A weight [rows, K] (bf16, fp16 or fp32; the rows of `parts` matrices of
+    one size) as codes with a scale per 128 x 128."""
+    kind = _check_type("w", w.dtype)
+    parts = int(parts)
+    if w.dim() != 2 or min(w.shape) < 1 or parts < 1 or w.shape[0] % parts:
+        raise ValueError(f"w must be [rows, channels], rows a multiple of {parts}; got {list(w.shape)}")
+    N, K = w.shape
+    nb = parts * blocks(N // parts)
+    if nb > 65535 or K >= 1 << 30:
+        raise ValueError(f"a weight of {N} x {K} in one call")
+    ld = _row_stride("w", w, (N, K))
+    require_gpu(w)
+    codes = _new_codes(N, K, w)
+    scales = torch.empty(nb, blocks(K), dtype=torch.float32, device=w.device)
+    _launch(lib().zkv_fp8_weight, w.device, (ptr(w), ld, N, K, kind, parts, ptr(codes), codes.shape[1], ptr(scales)))
+    return Fp8Weight(codes, scales, parts)
+
+
+def _check_product(codes, scales, weight: Fp8Weight, parts: int):
+    """(M, rows of a part of the weight, K, the operands' arguments)."""
+    if codes.dim() != 2 or weight.codes.dim() != 2 or codes.shape[1] != weight.codes.shape[1] or \
+            codes.shape[1] % BLOCK or not codes.shape[1]:
+        raise ValueError(f"codes and weight must have one length, a multiple of {BLOCK}; got {list(codes.shape)}, "
+                         f"{list(weight.codes.shape)}")
+    if weight.parts != parts:
+        raise ValueError(f"a weight in {weight.parts} part(s), not {parts}")
+    M, K = codes.shape
+    rows = weight.rows
+    if K > MAX_K:
+        raise ValueError(f"a product over {K} channels, at most {MAX_K}")
+    if rows < parts or rows % parts or rows >= 1 << 24 or M >= 1 << 20:
+        raise ValueError(f"a product of {M} rows with a weight of {rows} rows in {parts} part(s)")
+    x_ld = _check_codes("codes", codes, M, K, 16)
+    s_m, s_b = _check_scales("scales", scales, M, K, apart=False)
+    w_ld = _check_codes("the weight's codes", weight.codes, rows, K, 16)
+    nb = parts * blocks(rows // parts)
+    ws = weight.scales
+    if ws.dtype != torch.float32 or tuple(ws.shape) != (nb, K // BLOCK) or not ws.is_contiguous():
+        raise ValueError(f"the weight's scales must be contiguous float32 [{nb}, {K // BLOCK}]; got {ws.dtype} "
+                         f"{list(ws.shape)}")
+    _same_device(codes, scales=scales, weight=weight.codes, weight_scales=ws)
+    n = rows // parts
+    return M, n, K, (ptr(codes), x_ld, ptr(scales), s_m, s_b, ptr(weight.codes), w_ld, ptr(ws), M, n, K)
+
+
+# ---------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------
+def _linear_args(codes, scales, weight, out, out_dtype, residual):
+    M, N, _, operands = _check_product(codes, scales, weight, 1)
+    if out is None:
+        _check_type("out_dtype", out_dtype)
+        out = torch.empty(M, N, dtype=out_dtype, device=codes.device)
+    kind = _check_type("out", out.dtype)
+    out_ld = _row_stride("out", out, (M, N))
+    res_ld = 0
+    if residual is not None:
+        if residual.dtype != out.dtype:
+            raise TypeError(f"the residual must be {out.dtype}; got {residual.dtype}")
+        res_ld = _row_stride("residual", residual, (M, N))
+        if out.data_ptr() != residual.data_ptr() and _overlap(out, residual) or \
+                out.data_ptr() == residual.data_ptr() and _strides(out) != _strides(residual):
+            raise ValueError("out must be the residual itself or lie apart from it")
+    _same_device(codes, out=out, residual=residual)
+    require_gpu(codes)
+    args = (*operands, ptr(residual), res_ld, ptr(out), out_ld, kind)
+    return args, out, (codes, scales, weight.codes, weight.scales, residual, out)
+
+
+class LinearPlan(_Plan):
+    """``linear`` with its checks done once for fixed buffers."""
+
+    def __init__(self, codes, scales, weight, out=None, out_dtype=torch.bfloat16, residual=None):
+        args, result, keep = _linear_args(codes, scales, weight, out, out_dtype, residual)
+        super().__init__(lib().zkv_fp8_linear if codes.shape[0] else _nothing, codes.device, args, result, keep)
+
+
+def linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor | None = None,
+           out_dtype: torch.dtype = torch.bfloat16, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows (codes [M, K], scales float32 [M, K / 128] of any strides) times
+    weight.T [+ residual]: [M, rows of the weight] in bf16, fp16 or fp32, rounded
+    once.  out may be the residual."""
+    return LinearPlan(codes, scales, weight, out, out_dtype, residual).run()
+
+
+def _gated_args(codes, scales, weight, out_codes, out_scales, workspace):
+    M, F, _, operands = _check_product(codes, scales, weight, 2)
+    out_codes = _new_codes(M, F, codes) if out_codes is None else out_codes
+    out_scales = _new_scales(M, F, codes) if out_scales is None else out_scales
+    codes_ld = _check_codes("out_codes", out_codes, M, F, 8)
+    s_m, s_b = _check_scales("out_scales", out_scales, M, F, apart=True)
+    for name, a, b in (("out_codes", out_codes, codes), ("out_scales", out_scales, scales)):
+        if _overlap(a, b):
+            raise ValueError(f"{name} must lie apart from the input")
+    require_gpu(codes)
+    need = lib().zkv_fp8_gated_workspace_size(M, F)
+    ws = torch.empty(need, dtype=torch.uint8, device=codes.device) if workspace is None else workspace
+    if ws.dtype != torch.uint8 or ws.numel() < need or not ws.is_contiguous() or ws.data_ptr() % 16:
+        raise ValueError(f"workspace must be contiguous uint8 of at least {need} bytes on 16 bytes")
+    _same_device(codes, out_codes=out_codes, out_scales=out_scales, workspace=ws)
+    args = (*operands, ptr(out_codes), codes_ld, ptr(out_scales), s_m, s_b, ptr(ws), ws.numel())
+    return args, (out_codes, out_scales), (codes, scales, weight.codes, weight.scales, out_codes, out_scales, ws)
+
+
+class GatedLinearPlan(_Plan):
+    """``gated_linear`` with its checks done once for fixed buffers.  A plan has
+    a workspace of its own unless one is given; runs of one plan must not overlap
+    on the device."""
+
+    def __init__(self, codes, scales, weight, out_codes=None, out_scales=None, workspace=None):
+        args, result, keep = _gated_args(codes, scales, weight, out_codes, out_scales, workspace)
+        super().__init__(lib().zkv_fp8_gated_linear if codes.shape[0] else _nothing, codes.device, args, result, keep)
+
+
+def gated_linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out_codes: torch.Tensor | None = None,
+                 out_scales: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+    """silu(gate) * up of a gated feed-forward block, one launch: gate and up are
+    the rows (codes, scales) times the two parts of the weight ([2 F, K], parts =
+    2); returns codes [M, ceil(F / 128) * 128] and scales float32 [M, ceil(F /
+    128)] (new ones as columns of M), what ``linear`` takes for the down
+    projection.  The workspace (uint8, zkv_fp8_gated_workspace_size(M, F) bytes)
+    needs no clearing; calls that overlap on one race."""
+    return GatedLinearPlan(codes, scales, weight, out_codes, out_scales, workspace).run()
