@@ -300,27 +300,29 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
 }
 
-// 64 lanes x 16 bytes into LDS at dst + 16 lane (dst wave-uniform), not seen by the
+// 64 lanes x 16 bytes, each at its offset from a base (wave-uniform, as dst), into LDS at dst + 16 lane, not seen by the
 // compiler's wait counts: with the builtin every LDS read waits for all of them.
-__device__ __forceinline__ void dma16_tile(const void* src, uint32_t dst) {
-  asm volatile("global_load_lds_dwordx4 %0, off" : : "v"(src), "{m0}"(dst) : "memory");
+__device__ __forceinline__ void dma16_tile(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
 }
 
-// A lane's 64 codes of a row's block.
-struct Operand32 {
-  bf16x8_t v[8];
-  __device__ __forceinline__ void read(const uint8_t* row, uint32_t first) {
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      codes_to_bf16(*reinterpret_cast<const u32x4_t*>(row + (first ^ (16 * t))), v[2 * t], v[2 * t + 1]);
-  }
-};
+__device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
+  asm volatile("global_load_lds_dword %0, off" : : "v"(src), "{m0}"(dst) : "memory");
+}
 
-__device__ __forceinline__ float16_t block_sum(const Operand32& a, const Operand32& b) {
-  float16_t s = {};
+// 8 codes as an operand.
+__device__ __forceinline__ bf16x8_t codes8_to_bf16(uint32_t c0, uint32_t c1) {
+  u32x4_t a;
+#define ZKV_PAIR(w, half) __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, half))
+  a[0] = ZKV_PAIR(c0, false), a[1] = ZKV_PAIR(c0, true);
+  a[2] = ZKV_PAIR(c1, false), a[3] = ZKV_PAIR(c1, true);
+#undef ZKV_PAIR
+  return __builtin_bit_cast(bf16x8_t, a);
+}
+
+__device__ __forceinline__ void add_scaled(float16_t& acc, const float16_t& v, float s) {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[q], b.v[q], s, 0, 0, 0);
-  return s;
+  for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(v[i], s, acc[i]);
 }
 
 // Four neighbouring columns of a row of the output.
@@ -356,6 +358,8 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int m, int n, co
   }
 }
 
+constexpr int kStages = 3;
+
 template <bool kGated, int kWN, int kWM>
 struct TileShape {
   static constexpr int kRowsN = 64 * kWN, kRowsM = 64 * kWM;
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   constexpr int kWaves = kWN * kWM;
   constexpr int kDmas = Shape::kStage / 1024 / kWaves;  // per wave and block
   static_assert(Shape::kStage % (1024 * kWaves) == 0, "whole DMAs");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * Shape::kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * (Shape::kStage + 256 * (kWM + 1))];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 31, h = lane >> 5;
   const int wn = wave % kWN, wm = wave / kWN;
@@ -384,85 +388,138 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   const int tn = 4 * band + in_band % width, tm = in_band / width;
   const int n0 = tn * Shape::kCols, m0 = tm * Shape::kRowsM;
 
-  // where this lane's DMAs read: eight rows of 128 bytes each, slots permuted
+  // where the DMAs read: eight rows of 128 bytes each, slots permuted, at a lane's
+  // offset from a row of the wave's (host side: rows at most 8 MiB apart)
   const uint8_t* src[kDmas];
+  uint32_t off[kDmas];
 #pragma unroll
   for (int i = 0; i < kDmas; ++i) {
-    const int row = 8 * (wave * kDmas + i) + (lane >> 3);
-    const int chunk = (lane & 7) ^ ((row >> 1) & 7);
-    if (row < Shape::kRowsN) {
-      int n;
-      if constexpr (kGated)  // 32 gate rows and the 32 matching up rows in turn
-        n = min(n0 + (row >> 6) * 32 + (row & 31), p.N - 1) + (row & 32 ? p.N : 0);
-      else
-        n = min(n0 + row, p.N - 1);
-      src[i] = p.w + static_cast<int64_t>(n) * p.w_ld + 16 * chunk;
+    const int top = 8 * (wave * kDmas + i), row = top + (lane >> 3);
+    const uint32_t chunk = (lane & 7) ^ ((row >> 1) & 7);
+    if (top >= Shape::kRowsN) {
+      src[i] = p.x + m0 * p.x_ld;
+      off[i] = min(row - Shape::kRowsN, p.M - 1 - m0) * static_cast<uint32_t>(p.x_ld) + 16 * chunk;
+    } else if (kGated) {  // 32 gate rows and the 32 matching up rows in turn
+      src[i] = p.w + (static_cast<int64_t>(n0) + (top & 32 ? p.N : 0)) * p.w_ld;
+      off[i] = min((row >> 6) * 32 + (row & 31), p.N - 1 - n0) * static_cast<uint32_t>(p.w_ld) + 16 * chunk;
     } else {
-      src[i] = p.x + static_cast<int64_t>(min(m0 + row - Shape::kRowsN, p.M - 1)) * p.x_ld + 16 * chunk;
+      src[i] = p.w + n0 * p.w_ld;
+      off[i] = min(row, p.N - 1 - n0) * static_cast<uint32_t>(p.w_ld) + 16 * chunk;
     }
   }
   const uint32_t dst = lds_offset(lds) + wave * kDmas * 1024;
-  auto request = [&](int stage) {
-#pragma unroll
-    for (int i = 0; i < kDmas; ++i) {
-      dma16_tile(src[i], __builtin_amdgcn_readfirstlane(dst + stage * Shape::kStage + i * 1024));
-      src[i] += kFp8Block;
+  // scales of a block: of the tile's x rows, then of each wave row's weight rows (gated:
+  // gate and up), 64 to a wave's DMA
+  constexpr int kScaleWaves = kWM + 1;
+  const float* scale_src;
+  int64_t scale_step;
+  {
+    const int w = wave % kScaleWaves;
+    if (w < kWM) {
+      scale_src = p.xs + min(m0 + 64 * w + lane, p.M - 1) * p.xs_m;
+      scale_step = p.xs_b;
+    } else {
+      const int nb = (p.N + kFp8Block - 1) / kFp8Block, part = lane & 1, group = (lane >> 1) % kWN;
+      const int n = min(n0 + (kGated ? 32 : 64) * group, p.N - 1);
+      scale_src = p.ws + static_cast<int64_t>((kGated ? part * nb : 0) + n / kFp8Block) * p.nkb;
+      scale_step = 1;
+    }
+  }
+  const uint32_t scale_dst = lds_offset(lds) + kStages * Shape::kStage + (wave % kScaleWaves) * 256;
+  // the i-th DMA of the block that is requested next, into its stage; past the last
+  // block they repeat it, which keeps the counts of what is in flight
+  int req = 0, req_stage = 0;
+  auto request = [&](int i) {
+    const int step = req + 1 < p.nkb ? 1 : 0;
+    if (i < kDmas) {
+      dma16_tile(src[i], off[i], __builtin_amdgcn_readfirstlane(dst + req_stage * Shape::kStage + i * 1024));
+      src[i] += step * kFp8Block;
+    } else {
+      dma4_tile(scale_src, __builtin_amdgcn_readfirstlane(scale_dst + req_stage * 256 * kScaleWaves));
+      scale_src += step * scale_step;
+      req += step;
+      req_stage = req_stage + 1 == kStages ? 0 : req_stage + 1;
     }
   };
-  // scales: of this lane's two x rows, and of the wave's weight rows (one block; gate and up: two)
-  const float *xsp[2], *wsp[2];
-  int zero = 0;
-  asm("" : "+v"(zero));  // keeps the weight's scales out of scalar loads, whose waits are for all of them
-#pragma unroll
-  for (int j = 0; j < 2; ++j) xsp[j] = p.xs + min(m0 + 64 * wm + 32 * j + r, p.M - 1) * p.xs_m;
-  const int nb = (p.N + kFp8Block - 1) / kFp8Block;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int b = kGated ? i * nb + min(n0 + 32 * wn, p.N - 1) / kFp8Block : min(n0 + 64 * wn, p.N - 1) / kFp8Block;
-    wsp[i] = p.ws + static_cast<int64_t>(b) * p.nkb + zero;
-  }
-  float xs[2], ws[2];
-  auto request_scales = [&](int kb) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) xs[j] = xsp[j][kb * p.xs_b];
-#pragma unroll
-    for (int i = 0; i < (kGated ? 2 : 1); ++i) ws[i] = wsp[i][kb];
-  };
 
-  float16_t acc[2][2] = {};
+  // lane (r, h) reads chunks 4 h + t of its rows; pair t of a block is two slices of 16 k
   const uint32_t first = 16 * ((4 * h) ^ ((r >> 1) & 7));
   const uint8_t* rows_n = lds + (64 * wn + r) * kFp8Block;
   const uint8_t* rows_m = lds + (Shape::kRowsN + 64 * wm + r) * kFp8Block;
-  request(0);
-  request_scales(0);
+  u32x4_t raw[2][4];  // of two pairs: the rows of the weight's two products, then of x's
+  auto read_codes = [&](int i, uint32_t at, int t) {
+    raw[t & 1][i] =
+        *reinterpret_cast<const u32x4_t*>((i < 2 ? rows_n : rows_m) + 32 * (i & 1) * kFp8Block + at + (first ^ (16 * t)));
+  };
+  bf16x8_t op[2][4];  // operands of two slices
+  float16_t acc[2][2] = {}, part[2][2] = {};
+  float xs[2] = {0.0f, 0.0f}, ws[2] = {0.0f, 0.0f};  // of the block whose sums are in `part`
+
+  // a block's DMAs are spread over eight slices: those of block b from the fifth of
+  // block b - 3, where its stage is free, to the fourth of b - 2
+  constexpr int kPerSlice = (kDmas + 8) / 8, kHead = 4 * kPerSlice < kDmas + 1 ? 4 * kPerSlice : kDmas + 1;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int i = 0; i < (k < 2 ? kDmas + 1 : kHead); ++i) request(i);
+  wait_vmcnt<kDmas + 1 + kHead>();
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) read_codes(i, 0, t);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) op[0][i] = codes8_to_bf16(raw[0][i][0], raw[0][i][1]);
+  int stage = 0;
   for (int kb = 0; kb < p.nkb; ++kb) {
-    wait_vmcnt<0>();
-    __syncthreads();
-    float s[2][2];
+    const int next = stage + 1 == kStages ? 0 : stage + 1;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int q = 0; q < 8; ++q) {
+      if (q == 4) {
+        // the block's codes are in registers, the next one's have landed
+        wait_vmcnt<kDmas + 1>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // four products, and in their shadow the next slice's conversions, reads two
+      // pairs ahead and a DMA
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[i][j] = xs[j] * ws[kGated ? i : 0];
-    if (kb + 1 < p.nkb) {
-      request((kb + 1) & 1);
-      request_scales(kb + 1);
-    }
-    const int at = (kb & 1) * Shape::kStage;
-    Operand32 B[2];
+      for (int t = 0; t < 4; ++t) {
+        const int i = t >> 1, j = t & 1;
+        if (q == 0) {
+          add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
+          asm volatile("" : "+v"(acc[i][j]));  // (here: left to itself the compiler moves the sums behind the loop's branches and copies `part`)
+          part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[0][i], op[0][2 + j], float16_t{}, 0, 0, 0);
+        } else {
+          part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[q & 1][i], op[q & 1][2 + j], part[i][j], 0, 0, 0);
+        }
+        const u32x4_t c = raw[((q + 1) / 2) & 1][t];
+        op[(q + 1) & 1][t] = q & 1 ? codes8_to_bf16(c[0], c[1]) : codes8_to_bf16(c[2], c[3]);
+        if (q % 2 == 0) read_codes(t, (q < 4 ? stage : next) * Shape::kStage, (q / 2 + 2) & 3);
+        if (t == 1) {
+          const int n = (q + 4) % 8 * kPerSlice;  // of block kb + 3 from q = 4 on, else of kb + 2
 #pragma unroll
-    for (int j = 0; j < 2; ++j) B[j].read(rows_m + at + 32 * j * kFp8Block, first);
+          for (int k = n; k < n + kPerSlice && k <= kDmas; ++k) request(k);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (q == 0) {
+        const float* sc =
+            reinterpret_cast<const float*>(lds + kStages * Shape::kStage + stage * 256 * kScaleWaves);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      Operand32 A;
-      A.read(rows_n + at + 32 * i * kFp8Block, first);
+        for (int j = 0; j < 2; ++j) xs[j] = sc[64 * wm + 32 * j + r];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float16_t v = block_sum(A, B[j]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_fmaf(v[e], s[i][j], acc[i][j][e]);
+        for (int i = 0; i < (kGated ? 2 : 1); ++i) ws[i] = sc[64 * kWM + 2 * wn + i];
       }
     }
+    stage = next;
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
+  wait_vmcnt<0>();
 
   // lane (r, h) holds columns 8 q + 4 h + 0..3 of row r of each product
   if constexpr (!kGated) {
