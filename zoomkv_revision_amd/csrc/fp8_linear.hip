@@ -481,6 +481,11 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
       }
+      // a wave behind the other of its SIMD goes first: alone, neither fills it
+      if (q == 4) __builtin_amdgcn_s_setprio(3);
+      if (q == 6) __builtin_amdgcn_s_setprio(2);
+      if (q == 0) __builtin_amdgcn_s_setprio(1);
+      if (q == 2) __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       // four products, and in their shadow the next slice's conversions, reads two
       // pairs ahead and a DMA
