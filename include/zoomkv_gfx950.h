@@ -726,16 +726,19 @@ int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int part
 /* out[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in b} x[m, k] w[n, k]
  * [+ residual[m, n]], fp32 sums rounded once to `type` (out and residual; out may
  * be residual).  K is a multiple of 128, at most 16384; rows of codes start on 16
- * bytes. */
+ * bytes, less than 8 MiB apart.  workspace: zkv_fp8_linear_workspace_size(M, N, K)
+ * bytes (0 for most sizes) on 16, of any content; calls that overlap on one race. */
+size_t zkv_fp8_linear_workspace_size(int M, int N, int K);
 int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b, const uint8_t* w,
                    int64_t w_ld, const float* ws, int M, int N, int K, const void* residual, int64_t res_ld,
-                   void* out, int64_t out_ld, int type, zkv_stream_t stream);
+                   void* out, int64_t out_ld, int type, void* workspace, size_t workspace_bytes,
+                   zkv_stream_t stream);
 
 /* The same for a weight of 2 F rows in two parts, gate and up: codes and scales
  * of silu(gate) * up [M, F] (codes: rows of whole blocks of F, on 8 bytes).
- * workspace: zkv_fp8_gated_workspace_size(M, F) bytes on 16, of any content;
+ * workspace: zkv_fp8_gated_workspace_size(M, F, K) bytes on 16, of any content;
  * calls that overlap on one race. */
-size_t zkv_fp8_gated_workspace_size(int M, int F);
+size_t zkv_fp8_gated_workspace_size(int M, int F, int K);
 int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
                          const uint8_t* w, int64_t w_ld, const float* ws, int M, int F, int K, uint8_t* codes,
                          int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, void* workspace,

@@ -346,7 +346,7 @@ def test_refused_by_the_library():
     from zoomkv_revision_amd._lib import check, lib, ptr
     L = lib()
     args = lambda K, x: (x, 256, ptr(scales), 2, 1, ptr(w.codes), 256, ptr(w.scales), 4, 16, K, None, 0,
-                         ptr(torch.empty(4, 16, device=DEV)), 16, 2, 0)
+                         ptr(torch.empty(4, 16, device=DEV)), 16, 2, None, 0, 0)
     for K, x in ((200, ptr(codes)), (0, ptr(codes)), (256, None), (256, ptr(codes) + 8), (512, ptr(codes))):
         with pytest.raises(ZkvError):
             check(L.zkv_fp8_linear(*args(K, x)))

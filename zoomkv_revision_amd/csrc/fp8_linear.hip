@@ -42,37 +42,30 @@ struct LinearArgs {
   int64_t codes_ld;
   float* scales;
   int64_t s_m, s_b;
-  float* act;                 // [blocks of N][M][128]
-  unsigned long long* slots;  // arrivals per (block of N, group of x rows)
-  unsigned long long epoch;
+  // sums that a second launch goes on with: [part, split][M][sums_ld], the blocks of k
+  // in `splits` runs (null: the output is final)
+  float* sums;
+  int64_t sums_ld;
+  int splits;
 };
 
-// 16 codes as two operands of 8 bf16 values.
-__device__ __forceinline__ void codes_to_bf16(const u32x4_t c, bf16x8_t& lo, bf16x8_t& hi) {
-  u32x4_t a, b;
-#define ZKV_PAIR(w, half) __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, half))
-  a[0] = ZKV_PAIR(c[0], false), a[1] = ZKV_PAIR(c[0], true);
-  a[2] = ZKV_PAIR(c[1], false), a[3] = ZKV_PAIR(c[1], true);
-  b[0] = ZKV_PAIR(c[2], false), b[1] = ZKV_PAIR(c[2], true);
-  b[2] = ZKV_PAIR(c[3], false), b[3] = ZKV_PAIR(c[3], true);
-#undef ZKV_PAIR
-  lo = __builtin_bit_cast(bf16x8_t, a), hi = __builtin_bit_cast(bf16x8_t, b);
+// The part of the weight and the run of blocks [first, last) of a workgroup.
+struct Piece {
+  int part, first, last;
+};
+__device__ __forceinline__ Piece piece_of(const LinearArgs& p) {
+  const int part = blockIdx.z / p.splits, split = blockIdx.z - part * p.splits;
+  return Piece{part, split * p.nkb / p.splits, (split + 1) * p.nkb / p.splits};
 }
 
-// A lane's 32 codes of a row's block, for the 16 x 16 products.
-struct Operand16 {
-  bf16x8_t v[4];
-  __device__ __forceinline__ void set(const u32x4_t a, const u32x4_t b) {
-    codes_to_bf16(a, v[0], v[1]);
-    codes_to_bf16(b, v[2], v[3]);
-  }
-};
-
-__device__ __forceinline__ float4_t block_sum(const Operand16& a, const Operand16& b) {
-  float4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], s, 0, 0, 0);
-  return s;
+// 8 codes as an operand.
+__device__ __forceinline__ bf16x8_t codes8_to_bf16(uint32_t c0, uint32_t c1) {
+  u32x4_t a;
+#define ZKV_PAIR(w, half) __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, half))
+  a[0] = ZKV_PAIR(c0, false), a[1] = ZKV_PAIR(c0, true);
+  a[2] = ZKV_PAIR(c1, false), a[3] = ZKV_PAIR(c1, true);
+#undef ZKV_PAIR
+  return __builtin_bit_cast(bf16x8_t, a);
 }
 
 __device__ __forceinline__ void add_scaled(float4_t& acc, float4_t v, float s) {
@@ -96,237 +89,14 @@ __device__ __forceinline__ void store_out(const LinearArgs& p, int m, int n, flo
   }
 }
 
-// ---------------------------------------------------------------------------
-// Few rows of x: the weights stream from memory into registers.  A unit is R
-// (16, 8 or 4) weight rows (gated: R gate rows and the matching up rows) of 16 kMT rows
-// of x; the waves of a workgroup split its blocks of k (wave w takes blocks w, w +
-// nw, ...), so nothing is staged and every wave reads its own part of x.  Lanes
-// whose A row is past R, or whose B column is past M, repeat the last: no more
-// memory moves.  The waves' sums meet in LDS and are added in wave order.
-// ---------------------------------------------------------------------------
-template <int kTiles, int kMT>
-struct StreamWave {
-  float4_t acc[kTiles][kMT];
-
-  // kCnt blocks, three in flight
-  template <int kCnt>
-  __device__ __forceinline__ void run(const uint8_t* const (&wr)[kTiles], const float* const (&wsr)[kTiles],
-                                      const uint8_t* const (&xr)[kMT], const float* const (&xsr)[kMT], int64_t xs_b,
-                                      int wave, int nw) {
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-      for (int j = 0; j < kMT; ++j) acc[t][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (kCnt > 0) {
-      constexpr int kDepth = kCnt < 3 ? kCnt : 3;
-      u32x4_t a[kDepth][kTiles][2], b[kDepth][kMT][2];
-      float xs[kDepth][kMT], ws[kDepth][kTiles];
-      auto load = [&](int i) {
-        const int kb = wave + i * nw, d = i % kDepth;
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
-          a[d][t][0] = *reinterpret_cast<const u32x4_t*>(wr[t] + kb * kFp8Block);
-          a[d][t][1] = *reinterpret_cast<const u32x4_t*>(wr[t] + kb * kFp8Block + 64);
-          ws[d][t] = wsr[t][kb];
-        }
-#pragma unroll
-        for (int j = 0; j < kMT; ++j) {
-          b[d][j][0] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block);
-          b[d][j][1] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block + 64);
-          xs[d][j] = xsr[j][kb * xs_b];
-        }
-      };
-#pragma unroll
-      for (int i = 0; i < kDepth; ++i) load(i);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < kCnt; ++i) {
-        const int d = i % kDepth;
-        Operand16 A[kTiles];
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) A[t].set(a[d][t][0], a[d][t][1]);
-#pragma unroll
-        for (int j = 0; j < kMT; ++j) {
-          Operand16 B;
-          B.set(b[d][j][0], b[d][j][1]);
-#pragma unroll
-          for (int t = 0; t < kTiles; ++t) add_scaled(acc[t][j], block_sum(A[t], B), xs[d][j] * ws[d][t]);
-        }
-        if (i + kDepth < kCnt) load(i + kDepth);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  }
-};
-
-// The quantised output of one block of 128 gated values for rows [m0, m1): by the
-// workgroup that arrives last there.
-__device__ __forceinline__ void quantise_act(const LinearArgs& p, int jb, int m0, int m1) {
-  const int q = threadIdx.x & 15;
-  for (int m = m0 + (threadIdx.x >> 4); m < m1; m += blockDim.x >> 4) {
-    const unsigned long long* src =
-        reinterpret_cast<const unsigned long long*>(p.act + (static_cast<int64_t>(jb) * p.M + m) * kFp8Block + 8 * q);
-    float y[8];
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned long long v = __hip_atomic_load(src + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      y[2 * i] = __uint_as_float(static_cast<uint32_t>(v));
-      y[2 * i + 1] = __uint_as_float(static_cast<uint32_t>(v >> 32));
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (jb * kFp8Block + 8 * q + i >= p.N) y[i] = 0.0f;
-      amax = max(amax, abs_bits(y[i]));
-    }
-    const float s = fp8_scale(row_max(amax)), r = 1.0f / s;
-    *reinterpret_cast<u32x2_t*>(p.codes + m * p.codes_ld + jb * kFp8Block + 8 * q) =
-        u32x2_t{fp8_codes4(y, s, r), fp8_codes4(y + 4, s, r)};
-    if (q == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
-  }
-}
-
-template <bool kGated, int kMT, int kCnt>
-__global__ __launch_bounds__(1024) void fp8_stream_kernel(const LinearArgs p, int R) {
-  constexpr int kTiles = kGated ? 2 : 1;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][tile][x rows][lane]
-  const int nw = blockDim.x >> 6;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int c = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * R, m0 = blockIdx.y * 16 * kMT;
-  const int row = min(n0 + min(c, R - 1), p.N - 1);
-  const uint8_t *wr[kTiles], *xr[kMT];
-  const float *wsr[kTiles], *xsr[kMT];
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t) {
-    wr[t] = p.w + (static_cast<int64_t>(t) * p.N + row) * p.w_ld + 16 * g;
-    // (R divides 128: a unit lies in one block of rows)
-    wsr[t] = p.ws + static_cast<int64_t>(t * ((p.N + kFp8Block - 1) / kFp8Block) + n0 / kFp8Block) * p.nkb;
-  }
-#pragma unroll
-  for (int j = 0; j < kMT; ++j) {
-    const int m = min(m0 + 16 * j + c, p.M - 1);
-    xr[j] = p.x + m * p.x_ld + 16 * g;
-    xsr[j] = p.xs + m * p.xs_m;
-  }
-  // a wave's blocks are all there but for the last: one without it takes a
-  // straight line of its own
-  const bool full = wave + (kCnt - 1) * nw < p.nkb;
-  StreamWave<kTiles, kMT> s;
-  if (full) {
-    asm volatile("; all blocks");
-    s.template run<kCnt>(wr, wsr, xr, xsr, p.xs_b, wave, nw);
-  } else {
-    asm volatile("; one fewer");
-    s.template run<kCnt - 1>(wr, wsr, xr, xsr, p.xs_b, wave, nw);
-  }
-#pragma unroll
-  for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-    for (int j = 0; j < kMT; ++j) red[((wave * kTiles + t) * kMT + j) * 64 + lane] = s.acc[t][j];
-  __syncthreads();
-  // lane (c, g) holds rows 4 g + i of the unit for row c of x
-  for (int j = wave; j < kMT; j += nw) {
-    float4_t v[kTiles];
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      v[t] = red[(t * kMT + j) * 64 + lane];
-      for (int w = 1; w < nw; ++w) v[t] += red[((w * kTiles + t) * kMT + j) * 64 + lane];
-    }
-    const int m = m0 + 16 * j + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = 4 * g + i, n = n0 + r;
-      if (m >= p.M || r >= R || n >= p.N) continue;
-      if constexpr (kGated)
-        __hip_atomic_store(p.act + (static_cast<int64_t>(n / kFp8Block) * p.M + m) * kFp8Block + n % kFp8Block,
-                           silu_mul(v[0][i], v[kTiles - 1][i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      else
-        store_out(p, m, n, v[0][i]);
-    }
-  }
-  if constexpr (kGated) {
-    // the units of a block of 128 outputs: the last one quantises it.  Values go
-    // out and come back past the L2s, which the XCDs do not share; each lane's
-    // stores have been acknowledged before the workgroup counts itself in
-    __shared__ bool last;
-    const int jb = n0 / kFp8Block;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (threadIdx.x == 0)
-      last = arrive_last(p.slots + static_cast<int64_t>(jb) * gridDim.y + blockIdx.y, p.epoch,
-                         (min(kFp8Block, p.N - jb * kFp8Block) + R - 1) / R);
-    __syncthreads();
-    if (last) quantise_act(p, jb, m0, min(p.M, m0 + 16 * kMT));
-  }
-}
-
-template <bool kGated>
-int launch_stream(const LinearArgs& p, hipStream_t s) {
-  constexpr int kMT = 1;
-  const int R = 8;
-  const int cnt = std::max(std::min(8, (p.nkb + 7) / 8), (p.nkb + 15) / 16);
-  const int nw = (p.nkb + cnt - 1) / cnt;
-  const dim3 grid((p.N + R - 1) / R, (p.M + 16 * kMT - 1) / (16 * kMT));
-  const size_t lds = static_cast<size_t>(nw) * (kGated ? 2 : 1) * kMT * 1024;
-#define ZKV_CNT(C)                                                         \
-  case C:                                                                  \
-    fp8_stream_kernel<kGated, kMT, C><<<grid, 64 * nw, lds, s>>>(p, R);    \
-    break;
-  switch (cnt) {
-    ZKV_CNT(1) ZKV_CNT(2) ZKV_CNT(3) ZKV_CNT(4) ZKV_CNT(5) ZKV_CNT(6) ZKV_CNT(7) ZKV_CNT(8)
-    default:
-      return fail(ZKV_EINVAL, "fp8 linear: %d blocks per wave", cnt);
-  }
-#undef ZKV_CNT
-  return check_launch("fp8_stream_kernel");
-}
-
-// ---------------------------------------------------------------------------
-// Many rows of x: a workgroup of kWN x kWM waves computes 64 kWN weight rows (gated: 32
-// kWN gate rows and the matching up rows) for 64 kWM rows of x, a wave 64 x 64 of
-// it as 2 x 2 products of 32 x 32.  A block of 128 k of the tile's rows goes from
-// memory straight into one of two LDS stages while the other is computed on.
-//
-// LDS: a row is 8 chunks of 16 bytes, chunk c in slot c ^ ((row >> 1) & 7): the 16
-// lanes of a read phase, each with the same chunk of its own row, hit every bank
-// once.  A lane converts its codes after reading them (64 conversions per wave, block
-// and 32 rows): the LDS moves bytes, not bf16.
-// ---------------------------------------------------------------------------
-typedef float float16_t __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ uint32_t lds_offset(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
-}
-
-// 64 lanes x 16 bytes, each at its offset from a base (wave-uniform, as dst), into LDS at dst + 16 lane, not seen by the
-// compiler's wait counts: with the builtin every LDS read waits for all of them.
-__device__ __forceinline__ void dma16_tile(const void* base, uint32_t off, uint32_t dst) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
-}
-
-__device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
-  asm volatile("global_load_lds_dword %0, off" : : "v"(src), "{m0}"(dst) : "memory");
-}
-
-// 8 codes as an operand.
-__device__ __forceinline__ bf16x8_t codes8_to_bf16(uint32_t c0, uint32_t c1) {
-  u32x4_t a;
-#define ZKV_PAIR(w, half) __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, half))
-  a[0] = ZKV_PAIR(c0, false), a[1] = ZKV_PAIR(c0, true);
-  a[2] = ZKV_PAIR(c1, false), a[3] = ZKV_PAIR(c1, true);
-#undef ZKV_PAIR
-  return __builtin_bit_cast(bf16x8_t, a);
-}
-
-__device__ __forceinline__ void add_scaled(float16_t& acc, const float16_t& v, float s) {
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(v[i], s, acc[i]);
-}
-
 // Four neighbouring columns of a row of the output.
 __device__ __forceinline__ void store_out4(const LinearArgs& p, int m, int n, const float (&y)[4], bool vec) {
+  if (p.sums) {  // (rows of whole groups of four)
+    if (n < p.N)
+      *reinterpret_cast<float4_t*>(p.sums + (static_cast<int64_t>(blockIdx.z) * p.M + m) * p.sums_ld + n) =
+          float4_t{y[0], y[1], y[2], y[3]};
+    return;
+  }
   if (!vec || n + 4 > p.N) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -358,7 +128,305 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int m, int n, co
   }
 }
 
-constexpr int kStages = 3;
+// ---------------------------------------------------------------------------
+// Few rows of x, or few tiles: codes go from memory straight into registers.  A
+// workgroup computes 16 kNT weight rows (gated: half of them gate rows, half the matching
+// up rows) for 16 kMT rows of x; its waves split the blocks of k (wave w takes
+// blocks w, w + nw, ...), so nothing is staged, no wave waits for another, and their
+// sums meet in LDS at the end, added in wave order.  A unit may have R < 16 rows per
+// tile, to fill the CUs: lanes past R, N or M repeat the last row, which moves no
+// more memory.
+// ---------------------------------------------------------------------------
+template <int kNT, int kMT, int kDepth>
+struct WaveTile {
+  struct Block {
+    u32x4_t a[kNT][2], b[kMT][2];
+    float ws[kNT], xs[kMT];
+  };
+  const uint8_t *wr[kNT], *xr[kMT];
+  const float *wsr[kNT], *xsr[kMT];
+  int64_t xs_b;
+  float4_t acc[kNT][kMT];
+
+  // tile i: this lane's row of the weight, and the block of rows of its outputs
+  __device__ __forceinline__ void weight(const LinearArgs& p, int i, int part, int row, int block) {
+    wr[i] = p.w + (static_cast<int64_t>(part) * p.N + row) * p.w_ld + 16 * ((threadIdx.x >> 4) & 3);
+    wsr[i] = p.ws + static_cast<int64_t>(part * ((p.N + kFp8Block - 1) / kFp8Block) + block) * p.nkb;
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  __device__ __forceinline__ void rows(const LinearArgs& p, int m0) {
+    xs_b = p.xs_b;
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) {
+      const int m = min(m0 + 16 * j + static_cast<int>(threadIdx.x & 15), p.M - 1);
+      xr[j] = p.x + m * p.x_ld + 16 * ((threadIdx.x >> 4) & 3);
+      xsr[j] = p.xs + m * p.xs_m;
+    }
+  }
+  __device__ __forceinline__ void load_half(Block& v, int kb, int half) const {
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+      v.a[i][half] = *reinterpret_cast<const u32x4_t*>(wr[i] + kb * kFp8Block + 64 * half);
+#pragma unroll
+    for (int j = 0; j < kMT; ++j)
+      v.b[j][half] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block + 64 * half);
+  }
+  __device__ __forceinline__ void load_scales(Block& v, int kb) const {
+#pragma unroll
+    for (int i = 0; i < kNT; ++i) v.ws[i] = wsr[i][kb];
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) v.xs[j] = xsr[j][kb * xs_b];
+  }
+  __device__ __forceinline__ void load(Block& v, int kb) const {
+    load_half(v, kb, 0);
+    load_half(v, kb, 1);
+    load_scales(v, kb);
+  }
+  // adds a block; next >= 0: and loads that one in its place, as soon as a half has
+  // been converted
+  template <bool kNext>
+  __device__ __forceinline__ void add(Block& v, int next) {
+    float4_t part[kNT][kMT];
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        bf16x8_t A[kNT], B[kMT];
+#pragma unroll
+        for (int i = 0; i < kNT; ++i) A[i] = codes8_to_bf16(v.a[i][half][2 * q], v.a[i][half][2 * q + 1]);
+#pragma unroll
+        for (int j = 0; j < kMT; ++j) B[j] = codes8_to_bf16(v.b[j][half][2 * q], v.b[j][half][2 * q + 1]);
+        if (kNext && q == 1) load_half(v, next, half);
+#pragma unroll
+        for (int i = 0; i < kNT; ++i)
+#pragma unroll
+          for (int j = 0; j < kMT; ++j)
+            part[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                A[i], B[j], half + q ? part[i][j] : float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+      }
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int j = 0; j < kMT; ++j) add_scaled(acc[i][j], part[i][j], v.xs[j] * v.ws[i]);
+    if (kNext) load_scales(v, next);
+  }
+
+  // blocks first, first + step, ... below nkb, kDepth of them in flight
+  template <int kCnt>
+  __device__ __forceinline__ void run_all(int first, int step) {
+    if constexpr (kCnt > 0) {
+      constexpr int kD = kCnt < kDepth ? kCnt : kDepth;
+      Block v[kD];
+#pragma unroll
+      for (int i = 0; i < kD; ++i) load(v[i], first + i * step);
+      // (the barriers keep the loads where they are: the compiler sinks them to their uses)
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kCnt; ++i) {
+        if (i + kD < kCnt)
+          add<true>(v[i % kD], first + (i + kD) * step);
+        else
+          add<false>(v[i % kD], 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+  // kCnt > 0: each wave has kCnt blocks or one fewer, and a straight line for either
+  // (a load that some path skips makes the compiler wait for all of them)
+  template <int kCnt>
+  __device__ __forceinline__ void run(int first, int step, int nkb) {
+    if constexpr (kCnt > 0) {
+      if (first + (kCnt - 1) * step < nkb) {
+        asm volatile("; all blocks");
+        run_all<kCnt>(first, step);
+      } else {
+        asm volatile("; one fewer");
+        run_all<kCnt - 1>(first, step);
+      }
+    } else {
+      const int cnt = (nkb - first + step - 1) / step;
+      Block v[kDepth];
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (d < cnt) load(v[d], first + d * step);
+      int i = 0;
+      for (; i + 2 * kDepth <= cnt; i += kDepth) {
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+          add<true>(v[d], first + (i + kDepth + d) * step);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      // fewer than 2 kDepth blocks are left, kDepth of them loaded
+#pragma unroll
+      for (int t = 0; t < 2 * kDepth - 1; ++t) {
+        if (i + t < cnt) {
+          if (i + t + kDepth < cnt)
+            add<true>(v[t % kDepth], first + (i + t + kDepth) * step);
+          else
+            add<false>(v[t % kDepth], 0);
+        }
+      }
+    }
+  }
+};
+
+// kCnt > 0: so many blocks per wave, three in flight; 0: any number.
+template <int kNT, int kMT, int kWaves, int kCnt>
+__global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArgs p, int R, int vec) {
+  __shared__ float4_t red[kWaves * kNT * kMT * 64];  // [wave][weight tile][x tile][lane]
+  const int nw = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * R * kNT, m0 = blockIdx.y * 16 * kMT;
+  const Piece piece = piece_of(p);
+  WaveTile<kNT, kMT, kNT * kMT == 1 ? 3 : kNT * kMT == 4 ? 2 : 1> w;
+#pragma unroll
+  for (int i = 0; i < kNT; ++i) {
+    const int top = n0 + i * R;
+    // (the lane's four output columns lie in one block: R is a multiple of 4)
+    w.weight(p, i, piece.part, min(top + min(c, R - 1), p.N - 1), min(top + min(4 * g, R - 4), p.N - 1) / kFp8Block);
+  }
+  w.rows(p, m0);
+  w.template run<kCnt>(piece.first + wave, nw, piece.last);
+#pragma unroll
+  for (int i = 0; i < kNT; ++i)
+#pragma unroll
+    for (int j = 0; j < kMT; ++j) red[((wave * kNT + i) * kMT + j) * 64 + lane] = w.acc[i][j];
+  __syncthreads();
+  // lane (c, g) holds columns 4 g + 0..3 of a tile for row c of x
+  for (int t = wave; t < kNT * kMT; t += nw) {
+    const float4_t* src = red + t * 64 + lane;
+    float4_t v = src[0];
+    for (int k = 1; k < nw; ++k) v += src[k * kNT * kMT * 64];
+    const int m = m0 + 16 * (t % kMT) + c, n = n0 + t / kMT * R + 4 * g;
+    if (m >= p.M || 4 * g >= R) continue;
+    const float y[4] = {v[0], v[1], v[2], v[3]};
+    store_out4(p, m, n, y, vec);
+  }
+}
+
+int out_vec(const LinearArgs& p) {
+  const int item = p.type == kRowF32 ? 4 : 2;
+  return reinterpret_cast<uintptr_t>(p.out) % (4 * item) == 0 && p.out_ld % 4 == 0 &&
+         (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
+}
+
+// One tile of 16 weight rows and 16 rows of x per workgroup.
+int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
+  const int nw = std::min(p.nkb, p.nkb > 32 ? 16 : 4);
+  // (every wave has cnt or cnt - 1 of the blocks)
+  const int cnt = (p.nkb + nw - 1) / nw;
+  // rows per unit: the number of units is rounded up to whole rounds of 256 CUs
+  const int units = ((p.N + 15) / 16 + 255) / 256 * 256;
+  const int R = std::min(16, ((p.N + units - 1) / units + 3) / 4 * 4);
+  const dim3 grid((p.N + R - 1) / R, (p.M + 15) / 16, parts);
+#define ZKV_CNT(C)                                                                        \
+  case C:                                                                                 \
+    fp8_stream_kernel<1, 1, 16, C><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));            \
+    break;
+  switch (cnt) {
+    ZKV_CNT(1) ZKV_CNT(2) ZKV_CNT(3) ZKV_CNT(4) ZKV_CNT(5) ZKV_CNT(6) ZKV_CNT(7) ZKV_CNT(8)
+    default:
+      return fail(ZKV_EINVAL, "fp8 linear: %d blocks per wave", cnt);
+  }
+#undef ZKV_CNT
+  return check_launch("fp8_stream_kernel");
+}
+
+// 16 kNT weight rows and 16 kMT rows of x per workgroup.
+template <int kNT, int kMT>
+int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
+  const int nw = std::min(p.nkb, 8);
+  const dim3 grid((p.N + 16 * kNT - 1) / (16 * kNT), (p.M + 16 * kMT - 1) / (16 * kMT), parts);
+  fp8_stream_kernel<kNT, kMT, 8, 0><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
+  return check_launch("fp8_stream_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// The second launch where the first left sums: the splits added in order, then the
+// output's residual and rounding, or silu(gate) * up as codes.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float4_t sum_of(const LinearArgs& p, int part, int m, int n) {
+  const float* src = p.sums + (static_cast<int64_t>(part) * p.splits * p.M + m) * p.sums_ld + n;
+  float4_t v = *reinterpret_cast<const float4_t*>(src);
+  for (int k = 1; k < p.splits; ++k) v += *reinterpret_cast<const float4_t*>(src + k * p.M * p.sums_ld);
+  return v;
+}
+
+__global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p, int vec) {
+  const int n = 4 * (blockIdx.y * 256 + threadIdx.x), m = blockIdx.x;
+  if (n >= p.N) return;
+  const float4_t v = sum_of(p, 0, m, n);
+  LinearArgs q = p;
+  q.sums = nullptr;
+  const float y[4] = {v[0], v[1], v[2], v[3]};
+  store_out4(q, m, n, y, vec);
+}
+
+// 16 lanes per row and block of 128 outputs, 8 outputs each.
+__global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p) {
+  const int jb = blockIdx.y, m = blockIdx.x * 16 + (threadIdx.x >> 4), n = jb * kFp8Block + 8 * (threadIdx.x & 15);
+  if (m >= p.M) return;  // (whole groups of 16 lanes)
+  float y[8];
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float4_t g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
+    if (n + 4 * i < p.N) g = sum_of(p, 0, m, n + 4 * i), u = sum_of(p, 1, m, n + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[4 * i + e] = n + 4 * i + e < p.N ? silu_mul(g[e], u[e]) : 0.0f;
+      a = max(a, abs_bits(y[4 * i + e]));
+    }
+  }
+  const float s = fp8_scale(row_max(a)), r = 1.0f / s;
+  *reinterpret_cast<u32x2_t*>(p.codes + m * p.codes_ld + n) = u32x2_t{fp8_codes4(y, s, r), fp8_codes4(y + 4, s, r)};
+  if ((threadIdx.x & 15) == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
+}
+
+int launch_join(const LinearArgs& p, hipStream_t s) {
+  fp8_join_kernel<<<dim3(p.M, (p.N + 1023) / 1024), 256, 0, s>>>(p, out_vec(p));
+  return check_launch("fp8_join_kernel");
+}
+
+int launch_gated_join(const LinearArgs& p, hipStream_t s) {
+  fp8_gated_join_kernel<<<dim3((p.M + 15) / 16, (p.N + kFp8Block - 1) / kFp8Block), 256, 0, s>>>(p);
+  return check_launch("fp8_gated_join_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// Many rows of x: a workgroup of kWN x kWM waves computes 64 kWN weight rows (gated: 32
+// kWN gate rows and the matching up rows) for 64 kWM rows of x, a wave 64 x 64 of
+// it as 2 x 2 products of 32 x 32.  A block of 128 k of the tile's rows goes from
+// memory straight into one of two LDS stages while the other is computed on.
+//
+// LDS: a row is 8 chunks of 16 bytes, chunk c in slot c ^ ((row >> 1) & 7): the 16
+// lanes of a read phase, each with the same chunk of its own row, hit every bank
+// once.  A lane converts its codes after reading them (64 conversions per wave, block
+// and 32 rows): the LDS moves bytes, not bf16.
+// ---------------------------------------------------------------------------
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
+}
+
+// 64 lanes x 16 bytes, each at its offset from a base (wave-uniform, as dst), into LDS at dst + 16 lane, not seen by the
+// compiler's wait counts: with the builtin every LDS read waits for all of them.
+__device__ __forceinline__ void dma16_tile(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
+}
+
+__device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
+  asm volatile("global_load_lds_dword %0, off" : : "v"(src), "{m0}"(dst) : "memory");
+}
+
+__device__ __forceinline__ void add_scaled(float16_t& acc, const float16_t& v, float s) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(v[i], s, acc[i]);
+}
 
 template <bool kGated, int kWN, int kWM>
 struct TileShape {
@@ -367,7 +435,7 @@ struct TileShape {
   static constexpr int kStage = (kRowsN + kRowsM) * kFp8Block;
 };
 
-template <bool kGated, int kWN, int kWM>
+template <bool kGated, int kWN, int kWM, int kStages>
 __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const LinearArgs p, int tiles_n, int tiles_m,
                                                                     int vec) {
   using Shape = TileShape<kGated, kWN, kWM>;
@@ -387,6 +455,7 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   const int band = t / (4 * tiles_m), in_band = t - band * 4 * tiles_m, width = min(4, tiles_n - 4 * band);
   const int tn = 4 * band + in_band % width, tm = in_band / width;
   const int n0 = tn * Shape::kCols, m0 = tm * Shape::kRowsM;
+  const Piece piece = piece_of(p);
 
   // where the DMAs read: eight rows of 128 bytes each, slots permuted, at a lane's
   // offset from a row of the wave's (host side: rows at most 8 MiB apart)
@@ -397,13 +466,13 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
     const int top = 8 * (wave * kDmas + i), row = top + (lane >> 3);
     const uint32_t chunk = (lane & 7) ^ ((row >> 1) & 7);
     if (top >= Shape::kRowsN) {
-      src[i] = p.x + m0 * p.x_ld;
+      src[i] = p.x + m0 * p.x_ld + piece.first * kFp8Block;
       off[i] = min(row - Shape::kRowsN, p.M - 1 - m0) * static_cast<uint32_t>(p.x_ld) + 16 * chunk;
     } else if (kGated) {  // 32 gate rows and the 32 matching up rows in turn
-      src[i] = p.w + (static_cast<int64_t>(n0) + (top & 32 ? p.N : 0)) * p.w_ld;
+      src[i] = p.w + (static_cast<int64_t>(n0) + (top & 32 ? p.N : 0)) * p.w_ld + piece.first * kFp8Block;
       off[i] = min((row >> 6) * 32 + (row & 31), p.N - 1 - n0) * static_cast<uint32_t>(p.w_ld) + 16 * chunk;
     } else {
-      src[i] = p.w + n0 * p.w_ld;
+      src[i] = p.w + (static_cast<int64_t>(piece.part) * p.N + n0) * p.w_ld + piece.first * kFp8Block;
       off[i] = min(row, p.N - 1 - n0) * static_cast<uint32_t>(p.w_ld) + 16 * chunk;
     }
   }
@@ -416,21 +485,21 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   {
     const int w = wave % kScaleWaves;
     if (w < kWM) {
-      scale_src = p.xs + min(m0 + 64 * w + lane, p.M - 1) * p.xs_m;
+      scale_src = p.xs + min(m0 + 64 * w + lane, p.M - 1) * p.xs_m + piece.first * p.xs_b;
       scale_step = p.xs_b;
     } else {
-      const int nb = (p.N + kFp8Block - 1) / kFp8Block, part = lane & 1, group = (lane >> 1) % kWN;
-      const int n = min(n0 + (kGated ? 32 : 64) * group, p.N - 1);
-      scale_src = p.ws + static_cast<int64_t>((kGated ? part * nb : 0) + n / kFp8Block) * p.nkb;
+      const int nb = (p.N + kFp8Block - 1) / kFp8Block, part = kGated ? lane & 1 : piece.part;
+      const int n = min(n0 + (kGated ? 32 : 64) * ((lane >> 1) % kWN), p.N - 1);
+      scale_src = p.ws + static_cast<int64_t>(part * nb + n / kFp8Block) * p.nkb + piece.first;
       scale_step = 1;
     }
   }
   const uint32_t scale_dst = lds_offset(lds) + kStages * Shape::kStage + (wave % kScaleWaves) * 256;
   // the i-th DMA of the block that is requested next, into its stage; past the last
   // block they repeat it, which keeps the counts of what is in flight
-  int req = 0, req_stage = 0;
+  int req = piece.first, req_stage = 0;
   auto request = [&](int i) {
-    const int step = req + 1 < p.nkb ? 1 : 0;
+    const int step = req + 1 < piece.last ? 1 : 0;
     if (i < kDmas) {
       dma16_tile(src[i], off[i], __builtin_amdgcn_readfirstlane(dst + req_stage * Shape::kStage + i * 1024));
       src[i] += step * kFp8Block;
@@ -455,9 +524,12 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   float16_t acc[2][2] = {}, part[2][2] = {};
   float xs[2] = {0.0f, 0.0f}, ws[2] = {0.0f, 0.0f};  // of the block whose sums are in `part`
 
-  // a block's DMAs are spread over eight slices: those of block b from the fifth of
-  // block b - 3, where its stage is free, to the fourth of b - 2
-  constexpr int kPerSlice = (kDmas + 8) / 8, kHead = 4 * kPerSlice < kDmas + 1 ? 4 * kPerSlice : kDmas + 1;
+  // Three stages: a block's DMAs are spread over eight slices, those of block b from the
+  // fifth of block b - 3, where its stage is free, to the fourth of b - 2, and have landed
+  // a block later.  Two stages: over four, from the fifth of block b - 2.
+  static_assert(kStages == 2 || kStages == 3, "");
+  constexpr int kSlices = kStages == 3 ? 8 : 4, kPerSlice = (kDmas + kSlices) / kSlices;
+  constexpr int kHead = kStages == 2 ? 0 : 4 * kPerSlice < kDmas + 1 ? 4 * kPerSlice : kDmas + 1;
 #pragma unroll
   for (int k = 0; k < 3; ++k)
 #pragma unroll
@@ -471,13 +543,13 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
 #pragma unroll
   for (int i = 0; i < 4; ++i) op[0][i] = codes8_to_bf16(raw[0][i][0], raw[0][i][1]);
   int stage = 0;
-  for (int kb = 0; kb < p.nkb; ++kb) {
+  for (int kb = piece.first; kb < piece.last; ++kb) {
     const int next = stage + 1 == kStages ? 0 : stage + 1;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       if (q == 4) {
         // the block's codes are in registers, the next one's have landed
-        wait_vmcnt<kDmas + 1>();
+        wait_vmcnt<kStages == 3 ? kDmas + 1 : 0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
       }
@@ -503,7 +575,7 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
         op[(q + 1) & 1][t] = q & 1 ? codes8_to_bf16(c[0], c[1]) : codes8_to_bf16(c[2], c[3]);
         if (q % 2 == 0) read_codes(t, (q < 4 ? stage : next) * Shape::kStage, (q / 2 + 2) & 3);
         if (t == 1) {
-          const int n = (q + 4) % 8 * kPerSlice;  // of block kb + 3 from q = 4 on, else of kb + 2
+          const int n = (q + 4) % 8 * kPerSlice;  // of block kb + kStages from q = 4 on, else of kb + 2
 #pragma unroll
           for (int k = n; k < n + kPerSlice && k <= kDmas; ++k) request(k);
         }
@@ -576,16 +648,88 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   }
 }
 
-template <bool kGated, int kWN, int kWM>
-int launch_tile(const LinearArgs& p, hipStream_t s) {
+template <bool kGated, int kWN, int kWM, int kStages>
+int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
   using Shape = TileShape<kGated, kWN, kWM>;
   const int tiles_n = (p.N + Shape::kCols - 1) / Shape::kCols, tiles_m = (p.M + Shape::kRowsM - 1) / Shape::kRowsM;
-  const int item = p.type == kRowF32 ? 4 : 2;
-  const int vec = !kGated && reinterpret_cast<uintptr_t>(p.out) % (4 * item) == 0 && p.out_ld % 4 == 0 &&
-                  (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
-  const unsigned grid = (static_cast<unsigned>(tiles_n) * tiles_m + 7) / 8 * 8;
-  fp8_tile_kernel<kGated, kWN, kWM><<<grid, 64 * kWN * kWM, 0, s>>>(p, tiles_n, tiles_m, vec);
+  const dim3 grid((static_cast<unsigned>(tiles_n) * tiles_m + 7) / 8 * 8, 1, parts * p.splits);
+  fp8_tile_kernel<kGated, kWN, kWM, kStages><<<grid, 64 * kWN * kWM, 0, s>>>(p, tiles_n, tiles_m, out_vec(p));
   return check_launch("fp8_tile_kernel");
+}
+
+// ---------------------------------------------------------------------------
+// Which kernel, and in how many runs of k: the shortest by a model of their times, in
+// us: a start, and a time per block of k that grows as the CUs fill (which lowers the
+// clock).  Over 31 sizes of 17 to 16000 rows its choice took 1.04 times the best of the 15 that
+// were measured for each (geometric mean; at worst 1.3).
+// ---------------------------------------------------------------------------
+enum Variant : int { kStream, kSplit32, kSplit64, kTileBig, kTileMid, kTileFlat, kTileGated };
+
+struct Plan {
+  int variant, splits;
+  bool sums;
+};
+
+struct Pace {
+  double start;    // until the first block and behind the last
+  int most;        // workgroups at a time on a CU
+  double step[3];  // a block's time with 1, 2, 3 of them there
+};
+
+double rounds_us(int64_t groups, int steps, const Pace& pace) {
+  const int64_t per_round = 256 * pace.most, full = groups / per_round, rest = groups % per_round;
+  double us = pace.start + full * steps * pace.step[pace.most - 1];
+  if (rest) {
+    const int c = static_cast<int>((rest + 255) / 256);
+    const double low = c > 1 ? pace.step[c - 2] : 0.8 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
+    us += steps * (low + fill * (pace.step[c - 1] - low));
+  }
+  return us + 0.6 * pace.start * (full + (rest > 0) - 1);
+}
+
+int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
+
+// M rows of x, N weight rows in each of `parts`.  Two parts, gate and up, leave sums
+// for a second launch, but for the kernel that computes whole blocks of outputs.
+Plan plan_product(int M, int N, int nkb, int parts) {
+  const bool gated = parts == 2;
+  if (M <= 16) return Plan{kStream, 1, gated};
+  constexpr Pace kSplit32Pace{2.3, 1, {2.0}}, kSplit64Pace{2.3, 1, {3.0}}, kBigPace{4.6, 1, {1.62}},
+      kMidPace{4.6, 2, {1.08, 1.9}}, kFlatPace{4.6, 3, {0.95, 1.35, 1.8}};
+  Plan best{kTileBig, 1, gated};
+  double best_us = 1e30;
+  auto consider = [&](int variant, int splits, int64_t tiles, int steps, const Pace& pace, bool own) {
+    const bool sums = !own && (gated || splits > 1);
+    double us = rounds_us(tiles * splits * (own ? 1 : parts), steps, pace);
+    if (sums) us += 3.5 + 8.0 * parts * splits * M * static_cast<double>(N) / 6.5e6;  // (out and back)
+    if (us < best_us) best_us = us, best = Plan{variant, splits, sums};
+  };
+  consider(kSplit32, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 7) / 8, kSplit32Pace, false);
+  consider(kSplit64, 1, tiles_of(N, 32) * tiles_of(M, 64), (nkb + 7) / 8, kSplit64Pace, false);
+  for (int k = 1; k <= 8 && 2 * k <= nkb + 1; ++k) {
+    const int steps = (nkb + k - 1) / k;
+    consider(kTileBig, k, tiles_of(N, 256) * tiles_of(M, 128), steps, kBigPace, false);
+    consider(kTileMid, k, tiles_of(N, 128) * tiles_of(M, 128), steps, kMidPace, false);
+    consider(kTileFlat, k, tiles_of(N, 128) * tiles_of(M, 64), steps, kFlatPace, false);
+  }
+  if (gated) consider(kTileGated, 1, tiles_of(N, 128) * tiles_of(M, 128), nkb, kBigPace, true);
+  return best;
+}
+
+int launch_variant(const LinearArgs& p, int variant, int parts, hipStream_t s) {
+  switch (variant) {
+    case kStream: return launch_stream(p, parts, s);
+    case kSplit32: return launch_split<2, 2>(p, parts, s);
+    case kSplit64: return launch_split<2, 4>(p, parts, s);
+    case kTileBig: return launch_tile<false, 4, 2, 3>(p, parts, s);
+    case kTileMid: return launch_tile<false, 2, 2, 2>(p, parts, s);
+    case kTileFlat: return launch_tile<false, 2, 1, 2>(p, parts, s);
+    default: return launch_tile<true, 4, 2, 3>(p, 1, s);
+  }
+}
+
+size_t sums_bytes(const Plan& plan, int parts, int M, int N) {
+  return plan.sums ? static_cast<size_t>(parts) * plan.splits * M * ((N + 3) / 4 * 4) * 4 : 0;
 }
 
 int blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
@@ -598,6 +742,7 @@ const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, cons
   if (K % kFp8Block || K > 128 * kFp8Block) return "K is a multiple of 128, at most 16384";
   if (x_ld < K || w_ld < K || !rows_on_16(x, x_ld, 1) || !rows_on_16(w, w_ld, 1))
     return "rows of codes hold K bytes and start on 16";
+  if (x_ld >= 1 << 23 || w_ld >= 1 << 23) return "rows of codes lie less than 8 MiB apart";
   return nullptr;
 }
 
@@ -606,26 +751,35 @@ const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, cons
 
 using namespace zkv;
 
+extern "C" size_t zkv_fp8_linear_workspace_size(int M, int N, int K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return sums_bytes(plan_product(M, N, blocks_of(K), 1), 1, M, N);
+}
+
 extern "C" int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
                               const uint8_t* w, int64_t w_ld, const float* ws, int M, int N, int K,
                               const void* residual, int64_t res_ld, void* out, int64_t out_ld, int type,
-                              zkv_stream_t stream) {
+                              void* workspace, size_t workspace_bytes, zkv_stream_t stream) {
   const char* bad = check_operands(x, x_ld, xs, w, w_ld, ws, M, N, K);
   ZKV_REQUIRE(!bad, "zkv_fp8_linear: %s (M=%d N=%d K=%d)", bad, M, N, K);
   ZKV_REQUIRE(out && type >= kRowBf16 && type <= kRowF32, "zkv_fp8_linear: bad output");
+  const Plan plan = plan_product(M, N, K / kFp8Block, 1);
+  const size_t need = sums_bytes(plan, 1, M, N);
+  if (need && (workspace_bytes < need || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(ZKV_ESPACE, "zkv_fp8_linear: %zu bytes of workspace on 16 bytes, %zu needed", workspace_bytes, need);
   LinearArgs p{};
   p.x = x, p.x_ld = x_ld, p.xs = xs, p.xs_m = xs_m, p.xs_b = xs_b, p.w = w, p.w_ld = w_ld, p.ws = ws;
   p.M = M, p.N = N, p.nkb = K / kFp8Block;
   p.res = residual, p.res_ld = res_ld, p.out = out, p.out_ld = out_ld, p.type = type;
+  p.sums = plan.sums ? static_cast<float*>(workspace) : nullptr, p.sums_ld = (N + 3) / 4 * 4, p.splits = plan.splits;
   auto s = reinterpret_cast<hipStream_t>(stream);
-  if (M <= 64) return launch_stream<false>(p, s);
-  return launch_tile<false, 4, 2>(p, s);
+  const int rc = launch_variant(p, plan.variant, 1, s);
+  return rc != ZKV_OK || !plan.sums ? rc : launch_join(p, s);
 }
 
-extern "C" size_t zkv_fp8_gated_workspace_size(int M, int F) {
-  if (M < 1 || F < 1) return 0;
-  const size_t nb = blocks_of(F);
-  return (nb * ((M + 15) / 16) * 8 + 255) / 256 * 256 + nb * M * kFp8Block * 4;
+extern "C" size_t zkv_fp8_gated_workspace_size(int M, int F, int K) {
+  if (M < 1 || F < 1 || K < 1) return 0;
+  return sums_bytes(plan_product(M, F, blocks_of(K), 2), 2, M, F);
 }
 
 extern "C" int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b,
@@ -637,19 +791,17 @@ extern "C" int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float*
   ZKV_REQUIRE(codes && scales && codes_ld >= static_cast<int64_t>(blocks_of(F)) * kFp8Block && codes_ld % 8 == 0 &&
                   (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
               "zkv_fp8_gated_linear: rows of codes hold whole blocks of 128 and start on 8 bytes");
-  const size_t need = zkv_fp8_gated_workspace_size(M, F);
-  if (workspace_bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+  const Plan plan = plan_product(M, F, K / kFp8Block, 2);
+  const size_t need = sums_bytes(plan, 2, M, F);
+  if (need && (workspace_bytes < need || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
     return fail(ZKV_ESPACE, "zkv_fp8_gated_linear: %zu bytes of workspace on 16 bytes, %zu needed", workspace_bytes,
                 need);
   LinearArgs p{};
   p.x = x, p.x_ld = x_ld, p.xs = xs, p.xs_m = xs_m, p.xs_b = xs_b, p.w = w, p.w_ld = w_ld, p.ws = ws;
   p.M = M, p.N = F, p.nkb = K / kFp8Block;
   p.codes = codes, p.codes_ld = codes_ld, p.scales = scales, p.s_m = s_m, p.s_b = s_b;
-  p.slots = static_cast<unsigned long long*>(workspace);
-  p.act = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) +
-                                   (static_cast<size_t>(blocks_of(F)) * ((M + 15) / 16) * 8 + 255) / 256 * 256);
-  p.epoch = next_epoch();
+  p.sums = plan.sums ? static_cast<float*>(workspace) : nullptr, p.sums_ld = (F + 3) / 4 * 4, p.splits = plan.splits;
   auto s = reinterpret_cast<hipStream_t>(stream);
-  if (M <= 64) return launch_stream<true>(p, s);
-  return launch_tile<true, 4, 2>(p, s);
+  const int rc = launch_variant(p, plan.variant, 2, s);
+  return rc != ZKV_OK || !plan.sums ? rc : launch_gated_join(p, s);
 }

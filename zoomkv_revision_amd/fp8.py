@@ -246,6 +246,8 @@ def _check_product(codes, scales, weight: Fp8Weight, parts: int):
     if rows < parts or rows % parts or rows >= 1 << 24 or M >= 1 << 20:
         raise ValueError(f"a product of {M} rows with a weight of {rows} rows in {parts} part(s)")
     x_ld = _check_codes("codes", codes, M, K, 16)
+    if max(x_ld, weight.codes.stride(0)) >= 1 << 23:
+        raise ValueError("rows of codes must lie less than 8 MiB apart")
     s_m, s_b = _check_scales("scales", scales, M, K, apart=False)
     w_ld = _check_codes("the weight's codes", weight.codes, rows, K, 16)
     nb = parts * blocks(rows // parts)
@@ -261,8 +263,18 @@ def _check_product(codes, scales, weight: Fp8Weight, parts: int):
 # ---------------------------------------------------------------------------
 # products
 # ---------------------------------------------------------------------------
-def _linear_args(codes, scales, weight, out, out_dtype, residual):
-    M, N, _, operands = _check_product(codes, scales, weight, 1)
+def _workspace(need: int, given: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    """The workspace of a call, whose content does not matter: of its own unless
+    one is given (so calls on other streams, and graphs, never share one)."""
+    ws = torch.empty(need, dtype=torch.uint8, device=like.device) if given is None else given
+    if ws.dtype != torch.uint8 or ws.numel() < need or not ws.is_contiguous() or (need and ws.data_ptr() % 16):
+        raise ValueError(f"workspace must be contiguous uint8 of at least {need} bytes on 16 bytes")
+    _same_device(like, workspace=ws)
+    return ws
+
+
+def _linear_args(codes, scales, weight, out, out_dtype, residual, workspace):
+    M, N, K, operands = _check_product(codes, scales, weight, 1)
     if out is None:
         _check_type("out_dtype", out_dtype)
         out = torch.empty(M, N, dtype=out_dtype, device=codes.device)
@@ -278,28 +290,34 @@ def _linear_args(codes, scales, weight, out, out_dtype, residual):
             raise ValueError("out must be the residual itself or lie apart from it")
     _same_device(codes, out=out, residual=residual)
     require_gpu(codes)
-    args = (*operands, ptr(residual), res_ld, ptr(out), out_ld, kind)
-    return args, out, (codes, scales, weight.codes, weight.scales, residual, out)
+    ws = _workspace(lib().zkv_fp8_linear_workspace_size(M, N, K), workspace, codes)
+    args = (*operands, ptr(residual), res_ld, ptr(out), out_ld, kind, ptr(ws), ws.numel())
+    return args, out, (codes, scales, weight.codes, weight.scales, residual, out, ws)
 
 
 class LinearPlan(_Plan):
-    """``linear`` with its checks done once for fixed buffers."""
+    """``linear`` with its checks done once for fixed buffers.  A plan has a
+    workspace of its own unless one is given; runs of one plan must not overlap on
+    the device."""
 
-    def __init__(self, codes, scales, weight, out=None, out_dtype=torch.bfloat16, residual=None):
-        args, result, keep = _linear_args(codes, scales, weight, out, out_dtype, residual)
+    def __init__(self, codes, scales, weight, out=None, out_dtype=torch.bfloat16, residual=None, workspace=None):
+        args, result, keep = _linear_args(codes, scales, weight, out, out_dtype, residual, workspace)
         super().__init__(lib().zkv_fp8_linear if codes.shape[0] else _nothing, codes.device, args, result, keep)
 
 
 def linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor | None = None,
-           out_dtype: torch.dtype = torch.bfloat16, residual: torch.Tensor | None = None) -> torch.Tensor:
+           out_dtype: torch.dtype = torch.bfloat16, residual: torch.Tensor | None = None,
+           workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Rows (codes [M, K], scales float32 [M, K / 128] of any strides) times
     weight.T [+ residual]: [M, rows of the weight] in bf16, fp16 or fp32, rounded
-    once.  out may be the residual."""
-    return LinearPlan(codes, scales, weight, out, out_dtype, residual).run()
+    once.  out may be the residual.  The workspace (uint8,
+    zkv_fp8_linear_workspace_size(M, N, K) bytes: where few tiles meet a long K)
+    needs no clearing; calls that overlap on one race."""
+    return LinearPlan(codes, scales, weight, out, out_dtype, residual, workspace).run()
 
 
 def _gated_args(codes, scales, weight, out_codes, out_scales, workspace):
-    M, F, _, operands = _check_product(codes, scales, weight, 2)
+    M, F, K, operands = _check_product(codes, scales, weight, 2)
     out_codes = _new_codes(M, F, codes) if out_codes is None else out_codes
     out_scales = _new_scales(M, F, codes) if out_scales is None else out_scales
     codes_ld = _check_codes("out_codes", out_codes, M, F, 8)
@@ -308,11 +326,8 @@ def _gated_args(codes, scales, weight, out_codes, out_scales, workspace):
         if _overlap(a, b):
             raise ValueError(f"{name} must lie apart from the input")
     require_gpu(codes)
-    need = lib().zkv_fp8_gated_workspace_size(M, F)
-    ws = torch.empty(need, dtype=torch.uint8, device=codes.device) if workspace is None else workspace
-    if ws.dtype != torch.uint8 or ws.numel() < need or not ws.is_contiguous() or ws.data_ptr() % 16:
-        raise ValueError(f"workspace must be contiguous uint8 of at least {need} bytes on 16 bytes")
-    _same_device(codes, out_codes=out_codes, out_scales=out_scales, workspace=ws)
+    ws = _workspace(lib().zkv_fp8_gated_workspace_size(M, F, K), workspace, codes)
+    _same_device(codes, out_codes=out_codes, out_scales=out_scales)
     args = (*operands, ptr(out_codes), codes_ld, ptr(out_scales), s_m, s_b, ptr(ws), ws.numel())
     return args, (out_codes, out_scales), (codes, scales, weight.codes, weight.scales, out_codes, out_scales, ws)
 
@@ -329,10 +344,9 @@ class GatedLinearPlan(_Plan):
 
 def gated_linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out_codes: torch.Tensor | None = None,
                  out_scales: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
-    """silu(gate) * up of a gated feed-forward block, one launch: gate and up are
-    the rows (codes, scales) times the two parts of the weight ([2 F, K], parts =
+    """silu(gate) * up of a gated feed-forward block: gate and up are the rows (codes, scales) times the two parts of the weight ([2 F, K], parts =
     2); returns codes [M, ceil(F / 128) * 128] and scales float32 [M, ceil(F /
     128)] (new ones as columns of M), what ``linear`` takes for the down
-    projection.  The workspace (uint8, zkv_fp8_gated_workspace_size(M, F) bytes)
-    needs no clearing; calls that overlap on one race."""
+    projection.  The workspace (uint8, zkv_fp8_gated_workspace_size(M, F, K)
+    bytes) needs no clearing; calls that overlap on one race."""
     return GatedLinearPlan(codes, scales, weight, out_codes, out_scales, workspace).run()
