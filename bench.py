@@ -323,7 +323,7 @@ def run_c5(args):
     dev = torch.device("cuda:0")
     max_new = args.warmup + args.steps + interval + 64
     t0 = time.perf_counter()
-    model = ds.RandomQwen3(geo, dev, seed=42)
+    model = ds.RandomQwen3(geo, dev, seed=42, weights=args.weights)
 
     def run_mode(offload: bool, kv_format: str = "bf16"):
         """Timed steps, then untimed steps up to and through the first flush
@@ -425,7 +425,9 @@ def run_c5(args):
         "metric": "C5 full decode step (Qwen3-4B geometry, 36 layers): per-token latency, tokens/s",
         "value": batch / (ms * 1e-3), "unit": "tokens/s", "n_gpus": 1, "steps": args.steps,
         "warmup": args.warmup, "ms_per_step": ms, "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": None, "dtype": "bf16 model; 4-bit K (Format R) stage-2 scoring + bf16 K/V attention",
+        "vs_baseline": None,
+        "dtype": ("bf16 model" if args.weights == "bf16" else "8-bit projections (e4m3, scales per 128), bf16 model")
+        + "; 4-bit K (Format R) stage-2 scoring + bf16 K/V attention",
         "data": "synthetic (random-init weights seed 42; cache prefilled with seeded N(0,1) K/V)",
         "config": {"workload": "C5: one decode token through 36 layers + sampling, polar_cache sparse path",
                    "batch": batch, "context": context, "layers": geo.layers, "hidden": geo.hidden,
@@ -798,6 +800,8 @@ def main():
     ap.add_argument("--no-cpu", action="store_true", help="skip the CPU baseline leg")
     ap.add_argument("--no-offload", action="store_true",
                     help="c5: skip the run with the retrieval zone in pinned host memory")
+    ap.add_argument("--weights", choices=["bf16", "fp8"], default="bf16",
+                    help="c5: the layers' projections in bf16, or in 8 bits with scales per 128 x 128")
     ap.add_argument("--no-kivi4", action="store_true",
                     help="C5: skip the 4-bit K + V retrieval-zone mode")
     ap.add_argument("--no-flush", action="store_true",

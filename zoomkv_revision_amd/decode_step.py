@@ -24,6 +24,13 @@ projection with the residual add.  The torch ops of ``layer_decode_torch``
 the same layer written out op by op: the CPU path, and the check the fused
 kernels are tested against.
 
+With ``weights="fp8"`` the layers' projections are 8-bit products
+(``fp8``: e4m3 codes, a scale per 128 x 128 of a weight and per 128 channels of a
+row): the norms and the attention's output come out as codes, the residual's
+addition is part of the second norm and of the down projection, and the gated
+product passes codes on to the down projection.  Any number of rows takes these
+kernels.  The embedding and the head stay bf16.
+
 Over a ``paged_cache.paged_cache`` (requests of lengths of their own, full
 attention) the same step runs with each row's own position: the norm + RoPE
 launch writes the K / V rows into their page slots
@@ -34,8 +41,13 @@ from __future__ import annotations
 import os
 from dataclasses import dataclass
 
+from typing import TYPE_CHECKING
+
 import torch
 import torch.nn.functional as F
+
+if TYPE_CHECKING:
+    from .fp8 import Fp8Weight
 
 # The reference runner's ZoomKV environment (Z/run/eval_math_aime.py:216-238)
 # and cache knobs (polar_config, :177-213), restricted to what polar_cache reads.
@@ -134,11 +146,46 @@ def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_norm: torch.Ten
                                  v_dst.data_ptr(), v_dst.stride(0), v_dst.stride(1), stream_of(qkv)))
 
 
+def _normed(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
+    """RMSNorm of fp32 rows, unrounded."""
+    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * weight.float()
+
+
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     """RMSNorm over the last dim in fp32, weight applied in fp32, result in x's dtype."""
     xf = x.float()
     xf = xf * torch.rsqrt(xf.pow(2).mean(-1, keepdim=True) + eps)
     return (xf * weight.float()).to(x.dtype)
+
+
+def quantize_rows_torch(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """fp8.quantize_rows of fp32 rows in torch ops."""
+    M, K = x.shape
+    x = F.pad(x, (0, -K % 128)).view(M, -1, 128)
+    amax = x.abs().amax(-1)
+    scale = (amax / torch.full_like(amax, 448.0)).clamp(min=2.0 ** -100)
+    return (x / scale[..., None]).to(torch.float8_e4m3fn).view(M, -1), scale
+
+
+def quantize_weight_torch(w: torch.Tensor, parts: int = 1) -> "Fp8Weight":
+    """fp8.quantize_weight in torch ops (the CPU path)."""
+    from .fp8 import Fp8Weight
+    rows, K = w.shape
+    n = rows // parts
+    x = F.pad(w.float().view(parts, n, K), (0, -K % 128, 0, -n % 128))
+    x = x.view(parts, -1, 128, x.shape[2] // 128, 128)
+    amax = x.abs().amax((2, 4))
+    scale = (amax / torch.full_like(amax, 448.0)).clamp(min=2.0 ** -100)
+    codes = (x / scale[:, :, None, :, None]).to(torch.float8_e4m3fn).view(parts, -1, x.shape[3] * 128)[:, :n]
+    return Fp8Weight(codes.reshape(rows, -1).contiguous(), scale.view(-1, x.shape[3]), parts)
+
+
+def linear_fp8_torch(x: torch.Tensor, w: "Fp8Weight") -> torch.Tensor:
+    """Rows of x (fp32) through fp8.quantize_rows and fp8.linear in torch ops:
+    fp32, unrounded."""
+    codes, scale = quantize_rows_torch(x)
+    rows = codes.float().view(x.shape[0], -1, 128) * scale[..., None]
+    return rows.view(x.shape[0], -1) @ w.dequantize().T
 
 
 def _is_paged(cache) -> bool:
@@ -147,11 +194,15 @@ def _is_paged(cache) -> bool:
 
 
 class RandomQwen3:
-    """Random-init bf16 weights of a Qwen3 decoder (std 0.02, norms at 1), on one GPU."""
+    """Random-init bf16 weights of a Qwen3 decoder (std 0.02, norms at 1), on one
+    GPU; weights="fp8" keeps the layers' projections as 8-bit codes with scales."""
 
     def __init__(self, geo: Qwen3Geometry, device, seed: int = 42, max_position: int = 1 << 17,
-                 fused: bool = True):
+                 fused: bool = True, weights: str = "bf16"):
+        if weights not in ("bf16", "fp8"):
+            raise ValueError(f"weights must be bf16 or fp8; got {weights!r}")
         self.geo = geo
+        self.weights = weights
         self.device = torch.device(device)
         self.fused = fused  # on the GPU: the fused kernels (False: the torch ops, for checks)
         g = torch.Generator(device=self.device)
@@ -161,6 +212,15 @@ class RandomQwen3:
         def w(*shape):
             return (torch.randn(*shape, generator=g, device=self.device) * 0.02).to(torch.bfloat16)
 
+        def proj(rows, cols, parts=1):
+            t = w(rows, cols)
+            if weights == "bf16":
+                return t
+            if t.is_cuda:
+                from .fp8 import quantize_weight
+                return quantize_weight(t, parts)
+            return quantize_weight_torch(t, parts)
+
         qd, kd = geo.heads * geo.head_dim, geo.kv_heads * geo.head_dim
         self.embed = w(geo.vocab, geo.hidden)             # tied with the LM head
         self.final_norm = torch.ones(geo.hidden, **bf)
@@ -169,12 +229,12 @@ class RandomQwen3:
             self.layers.append({
                 "input_ln": torch.ones(geo.hidden, **bf),
                 "post_ln": torch.ones(geo.hidden, **bf),
-                "wqkv": w(qd + 2 * kd, geo.hidden),
+                "wqkv": proj(qd + 2 * kd, geo.hidden),
                 "q_norm": torch.ones(geo.head_dim, **bf),
                 "k_norm": torch.ones(geo.head_dim, **bf),
-                "wo": w(geo.hidden, qd),
-                "gate_up": w(2 * geo.ffn, geo.hidden),
-                "down": w(geo.hidden, geo.ffn),
+                "wo": proj(geo.hidden, qd),
+                "gate_up": proj(2 * geo.ffn, geo.hidden, 2),
+                "down": proj(geo.hidden, geo.ffn),
             })
         # RoPE cos / sin (rotate-half form), fp32 [max_position, head_dim / 2]
         inv = 1.0 / (geo.rope_theta ** (torch.arange(0, geo.head_dim, 2, dtype=torch.float32,
@@ -184,10 +244,11 @@ class RandomQwen3:
         self.cos, self.sin = freqs.cos(), freqs.sin()
 
     def parameter_bytes(self) -> int:
-        n = self.embed.numel() + self.final_norm.numel()
+        tensors = [self.embed, self.final_norm]
         for L in self.layers:
-            n += sum(t.numel() for t in L.values())
-        return 2 * n
+            for t in L.values():
+                tensors += [t] if isinstance(t, torch.Tensor) else [t.codes, t.scales]
+        return sum(t.numel() * t.element_size() for t in tensors)
 
     def _rope(self, x: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
         """x [bs, 1, heads, 128] rotated at position pos, or row b at pos[b]
@@ -204,8 +265,40 @@ class RandomQwen3:
     def layer_decode(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
         """One layer of one decode token (LLM.py:208-251); hidden [bs, 1, hidden]."""
         if hidden.is_cuda and self.fused:
+            if self.weights == "fp8":
+                return self.layer_decode_fp8(ldx, hidden, cache)
             return self.layer_decode_fused(ldx, hidden, cache)
         return self.layer_decode_torch(ldx, hidden, cache)
+
+    def _attend(self, ldx: int, qkv: torch.Tensor, cache) -> torch.Tensor:
+        """q / k norm, RoPE, the K / V rows and the attention: qkv [bs, (heads + 2
+        kv_heads) * 128] -> [bs, 1, heads, 128]."""
+        geo, L = self.geo, self.layers[ldx]
+        bs = qkv.shape[0]
+        if _is_paged(cache):
+            cache.decode_begin(ldx, self.cos.shape[0])
+            q = cache.decode_norm_rope(qkv, L["q_norm"], L["k_norm"], geo.eps, self.cos, self.sin, ldx)
+        else:
+            pos = cache.context
+            row = cache.decode_reserve_row(ldx)
+            q = torch.empty(bs, 1, geo.heads, geo.head_dim, dtype=torch.bfloat16, device=qkv.device)
+            qk_norm_rope(qkv, geo.heads, geo.kv_heads, L["q_norm"], L["k_norm"], geo.eps, self.cos[pos],
+                         self.sin[pos], q, cache.unified_keys[ldx][:, :, row], cache.unified_values[ldx][:, :, row])
+        return cache.compute(q, ldx)
+
+    def layer_decode_fp8(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
+        """layer_decode with 8-bit projections: seven launches (eight or nine where
+        a product takes two) around cache.compute."""
+        from . import fp8
+        geo, L = self.geo, self.layers[ldx]
+        bs = hidden.shape[0]
+        x = hidden.reshape(bs, geo.hidden)
+        qkv = fp8.linear(*fp8.rms_norm_quant(x, L["input_ln"], geo.eps), L["wqkv"])
+        attn = self._attend(ldx, qkv, cache)
+        o = fp8.linear(*fp8.quantize_rows(attn.reshape(bs, -1)), L["wo"])
+        codes, scales, h1 = fp8.rms_norm_quant(o, L["post_ln"], geo.eps, residual=x)
+        act = fp8.gated_linear(codes, scales, L["gate_up"])
+        return fp8.linear(*act, L["down"], residual=h1).view(bs, 1, geo.hidden)
 
     def layer_decode_fused(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
         """layer_decode in five kernels around cache.compute (see the module
@@ -216,16 +309,7 @@ class RandomQwen3:
         x = hidden.reshape(bs, geo.hidden)
         qkv = torch.empty(bs, qd + 2 * kd, dtype=torch.bfloat16, device=hidden.device)
         _layer_linear(x, L["wqkv"], qkv, norm_w=L["input_ln"], eps=geo.eps)
-        if _is_paged(cache):
-            cache.decode_begin(ldx, self.cos.shape[0])
-            q = cache.decode_norm_rope(qkv, L["q_norm"], L["k_norm"], geo.eps, self.cos, self.sin, ldx)
-        else:
-            pos = cache.context
-            row = cache.decode_reserve_row(ldx)
-            q = torch.empty(bs, 1, geo.heads, geo.head_dim, dtype=torch.bfloat16, device=hidden.device)
-            qk_norm_rope(qkv, geo.heads, geo.kv_heads, L["q_norm"], L["k_norm"], geo.eps, self.cos[pos],
-                         self.sin[pos], q, cache.unified_keys[ldx][:, :, row], cache.unified_values[ldx][:, :, row])
-        attn = cache.compute(q, ldx)                                   # [bs, 1, heads, 128]
+        attn = self._attend(ldx, qkv, cache)                           # [bs, 1, heads, 128]
         h1 = torch.empty(bs, geo.hidden, dtype=torch.bfloat16, device=hidden.device)
         _layer_linear(attn.reshape(bs, qd), L["wo"], h1, residual=x)
         act = torch.empty(bs, geo.ffn, dtype=torch.bfloat16, device=hidden.device)
@@ -239,8 +323,11 @@ class RandomQwen3:
         geo, L = self.geo, self.layers[ldx]
         bs = hidden.shape[0]
         residual = hidden
-        x = rms_norm(hidden, L["input_ln"], geo.eps)
-        qkv = F.linear(x, L["wqkv"])
+        if self.weights == "fp8":
+            qkv = linear_fp8_torch(_normed(hidden[:, 0].float(), L["input_ln"], geo.eps), L["wqkv"])
+            qkv = qkv.to(hidden.dtype).unsqueeze(1)
+        else:
+            qkv = F.linear(rms_norm(hidden, L["input_ln"], geo.eps), L["wqkv"])
         qd, kd = geo.heads * geo.head_dim, geo.kv_heads * geo.head_dim
         q, k, v = qkv.split([qd, kd, kd], dim=-1)
         q = rms_norm(q.reshape(bs, 1, geo.heads, geo.head_dim), L["q_norm"], geo.eps)
@@ -256,6 +343,12 @@ class RandomQwen3:
         else:
             cache.decode_update_kv_cache(k, v, ldx)
         attn = cache.compute(q, ldx)                                   # [bs, 1, heads, 128]
+        if self.weights == "fp8":
+            o = linear_fp8_torch(attn.reshape(bs, qd).float(), L["wo"]).to(hidden.dtype)
+            h = residual[:, 0].float() + o.float()
+            gate, up = linear_fp8_torch(_normed(h, L["post_ln"], geo.eps), L["gate_up"]).chunk(2, dim=-1)
+            down = linear_fp8_torch(gate / (1.0 + torch.exp(-gate)) * up, L["down"])
+            return (h.to(hidden.dtype).float() + down).to(hidden.dtype).unsqueeze(1)
         hidden = residual + F.linear(attn.reshape(bs, 1, qd), L["wo"])
         residual = hidden
         x = rms_norm(hidden, L["post_ln"], geo.eps)
