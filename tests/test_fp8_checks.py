@@ -5,7 +5,7 @@ import torch
 
 from fp8_cases import E4M3
 from zoomkv_revision_amd import fp8
-from zoomkv_revision_amd._lib import ZkvError
+from zoomkv_revision_amd._lib import ZkvError, lib
 
 BF = torch.bfloat16
 M, N, K = 3, 40, 200
@@ -148,3 +148,13 @@ def test_gated_output_over_its_input_is_refused():
 def test_weight_refusals(w, parts, text):
     with pytest.raises((ValueError, TypeError), match=text):
         fp8.quantize_weight(w, parts)
+
+
+@pytest.mark.parametrize("entry", ["zkv_fp8_linear", "zkv_fp8_gated_linear"])
+@pytest.mark.parametrize("sizes", [(0, 8, 128), (8, 0, 128), (8, 8, 0), (8, 8, 130), (8, 8, 16512), (1 << 20, 8, 128),
+                                   (8, 1 << 22, 128), (1 << 19, 1 << 19, 128), (-5, 8, 128)])
+def test_the_library_refuses_sizes_its_grids_do_not_hold(entry, sizes):
+    """The entry points' own checks, before any launch (the addresses are never read)."""
+    at, (m, n, k) = 4096, sizes
+    tail = ((0, 0, at, n, 0) if entry == "zkv_fp8_linear" else (at, 1 << 23, at, 1, 1)) + (0, 0, 0)
+    assert getattr(lib(), entry)(at, 1 << 20, at, 1, 1, at, 1 << 20, at, m, n, k, *tail) != 0

@@ -53,8 +53,8 @@ struct LinearArgs {
 struct Piece {
   int part, first, last;
 };
-__device__ __forceinline__ Piece piece_of(const LinearArgs& p) {
-  const int part = blockIdx.z / p.splits, split = blockIdx.z - part * p.splits;
+__device__ __forceinline__ Piece piece_of(const LinearArgs& p, int z) {
+  const int part = z / p.splits, split = z - part * p.splits;
   return Piece{part, split * p.nkb / p.splits, (split + 1) * p.nkb / p.splits};
 }
 
@@ -89,11 +89,22 @@ __device__ __forceinline__ void store_out(const LinearArgs& p, int m, int n, flo
   }
 }
 
+// Outputs 8 l + 0..7 of block jb of row m, from each of 16 neighbouring lanes.
+__device__ __forceinline__ void put_gated(const LinearArgs& p, int m, int jb, int l, const float (&y)[8]) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, abs_bits(y[i]));
+  const float s = fp8_scale(row_max(a)), r = 1.0f / s;
+  *reinterpret_cast<u32x2_t*>(p.codes + m * p.codes_ld + jb * kFp8Block + 8 * l) =
+      u32x2_t{fp8_codes4(y, s, r), fp8_codes4(y + 4, s, r)};
+  if (l == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
+}
+
 // Four neighbouring columns of a row of the output.
-__device__ __forceinline__ void store_out4(const LinearArgs& p, int m, int n, const float (&y)[4], bool vec) {
+__device__ __forceinline__ void store_out4(const LinearArgs& p, int z, int m, int n, const float (&y)[4], bool vec) {
   if (p.sums) {  // (rows of whole groups of four)
     if (n < p.N)
-      *reinterpret_cast<float4_t*>(p.sums + (static_cast<int64_t>(blockIdx.z) * p.M + m) * p.sums_ld + n) =
+      *reinterpret_cast<float4_t*>(p.sums + (static_cast<int64_t>(z) * p.M + m) * p.sums_ld + n) =
           float4_t{y[0], y[1], y[2], y[3]};
     return;
   }
@@ -280,8 +291,8 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArg
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * R * kNT, m0 = blockIdx.y * 16 * kMT;
-  const Piece piece = piece_of(p);
-  WaveTile<kNT, kMT, kNT * kMT == 1 ? 3 : kNT * kMT == 4 ? 2 : 1> w;
+  const Piece piece = piece_of(p, blockIdx.z);
+  WaveTile<kNT, kMT, kNT * kMT == 1 ? 3 : 2> w;
 #pragma unroll
   for (int i = 0; i < kNT; ++i) {
     const int top = n0 + i * R;
@@ -303,7 +314,7 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArg
     const int m = m0 + 16 * (t % kMT) + c, n = n0 + t / kMT * R + 4 * g;
     if (m >= p.M || 4 * g >= R) continue;
     const float y[4] = {v[0], v[1], v[2], v[3]};
-    store_out4(p, m, n, y, vec);
+    store_out4(p, blockIdx.z, m, n, y, vec);
   }
 }
 
@@ -335,12 +346,11 @@ int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
   return check_launch("fp8_stream_kernel");
 }
 
-// 16 kNT weight rows and 16 kMT rows of x per workgroup.
-template <int kNT, int kMT>
+// 32 weight rows and 32 rows of x per workgroup.
 int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
   const int nw = std::min(p.nkb, 8);
-  const dim3 grid((p.N + 16 * kNT - 1) / (16 * kNT), (p.M + 16 * kMT - 1) / (16 * kMT), parts);
-  fp8_stream_kernel<kNT, kMT, 8, 0><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
+  const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts);
+  fp8_stream_kernel<2, 2, 8, 0><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
   return check_launch("fp8_stream_kernel");
 }
 
@@ -362,7 +372,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p, int v
   LinearArgs q = p;
   q.sums = nullptr;
   const float y[4] = {v[0], v[1], v[2], v[3]};
-  store_out4(q, m, n, y, vec);
+  store_out4(q, 0, m, n, y, vec);
 }
 
 // 16 lanes per row and block of 128 outputs, 8 outputs each.
@@ -370,20 +380,14 @@ __global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p)
   const int jb = blockIdx.y, m = blockIdx.x * 16 + (threadIdx.x >> 4), n = jb * kFp8Block + 8 * (threadIdx.x & 15);
   if (m >= p.M) return;  // (whole groups of 16 lanes)
   float y[8];
-  uint32_t a = 0;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float4_t g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
     if (n + 4 * i < p.N) g = sum_of(p, 0, m, n + 4 * i), u = sum_of(p, 1, m, n + 4 * i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[4 * i + e] = n + 4 * i + e < p.N ? silu_mul(g[e], u[e]) : 0.0f;
-      a = max(a, abs_bits(y[4 * i + e]));
-    }
+    for (int e = 0; e < 4; ++e) y[4 * i + e] = n + 4 * i + e < p.N ? silu_mul(g[e], u[e]) : 0.0f;
   }
-  const float s = fp8_scale(row_max(a)), r = 1.0f / s;
-  *reinterpret_cast<u32x2_t*>(p.codes + m * p.codes_ld + n) = u32x2_t{fp8_codes4(y, s, r), fp8_codes4(y + 4, s, r)};
-  if ((threadIdx.x & 15) == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
+  put_gated(p, m, jb, threadIdx.x & 15, y);
 }
 
 int launch_join(const LinearArgs& p, hipStream_t s) {
@@ -397,15 +401,25 @@ int launch_gated_join(const LinearArgs& p, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows of x: a workgroup of kWN x kWM waves computes 64 kWN weight rows (gated: 32
-// kWN gate rows and the matching up rows) for 64 kWM rows of x, a wave 64 x 64 of
-// it as 2 x 2 products of 32 x 32.  A block of 128 k of the tile's rows goes from
-// memory straight into one of two LDS stages while the other is computed on.
+// Many rows of x: a workgroup of kWN x kWM waves, each with kI x kJ products of 32 x
+// 32, computes 32 kI kWN weight rows (gated: half of them gate rows, half the matching up
+// rows) for 32 kJ kWM rows of x.  A block of 128 k of the tile's rows goes from memory
+// straight into one of three LDS stages, two blocks ahead of the one that is computed on.
 //
 // LDS: a row is 8 chunks of 16 bytes, chunk c in slot c ^ ((row >> 1) & 7): the 16
 // lanes of a read phase, each with the same chunk of its own row, hit every bank
-// once.  A lane converts its codes after reading them (64 conversions per wave, block
-// and 32 rows): the LDS moves bytes, not bf16.
+// once.  A lane converts its codes after reading them (8 instructions per 16 of
+// them): the LDS moves bytes, not bf16.
+//
+//   tile of w x x  waves  products  workgroups on a CU
+//     256 x 128      8     2 x 2           1   the fewest bytes and conversions per product
+//     128 x 128      8     2 x 1           1
+//     128 x 64       8     1 x 1           2   more of them run
+//      64 x 64       4     1 x 1           3   at a time where there are few
+//
+// 8192^3 takes 860 us with the first (1278 TF, 857 at the rate of a bf16 product of the
+// library), 512 x 6144 x 2560 33.6, 22.5, 24.8 and 23.6 with the four, 300 x 4096 x 4096
+// 44.8, 29.2, 21.8 and 23.4.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -428,34 +442,50 @@ __device__ __forceinline__ void add_scaled(float16_t& acc, const float16_t& v, f
   for (int i = 0; i < 16; ++i) acc[i] = __builtin_fmaf(v[i], s, acc[i]);
 }
 
-template <bool kGated, int kWN, int kWM>
+// kWN x kWM waves of kI x kJ products of 32 x 32.
+template <bool kGated, int kWN, int kWM, int kI, int kJ>
 struct TileShape {
-  static constexpr int kRowsN = 64 * kWN, kRowsM = 64 * kWM;
+  static constexpr int kWaves = kWN * kWM;
+  static constexpr int kRowsN = 32 * kI * kWN, kRowsM = 32 * kJ * kWM;
   static constexpr int kCols = kGated ? kRowsN / 2 : kRowsN;  // output columns
   static constexpr int kStage = (kRowsN + kRowsM) * kFp8Block;
+  static constexpr int kDmas = kStage / 1024 / kWaves;  // per wave and block
+  static constexpr int kScaleWaves = kRowsM / 64 + 1;
+  static_assert(kStage % (1024 * kWaves) == 0 && kRowsM % 64 == 0 && kScaleWaves <= kWaves, "whole DMAs");
+  static_assert(!kGated || (kI == 2 && kCols == kFp8Block), "gate and up, and one block of outputs");
 };
 
-template <bool kGated, int kWN, int kWM, int kStages>
-__global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const LinearArgs p, int tiles_n, int tiles_m,
-                                                                    int vec) {
-  using Shape = TileShape<kGated, kWN, kWM>;
-  constexpr int kWaves = kWN * kWM;
-  constexpr int kDmas = Shape::kStage / 1024 / kWaves;  // per wave and block
-  static_assert(Shape::kStage % (1024 * kWaves) == 0, "whole DMAs");
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * (Shape::kStage + 256 * (kWM + 1))];
+// What every wave has requested by DMA, but for the last kLeft, is in the LDS for all
+// of the workgroup, and what they read before has been read.
+template <int kLeft>
+__device__ __forceinline__ void tile_barrier() {
+  wait_vmcnt<kLeft>();
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");  // (to the compiler the barrier touches no memory)
+}
+
+template <bool kGated, int kWN, int kWM, int kI, int kJ>
+__global__ __launch_bounds__(64 * kWN * kWM, kI * kJ > 1 ? 2 : kWN * kWM > 4 ? 4 : 3) void fp8_tile_kernel(const LinearArgs p, int tiles_n,
+                                                                                      int tiles_m, int parts, int vec) {
+  using Shape = TileShape<kGated, kWN, kWM, kI, kJ>;
+  constexpr int kStages = 3, kDmas = Shape::kDmas, kScaleWaves = Shape::kScaleWaves;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * (Shape::kStage + 256 * kScaleWaves)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 31, h = lane >> 5;
   const int wn = wave % kWN, wm = wave / kWN;
 
-  // Workgroups go to the eight XCDs in turn: each takes a run of tiles, in bands of
-  // four tiles of weight rows, so that those at work at one time share rows in its L2
-  const int T = tiles_n * tiles_m, per = (T + 7) / 8;
-  const int t = static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3);
-  if (t >= T || static_cast<int>(blockIdx.x >> 3) >= per) return;
+  // Workgroups go to the eight XCDs in turn: each takes a run of the tiles of the first
+  // run of k, then of the next, in bands of four tiles of weight rows, so that those
+  // at work at one time share rows in its L2
+  const int T = tiles_n * tiles_m, all = T * p.splits * parts, per = (all + 7) / 8;
+  const int item = static_cast<int>(blockIdx.x & 7) * per + static_cast<int>(blockIdx.x >> 3);
+  if (item >= all || static_cast<int>(blockIdx.x >> 3) >= per) return;
+  const int z = item / T, t = item - z * T;
   const int band = t / (4 * tiles_m), in_band = t - band * 4 * tiles_m, width = min(4, tiles_n - 4 * band);
   const int tn = 4 * band + in_band % width, tm = in_band / width;
   const int n0 = tn * Shape::kCols, m0 = tm * Shape::kRowsM;
-  const Piece piece = piece_of(p);
+  const Piece piece = piece_of(p, z);
 
   // where the DMAs read: eight rows of 128 bytes each, slots permuted, at a lane's
   // offset from a row of the wave's (host side: rows at most 8 MiB apart)
@@ -479,17 +509,16 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
   const uint32_t dst = lds_offset(lds) + wave * kDmas * 1024;
   // scales of a block: of the tile's x rows, then of each wave row's weight rows (gated:
   // gate and up), 64 to a wave's DMA
-  constexpr int kScaleWaves = kWM + 1;
   const float* scale_src;
   int64_t scale_step;
   {
     const int w = wave % kScaleWaves;
-    if (w < kWM) {
+    if (w < kScaleWaves - 1) {
       scale_src = p.xs + min(m0 + 64 * w + lane, p.M - 1) * p.xs_m + piece.first * p.xs_b;
       scale_step = p.xs_b;
     } else {
       const int nb = (p.N + kFp8Block - 1) / kFp8Block, part = kGated ? lane & 1 : piece.part;
-      const int n = min(n0 + (kGated ? 32 : 64) * ((lane >> 1) % kWN), p.N - 1);
+      const int n = min(n0 + (kGated ? 32 : 32 * kI) * ((lane >> 1) % kWN), p.N - 1);
       scale_src = p.ws + static_cast<int64_t>(part * nb + n / kFp8Block) * p.nkb + piece.first;
       scale_step = 1;
     }
@@ -513,69 +542,71 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
 
   // lane (r, h) reads chunks 4 h + t of its rows; pair t of a block is two slices of 16 k
   const uint32_t first = 16 * ((4 * h) ^ ((r >> 1) & 7));
-  const uint8_t* rows_n = lds + (64 * wn + r) * kFp8Block;
-  const uint8_t* rows_m = lds + (Shape::kRowsN + 64 * wm + r) * kFp8Block;
-  u32x4_t raw[2][4];  // of two pairs: the rows of the weight's two products, then of x's
+  const uint8_t* rows_n = lds + (32 * kI * wn + r) * kFp8Block;
+  const uint8_t* rows_m = lds + (Shape::kRowsN + 32 * kJ * wm + r) * kFp8Block;
+  constexpr int kOps = kI + kJ;
+  u32x4_t raw[2][kOps];  // of two pairs: the weight rows of the products, then x's
   auto read_codes = [&](int i, uint32_t at, int t) {
-    raw[t & 1][i] =
-        *reinterpret_cast<const u32x4_t*>((i < 2 ? rows_n : rows_m) + 32 * (i & 1) * kFp8Block + at + (first ^ (16 * t)));
+    raw[t & 1][i] = *reinterpret_cast<const u32x4_t*>((i < kI ? rows_n + 32 * i * kFp8Block
+                                                              : rows_m + 32 * (i - kI) * kFp8Block) +
+                                                      at + (first ^ (16 * t)));
   };
-  bf16x8_t op[2][4];  // operands of two slices
-  float16_t acc[2][2] = {}, part[2][2] = {};
-  float xs[2] = {0.0f, 0.0f}, ws[2] = {0.0f, 0.0f};  // of the block whose sums are in `part`
+  bf16x8_t op[2][kOps];  // operands of two slices
+  float16_t acc[kI][kJ] = {}, part[kI][kJ] = {};
+  float xs[kJ] = {}, ws[2] = {0.0f, 0.0f};  // of the block whose sums are in `part`
 
-  // Three stages: a block's DMAs are spread over eight slices, those of block b from the
-  // fifth of block b - 3, where its stage is free, to the fourth of b - 2, and have landed
-  // a block later.  Two stages: over four, from the fifth of block b - 2.
-  static_assert(kStages == 2 || kStages == 3, "");
-  constexpr int kSlices = kStages == 3 ? 8 : 4, kPerSlice = (kDmas + kSlices) / kSlices;
-  constexpr int kHead = kStages == 2 ? 0 : 4 * kPerSlice < kDmas + 1 ? 4 * kPerSlice : kDmas + 1;
+  // A block's DMAs are spread over eight slices, those of block b from the fifth of
+  // block b - kStages, where its stage is free, and have landed by the fifth of b - 1
+  constexpr int kPerSlice = (kDmas + 8) / 8, kHead = 4 * kPerSlice < kDmas + 1 ? 4 * kPerSlice : kDmas + 1;
+  constexpr int kLater = (kStages - 2) * (kDmas + 1);  // requested behind a block that has to be there
 #pragma unroll
-  for (int k = 0; k < 3; ++k)
+  for (int k = 0; k < kStages; ++k)
 #pragma unroll
-    for (int i = 0; i < (k < 2 ? kDmas + 1 : kHead); ++i) request(i);
-  wait_vmcnt<kDmas + 1 + kHead>();
-  __builtin_amdgcn_s_barrier();
+    for (int i = 0; i < (k < kStages - 1 ? kDmas + 1 : kHead); ++i) request(i);
+  tile_barrier<kLater + kHead>();
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) read_codes(i, 0, t);
+    for (int i = 0; i < kOps; ++i) read_codes(i, 0, t);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) op[0][i] = codes8_to_bf16(raw[0][i][0], raw[0][i][1]);
+  for (int i = 0; i < kOps; ++i) op[0][i] = codes8_to_bf16(raw[0][i][0], raw[0][i][1]);
   int stage = 0;
   for (int kb = piece.first; kb < piece.last; ++kb) {
     const int next = stage + 1 == kStages ? 0 : stage + 1;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      if (q == 4) {
-        // the block's codes are in registers, the next one's have landed
-        wait_vmcnt<kStages == 3 ? kDmas + 1 : 0>();
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-      }
+      // the block's codes are in registers, the next one's have landed
+      if (q == 4) tile_barrier<kLater>();
       // a wave behind the other of its SIMD goes first: alone, neither fills it
       if (q == 4) __builtin_amdgcn_s_setprio(3);
       if (q == 6) __builtin_amdgcn_s_setprio(2);
       if (q == 0) __builtin_amdgcn_s_setprio(1);
       if (q == 2) __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
-      // four products, and in their shadow the next slice's conversions, reads two
+      // the products, and in their shadow the next slice's conversions, reads two
       // pairs ahead and a DMA
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int i = t >> 1, j = t & 1;
-        if (q == 0) {
-          add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
-          asm volatile("" : "+v"(acc[i][j]));  // (here: left to itself the compiler moves the sums behind the loop's branches and copies `part`)
-          part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[0][i], op[0][2 + j], float16_t{}, 0, 0, 0);
-        } else {
-          part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[q & 1][i], op[q & 1][2 + j], part[i][j], 0, 0, 0);
+      for (int t = 0; t < (kI * kJ > kOps ? kI * kJ : kOps); ++t) {
+        if (t < kI * kJ) {
+          const int i = t / kJ, j = t % kJ;
+          if (q == 0) {
+            add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
+            // (here: left to itself the compiler moves the sums behind the loop's branches
+            // and copies `part`)
+            asm volatile("" : "+v"(acc[i][j]));
+            part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[0][i], op[0][kI + j], float16_t{}, 0, 0, 0);
+          } else {
+            part[i][j] =
+                __builtin_amdgcn_mfma_f32_32x32x16_bf16(op[q & 1][i], op[q & 1][kI + j], part[i][j], 0, 0, 0);
+          }
         }
-        const u32x4_t c = raw[((q + 1) / 2) & 1][t];
-        op[(q + 1) & 1][t] = q & 1 ? codes8_to_bf16(c[0], c[1]) : codes8_to_bf16(c[2], c[3]);
-        if (q % 2 == 0) read_codes(t, (q < 4 ? stage : next) * Shape::kStage, (q / 2 + 2) & 3);
-        if (t == 1) {
-          const int n = (q + 4) % 8 * kPerSlice;  // of block kb + kStages from q = 4 on, else of kb + 2
+        if (t < kOps) {
+          const u32x4_t c = raw[((q + 1) / 2) & 1][t];
+          op[(q + 1) & 1][t] = q & 1 ? codes8_to_bf16(c[0], c[1]) : codes8_to_bf16(c[2], c[3]);
+          if (q % 2 == 0) read_codes(t, (q < 4 ? stage : next) * Shape::kStage, (q / 2 + 2) & 3);
+        }
+        if (t == kOps / 2 - 1) {
+          const int n = (q + 4) % 8 * kPerSlice;  // of the block kStages on from q = 4, else one nearer
 #pragma unroll
           for (int k = n; k < n + kPerSlice && k <= kDmas; ++k) request(k);
         }
@@ -585,85 +616,87 @@ __global__ __launch_bounds__(64 * kWN * kWM, 2) void fp8_tile_kernel(const Linea
         const float* sc =
             reinterpret_cast<const float*>(lds + kStages * Shape::kStage + stage * 256 * kScaleWaves);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) xs[j] = sc[64 * wm + 32 * j + r];
+        for (int j = 0; j < kJ; ++j) xs[j] = sc[32 * kJ * wm + 32 * j + r];
 #pragma unroll
-        for (int i = 0; i < (kGated ? 2 : 1); ++i) ws[i] = sc[64 * kWM + 2 * wn + i];
+        for (int i = 0; i < (kGated ? 2 : 1); ++i) ws[i] = sc[Shape::kRowsM + 2 * wn + i];
       }
     }
     stage = next;
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < kI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
-  wait_vmcnt<0>();
+    for (int j = 0; j < kJ; ++j) add_scaled(acc[i][j], part[i][j], xs[j] * ws[kGated ? i : 0]);
 
-  // lane (r, h) holds columns 8 q + 4 h + 0..3 of row r of each product
+  // The sums go through the LDS, [row of x][weight row], 16-byte chunks of a row
+  // permuted: what follows is a loop over whole rows, written out once (unrolled over the
+  // registers it was 80 KB of code, which no tile finds in the instruction cache) and
+  // with whole lines stored
+  tile_barrier<0>();
+  float4_t* tile = reinterpret_cast<float4_t*>(lds);
+  constexpr int kChunks = Shape::kRowsN / 4, kThreads = 64 * Shape::kWaves;
+  static_assert(Shape::kRowsM * kChunks * 16 <= sizeof(lds), "");
+#pragma unroll
+  for (int i = 0; i < kI; ++i)
+#pragma unroll
+    for (int j = 0; j < kJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        // lane (r, h) holds weight rows 8 q + 4 h + 0..3 of row r of each product
+        const int row = 32 * (kJ * wm + j) + r;
+        const float16_t& v = acc[i][j];
+        tile[row * kChunks + ((8 * (kI * wn + i) + 2 * q + h) ^ (row & 15))] =
+            float4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+      }
+  __syncthreads();
   if constexpr (!kGated) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int m = m0 + 64 * wm + 32 * j + r;
-      if (m >= p.M) continue;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float y[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          store_out4(p, m, n0 + 64 * wn + 32 * i + 8 * q + 4 * h, y, vec);
-        }
+#pragma unroll 2
+    for (int t = threadIdx.x; t < Shape::kRowsM * kChunks; t += kThreads) {
+      const int row = t / kChunks, c = t % kChunks;
+      if (m0 + row >= p.M) break;
+      const float4_t v = tile[row * kChunks + (c ^ (row & 15))];
+      const float y[4] = {v[0], v[1], v[2], v[3]};
+      store_out4(p, z, m0 + row, n0 + 4 * c, y, vec);
     }
   } else {
-    // 128 columns, one block: its largest magnitudes meet in LDS, [wn][row]
-    static_assert(Shape::kCols == kFp8Block, "one block of outputs");
-    __syncthreads();
-    uint32_t* amax = reinterpret_cast<uint32_t*>(lds);
-    float y[2][16];
+    // 128 columns, one block: 16 lanes per row, 8 outputs each (weight rows 64 w + 0..31
+    // of the tile are gate, 64 w + 32..63 the matching up)
+#pragma unroll 1
+    for (int t = threadIdx.x; t < Shape::kRowsM * 16; t += kThreads) {
+      const int row = t >> 4, l = t & 15, m = m0 + row;
+      if (m >= p.M) break;  // (whole groups of 16 lanes)
+      float y[8];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t a = 0;
+      for (int i = 0; i < 2; ++i) {
+        const int c = 16 * (l >> 2) + 2 * (l & 3) + i;
+        const float4_t g = tile[row * kChunks + (c ^ (row & 15))], u = tile[row * kChunks + ((c + 8) ^ (row & 15))];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int n = n0 + 32 * wn + 8 * (e >> 2) + 4 * h + (e & 3);
-        y[j][e] = n < p.N ? silu_mul(acc[0][j][e], acc[1][j][e]) : 0.0f;
-        a = max(a, abs_bits(y[j][e]));
+        for (int e = 0; e < 4; ++e)
+          y[4 * i + e] = n0 + 8 * l + 4 * i + e < p.N ? silu_mul(g[e], u[e]) : 0.0f;
       }
-      a = max(a, static_cast<uint32_t>(__shfl_xor(static_cast<int>(a), 32)));
-      if (h == 0) amax[wn * Shape::kRowsM + 64 * wm + 32 * j + r] = a;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = 64 * wm + 32 * j + r, m = m0 + row;
-      uint32_t a = amax[row];
-#pragma unroll
-      for (int w = 1; w < kWN; ++w) a = max(a, amax[w * Shape::kRowsM + row]);
-      const float sc = fp8_scale(a), rc = 1.0f / sc;
-      if (m >= p.M) continue;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint32_t*>(p.codes + m * p.codes_ld + n0 + 32 * wn + 8 * q + 4 * h) =
-            fp8_codes4(y[j] + 4 * q, sc, rc);
-      if (wn == 0 && h == 0) p.scales[m * p.s_m + tn * p.s_b] = sc;
+      put_gated(p, m, tn, l, y);
     }
   }
 }
 
-template <bool kGated, int kWN, int kWM, int kStages>
+template <bool kGated, int kWN, int kWM, int kI, int kJ>
 int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
-  using Shape = TileShape<kGated, kWN, kWM>;
+  using Shape = TileShape<kGated, kWN, kWM, kI, kJ>;
   const int tiles_n = (p.N + Shape::kCols - 1) / Shape::kCols, tiles_m = (p.M + Shape::kRowsM - 1) / Shape::kRowsM;
-  const dim3 grid((static_cast<unsigned>(tiles_n) * tiles_m + 7) / 8 * 8, 1, parts * p.splits);
-  fp8_tile_kernel<kGated, kWN, kWM, kStages><<<grid, 64 * kWN * kWM, 0, s>>>(p, tiles_n, tiles_m, out_vec(p));
+  const unsigned grid = (static_cast<unsigned>(tiles_n) * tiles_m * p.splits * parts + 7) / 8 * 8;
+  fp8_tile_kernel<kGated, kWN, kWM, kI, kJ>
+      <<<grid, 64 * Shape::kWaves, 0, s>>>(p, tiles_n, tiles_m, parts, out_vec(p));
   return check_launch("fp8_tile_kernel");
 }
 
 // ---------------------------------------------------------------------------
 // Which kernel, and in how many runs of k: the shortest by a model of their times, in
 // us: a start, and a time per block of k that grows as the CUs fill (which lowers the
-// clock).  Over 31 sizes of 17 to 16000 rows its choice took 1.04 times the best of the 15 that
-// were measured for each (geometric mean; at worst 1.3).
+// clock); and where the runs are joined by a second launch, that and the sums' way out and
+// back.  Over 42 sizes of 17 to 16000 rows its choice took 1.01 times the best of the 25
+// that were measured for each (geometric mean; at worst 1.17).
 // ---------------------------------------------------------------------------
-enum Variant : int { kStream, kSplit32, kSplit64, kTileBig, kTileMid, kTileFlat, kTileGated };
+enum Variant : int { kStream, kSplit, kTile256, kTile128, kTileFlat, kTile64, kTileGated };
 
 struct Plan {
   int variant, splits;
@@ -672,8 +705,8 @@ struct Plan {
 
 struct Pace {
   double start;    // until the first block and behind the last
-  int most;        // workgroups at a time on a CU
-  double step[3];  // a block's time with 1, 2, 3 of them there
+  int most;        // steps of the list
+  double step[4];  // a block's time with 256, 512, ... workgroups at work
 };
 
 double rounds_us(int64_t groups, int steps, const Pace& pace) {
@@ -681,10 +714,10 @@ double rounds_us(int64_t groups, int steps, const Pace& pace) {
   double us = pace.start + full * steps * pace.step[pace.most - 1];
   if (rest) {
     const int c = static_cast<int>((rest + 255) / 256);
-    const double low = c > 1 ? pace.step[c - 2] : 0.8 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
+    const double low = c > 1 ? pace.step[c - 2] : 0.62 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
     us += steps * (low + fill * (pace.step[c - 1] - low));
   }
-  return us + 0.6 * pace.start * (full + (rest > 0) - 1);
+  return us + 0.44 * pace.start * (full + (rest > 0) - 1);
 }
 
 int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
@@ -694,37 +727,37 @@ int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
 Plan plan_product(int M, int N, int nkb, int parts) {
   const bool gated = parts == 2;
   if (M <= 16) return Plan{kStream, 1, gated};
-  constexpr Pace kSplit32Pace{2.3, 1, {2.0}}, kSplit64Pace{2.3, 1, {3.0}}, kBigPace{4.6, 1, {1.62}},
-      kMidPace{4.6, 2, {1.08, 1.9}}, kFlatPace{4.6, 3, {0.95, 1.35, 1.8}};
-  Plan best{kTileBig, 1, gated};
+  constexpr Pace kSplitPace{2.25, 1, {2.25}}, k256Pace{7.3, 1, {1.48}}, k128Pace{7.3, 2, {0.85, 2.5}},
+      kFlatPace{7.3, 2, {0.58, 1.35}}, k64Pace{7.3, 4, {0.41, 0.77, 0.84, 1.3}}, kGatedPace{9.6, 1, {1.62}};
+  Plan best{kTile256, 1, gated};
   double best_us = 1e30;
   auto consider = [&](int variant, int splits, int64_t tiles, int steps, const Pace& pace, bool own) {
     const bool sums = !own && (gated || splits > 1);
     double us = rounds_us(tiles * splits * (own ? 1 : parts), steps, pace);
-    if (sums) us += 3.5 + 8.0 * parts * splits * M * static_cast<double>(N) / 6.5e6;  // (out and back)
+    if (sums) us += (gated ? 3.6 : 0.65) + 8.0 * parts * splits * M * static_cast<double>(N) / 6.1e6;
     if (us < best_us) best_us = us, best = Plan{variant, splits, sums};
   };
-  consider(kSplit32, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 7) / 8, kSplit32Pace, false);
-  consider(kSplit64, 1, tiles_of(N, 32) * tiles_of(M, 64), (nkb + 7) / 8, kSplit64Pace, false);
-  for (int k = 1; k <= 8 && 2 * k <= nkb + 1; ++k) {
+  consider(kSplit, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 7) / 8, kSplitPace, false);
+  for (int k = 1; k <= 8 && (k == 1 || 2 * k <= nkb + 1); ++k) {
     const int steps = (nkb + k - 1) / k;
-    consider(kTileBig, k, tiles_of(N, 256) * tiles_of(M, 128), steps, kBigPace, false);
-    consider(kTileMid, k, tiles_of(N, 128) * tiles_of(M, 128), steps, kMidPace, false);
+    consider(kTile256, k, tiles_of(N, 256) * tiles_of(M, 128), steps, k256Pace, false);
+    consider(kTile128, k, tiles_of(N, 128) * tiles_of(M, 128), steps, k128Pace, false);
     consider(kTileFlat, k, tiles_of(N, 128) * tiles_of(M, 64), steps, kFlatPace, false);
+    consider(kTile64, k, tiles_of(N, 64) * tiles_of(M, 64), steps, k64Pace, false);
   }
-  if (gated) consider(kTileGated, 1, tiles_of(N, 128) * tiles_of(M, 128), nkb, kBigPace, true);
+  if (gated) consider(kTileGated, 1, tiles_of(N, 128) * tiles_of(M, 128), nkb, kGatedPace, true);
   return best;
 }
 
 int launch_variant(const LinearArgs& p, int variant, int parts, hipStream_t s) {
   switch (variant) {
     case kStream: return launch_stream(p, parts, s);
-    case kSplit32: return launch_split<2, 2>(p, parts, s);
-    case kSplit64: return launch_split<2, 4>(p, parts, s);
-    case kTileBig: return launch_tile<false, 4, 2, 3>(p, parts, s);
-    case kTileMid: return launch_tile<false, 2, 2, 2>(p, parts, s);
-    case kTileFlat: return launch_tile<false, 2, 1, 2>(p, parts, s);
-    default: return launch_tile<true, 4, 2, 3>(p, 1, s);
+    case kSplit: return launch_split(p, parts, s);
+    case kTile256: return launch_tile<false, 4, 2, 2, 2>(p, parts, s);
+    case kTile128: return launch_tile<false, 2, 4, 2, 1>(p, parts, s);
+    case kTileFlat: return launch_tile<false, 4, 2, 1, 1>(p, parts, s);
+    case kTile64: return launch_tile<false, 2, 2, 1, 1>(p, parts, s);
+    default: return launch_tile<true, 4, 2, 2, 2>(p, 1, s);
   }
 }
 
@@ -739,6 +772,8 @@ const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, cons
                            const float* ws, int M, int N, int K) {
   if (!x || !xs || !w || !ws) return "null pointer";
   if (M < 1 || N < 1 || K < 1) return "empty product";
+  if (M >= 1 << 20 || N >= 1 << 22 || static_cast<int64_t>(M) * N > int64_t{1} << 37)
+    return "below 2^20 rows of x, 2^22 rows of the weight, and at most 2^37 outputs";
   if (K % kFp8Block || K > 128 * kFp8Block) return "K is a multiple of 128, at most 16384";
   if (x_ld < K || w_ld < K || !rows_on_16(x, x_ld, 1) || !rows_on_16(w, w_ld, 1))
     return "rows of codes hold K bytes and start on 16";
