@@ -167,6 +167,36 @@ class QuantizeRowsPlan(_Plan):
         super().__init__(lib().zkv_fp8_rows if x.shape[0] else _nothing, x.device, args, result, keep)
 
 
+def _fresh_rows(x, weight, eps, residual):
+    """The call over contiguous inputs, with outputs of its own: what _rows_args
+    checks in fewer steps, or None where it has to be asked (which names what is
+    wrong)."""
+    kind = _TYPES.get(x.dtype)
+    if kind is None or x.dim() != 2 or not x.is_contiguous() or not x.is_cuda:
+        return None
+    M, K = shape = x.shape
+    device = x.device
+    if not 0 < M < 1 << 27 or not 0 < K <= MAX_NORM_K:
+        return None
+    if weight is not None and (weight.dtype != x.dtype or weight.shape != shape[1:] or not weight.is_contiguous() or
+                               weight.device != device):
+        return None
+    total = None
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != shape or not residual.is_contiguous() or \
+                residual.device != device:
+            return None
+        total = torch.empty(shape, dtype=x.dtype, device=device)
+    kb = -(-K // BLOCK)
+    codes = torch.empty((M, kb * BLOCK), dtype=E4M3, device=device)
+    scales = torch.empty_strided((M, kb), (1, M), dtype=torch.float32, device=device)
+    _launch(lib().zkv_fp8_rows, device,
+            (x.data_ptr(), K, M, K, kind, None if weight is None else weight.data_ptr(), float(eps),
+             None if total is None else residual.data_ptr(), K, None if total is None else total.data_ptr(), K,
+             codes.data_ptr(), kb * BLOCK, scales.data_ptr(), 1, M))
+    return (codes, scales) if total is None else (codes, scales, total)
+
+
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: torch.Tensor | None = None,
                    sum_out: torch.Tensor | None = None, codes: torch.Tensor | None = None,
                    scales: torch.Tensor | None = None):
@@ -178,12 +208,20 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float, residual: 
     type where it is stored.  Returns (codes, scales), and with a residual (codes,
     scales, sum_out); sum_out may be x or residual.  New scales are laid out as
     columns of M."""
+    if sum_out is None and codes is None and scales is None and weight is not None:
+        got = _fresh_rows(x, weight, eps, residual)
+        if got is not None:
+            return got
     return RmsNormQuantPlan(x, weight, eps, residual, sum_out, codes, scales).run()
 
 
 def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scales: torch.Tensor | None = None):
     """The rows of x [M, K] (bf16, fp16 or fp32) as codes [M, ceil(K / 128) *
     128] and scales float32 [M, ceil(K / 128)]."""
+    if codes is None and scales is None:
+        got = _fresh_rows(x, None, 0.0, None)
+        if got is not None:
+            return got
     return QuantizeRowsPlan(x, codes, scales).run()
 
 
@@ -305,6 +343,68 @@ class LinearPlan(_Plan):
         super().__init__(lib().zkv_fp8_linear if codes.shape[0] else _nothing, codes.device, args, result, keep)
 
 
+def _fresh_operands(codes, scales, weight: Fp8Weight, parts: int):
+    """_check_product of contiguous operands in fewer steps, or None where it has
+    to be asked."""
+    w, ws = weight.codes, weight.scales
+    if codes.dtype != E4M3 or w.dtype != E4M3 or codes.dim() != 2 or w.dim() != 2 or weight.parts != parts or \
+            not codes.is_contiguous() or not w.is_contiguous() or not codes.is_cuda:
+        return None
+    (M, K), (rows, wide), device = codes.shape, w.shape, codes.device
+    if wide != K or K % BLOCK or not 0 < K <= MAX_K or not 0 < M < 1 << 20 or not parts <= rows < 1 << 24 or \
+            rows % parts:
+        return None
+    n, kb = rows // parts, K // BLOCK
+    if scales.dtype != torch.float32 or scales.shape != (M, kb) or ws.dtype != torch.float32 or \
+            ws.shape != (parts * -(-n // BLOCK), kb) or not ws.is_contiguous():
+        return None
+    if scales.device != device or w.device != device or ws.device != device:
+        return None
+    x_ptr, w_ptr = codes.data_ptr(), w.data_ptr()
+    if (x_ptr | w_ptr) % 16:
+        return None
+    s_m, s_b = scales.stride()
+    return M, n, K, (x_ptr, K, scales.data_ptr(), s_m, s_b, w_ptr, K, ws.data_ptr(), M, n, K)
+
+
+def _fresh_linear(codes, scales, weight, out_dtype, residual):
+    """The call over contiguous inputs, with an output of its own; None where
+    _linear_args has to be asked."""
+    operands, kind = _fresh_operands(codes, scales, weight, 1), _TYPES.get(out_dtype)
+    if operands is None or kind is None:
+        return None
+    M, N, K, args = operands
+    if residual is not None and (residual.dtype != out_dtype or residual.shape != (M, N) or
+                                 not residual.is_contiguous() or residual.device != codes.device):
+        return None
+    device = codes.device
+    out = torch.empty((M, N), dtype=out_dtype, device=device)
+    L = lib()
+    need = L.zkv_fp8_linear_workspace_size(M, N, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch(L.zkv_fp8_linear, device,
+            (*args, None if residual is None else residual.data_ptr(), N, out.data_ptr(), N, kind,
+             None if ws is None else ws.data_ptr(), need))
+    return out
+
+
+def _fresh_gated(codes, scales, weight):
+    operands = _fresh_operands(codes, scales, weight, 2)
+    if operands is None:
+        return None
+    M, F, K, args = operands
+    device, nb = codes.device, -(-F // BLOCK)
+    out_codes = torch.empty((M, nb * BLOCK), dtype=E4M3, device=device)
+    out_scales = torch.empty_strided((M, nb), (1, M), dtype=torch.float32, device=device)
+    L = lib()
+    need = L.zkv_fp8_gated_workspace_size(M, F, K)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _launch(L.zkv_fp8_gated_linear, device,
+            (*args, out_codes.data_ptr(), nb * BLOCK, out_scales.data_ptr(), 1, M,
+             None if ws is None else ws.data_ptr(), need))
+    return out_codes, out_scales
+
+
 def linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: torch.Tensor | None = None,
            out_dtype: torch.dtype = torch.bfloat16, residual: torch.Tensor | None = None,
            workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -313,6 +413,10 @@ def linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out: to
     once.  out may be the residual.  The workspace (uint8,
     zkv_fp8_linear_workspace_size(M, N, K) bytes: where few tiles meet a long K)
     needs no clearing; calls that overlap on one race."""
+    if out is None and workspace is None:
+        got = _fresh_linear(codes, scales, weight, out_dtype, residual)
+        if got is not None:
+            return got
     return LinearPlan(codes, scales, weight, out, out_dtype, residual, workspace).run()
 
 
@@ -344,9 +448,14 @@ class GatedLinearPlan(_Plan):
 
 def gated_linear(codes: torch.Tensor, scales: torch.Tensor, weight: Fp8Weight, out_codes: torch.Tensor | None = None,
                  out_scales: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
-    """silu(gate) * up of a gated feed-forward block: gate and up are the rows (codes, scales) times the two parts of the weight ([2 F, K], parts =
-    2); returns codes [M, ceil(F / 128) * 128] and scales float32 [M, ceil(F /
-    128)] (new ones as columns of M), what ``linear`` takes for the down
-    projection.  The workspace (uint8, zkv_fp8_gated_workspace_size(M, F, K)
-    bytes) needs no clearing; calls that overlap on one race."""
+    """silu(gate) * up of a gated feed-forward block: gate and up are the rows
+    (codes, scales) times the two parts of the weight ([2 F, K], parts = 2); returns
+    codes [M, ceil(F / 128) * 128] and scales float32 [M, ceil(F / 128)] (new ones as
+    columns of M), what ``linear`` takes for the down projection.  The workspace
+    (uint8, zkv_fp8_gated_workspace_size(M, F, K) bytes) needs no clearing; calls
+    that overlap on one race."""
+    if out_codes is None and out_scales is None and workspace is None:
+        got = _fresh_gated(codes, scales, weight)
+        if got is not None:
+            return got
     return GatedLinearPlan(codes, scales, weight, out_codes, out_scales, workspace).run()
