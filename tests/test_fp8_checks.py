@@ -158,3 +158,28 @@ def test_the_library_refuses_sizes_its_grids_do_not_hold(entry, sizes):
     at, (m, n, k) = 4096, sizes
     tail = ((0, 0, at, n, 0) if entry == "zkv_fp8_linear" else (at, 1 << 23, at, 1, 1)) + (0, 0, 0)
     assert getattr(lib(), entry)(at, 1 << 20, at, 1, 1, at, 1 << 20, at, m, n, k, *tail) != 0
+
+
+def _raw(t):
+    return t.view(-1).view(torch.uint8)
+
+
+def test_outputs_over_inputs_are_refused():
+    """An output or a workspace that lies in what other workgroups still read."""
+    square, ones = _codes(256), torch.ones(256, 2)
+    gate = fp8.Fp8Weight(_codes(512), torch.ones(4, 2), parts=2)
+    half = fp8.Fp8Weight(_codes(128), torch.ones(1, 2))
+    x, single = torch.zeros(256, 256, dtype=BF), torch.zeros(256, 256)
+    flat = torch.zeros(256 * 256 * 2, dtype=torch.uint8)
+    for call in (
+            lambda: fp8.rms_norm_quant(flat.view(BF).view(256, 256), x[0], 1e-6,
+                                       codes=flat[:1 << 16].view(E4M3).view(256, 256)),
+            lambda: fp8.rms_norm_quant(x.clone(), x[0], 1e-6, residual=x.clone(), sum_out=x),
+            lambda: fp8.quantize_rows(single, scales=single[:, :2]),
+            lambda: fp8.linear(square, ones, half, out=_raw(square).view(BF).view(256, 128)),
+            lambda: fp8.gated_linear(square, ones, gate, out_codes=square),
+            lambda: fp8.gated_linear(square, ones, gate, out_scales=ones),
+            lambda: fp8.gated_linear(square, ones, gate, out_codes=gate.codes[:256]),
+            lambda: fp8.gated_linear(square[:17], ones[:17], gate, workspace=_raw(gate.codes))):
+        with pytest.raises(ValueError, match="apart from the input"):
+            call()

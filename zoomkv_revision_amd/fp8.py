@@ -92,6 +92,26 @@ def _new_scales(rows: int, K: int, like: torch.Tensor) -> torch.Tensor:
     return torch.empty(blocks(K), rows, dtype=torch.float32, device=like.device).t()
 
 
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes that a tensor's elements lie in."""
+    if not t.numel():
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a0 < b1 and b0 < a1
+
+
+def _check_apart(name: str, out: torch.Tensor, *others) -> None:
+    """`out` is written while other workgroups still read the inputs."""
+    for t in others:
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{name} must lie apart from the inputs and the other outputs")
+
+
 # ---------------------------------------------------------------------------
 # rows
 # ---------------------------------------------------------------------------
@@ -129,24 +149,15 @@ def _rows_args(x, weight, eps, residual, sum_out, codes, scales):
     codes_ld = _check_codes("codes", codes, M, K, 8)
     s_m, s_b = _check_scales("scales", scales, M, K, apart=True)
     _same_device(x, weight=weight, residual=residual, sum_out=sum_out, codes=codes, scales=scales)
+    for name, t in (("codes", codes), ("scales", scales)):
+        _check_apart(name, t, x, weight, residual, sum_out)
+    if sum_out is not None:
+        _check_apart("sum_out", sum_out, weight)
     require_gpu(x)
     args = (ptr(x), x_ld, M, K, kind, ptr(weight), float(eps), ptr(residual), res_ld, ptr(sum_out), sum_ld,
             ptr(codes), codes_ld, ptr(scales), s_m, s_b)
     result = (codes, scales) if residual is None else (codes, scales, sum_out)
     return args, result, (x, weight, residual, sum_out, codes, scales)
-
-
-def _extent(t: torch.Tensor) -> tuple[int, int]:
-    """The bytes that a tensor's elements lie in."""
-    if not t.numel():
-        return 0, 0
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _extent(a), _extent(b)
-    return a0 < b1 and b0 < a1
 
 
 class RmsNormQuantPlan(_Plan):
@@ -281,7 +292,7 @@ def _check_product(codes, scales, weight: Fp8Weight, parts: int):
     rows = weight.rows
     if K > MAX_K:
         raise ValueError(f"a product over {K} channels, at most {MAX_K}")
-    if rows < parts or rows % parts or rows >= 1 << 24 or M >= 1 << 20:
+    if rows < parts or rows % parts or rows >= parts << 22 or M >= 1 << 20 or M * (rows // parts) > 1 << 37:
         raise ValueError(f"a product of {M} rows with a weight of {rows} rows in {parts} part(s)")
     x_ld = _check_codes("codes", codes, M, K, 16)
     if max(x_ld, weight.codes.stride(0)) >= 1 << 23:
@@ -327,8 +338,11 @@ def _linear_args(codes, scales, weight, out, out_dtype, residual, workspace):
                 out.data_ptr() == residual.data_ptr() and _strides(out) != _strides(residual):
             raise ValueError("out must be the residual itself or lie apart from it")
     _same_device(codes, out=out, residual=residual)
-    require_gpu(codes)
+    inputs = codes, scales, weight.codes, weight.scales
+    _check_apart("out", out, *inputs)
     ws = _workspace(lib().zkv_fp8_linear_workspace_size(M, N, K), workspace, codes)
+    _check_apart("workspace", ws, *inputs, residual, out)
+    require_gpu(codes)
     args = (*operands, ptr(residual), res_ld, ptr(out), out_ld, kind, ptr(ws), ws.numel())
     return args, out, (codes, scales, weight.codes, weight.scales, residual, out, ws)
 
@@ -351,8 +365,8 @@ def _fresh_operands(codes, scales, weight: Fp8Weight, parts: int):
             not codes.is_contiguous() or not w.is_contiguous() or not codes.is_cuda:
         return None
     (M, K), (rows, wide), device = codes.shape, w.shape, codes.device
-    if wide != K or K % BLOCK or not 0 < K <= MAX_K or not 0 < M < 1 << 20 or not parts <= rows < 1 << 24 or \
-            rows % parts:
+    if wide != K or K % BLOCK or not 0 < K <= MAX_K or not 0 < M < 1 << 20 or not parts <= rows < parts << 22 or \
+            rows % parts or M * rows > 1 << 37:
         return None
     n, kb = rows // parts, K // BLOCK
     if scales.dtype != torch.float32 or scales.shape != (M, kb) or ws.dtype != torch.float32 or \
@@ -426,12 +440,13 @@ def _gated_args(codes, scales, weight, out_codes, out_scales, workspace):
     out_scales = _new_scales(M, F, codes) if out_scales is None else out_scales
     codes_ld = _check_codes("out_codes", out_codes, M, F, 8)
     s_m, s_b = _check_scales("out_scales", out_scales, M, F, apart=True)
-    for name, a, b in (("out_codes", out_codes, codes), ("out_scales", out_scales, scales)):
-        if _overlap(a, b):
-            raise ValueError(f"{name} must lie apart from the input")
-    require_gpu(codes)
-    ws = _workspace(lib().zkv_fp8_gated_workspace_size(M, F, K), workspace, codes)
+    inputs = codes, scales, weight.codes, weight.scales
+    _check_apart("out_codes", out_codes, *inputs)
+    _check_apart("out_scales", out_scales, *inputs)
     _same_device(codes, out_codes=out_codes, out_scales=out_scales)
+    ws = _workspace(lib().zkv_fp8_gated_workspace_size(M, F, K), workspace, codes)
+    _check_apart("workspace", ws, *inputs, out_codes, out_scales)
+    require_gpu(codes)
     args = (*operands, ptr(out_codes), codes_ld, ptr(out_scales), s_m, s_b, ptr(ws), ws.numel())
     return args, (out_codes, out_scales), (codes, scales, weight.codes, weight.scales, out_codes, out_scales, ws)
 
