@@ -718,6 +718,25 @@ int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type, const void
                  const void* residual, int64_t res_ld, void* sum_out, int64_t sum_ld, uint8_t* codes,
                  int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, zkv_stream_t stream);
 
+/* The arguments of a call but its stream, in its order: what a caller with fixed
+ * buffers keeps, and passes with each call as one address. */
+typedef struct {
+  const void* x;
+  int64_t x_ld;
+  int M, K, type;
+  const void* norm_w;
+  float eps;
+  const void* residual;
+  int64_t res_ld;
+  void* sum_out;
+  int64_t sum_ld;
+  uint8_t* codes;
+  int64_t codes_ld;
+  float* scales;
+  int64_t s_m, s_b;
+} zkv_fp8_rows_args;
+int zkv_fp8_rows_call(const zkv_fp8_rows_args* args, zkv_stream_t stream);
+
 /* A weight w [N, K] of `type`, `parts` matrices of N / parts rows one behind the
  * other, each with blocks of its own: scales [parts * ceil(N / parts / 128), B]. */
 int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int parts, uint8_t* codes, int64_t codes_ld,
@@ -725,7 +744,8 @@ int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int part
 
 /* out[m, n] = sum_b xs[m, b] ws[n / 128, b] sum_{k in b} x[m, k] w[n, k]
  * [+ residual[m, n]], fp32 sums rounded once to `type` (out and residual; out may
- * be residual).  K is a multiple of 128, at most 16384; rows of codes start on 16
+ * be residual).  K is a multiple of 128, at most 16384; M < 2^20, N < 2^22, M * N
+ * at most 2^37; rows of codes start on 16
  * bytes, less than 8 MiB apart.  workspace: zkv_fp8_linear_workspace_size(M, N, K)
  * bytes (0 for most sizes) on 16, of any content; calls that overlap on one race. */
 size_t zkv_fp8_linear_workspace_size(int M, int N, int K);
@@ -733,6 +753,24 @@ int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m
                    int64_t w_ld, const float* ws, int M, int N, int K, const void* residual, int64_t res_ld,
                    void* out, int64_t out_ld, int type, void* workspace, size_t workspace_bytes,
                    zkv_stream_t stream);
+typedef struct {
+  const uint8_t* x;
+  int64_t x_ld;
+  const float* xs;
+  int64_t xs_m, xs_b;
+  const uint8_t* w;
+  int64_t w_ld;
+  const float* ws;
+  int M, N, K;
+  const void* residual;
+  int64_t res_ld;
+  void* out;
+  int64_t out_ld;
+  int type;
+  void* workspace;
+  size_t workspace_bytes;
+} zkv_fp8_linear_args;
+int zkv_fp8_linear_call(const zkv_fp8_linear_args* args, zkv_stream_t stream);
 
 /* The same for a weight of 2 F rows in two parts, gate and up: codes and scales
  * of silu(gate) * up [M, F] (codes: rows of whole blocks of F, on 8 bytes).
@@ -743,6 +781,23 @@ int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_
                          const uint8_t* w, int64_t w_ld, const float* ws, int M, int F, int K, uint8_t* codes,
                          int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, void* workspace,
                          size_t workspace_bytes, zkv_stream_t stream);
+typedef struct {
+  const uint8_t* x;
+  int64_t x_ld;
+  const float* xs;
+  int64_t xs_m, xs_b;
+  const uint8_t* w;
+  int64_t w_ld;
+  const float* ws;
+  int M, F, K;
+  uint8_t* codes;
+  int64_t codes_ld;
+  float* scales;
+  int64_t s_m, s_b;
+  void* workspace;
+  size_t workspace_bytes;
+} zkv_fp8_gated_linear_args;
+int zkv_fp8_gated_linear_call(const zkv_fp8_gated_linear_args* args, zkv_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,11 +1,13 @@
 """What the 8-bit linear calls refuse before any launch (host checks only, on CPU
 tensors: the last check is that they are on the GPU)."""
+import ctypes
+
 import pytest
 import torch
 
 from fp8_cases import E4M3
 from zoomkv_revision_amd import fp8
-from zoomkv_revision_amd._lib import ZkvError, lib
+from zoomkv_revision_amd._lib import SIGNATURES, ZkvError, lib, packed_args
 
 BF = torch.bfloat16
 M, N, K = 3, 40, 200
@@ -183,3 +185,15 @@ def test_outputs_over_inputs_are_refused():
             lambda: fp8.gated_linear(square[:17], ones[:17], gate, workspace=_raw(gate.codes))):
         with pytest.raises(ValueError, match="apart from the input"):
             call()
+
+
+@pytest.mark.parametrize("entry", ["zkv_fp8_rows", "zkv_fp8_linear", "zkv_fp8_gated_linear"])
+def test_packed_arguments_are_the_entrys_own(entry):
+    """A null operand with packed arguments is refused as without."""
+    values = [0] * (len(SIGNATURES[entry][1]) - 1)
+    assert getattr(lib(), entry)(*values, 0) != 0
+    text = lib().zkv_last_error()
+    packed = packed_args(entry, values)
+    assert getattr(lib(), entry + "_call")(ctypes.addressof(packed), 0) != 0
+    assert lib().zkv_last_error() == text and b"null pointer" in text
+    assert getattr(lib(), entry + "_call")(0, 0) != 0

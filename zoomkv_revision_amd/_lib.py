@@ -106,6 +106,9 @@ SIGNATURES = {
     "zkv_fp8_linear": (I32, [P, I64, P, I64, I64, P, I64, P, I32, I32, I32, P, I64, P, I64, I32, P, SZ, P]),
     "zkv_fp8_gated_workspace_size": (SZ, [I32, I32, I32]),
     "zkv_fp8_gated_linear": (I32, [P, I64, P, I64, I64, P, I64, P, I32, I32, I32, P, I64, P, I64, I64, P, SZ, P]),
+    "zkv_fp8_rows_call": (I32, [P, P]),
+    "zkv_fp8_linear_call": (I32, [P, P]),
+    "zkv_fp8_gated_linear_call": (I32, [P, P]),
 }
 
 _lib = None
@@ -130,6 +133,13 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def packed_args(name: str, args) -> C.Structure:
+    """The arguments of an entry but its stream as the struct that its `_call`
+    entry takes."""
+    fields = [(f"a{i}", t) for i, t in enumerate(SIGNATURES[name][1][:-1])]
+    return type(f"{name}_args", (C.Structure,), {"_fields_": fields})(*args)
 
 
 def check(rc: int) -> None:

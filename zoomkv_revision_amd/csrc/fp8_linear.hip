@@ -812,6 +812,12 @@ extern "C" int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, i
   return rc != ZKV_OK || !plan.sums ? rc : launch_join(p, s);
 }
 
+extern "C" int zkv_fp8_linear_call(const zkv_fp8_linear_args* a, zkv_stream_t stream) {
+  ZKV_REQUIRE(a, "zkv_fp8_linear: null pointer");
+  return zkv_fp8_linear(a->x, a->x_ld, a->xs, a->xs_m, a->xs_b, a->w, a->w_ld, a->ws, a->M, a->N, a->K, a->residual,
+                        a->res_ld, a->out, a->out_ld, a->type, a->workspace, a->workspace_bytes, stream);
+}
+
 extern "C" size_t zkv_fp8_gated_workspace_size(int M, int F, int K) {
   if (M < 1 || F < 1 || K < 1) return 0;
   return sums_bytes(plan_product(M, F, blocks_of(K), 2), 2, M, F);
@@ -839,4 +845,10 @@ extern "C" int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float*
   auto s = reinterpret_cast<hipStream_t>(stream);
   const int rc = launch_variant(p, plan.variant, 2, s);
   return rc != ZKV_OK || !plan.sums ? rc : launch_gated_join(p, s);
+}
+
+extern "C" int zkv_fp8_gated_linear_call(const zkv_fp8_gated_linear_args* a, zkv_stream_t stream) {
+  ZKV_REQUIRE(a, "zkv_fp8_gated_linear: null pointer");
+  return zkv_fp8_gated_linear(a->x, a->x_ld, a->xs, a->xs_m, a->xs_b, a->w, a->w_ld, a->ws, a->M, a->F, a->K, a->codes,
+                              a->codes_ld, a->scales, a->s_m, a->s_b, a->workspace, a->workspace_bytes, stream);
 }

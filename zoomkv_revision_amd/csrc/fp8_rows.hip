@@ -216,6 +216,12 @@ extern "C" int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type,
   return check_launch("fp8_norm_rows_kernel");
 }
 
+extern "C" int zkv_fp8_rows_call(const zkv_fp8_rows_args* a, zkv_stream_t stream) {
+  ZKV_REQUIRE(a, "zkv_fp8_rows: null pointer");
+  return zkv_fp8_rows(a->x, a->x_ld, a->M, a->K, a->type, a->norm_w, a->eps, a->residual, a->res_ld, a->sum_out,
+                      a->sum_ld, a->codes, a->codes_ld, a->scales, a->s_m, a->s_b, stream);
+}
+
 extern "C" int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int parts, uint8_t* codes,
                               int64_t codes_ld, float* scales, zkv_stream_t stream) {
   ZKV_REQUIRE(w && codes && scales, "zkv_fp8_weight: null pointer");
