@@ -140,177 +140,157 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int z, int m, in
 }
 
 // ---------------------------------------------------------------------------
-// Few rows of x, or few tiles: codes go from memory straight into registers.  A
-// workgroup computes 16 kNT weight rows (gated: half of them gate rows, half the matching
-// up rows) for 16 kMT rows of x; its waves split the blocks of k (wave w takes
-// blocks w, w + nw, ...), so nothing is staged, no wave waits for another, and their
-// sums meet in LDS at the end, added in wave order.  A unit may have R < 16 rows per
-// tile, to fill the CUs: lanes past R, N or M repeat the last row, which moves no
-// more memory.
+// What the LDS kernels share.  A row of a block of k is 128 bytes there, 8 chunks of 16,
+// chunk c in slot c ^ ((row >> 1) & 7): the 16 lanes of a read phase, each with the
+// same chunk of its own row, hit every bank once.
 // ---------------------------------------------------------------------------
-template <int kNT, int kMT, int kDepth>
-struct WaveTile {
-  struct Block {
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
+}
+
+// 64 lanes x 16 bytes, each at its offset from a base (wave-uniform, as dst), into LDS at
+// dst + 16 lane, not seen by the compiler's wait counts: with the builtin every LDS read
+// waits for all of them.
+__device__ __forceinline__ void dma16_tile(const void* base, uint32_t off, uint32_t dst) {
+  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
+}
+
+__device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
+  asm volatile("global_load_lds_dword %0, off" : : "v"(src), "{m0}"(dst) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Few rows of x, or few tiles: a unit computes 16 kNT weight rows for kXR rows of x (8,
+// or 16 kMT); its waves split the blocks of k (wave w takes blocks w, w + nw, ...), so
+// no wave waits for another, and their sums meet at the end, added in wave order.  Each
+// wave has kD blocks on their way into its own part of the LDS, eight whole lines to
+// a load: straight into the registers of a product's operands, a load's neighbouring
+// lanes are in different rows, which the address unit takes one by one, and at 64
+// cycles a load it was what bounded the kernel (16 x 2560 x 9728 12.7 -> 10.4 us, 100 x
+// 1000 x 2600 8.4 -> 6.1, gated 4 x 9728 x 2560 16.0 -> 14.5 with its second launch).
+// A unit may have R < 16 weight rows per tile, to fill the CUs: lanes past R, N or M
+// repeat the last row, which moves no more memory.
+// ---------------------------------------------------------------------------
+template <int kNT, int kXR, int kWaves, int kD>
+__global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArgs p, int R, int vec) {
+  constexpr int kMT = (kXR + 15) / 16, kDmas = (16 * kNT + kXR) / 8;
+  constexpr int kRegion = kDmas * 1024 + 256;  // a block: rows of the weight, rows of x, scales
+  static_assert(kXR + 4 * kNT <= 64 && kD >= 2 && kD <= 3 && kNT * kMT * 1024 <= kD * kRegion, "");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[kWaves * kD * kRegion];
+  const int nw = blockDim.x >> 6;
+  // (turned from unit to unit, so that those at work at one time do not all ask for the
+  // same part of x first: 1 x 6144 x 2560 6.37 -> 6.20 us, 16 x 6144 x 2560 8.59 -> 8.35)
+  const int wave = __builtin_amdgcn_readfirstlane(((threadIdx.x >> 6) + blockIdx.x) % nw), lane = threadIdx.x & 63;
+  const int c = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * R * kNT, m0 = blockIdx.y * 16 * kMT;
+  const Piece piece = piece_of(p, blockIdx.z);
+
+  // where the loads read (host side: rows at most 8 MiB apart)
+  const int first = piece.first + wave;
+  const uint8_t* wb = p.w + (static_cast<int64_t>(piece.part) * p.N + n0) * p.w_ld + first * kFp8Block;
+  const uint8_t* xb = p.x + m0 * p.x_ld + first * kFp8Block;
+  uint32_t off[kDmas];
+#pragma unroll
+  for (int i = 0; i < kDmas; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    const uint32_t chunk = 16 * ((lane & 7) ^ ((row >> 1) & 7));
+    if (i < 2 * kNT)
+      off[i] = min(row / 16 * R + min(row % 16, R - 1), p.N - 1 - n0) * static_cast<uint32_t>(p.w_ld) + chunk;
+    else
+      off[i] = min(row - 16 * kNT, p.M - 1 - m0) * static_cast<uint32_t>(p.x_ld) + chunk;
+  }
+  // scales: of the rows of x, then of each four columns of the weight's tiles (in one block
+  // each: R is a multiple of 4)
+  const float* sb;
+  int64_t s_step;
+  if (lane < kXR) {
+    sb = p.xs + min(m0 + lane, p.M - 1) * p.xs_m + first * p.xs_b;
+    s_step = nw * p.xs_b;
+  } else {
+    const int j = min(lane - kXR, 4 * kNT - 1);
+    const int n = min(n0 + (j >> 2) * R + min(4 * (j & 3), R - 4), p.N - 1);
+    const int nb = (p.N + kFp8Block - 1) / kFp8Block;
+    sb = p.ws + static_cast<int64_t>(piece.part * nb + n / kFp8Block) * p.nkb + first;
+    s_step = nw;
+  }
+  uint8_t* const mine = lds + wave * kD * kRegion;
+  const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_offset(mine));
+  auto request = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kDmas; ++i) dma16_tile(i < 2 * kNT ? wb : xb, off[i], dst + stage * kRegion + i * 1024);
+    dma4_tile(sb, dst + stage * kRegion + kDmas * 1024);
+    wb += nw * kFp8Block, xb += nw * kFp8Block, sb += s_step;
+  };
+
+  const int cnt = (piece.last - first + nw - 1) / nw;  // (at least 1)
+#pragma unroll
+  for (int d = 0; d < kD; ++d)
+    if (d < cnt) request(d);
+  const uint32_t at = c * kFp8Block + 16 * (g ^ ((c >> 1) & 7));
+  float4_t acc[kNT][kMT] = {};
+  int stage = 0;
+  for (int i = 0; i < cnt; ++i) {
+    const int left = cnt - 1 - i;  // behind this block, min(left, kD - 1) of them requested
+    if (left >= kD - 1)
+      wait_vmcnt<(kD - 1) * (kDmas + 1)>();
+    else if (kD > 2 && left == 1)
+      wait_vmcnt<kDmas + 1>();
+    else
+      wait_vmcnt<0>();
+    const uint8_t* src = mine + stage * kRegion;
     u32x4_t a[kNT][2], b[kMT][2];
     float ws[kNT], xs[kMT];
-  };
-  const uint8_t *wr[kNT], *xr[kMT];
-  const float *wsr[kNT], *xsr[kMT];
-  int64_t xs_b;
-  float4_t acc[kNT][kMT];
-
-  // tile i: this lane's row of the weight, and the block of rows of its outputs
-  __device__ __forceinline__ void weight(const LinearArgs& p, int i, int part, int row, int block) {
-    wr[i] = p.w + (static_cast<int64_t>(part) * p.N + row) * p.w_ld + 16 * ((threadIdx.x >> 4) & 3);
-    wsr[i] = p.ws + static_cast<int64_t>(part * ((p.N + kFp8Block - 1) / kFp8Block) + block) * p.nkb;
 #pragma unroll
-    for (int j = 0; j < kMT; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  __device__ __forceinline__ void rows(const LinearArgs& p, int m0) {
-    xs_b = p.xs_b;
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < kMT; ++j) {
-      const int m = min(m0 + 16 * j + static_cast<int>(threadIdx.x & 15), p.M - 1);
-      xr[j] = p.x + m * p.x_ld + 16 * ((threadIdx.x >> 4) & 3);
-      xsr[j] = p.xs + m * p.xs_m;
+      for (int t = 0; t < kNT; ++t) a[t][h] = *reinterpret_cast<const u32x4_t*>(src + t * 2048 + (at ^ (64 * h)));
+#pragma unroll
+      for (int t = 0; t < kMT; ++t)
+        b[t][h] = *reinterpret_cast<const u32x4_t*>(src + (kNT + t) * 2048 + ((kXR < 16 ? at & ~1024u : at) ^ (64 * h)));
     }
-  }
-  __device__ __forceinline__ void load_half(Block& v, int kb, int half) const {
+    const float* sc = reinterpret_cast<const float*>(src + kDmas * 1024);
 #pragma unroll
-    for (int i = 0; i < kNT; ++i)
-      v.a[i][half] = *reinterpret_cast<const u32x4_t*>(wr[i] + kb * kFp8Block + 64 * half);
+    for (int t = 0; t < kNT; ++t) ws[t] = sc[kXR + 4 * t + g];
 #pragma unroll
-    for (int j = 0; j < kMT; ++j)
-      v.b[j][half] = *reinterpret_cast<const u32x4_t*>(xr[j] + kb * kFp8Block + 64 * half);
-  }
-  __device__ __forceinline__ void load_scales(Block& v, int kb) const {
-#pragma unroll
-    for (int i = 0; i < kNT; ++i) v.ws[i] = wsr[i][kb];
-#pragma unroll
-    for (int j = 0; j < kMT; ++j) v.xs[j] = xsr[j][kb * xs_b];
-  }
-  __device__ __forceinline__ void load(Block& v, int kb) const {
-    load_half(v, kb, 0);
-    load_half(v, kb, 1);
-    load_scales(v, kb);
-  }
-  // adds a block; next >= 0: and loads that one in its place, as soon as a half has
-  // been converted
-  template <bool kNext>
-  __device__ __forceinline__ void add(Block& v, int next) {
+    for (int t = 0; t < kMT; ++t) xs[t] = sc[16 * t + (kXR < 16 ? c & 7 : c)];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (left >= kD) request(stage);
+    stage = stage + 1 == kD ? 0 : stage + 1;
     float4_t part[kNT][kMT];
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         bf16x8_t A[kNT], B[kMT];
 #pragma unroll
-        for (int i = 0; i < kNT; ++i) A[i] = codes8_to_bf16(v.a[i][half][2 * q], v.a[i][half][2 * q + 1]);
+        for (int t = 0; t < kNT; ++t) A[t] = codes8_to_bf16(a[t][h][2 * q], a[t][h][2 * q + 1]);
 #pragma unroll
-        for (int j = 0; j < kMT; ++j) B[j] = codes8_to_bf16(v.b[j][half][2 * q], v.b[j][half][2 * q + 1]);
-        if (kNext && q == 1) load_half(v, next, half);
+        for (int t = 0; t < kMT; ++t) B[t] = codes8_to_bf16(b[t][h][2 * q], b[t][h][2 * q + 1]);
 #pragma unroll
-        for (int i = 0; i < kNT; ++i)
+        for (int t = 0; t < kNT; ++t)
 #pragma unroll
           for (int j = 0; j < kMT; ++j)
-            part[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                A[i], B[j], half + q ? part[i][j] : float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            part[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                A[t], B[j], h + q ? part[t][j] : float4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
       }
 #pragma unroll
-    for (int i = 0; i < kNT; ++i)
+    for (int t = 0; t < kNT; ++t)
 #pragma unroll
-      for (int j = 0; j < kMT; ++j) add_scaled(acc[i][j], part[i][j], v.xs[j] * v.ws[i]);
-    if (kNext) load_scales(v, next);
+      for (int j = 0; j < kMT; ++j) add_scaled(acc[t][j], part[t][j], xs[j] * ws[t]);
   }
-
-  // blocks first, first + step, ... below nkb, kDepth of them in flight
-  template <int kCnt>
-  __device__ __forceinline__ void run_all(int first, int step) {
-    if constexpr (kCnt > 0) {
-      constexpr int kD = kCnt < kDepth ? kCnt : kDepth;
-      Block v[kD];
+  // nothing is on its way into this wave's part any more: [weight tile][x tile][lane]
+  float4_t* red = reinterpret_cast<float4_t*>(lds);
+  constexpr int kStep = kD * kRegion / 16;
 #pragma unroll
-      for (int i = 0; i < kD; ++i) load(v[i], first + i * step);
-      // (the barriers keep the loads where they are: the compiler sinks them to their uses)
-      __builtin_amdgcn_sched_barrier(0);
+  for (int t = 0; t < kNT; ++t)
 #pragma unroll
-      for (int i = 0; i < kCnt; ++i) {
-        if (i + kD < kCnt)
-          add<true>(v[i % kD], first + (i + kD) * step);
-        else
-          add<false>(v[i % kD], 0);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  }
-  // kCnt > 0: each wave has kCnt blocks or one fewer, and a straight line for either
-  // (a load that some path skips makes the compiler wait for all of them)
-  template <int kCnt>
-  __device__ __forceinline__ void run(int first, int step, int nkb) {
-    if constexpr (kCnt > 0) {
-      if (first + (kCnt - 1) * step < nkb) {
-        asm volatile("; all blocks");
-        run_all<kCnt>(first, step);
-      } else {
-        asm volatile("; one fewer");
-        run_all<kCnt - 1>(first, step);
-      }
-    } else {
-      const int cnt = (nkb - first + step - 1) / step;
-      Block v[kDepth];
-#pragma unroll
-      for (int d = 0; d < kDepth; ++d)
-        if (d < cnt) load(v[d], first + d * step);
-      int i = 0;
-      for (; i + 2 * kDepth <= cnt; i += kDepth) {
-#pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-          add<true>(v[d], first + (i + kDepth + d) * step);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      // fewer than 2 kDepth blocks are left, kDepth of them loaded
-#pragma unroll
-      for (int t = 0; t < 2 * kDepth - 1; ++t) {
-        if (i + t < cnt) {
-          if (i + t + kDepth < cnt)
-            add<true>(v[t % kDepth], first + (i + t + kDepth) * step);
-          else
-            add<false>(v[t % kDepth], 0);
-        }
-      }
-    }
-  }
-};
-
-// kCnt > 0: so many blocks per wave, three in flight; 0: any number.
-template <int kNT, int kMT, int kWaves, int kCnt>
-__global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArgs p, int R, int vec) {
-  __shared__ float4_t red[kWaves * kNT * kMT * 64];  // [wave][weight tile][x tile][lane]
-  const int nw = blockDim.x >> 6;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int c = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * R * kNT, m0 = blockIdx.y * 16 * kMT;
-  const Piece piece = piece_of(p, blockIdx.z);
-  WaveTile<kNT, kMT, kNT * kMT == 1 ? 3 : 2> w;
-#pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    const int top = n0 + i * R;
-    // (the lane's four output columns lie in one block: R is a multiple of 4)
-    w.weight(p, i, piece.part, min(top + min(c, R - 1), p.N - 1), min(top + min(4 * g, R - 4), p.N - 1) / kFp8Block);
-  }
-  w.rows(p, m0);
-  w.template run<kCnt>(piece.first + wave, nw, piece.last);
-#pragma unroll
-  for (int i = 0; i < kNT; ++i)
-#pragma unroll
-    for (int j = 0; j < kMT; ++j) red[((wave * kNT + i) * kMT + j) * 64 + lane] = w.acc[i][j];
+    for (int j = 0; j < kMT; ++j) red[wave * kStep + (t * kMT + j) * 64 + lane] = acc[t][j];
   __syncthreads();
   // lane (c, g) holds columns 4 g + 0..3 of a tile for row c of x
   for (int t = wave; t < kNT * kMT; t += nw) {
     const float4_t* src = red + t * 64 + lane;
     float4_t v = src[0];
-    for (int k = 1; k < nw; ++k) v += src[k * kNT * kMT * 64];
+    for (int k = 1; k < nw; ++k) v += src[k * kStep];
     const int m = m0 + 16 * (t % kMT) + c, n = n0 + t / kMT * R + 4 * g;
     if (m >= p.M || 4 * g >= R) continue;
     const float y[4] = {v[0], v[1], v[2], v[3]};
@@ -327,22 +307,21 @@ int out_vec(const LinearArgs& p) {
 // One tile of 16 weight rows and 16 rows of x per workgroup.
 int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
   const int nw = std::min(p.nkb, p.nkb > 32 ? 16 : 4);
-  // (every wave has cnt or cnt - 1 of the blocks)
-  const int cnt = (p.nkb + nw - 1) / nw;
   // rows per unit: the number of units is rounded up to whole rounds of 256 CUs
   const int units = ((p.N + 15) / 16 + 255) / 256 * 256;
   const int R = std::min(16, ((p.N + units - 1) / units + 3) / 4 * 4);
-  const dim3 grid((p.N + R - 1) / R, (p.M + 15) / 16, parts);
-#define ZKV_CNT(C)                                                                        \
-  case C:                                                                                 \
-    fp8_stream_kernel<1, 1, 16, C><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));            \
-    break;
-  switch (cnt) {
-    ZKV_CNT(1) ZKV_CNT(2) ZKV_CNT(3) ZKV_CNT(4) ZKV_CNT(5) ZKV_CNT(6) ZKV_CNT(7) ZKV_CNT(8)
-    default:
-      return fail(ZKV_EINVAL, "fp8 linear: %d blocks per wave", cnt);
+  const dim3 grid((p.N + R - 1) / R, 1, parts);
+  if (nw > 4) {
+    if (p.M <= 8)
+      fp8_stream_kernel<1, 8, 16, 3><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    else
+      fp8_stream_kernel<1, 16, 16, 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+  } else {
+    if (p.M <= 8)
+      fp8_stream_kernel<1, 8, 4, 3><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    else
+      fp8_stream_kernel<1, 16, 4, 3><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
   }
-#undef ZKV_CNT
   return check_launch("fp8_stream_kernel");
 }
 
@@ -350,7 +329,7 @@ int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
 int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
   const int nw = std::min(p.nkb, 8);
   const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts);
-  fp8_stream_kernel<2, 2, 8, 0><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
+  fp8_stream_kernel<2, 32, 8, 2><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
   return check_launch("fp8_stream_kernel");
 }
 
@@ -405,11 +384,8 @@ int launch_gated_join(const LinearArgs& p, hipStream_t s) {
 // 32, computes 32 kI kWN weight rows (gated: half of them gate rows, half the matching up
 // rows) for 32 kJ kWM rows of x.  A block of 128 k of the tile's rows goes from memory
 // straight into one of three LDS stages, two blocks ahead of the one that is computed on.
-//
-// LDS: a row is 8 chunks of 16 bytes, chunk c in slot c ^ ((row >> 1) & 7): the 16
-// lanes of a read phase, each with the same chunk of its own row, hit every bank
-// once.  A lane converts its codes after reading them (8 instructions per 16 of
-// them): the LDS moves bytes, not bf16.
+// A lane converts its codes after reading them (8 instructions per 16 of them): the
+// LDS moves bytes, not bf16.
 //
 //   tile of w x x  waves  products  workgroups on a CU
 //     256 x 128      8     2 x 2           1   the fewest bytes and conversions per product
@@ -422,20 +398,6 @@ int launch_gated_join(const LinearArgs& p, hipStream_t s) {
 // 44.8, 29.2, 21.8 and 23.4.
 // ---------------------------------------------------------------------------
 typedef float float16_t __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ uint32_t lds_offset(const void* p) {
-  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const lds_void_t*)(p)));
-}
-
-// 64 lanes x 16 bytes, each at its offset from a base (wave-uniform, as dst), into LDS at dst + 16 lane, not seen by the
-// compiler's wait counts: with the builtin every LDS read waits for all of them.
-__device__ __forceinline__ void dma16_tile(const void* base, uint32_t off, uint32_t dst) {
-  asm volatile("global_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "{m0}"(dst) : "memory");
-}
-
-__device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
-  asm volatile("global_load_lds_dword %0, off" : : "v"(src), "{m0}"(dst) : "memory");
-}
 
 __device__ __forceinline__ void add_scaled(float16_t& acc, const float16_t& v, float s) {
 #pragma unroll
