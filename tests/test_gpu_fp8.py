@@ -171,11 +171,11 @@ def _product(codes, scales, weight):
 SIZES = [(1, 1, 1), (1, 16, 128), (2, 7, 130), (4, 384, 2560), (5, 100, 384), (16, 130, 1000), (17, 24, 256),
          (33, 257, 640), (48, 72, 9728), (64, 200, 2600), (65, 64, 128), (66, 1, 256), (127, 129, 384),
          (128, 256, 1152), (129, 300, 640), (200, 1000, 2600), (257, 513, 16384), (600, 2560, 640), (1100, 80, 256),
-         # each tile with whole k (and odd edges), then with k in runs, then as the gated product has them
+         # sizes at which each of the kernels is chosen, with k whole and in runs, as linear and as gated product
          (2376, 2390, 600), (971, 2482, 300), (129, 7420, 700), (66, 5164, 69), (67, 6274, 2960), (39, 7542, 1835),
          (33, 5894, 1093), (65, 4787, 1262), (37, 4675, 336), (38, 5186, 649), (19, 300, 4518), (700, 2235, 600),
          (67, 5539, 4103), (454, 3494, 130), (34, 3588, 9044), (38, 38, 15934), (67, 7803, 357), (18, 1813, 9498),
-         (194, 4874, 1095), (78, 5919, 6368)]
+         (194, 4874, 1095), (78, 5919, 6368), (67, 5553, 67), (34, 65, 16047), (7, 333, 5000), (13, 200, 6000), (30, 40, 16384)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

@@ -304,31 +304,32 @@ int out_vec(const LinearArgs& p) {
          (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
 }
 
-// Units of up to 16 weight rows.  More waves where k is long; and so many weight rows
+// Units of up to 16 weight rows.  Eight waves where k is long (4 x 2560 x 4096 5.9 us with
+// four, 5.3; 4 x 6144 x 2560 6.2, with eight 6.6; gated 4 x 1024 x 8192 14.6 with 16, 12.5); and so many weight rows
 // that the number of units is rounded up to whole rounds of 256 CUs.
-int stream_waves(int nkb, int most) { return std::min(nkb, nkb > 32 ? most : 4); }
+int stream_waves(int nkb) { return nkb > 26 ? 8 : std::min(nkb, 4); }
 
 int stream_rows(int N) {
   const int units = ((N + 15) / 16 + 255) / 256 * 256;
   return std::min(16, ((N + units - 1) / units + 3) / 4 * 4);
 }
 
-template <int kXR, int kMost, int kDeep>
+template <int kXR>
 int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
-  const int nw = stream_waves(p.nkb, kMost), R = stream_rows(p.N);
+  const int nw = stream_waves(p.nkb), R = stream_rows(p.N);
   const dim3 grid((p.N + R - 1) / R, (p.M + kXR - 1) / kXR, parts);
   if (nw > 4)
-    fp8_stream_kernel<1, kXR, kMost, kDeep><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    fp8_stream_kernel<1, kXR, 8, kXR == 8 ? 3 : 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
   else
-    fp8_stream_kernel<1, kXR, 4, 3><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    fp8_stream_kernel<1, kXR, 4, 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
   return check_launch("fp8_stream_kernel");
 }
 
 // 32 weight rows and 32 rows of x per workgroup.
 int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
-  const int nw = std::min(p.nkb, 8);
+  const int nw = std::min(p.nkb, 4);
   const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts);
-  fp8_stream_kernel<2, 32, 8, 2><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
+  fp8_stream_kernel<2, 32, 4, 2><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
   return check_launch("fp8_stream_kernel");
 }
 
@@ -654,7 +655,7 @@ int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
 // Which kernel, and in how many runs of k: the shortest by a model of their times, in
 // us: a start, and a time per block of k that grows as the CUs fill (which lowers the
 // clock); and where the runs are joined by a second launch, that and the sums' way out and
-// back.  Over 56 sizes of 17 to 16000 rows its choice took 1.014 times the best of the 6 to
+// back.  Over 56 sizes of 17 to 16000 rows its choice took 1.012 times the best of the 6 to
 // 27 that were measured for each (geometric mean; at worst 1.20).  Up to 16 rows a tile of
 // the matrix instruction holds them all, and units of 16 weight rows are the smallest.
 // ---------------------------------------------------------------------------
@@ -676,10 +677,10 @@ double rounds_us(int64_t groups, int steps, const Pace& pace) {
   double us = pace.start + full * steps * pace.step[pace.most - 1];
   if (rest) {
     const int c = static_cast<int>((rest + 255) / 256);
-    const double low = c > 1 ? pace.step[c - 2] : 0.47 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
+    const double low = c > 1 ? pace.step[c - 2] : 0.48 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
     us += steps * (low + fill * (pace.step[c - 1] - low));
   }
-  return us + 0.48 * pace.start * (full + (rest > 0) - 1);
+  return us + 0.57 * pace.start * (full + (rest > 0) - 1);
 }
 
 int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
@@ -689,21 +690,21 @@ int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
 Plan plan_product(int M, int N, int nkb, int parts) {
   const bool gated = parts == 2;
   if (M <= 16) return Plan{M <= 8 ? kStream8 : kStream16, 1, gated};
-  constexpr Pace kStreamPace{3.1, 2, {0.42, 0.94}}, kStreamLongPace{3.1, 1, {0.85}}, kSplitPace{2.82, 2, {1.68, 2.83}},
-      k256Pace{7.03, 1, {1.78}}, k128Pace{7.03, 2, {1.03, 2.64}}, kFlatPace{7.03, 2, {0.71, 1.29}},
-      k64Pace{7.03, 4, {0.44, 0.77, 1.09, 1.3}}, kGatedPace{10.6, 1, {1.76}};
+  constexpr Pace kStreamPace{2.81, 2, {0.58, 0.84}}, kStreamLongPace{2.81, 1, {0.86}}, kSplitPace{3.06, 2, {0.85, 1.04}},
+      k256Pace{7.23, 1, {1.65}}, k128Pace{7.23, 2, {1.02, 2.9}}, kFlatPace{7.23, 2, {0.76, 1.29}},
+      k64Pace{7.23, 4, {0.46, 0.81, 1.14, 1.24}}, kGatedPace{11.1, 1, {1.75}};
   Plan best{kTile256, 1, gated};
   double best_us = 1e30;
   auto consider = [&](int variant, int splits, int64_t tiles, int steps, const Pace& pace, bool own) {
     const bool sums = !own && (gated || splits > 1);
     double us = rounds_us(tiles * splits * (own ? 1 : parts), steps, pace);
-    if (sums) us += (gated ? 3.0 : 1.54) + 8.0 * parts * splits * M * static_cast<double>(N) / 5.13e6;
+    if (sums) us += (gated ? 2.64 : 1.01) + 8.0 * parts * splits * M * static_cast<double>(N) / 4.62e6;
     if (us < best_us) best_us = us, best = Plan{variant, splits, sums};
   };
-  const int waves = stream_waves(nkb, 8);
+  const int waves = stream_waves(nkb);
   consider(kStream32, 1, tiles_of(N, stream_rows(N)) * tiles_of(M, 32), (nkb + waves - 1) / waves,
-           nkb > 32 ? kStreamLongPace : kStreamPace, false);
-  consider(kSplit, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 7) / 8, kSplitPace, false);
+           nkb > 26 ? kStreamLongPace : kStreamPace, false);
+  consider(kSplit, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 3) / 4, kSplitPace, false);
   for (int k = 1; k <= 8 && (k == 1 || 2 * k <= nkb + 1); ++k) {
     const int steps = (nkb + k - 1) / k;
     consider(kTile256, k, tiles_of(N, 256) * tiles_of(M, 128), steps, k256Pace, false);
@@ -717,9 +718,9 @@ Plan plan_product(int M, int N, int nkb, int parts) {
 
 int launch_variant(const LinearArgs& p, int variant, int parts, hipStream_t s) {
   switch (variant) {
-    case kStream8: return launch_stream<8, 16, 3>(p, parts, s);
-    case kStream16: return launch_stream<16, 16, 2>(p, parts, s);
-    case kStream32: return launch_stream<32, 8, 3>(p, parts, s);
+    case kStream8: return launch_stream<8>(p, parts, s);
+    case kStream16: return launch_stream<16>(p, parts, s);
+    case kStream32: return launch_stream<32>(p, parts, s);
     case kSplit: return launch_split(p, parts, s);
     case kTile256: return launch_tile<false, 4, 2, 2, 2>(p, parts, s);
     case kTile128: return launch_tile<false, 2, 4, 2, 1>(p, parts, s);
