@@ -267,7 +267,8 @@ def test_gates_far_from_zero():
     assert abs(v[2] + 2 / (1 + math.e)) <= 2 / (1 + math.e) * 2.0 ** -4 + 2 * 2.0 ** -10
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 100, 384), (40, 200, 640), (150, 300, 384)])
+@pytest.mark.parametrize("M,N,K", [(3, 100, 384), (40, 200, 640), (150, 300, 384), (257, 513, 16384), (971, 2482, 300),
+                                   (2376, 2390, 600)])
 def test_products_of_other_strides(M, N, K):
     """Rows, scales, outputs and residuals as views of wider buffers; what lies
     between them stays."""
@@ -297,17 +298,18 @@ def test_products_of_other_strides(M, N, K):
     assert torch.equal(fp8.linear(codes, one, w), fp8.linear(codes, one.contiguous(), w))
 
 
-def test_gated_products_of_other_strides():
-    M, F, K = 70, 200, 384
+@pytest.mark.parametrize("M,F,K", [(70, 200, 384), (300, 2048, 4096), (700, 2235, 600)])
+def test_gated_products_of_other_strides(M, F, K):
     codes, scales, w = _whole_product(3, M, F, K, parts=2)
+    wide = blocks(F) * B
     for m in (5, M):
         want = fp8.gated_linear(codes[:m], scales[:m], w)
-        place = torch.full((m, 512), 7, dtype=torch.uint8, device=DEV).view(E4M3)
-        s = torch.full((m, 4), -1.0, device=DEV)
-        got = fp8.gated_linear(codes[:m], scales[:m], w, out_codes=place[:, 128:384], out_scales=s[:, 1:3])
+        place = torch.full((m, wide + 256), 7, dtype=torch.uint8, device=DEV).view(E4M3)
+        s = torch.full((m, blocks(F) + 2), -1.0, device=DEV)
+        got = fp8.gated_linear(codes[:m], scales[:m], w, out_codes=place[:, 128:-128], out_scales=s[:, 1:-1])
         assert _same_codes(got[0].contiguous(), want[0]) and torch.equal(got[1], want[1])
         raw = place.view(torch.uint8)
-        assert (raw[:, :128] == 7).all() and (raw[:, 384:] == 7).all() and (s[:, 0] == -1).all() and (s[:, 3] == -1).all()
+        assert (raw[:, :128] == 7).all() and (raw[:, -128:] == 7).all() and (s[:, 0] == -1).all() and (s[:, -1] == -1).all()
 
 
 def test_no_rows():
@@ -407,6 +409,35 @@ def test_captured_and_replayed(M):
         graphs[i % 2].replay()
         torch.cuda.synchronize()
         assert torch.equal(outs[i % 2], want)
+
+
+@pytest.mark.parametrize("M,F,K", [(257, 513, 16384), (300, 2048, 4096), (700, 2235, 600), (4, 1000, 6000)])
+def test_larger_products_at_once_and_replayed(M, F, K):
+    """Tiles, and runs of k in a workspace, on two streams and in two graphs at once."""
+    codes, scales, w = _whole_product(M, M, F, K, parts=2)
+    one = fp8.Fp8Weight(w.codes[:F], w.scales[:blocks(F)])
+    both = lambda: (*fp8.gated_linear(codes, scales, w), fp8.linear(codes, scales, one, out_dtype=torch.float32))
+    want = [t.clone() for t in both()]
+    same = lambda got: _same_codes(got[0], want[0]) and all(torch.equal(g, t) for g, t in zip(got[1:], want[1:]))
+    streams, graphs, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [], []
+    torch.cuda.synchronize()
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(both())
+        graphs.append(g)
+    for _ in range(4):
+        got = []
+        for o in outs:
+            for t in o:
+                (t.view(torch.uint8) if t.dtype == E4M3 else t).zero_()
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+                got.append(both())
+        torch.cuda.synchronize()
+        assert all(same(g) for g in got) and all(same(o) for o in outs)
 
 
 @pytest.mark.parametrize("M", [3, 100])
