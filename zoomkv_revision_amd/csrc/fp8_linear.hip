@@ -304,19 +304,20 @@ int out_vec(const LinearArgs& p) {
          (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
 }
 
-// Units of up to 16 weight rows.  Eight waves where k is long (4 x 2560 x 4096 5.9 us with
-// four, 5.3; 4 x 6144 x 2560 6.2, with eight 6.6; gated 4 x 1024 x 8192 14.6 with 16, 12.5); and so many weight rows
-// that the number of units is rounded up to whole rounds of 256 CUs.
+// Units of up to 16 weight rows: eight waves where k is long (4 x 2560 x 4096 5.9 us with
+// four, 5.3 with eight; 4 x 6144 x 2560 6.2 and 6.6), and so many weight rows that the
+// number of units is rounded up to whole rounds of 256 CUs (4 x 2560 x 9728, 12 rows each
+// 8.15 us, 16 rows 8.6, 8 rows 10.8).
 int stream_waves(int nkb) { return nkb > 26 ? 8 : std::min(nkb, 4); }
 
-int stream_rows(int N) {
-  const int units = ((N + 15) / 16 + 255) / 256 * 256;
+int stream_rows(int N, int parts) {
+  const int units = ((N + 15) / 16 * parts + 255) / 256 * 256 / parts;
   return std::min(16, ((N + units - 1) / units + 3) / 4 * 4);
 }
 
 template <int kXR>
 int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
-  const int nw = stream_waves(p.nkb), R = stream_rows(p.N);
+  const int nw = stream_waves(p.nkb), R = stream_rows(p.N, parts);
   const dim3 grid((p.N + R - 1) / R, (p.M + kXR - 1) / kXR, parts);
   if (nw > 4)
     fp8_stream_kernel<1, kXR, 8, kXR == 8 ? 3 : 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
@@ -702,7 +703,7 @@ Plan plan_product(int M, int N, int nkb, int parts) {
     if (us < best_us) best_us = us, best = Plan{variant, splits, sums};
   };
   const int waves = stream_waves(nkb);
-  consider(kStream32, 1, tiles_of(N, stream_rows(N)) * tiles_of(M, 32), (nkb + waves - 1) / waves,
+  consider(kStream32, 1, tiles_of(N, stream_rows(N, parts)) * tiles_of(M, 32), (nkb + waves - 1) / waves,
            nkb > 26 ? kStreamLongPace : kStreamPace, false);
   consider(kSplit, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 3) / 4, kSplitPace, false);
   for (int k = 1; k <= 8 && (k == 1 || 2 * k <= nkb + 1); ++k) {
