@@ -112,6 +112,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_packed = {}  # structs of entries' arguments
 
 
 class ZkvError(RuntimeError):
@@ -138,8 +139,11 @@ def lib() -> C.CDLL:
 def packed_args(name: str, args) -> C.Structure:
     """The arguments of an entry but its stream as the struct that its `_call`
     entry takes."""
-    fields = [(f"a{i}", t) for i, t in enumerate(SIGNATURES[name][1][:-1])]
-    return type(f"{name}_args", (C.Structure,), {"_fields_": fields})(*args)
+    struct = _packed.get(name)
+    if struct is None:
+        fields = [(f"a{i}", t) for i, t in enumerate(SIGNATURES[name][1][:-1])]
+        struct = _packed[name] = type(f"{name}_args", (C.Structure,), {"_fields_": fields})
+    return struct(*args)
 
 
 def check(rc: int) -> None:
