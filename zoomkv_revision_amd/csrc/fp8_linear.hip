@@ -100,33 +100,33 @@ __device__ __forceinline__ void put_gated(const LinearArgs& p, int m, int jb, in
   if (l == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
 }
 
-// Four neighbouring columns of a row of the output.
-__device__ __forceinline__ void store_out4(const LinearArgs& p, int z, int m, int n, const float (&y)[4], bool vec) {
-  if (p.sums) {  // (rows of whole groups of four)
-    if (n < p.N)
-      *reinterpret_cast<float4_t*>(p.sums + (static_cast<int64_t>(z) * p.M + m) * p.sums_ld + n) =
-          float4_t{y[0], y[1], y[2], y[3]};
-    return;
-  }
-  if (!vec || n + 4 > p.N) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) store_out(p, m, n + i, y[i]);
-    return;
-  }
-  const int64_t o = m * p.out_ld + n, r = m * p.res_ld + n;
+// Rows of the output and the residual start anywhere: wide accesses at any element.
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
+// Four neighbouring columns of a row of the residual, as they are stored.
+__device__ __forceinline__ u32x4_t load_res4(const LinearArgs& p, int m, int n) {
+  const int64_t r = m * p.res_ld + n;
+  if (p.type == kRowF32) return *reinterpret_cast<const u32x4_any*>(static_cast<const float*>(p.res) + r);
+  const u32x2_any h = *reinterpret_cast<const u32x2_any*>(static_cast<const uint16_t*>(p.res) + r);
+  return u32x4_t{h[0], h[1], 0, 0};
+}
+
+// Four columns of the output, all of them in it; res where there is a residual.
+__device__ __forceinline__ void store_whole4(const LinearArgs& p, int m, int n, const float (&y)[4], u32x4_t res) {
+  const int64_t o = m * p.out_ld + n;
   if (p.type == kRowF32) {
-    float4_t v = {y[0], y[1], y[2], y[3]};
-    if (p.res) v += *reinterpret_cast<const float4_t*>(static_cast<const float*>(p.res) + r);
-    *reinterpret_cast<float4_t*>(static_cast<float*>(p.out) + o) = v;
+    u32x4_t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __float_as_uint(p.res ? y[i] + __uint_as_float(res[i]) : y[i]);
+    *reinterpret_cast<u32x4_any*>(static_cast<float*>(p.out) + o) = v;
   } else {
     float v[4] = {y[0], y[1], y[2], y[3]};
     const bool bf = p.type == kRowBf16;
     if (p.res) {
-      const u32x2_t h = *reinterpret_cast<const u32x2_t*>(static_cast<const uint16_t*>(p.res) + r);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t e = i & 1 ? h[i >> 1] >> 16 : h[i >> 1] & 0xFFFFu;
+        const uint32_t e = i & 1 ? res[i >> 1] >> 16 : res[i >> 1] & 0xFFFFu;
         v[i] += bf ? elem_to_f32<kBf16>(e) : elem_to_f32<kF16>(e);
       }
     }
@@ -135,7 +135,22 @@ __device__ __forceinline__ void store_out4(const LinearArgs& p, int z, int m, in
     for (int i = 0; i < 2; ++i)
       q[i] = bf ? f32_to_elem<kBf16>(v[2 * i]) | (f32_to_elem<kBf16>(v[2 * i + 1]) << 16)
                 : f32_to_elem<kF16>(v[2 * i]) | (f32_to_elem<kF16>(v[2 * i + 1]) << 16);
-    *reinterpret_cast<u32x2_t*>(static_cast<uint16_t*>(p.out) + o) = q;
+    *reinterpret_cast<u32x2_any*>(static_cast<uint16_t*>(p.out) + o) = q;
+  }
+}
+
+// Four columns of the output, or of the sums that a second launch goes on with.
+__device__ __forceinline__ void store_out4(const LinearArgs& p, int z, int m, int n, const float (&y)[4]) {
+  if (p.sums) {  // (rows of whole groups of four)
+    if (n < p.N)
+      *reinterpret_cast<float4_t*>(p.sums + (static_cast<int64_t>(z) * p.M + m) * p.sums_ld + n) =
+          float4_t{y[0], y[1], y[2], y[3]};
+  } else if (n + 4 > p.N) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) store_out(p, m, n + i, y[i]);
+  } else {
+    store_whole4(p, m, n, y, p.res ? load_res4(p, m, n) : u32x4_t{});
   }
 }
 
@@ -172,7 +187,7 @@ __device__ __forceinline__ void dma4_tile(const void* src, uint32_t dst) {
 // repeat the last row, which moves no more memory.
 // ---------------------------------------------------------------------------
 template <int kNT, int kXR, int kWaves, int kD>
-__global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArgs p, int R, int vec) {
+__global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArgs p, int R) {
   constexpr int kMT = (kXR + 15) / 16, kDmas = (16 * kNT + kXR) / 8;
   constexpr int kRegion = kDmas * 1024 + 256;  // a block: rows of the weight, rows of x, scales
   static_assert(kXR + 4 * kNT <= 64 && kD >= 2 && kD <= 3 && kNT * kMT * 1024 <= kD * kRegion, "");
@@ -294,14 +309,8 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArg
     const int m = m0 + 16 * (t % kMT) + c, n = n0 + t / kMT * R + 4 * g;
     if (m >= p.M || 4 * g >= R) continue;
     const float y[4] = {v[0], v[1], v[2], v[3]};
-    store_out4(p, blockIdx.z, m, n, y, vec);
+    store_out4(p, blockIdx.z, m, n, y);
   }
-}
-
-int out_vec(const LinearArgs& p) {
-  const int item = p.type == kRowF32 ? 4 : 2;
-  return reinterpret_cast<uintptr_t>(p.out) % (4 * item) == 0 && p.out_ld % 4 == 0 &&
-         (!p.res || (reinterpret_cast<uintptr_t>(p.res) % (4 * item) == 0 && p.res_ld % 4 == 0));
 }
 
 // Units of up to 16 weight rows: eight waves where k is long (4 x 2560 x 4096 5.9 us with
@@ -320,9 +329,9 @@ int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
   const int nw = stream_waves(p.nkb), R = stream_rows(p.N, parts);
   const dim3 grid((p.N + R - 1) / R, (p.M + kXR - 1) / kXR, parts);
   if (nw > 4)
-    fp8_stream_kernel<1, kXR, 8, kXR == 8 ? 3 : 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    fp8_stream_kernel<1, kXR, 8, kXR == 8 ? 3 : 2><<<grid, 64 * nw, 0, s>>>(p, R);
   else
-    fp8_stream_kernel<1, kXR, 4, 2><<<grid, 64 * nw, 0, s>>>(p, R, out_vec(p));
+    fp8_stream_kernel<1, kXR, 4, 2><<<grid, 64 * nw, 0, s>>>(p, R);
   return check_launch("fp8_stream_kernel");
 }
 
@@ -330,7 +339,7 @@ int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
 int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
   const int nw = std::min(p.nkb, 4);
   const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts);
-  fp8_stream_kernel<2, 32, 4, 2><<<grid, 64 * nw, 0, s>>>(p, 16, out_vec(p));
+  fp8_stream_kernel<2, 32, 4, 2><<<grid, 64 * nw, 0, s>>>(p, 16);
   return check_launch("fp8_stream_kernel");
 }
 
@@ -345,14 +354,14 @@ __device__ __forceinline__ float4_t sum_of(const LinearArgs& p, int part, int m,
   return v;
 }
 
-__global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p, int vec) {
+__global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p) {
   const int n = 4 * (blockIdx.y * 256 + threadIdx.x), m = blockIdx.x;
   if (n >= p.N) return;
   const float4_t v = sum_of(p, 0, m, n);
   LinearArgs q = p;
   q.sums = nullptr;
   const float y[4] = {v[0], v[1], v[2], v[3]};
-  store_out4(q, 0, m, n, y, vec);
+  store_out4(q, 0, m, n, y);
 }
 
 // 16 lanes per row and block of 128 outputs, 8 outputs each.
@@ -371,7 +380,7 @@ __global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p)
 }
 
 int launch_join(const LinearArgs& p, hipStream_t s) {
-  fp8_join_kernel<<<dim3(p.M, (p.N + 1023) / 1024), 256, 0, s>>>(p, out_vec(p));
+  fp8_join_kernel<<<dim3(p.M, (p.N + 1023) / 1024), 256, 0, s>>>(p);
   return check_launch("fp8_join_kernel");
 }
 
@@ -429,8 +438,8 @@ __device__ __forceinline__ void tile_barrier() {
 }
 
 template <bool kGated, int kWN, int kWM, int kI, int kJ>
-__global__ __launch_bounds__(64 * kWN * kWM, kI * kJ > 1 ? 2 : kWN * kWM > 4 ? 4 : 3) void fp8_tile_kernel(const LinearArgs p, int tiles_n,
-                                                                                      int tiles_m, int parts, int vec) {
+__global__ __launch_bounds__(64 * kWN * kWM, kI * kJ > 1 ? 2 : kWN * kWM > 4 ? 4 : 3) void fp8_tile_kernel(
+    const LinearArgs p, int tiles_n, int tiles_m, int parts) {
   using Shape = TileShape<kGated, kWN, kWM, kI, kJ>;
   constexpr int kStages = 3, kDmas = Shape::kDmas, kScaleWaves = Shape::kScaleWaves;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[kStages * (Shape::kStage + 256 * kScaleWaves)];
@@ -613,13 +622,41 @@ __global__ __launch_bounds__(64 * kWN * kWM, kI * kJ > 1 ? 2 : kWN * kWM > 4 ? 4
       }
   __syncthreads();
   if constexpr (!kGated) {
+    constexpr int kSteps = Shape::kRowsM * kChunks / kThreads, kGroup = kSteps < 8 ? kSteps : 8;
+    static_assert(Shape::kRowsM * kChunks % kThreads == 0 && kSteps % kGroup == 0, "");
+    if (p.res && !p.sums && p.N >= 4) {
+      // (eight rows of the residual on their way at a time: with one or two, what comes
+      // after the products took longer than they did at short k.  Past the edges a load
+      // repeats the last whole group, which is not used)
+#pragma unroll 1
+      for (int first = threadIdx.x; first < kSteps * kThreads; first += kGroup * kThreads) {
+        u32x4_t res[kGroup];
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const int t = first + i * kThreads;
+          res[i] = load_res4(p, min(m0 + t / kChunks, p.M - 1), min(n0 + 4 * (t % kChunks), p.N - 4));
+        }
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const int t = first + i * kThreads, row = t / kChunks, c = t % kChunks, n = n0 + 4 * c;
+          const float4_t v = tile[row * kChunks + (c ^ (row & 15))];
+          const float y[4] = {v[0], v[1], v[2], v[3]};
+          if (m0 + row >= p.M) continue;
+          if (n + 4 <= p.N)
+            store_whole4(p, m0 + row, n, y, res[i]);
+          else
+            store_out4(p, z, m0 + row, n, y);
+        }
+      }
+    } else {
 #pragma unroll 2
-    for (int t = threadIdx.x; t < Shape::kRowsM * kChunks; t += kThreads) {
-      const int row = t / kChunks, c = t % kChunks;
-      if (m0 + row >= p.M) break;
-      const float4_t v = tile[row * kChunks + (c ^ (row & 15))];
-      const float y[4] = {v[0], v[1], v[2], v[3]};
-      store_out4(p, z, m0 + row, n0 + 4 * c, y, vec);
+      for (int t = threadIdx.x; t < kSteps * kThreads; t += kThreads) {
+        const int row = t / kChunks, c = t % kChunks;
+        if (m0 + row >= p.M) break;
+        const float4_t v = tile[row * kChunks + (c ^ (row & 15))];
+        const float y[4] = {v[0], v[1], v[2], v[3]};
+        store_out4(p, z, m0 + row, n0 + 4 * c, y);
+      }
     }
   } else {
     // 128 columns, one block: 16 lanes per row, 8 outputs each (weight rows 64 w + 0..31
@@ -648,7 +685,7 @@ int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
   const int tiles_n = (p.N + Shape::kCols - 1) / Shape::kCols, tiles_m = (p.M + Shape::kRowsM - 1) / Shape::kRowsM;
   const unsigned grid = (static_cast<unsigned>(tiles_n) * tiles_m * p.splits * parts + 7) / 8 * 8;
   fp8_tile_kernel<kGated, kWN, kWM, kI, kJ>
-      <<<grid, 64 * Shape::kWaves, 0, s>>>(p, tiles_n, tiles_m, parts, out_vec(p));
+      <<<grid, 64 * Shape::kWaves, 0, s>>>(p, tiles_n, tiles_m, parts);
   return check_launch("fp8_tile_kernel");
 }
 
