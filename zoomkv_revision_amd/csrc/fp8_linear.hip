@@ -100,10 +100,6 @@ __device__ __forceinline__ void put_gated(const LinearArgs& p, int m, int jb, in
   if (l == 0) p.scales[m * p.s_m + jb * p.s_b] = s;
 }
 
-// Rows of the output and the residual start anywhere: wide accesses at any element.
-typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-
 // Four neighbouring columns of a row of the residual, as they are stored.
 __device__ __forceinline__ u32x4_t load_res4(const LinearArgs& p, int m, int n) {
   const int64_t r = m * p.res_ld + n;

@@ -33,11 +33,10 @@ struct RowsParams {
   float eps;
   int M, K;
   int rows_per_xcd;
-  int vec;  // every row starts on 16 bytes
 };
 
-// Workgroups go to the eight XCDs in turn: workgroup b takes a row of the b % 8-th
-// eighth of the rows, so that neighbouring rows' scales (4 bytes each, columns of
+// Workgroups go to the eight XCDs in turn: workgroup b takes a row (or group of rows) of
+// the b % 8-th eighth of them, so that neighbouring rows' scales (4 bytes each, columns of
 // M) meet in one L2.
 __device__ __forceinline__ int xcd_row(const RowsParams& p) {
   return static_cast<int>(blockIdx.x & 7) * p.rows_per_xcd + static_cast<int>(blockIdx.x >> 3);
@@ -63,20 +62,26 @@ __global__ __launch_bounds__(1024) void fp8_norm_rows_kernel(const RowsParams p)
   if (row >= p.M) return;
   constexpr int kItem = kType == kRowF32 ? 4 : 2;
   const int nw = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const bool vec = p.vec;
   const void* x = static_cast<const uint8_t*>(p.x) + row * p.x_ld * kItem;
   float h[kC][8];
 #pragma unroll
-  for (int c = 0; c < kC; ++c) load_row8<kType>(x, 8 * (threadIdx.x + c * blockDim.x), p.K, vec, h[c]);
+  for (int c = 0; c < kC; ++c) load_row8<kType>(x, 8 * (threadIdx.x + c * blockDim.x), p.K, h[c]);
   if (p.res) {
     const void* res = static_cast<const uint8_t*>(p.res) + row * p.res_ld * kItem;
     float a[kC][8];
 #pragma unroll
-    for (int c = 0; c < kC; ++c) load_row8<kType>(res, 8 * (threadIdx.x + c * blockDim.x), p.K, vec, a[c]);
+    for (int c = 0; c < kC; ++c) load_row8<kType>(res, 8 * (threadIdx.x + c * blockDim.x), p.K, a[c]);
 #pragma unroll
     for (int c = 0; c < kC; ++c)
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[c][i] += a[c][i];
+  }
+  // (the norm's weight with them, where the registers hold it: a round trip less)
+  constexpr bool kEarly = kC <= 2;
+  float w[kC][8];
+  if (kEarly) {
+#pragma unroll
+    for (int c = 0; c < kC; ++c) load_row8<kType>(p.w, 8 * (threadIdx.x + c * blockDim.x), p.K, w[c]);
   }
   float ss = 0.0f;
 #pragma unroll
@@ -89,7 +94,7 @@ __global__ __launch_bounds__(1024) void fp8_norm_rows_kernel(const RowsParams p)
   if (p.sum) {
     void* sum = static_cast<uint8_t*>(p.sum) + row * p.sum_ld * kItem;
 #pragma unroll
-    for (int c = 0; c < kC; ++c) store_row8<kType>(sum, 8 * (threadIdx.x + c * blockDim.x), p.K, vec, h[c]);
+    for (int c = 0; c < kC; ++c) store_row8<kType>(sum, 8 * (threadIdx.x + c * blockDim.x), p.K, h[c]);
   }
   __syncthreads();
   float total = red[0];
@@ -98,12 +103,43 @@ __global__ __launch_bounds__(1024) void fp8_norm_rows_kernel(const RowsParams p)
 #pragma unroll
   for (int c = 0; c < kC; ++c) {
     const int chunk = threadIdx.x + c * blockDim.x;
-    float w[8], y[8];
-    load_row8<kType>(p.w, 8 * chunk, p.K, vec, w);
+    float y[8];
+    if (!kEarly) load_row8<kType>(p.w, 8 * chunk, p.K, w[c]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = h[c][i] * r * w[i];
+    for (int i = 0; i < 8; ++i) y[i] = h[c][i] * r * w[c][i];
     put_codes(p, row, chunk, y);
   }
+}
+
+// Rows of up to 8 kLanes channels: 256 / kLanes rows per workgroup, a chunk per lane, and
+// no barrier.  (A workgroup of one wave per row was bound by the rate at which they
+// start: 49150 rows of 68 26 us.)
+template <int kType, int kLanes, bool kNorm>
+__global__ __launch_bounds__(256) void fp8_short_rows_kernel(const RowsParams p) {
+  const int row = xcd_row(p) * (256 / kLanes) + static_cast<int>(threadIdx.x) / kLanes, chunk = threadIdx.x % kLanes;
+  if (row >= p.M) return;  // (whole groups of lanes)
+  constexpr int kItem = kType == kRowF32 ? 4 : 2;
+  float h[8];
+  load_row8<kType>(static_cast<const uint8_t*>(p.x) + row * p.x_ld * kItem, 8 * chunk, p.K, h);
+  if constexpr (kNorm) {
+    float w[8], ss = 0.0f;
+    load_row8<kType>(p.w, 8 * chunk, p.K, w);
+    if (p.res) {
+      float a[8];
+      load_row8<kType>(static_cast<const uint8_t*>(p.res) + row * p.res_ld * kItem, 8 * chunk, p.K, a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] += a[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(h[i], h[i], ss);
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d >>= 1) ss += __shfl_xor(ss, d);
+    if (p.sum) store_row8<kType>(static_cast<uint8_t*>(p.sum) + row * p.sum_ld * kItem, 8 * chunk, p.K, h);
+    const float r = rsqrtf(ss / static_cast<float>(p.K) + p.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = h[i] * r * w[i];
+  }
+  put_codes(p, row, chunk, h);
 }
 
 // Blocks are independent: a row's chunks in strides of the workgroup.
@@ -115,7 +151,7 @@ __global__ __launch_bounds__(1024) void fp8_rows_kernel(const RowsParams p) {
   const int chunks = (p.K + kFp8Block - 1) / kFp8Block * (kFp8Block / 8);
   for (int first = 0; first < chunks; first += blockDim.x) {
     float v[8];
-    load_row8<kType>(x, 8 * (first + threadIdx.x), p.K, p.vec, v);
+    load_row8<kType>(x, 8 * (first + threadIdx.x), p.K, v);
     put_codes(p, row, first + threadIdx.x, v);
   }
 }
@@ -127,7 +163,6 @@ struct WeightParams {
   uint8_t* codes;
   int64_t codes_ld;
   float* scales;  // [parts * blocks of a part's rows, blocks of K]
-  int vec;
 };
 
 // One workgroup per block of 128 x 128: thread t holds chunk t % 16 of rows t / 16 + 16 i.
@@ -144,7 +179,7 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const WeightParams p) {
     const int r = b * kFp8Block + (threadIdx.x >> 4) + 16 * i;
     const void* src = static_cast<const uint8_t*>(p.w) +
                       (static_cast<int64_t>(part) * rows + min(r, rows - 1)) * p.w_ld * (kType == kRowF32 ? 4 : 2);
-    load_row8<kType>(src, k, p.K, p.vec, v[i]);
+    load_row8<kType>(src, k, p.K, v[i]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[i][j]));
   }
@@ -177,22 +212,40 @@ extern "C" int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type,
                             const void* residual, int64_t res_ld, void* sum_out, int64_t sum_ld, uint8_t* codes,
                             int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, zkv_stream_t stream) {
   ZKV_REQUIRE(x && codes && scales, "zkv_fp8_rows: null pointer");
-  ZKV_REQUIRE(M >= 1 && K >= 1 && K <= (1 << 30), "zkv_fp8_rows: M=%d K=%d", M, K);
+  ZKV_REQUIRE(M >= 1 && M < (1 << 27) && K >= 1 && K <= (1 << 30), "zkv_fp8_rows: M=%d K=%d", M, K);
   ZKV_REQUIRE(type >= kRowBf16 && type <= kRowF32, "zkv_fp8_rows: type %d", type);
   ZKV_REQUIRE(norm_w || (!residual && !sum_out), "zkv_fp8_rows: a residual goes with a norm");
   ZKV_REQUIRE(!norm_w || K <= kNormMaxK, "zkv_fp8_rows: rows of %d, at most %d with a norm", K, kNormMaxK);
   ZKV_REQUIRE(codes_ld >= static_cast<int64_t>(blocks_of(K)) * kFp8Block && codes_ld % 8 == 0 &&
                   (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
               "zkv_fp8_rows: rows of codes hold whole blocks of 128 and start on 8 bytes");
-  const int item = type == kRowF32 ? 4 : 2;
-  const bool vec = rows_on_16(x, x_ld, item) && (!norm_w || rows_on_16(norm_w, 0, item)) &&
-                   (!residual || rows_on_16(residual, res_ld, item)) &&
-                   (!sum_out || rows_on_16(sum_out, sum_ld, item));
   const int per = (M + 7) / 8;
   const RowsParams p{x, x_ld, norm_w, residual, res_ld, sum_out, sum_ld, codes, codes_ld, scales,
-                     s_m, s_b, eps, M, K, per, vec};
+                     s_m, s_b, eps, M, K, per};
   auto s = reinterpret_cast<hipStream_t>(stream);
   const int chunks = blocks_of(K) * (kFp8Block / 8);
+  if (chunks <= 64) {
+    const int lanes = chunks <= 16 ? 16 : chunks <= 32 ? 32 : 64, groups = ((M + 256 / lanes - 1) / (256 / lanes) + 7) / 8;
+    RowsParams q = p;
+    q.rows_per_xcd = groups;
+#define ZKV_SHORT(T, L)                                                        \
+  do {                                                                         \
+    if (norm_w) fp8_short_rows_kernel<T, L, true><<<groups * 8, 256, 0, s>>>(q); \
+    else fp8_short_rows_kernel<T, L, false><<<groups * 8, 256, 0, s>>>(q);     \
+  } while (0)
+#define ZKV_SHORT_TYPE(T)                                                      \
+  do {                                                                         \
+    if (lanes == 16) ZKV_SHORT(T, 16);                                         \
+    else if (lanes == 32) ZKV_SHORT(T, 32);                                    \
+    else ZKV_SHORT(T, 64);                                                     \
+  } while (0)
+    if (type == kRowBf16) ZKV_SHORT_TYPE(kRowBf16);
+    else if (type == kRowF16) ZKV_SHORT_TYPE(kRowF16);
+    else ZKV_SHORT_TYPE(kRowF32);
+#undef ZKV_SHORT_TYPE
+#undef ZKV_SHORT
+    return check_launch("fp8_short_rows_kernel");
+  }
   if (!norm_w) {
     const int threads = std::min((chunks + 63) / 64, 16) * 64;
     if (type == kRowBf16) fp8_rows_kernel<kRowBf16><<<per * 8, threads, 0, s>>>(p);
@@ -233,8 +286,7 @@ extern "C" int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int typ
               "zkv_fp8_weight: rows of codes hold whole blocks of 128 and start on 8 bytes");
   const int64_t nb = static_cast<int64_t>(parts) * blocks_of(N / parts);
   ZKV_REQUIRE(nb <= 65535, "zkv_fp8_weight: %lld blocks of rows, at most 65535", static_cast<long long>(nb));
-  const int item = type == kRowF32 ? 4 : 2;
-  const WeightParams p{w, w_ld, N, K, parts, codes, codes_ld, scales, rows_on_16(w, w_ld, item)};
+  const WeightParams p{w, w_ld, N, K, parts, codes, codes_ld, scales};
   const dim3 grid(blocks_of(K), static_cast<unsigned>(nb));
   auto s = reinterpret_cast<hipStream_t>(stream);
   if (type == kRowBf16) fp8_weight_kernel<kRowBf16><<<grid, 256, 0, s>>>(p);
