@@ -175,7 +175,8 @@ SIZES = [(1, 1, 1), (1, 16, 128), (2, 7, 130), (4, 384, 2560), (5, 100, 384), (1
          (2376, 2390, 600), (971, 2482, 300), (129, 7420, 700), (66, 5164, 69), (67, 6274, 2960), (39, 7542, 1835),
          (33, 5894, 1093), (65, 4787, 1262), (37, 4675, 336), (38, 5186, 649), (19, 300, 4518), (700, 2235, 600),
          (67, 5539, 4103), (454, 3494, 130), (34, 3588, 9044), (38, 38, 15934), (67, 7803, 357), (18, 1813, 9498),
-         (194, 4874, 1095), (78, 5919, 6368), (67, 5553, 67), (34, 65, 16047), (7, 333, 5000), (13, 200, 6000), (30, 40, 16384)]
+         (194, 4874, 1095), (78, 5919, 6368), (67, 5553, 67), (34, 65, 16047), (7, 333, 5000), (13, 200, 6000), (30, 40, 16384),
+         (3, 100, 16000), (12, 60, 14000), (37, 2704, 12343), (33, 6774, 8170), (915, 1194, 4974), (2730, 69, 2190)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArg
     wb += nw * kFp8Block, xb += nw * kFp8Block, sb += s_step;
   };
 
-  const int cnt = (piece.last - first + nw - 1) / nw;  // (at least 1)
+  const int cnt = (piece.last - first + nw - 1) / nw;  // (0 for the last wave of a shorter run of k)
 #pragma unroll
   for (int d = 0; d < kD; ++d)
     if (d < cnt) request(d);
@@ -322,8 +322,8 @@ int stream_rows(int N, int parts) {
 
 template <int kXR>
 int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
-  const int nw = stream_waves(p.nkb), R = stream_rows(p.N, parts);
-  const dim3 grid((p.N + R - 1) / R, (p.M + kXR - 1) / kXR, parts);
+  const int nw = stream_waves((p.nkb + p.splits - 1) / p.splits), R = stream_rows(p.N, parts);
+  const dim3 grid((p.N + R - 1) / R, (p.M + kXR - 1) / kXR, parts * p.splits);
   if (nw > 4)
     fp8_stream_kernel<1, kXR, 8, kXR == 8 ? 3 : 2><<<grid, 64 * nw, 0, s>>>(p, R);
   else
@@ -333,8 +333,8 @@ int launch_stream(const LinearArgs& p, int parts, hipStream_t s) {
 
 // 32 weight rows and 32 rows of x per workgroup.
 int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
-  const int nw = std::min(p.nkb, 4);
-  const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts);
+  const int nw = std::min((p.nkb + p.splits - 1) / p.splits, 4);
+  const dim3 grid((p.N + 31) / 32, (p.M + 31) / 32, parts * p.splits);
   fp8_stream_kernel<2, 32, 4, 2><<<grid, 64 * nw, 0, s>>>(p, 16);
   return check_launch("fp8_stream_kernel");
 }
@@ -343,17 +343,22 @@ int launch_split(const LinearArgs& p, int parts, hipStream_t s) {
 // The second launch where the first left sums: the splits added in order, then the
 // output's residual and rounding, or silu(gate) * up as codes.
 // ---------------------------------------------------------------------------
+template <int kSplits>
 __device__ __forceinline__ float4_t sum_of(const LinearArgs& p, int part, int m, int n) {
-  const float* src = p.sums + (static_cast<int64_t>(part) * p.splits * p.M + m) * p.sums_ld + n;
-  float4_t v = *reinterpret_cast<const float4_t*>(src);
-  for (int k = 1; k < p.splits; ++k) v += *reinterpret_cast<const float4_t*>(src + k * p.M * p.sums_ld);
-  return v;
+  const float* src = p.sums + (static_cast<int64_t>(part) * kSplits * p.M + m) * p.sums_ld + n;
+  float4_t v[kSplits];  // (requested together)
+#pragma unroll
+  for (int k = 0; k < kSplits; ++k) v[k] = *reinterpret_cast<const float4_t*>(src + k * p.M * p.sums_ld);
+#pragma unroll
+  for (int k = 1; k < kSplits; ++k) v[0] += v[k];
+  return v[0];
 }
 
+template <int kSplits>
 __global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p) {
   const int n = 4 * (blockIdx.y * 256 + threadIdx.x), m = blockIdx.x;
   if (n >= p.N) return;
-  const float4_t v = sum_of(p, 0, m, n);
+  const float4_t v = sum_of<kSplits>(p, 0, m, n);
   LinearArgs q = p;
   q.sums = nullptr;
   const float y[4] = {v[0], v[1], v[2], v[3]};
@@ -361,6 +366,7 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const LinearArgs p) {
 }
 
 // 16 lanes per row and block of 128 outputs, 8 outputs each.
+template <int kSplits>
 __global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p) {
   const int jb = blockIdx.y, m = blockIdx.x * 16 + (threadIdx.x >> 4), n = jb * kFp8Block + 8 * (threadIdx.x & 15);
   if (m >= p.M) return;  // (whole groups of 16 lanes)
@@ -368,21 +374,28 @@ __global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p)
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     float4_t g = {0.0f, 0.0f, 0.0f, 0.0f}, u = g;
-    if (n + 4 * i < p.N) g = sum_of(p, 0, m, n + 4 * i), u = sum_of(p, 1, m, n + 4 * i);
+    if (n + 4 * i < p.N) g = sum_of<kSplits>(p, 0, m, n + 4 * i), u = sum_of<kSplits>(p, 1, m, n + 4 * i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[4 * i + e] = n + 4 * i + e < p.N ? silu_mul(g[e], u[e]) : 0.0f;
   }
   put_gated(p, m, jb, threadIdx.x & 15, y);
 }
 
-int launch_join(const LinearArgs& p, hipStream_t s) {
-  fp8_join_kernel<<<dim3(p.M, (p.N + 1023) / 1024), 256, 0, s>>>(p);
-  return check_launch("fp8_join_kernel");
-}
+constexpr int kMaxSplits = 8;
 
-int launch_gated_join(const LinearArgs& p, hipStream_t s) {
-  fp8_gated_join_kernel<<<dim3((p.M + 15) / 16, (p.N + kFp8Block - 1) / kFp8Block), 256, 0, s>>>(p);
-  return check_launch("fp8_gated_join_kernel");
+int launch_join(const LinearArgs& p, bool gated, hipStream_t s) {
+  const dim3 grid = gated ? dim3((p.M + 15) / 16, (p.N + kFp8Block - 1) / kFp8Block) : dim3(p.M, (p.N + 1023) / 1024);
+#define ZKV_JOIN(S)                                                  \
+  case S:                                                            \
+    if (gated) fp8_gated_join_kernel<S><<<grid, 256, 0, s>>>(p);     \
+    else fp8_join_kernel<S><<<grid, 256, 0, s>>>(p);                 \
+    break;
+  switch (p.splits) {
+    ZKV_JOIN(1) ZKV_JOIN(2) ZKV_JOIN(3) ZKV_JOIN(4) ZKV_JOIN(5) ZKV_JOIN(6) ZKV_JOIN(7) ZKV_JOIN(8)
+    default: return fail(ZKV_EINVAL, "fp8 linear: %d runs of k", p.splits);
+  }
+#undef ZKV_JOIN
+  return check_launch("fp8_join_kernel");
 }
 
 // ---------------------------------------------------------------------------
@@ -687,11 +700,13 @@ int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
 
 // ---------------------------------------------------------------------------
 // Which kernel, and in how many runs of k: the shortest by a model of their times, in
-// us: a start, and a time per block of k that grows as the CUs fill (which lowers the
-// clock); and where the runs are joined by a second launch, that and the sums' way out and
-// back.  Over 56 sizes of 17 to 16000 rows its choice took 1.012 times the best of the 6 to
-// 27 that were measured for each (geometric mean; at worst 1.20).  Up to 16 rows a tile of
-// the matrix instruction holds them all, and units of 16 weight rows are the smallest.
+// us: a start, and a time per block of k (per wave, where waves share k) that grows as the
+// CUs fill, which lowers the clock; and where the runs are joined by a second launch,
+// that and the sums' way out and back.  Over 164 sizes its choice took 1.009 times the
+// best of those measured for each (geometric mean; at worst 1.16).  With as many runs as
+// it takes 64 x 1024 x 9728 went from 15.0 to 9.3 us, 64 x 256 x 16384 from 16.7 to 7.9,
+// gated 16 x 256 x 16384 from 11.3 to 9.4.  Up to 16 rows a tile of the matrix instruction
+// holds them all, and units of 16 weight rows are the smallest.
 // ---------------------------------------------------------------------------
 enum Variant : int { kStream8, kStream16, kStream32, kSplit, kTile256, kTile128, kTileFlat, kTile64, kTileGated };
 
@@ -704,6 +719,7 @@ struct Pace {
   double start;    // until the first block and behind the last
   int most;        // steps of the list
   double step[4];  // a block's time with 256, 512, ... workgroups at work
+  double low;      // of the first of them where nearly all CUs are idle
 };
 
 double rounds_us(int64_t groups, int steps, const Pace& pace) {
@@ -711,10 +727,10 @@ double rounds_us(int64_t groups, int steps, const Pace& pace) {
   double us = pace.start + full * steps * pace.step[pace.most - 1];
   if (rest) {
     const int c = static_cast<int>((rest + 255) / 256);
-    const double low = c > 1 ? pace.step[c - 2] : 0.48 * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
+    const double low = c > 1 ? pace.step[c - 2] : pace.low * pace.step[0], fill = (rest - (c - 1) * 256) / 256.0;
     us += steps * (low + fill * (pace.step[c - 1] - low));
   }
-  return us + 0.57 * pace.start * (full + (rest > 0) - 1);
+  return us + 0.074 * pace.start * (full + (rest > 0) - 1);
 }
 
 int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
@@ -723,30 +739,34 @@ int64_t tiles_of(int a, int b) { return (a + b - 1) / b; }
 // for a second launch, but for the kernel that computes whole blocks of outputs.
 Plan plan_product(int M, int N, int nkb, int parts) {
   const bool gated = parts == 2;
-  if (M <= 16) return Plan{M <= 8 ? kStream8 : kStream16, 1, gated};
-  constexpr Pace kStreamPace{2.81, 2, {0.58, 0.84}}, kStreamLongPace{2.81, 1, {0.86}}, kSplitPace{3.06, 2, {0.85, 1.04}},
-      k256Pace{7.23, 1, {1.65}}, k128Pace{7.23, 2, {1.02, 2.9}}, kFlatPace{7.23, 2, {0.76, 1.29}},
-      k64Pace{7.23, 4, {0.46, 0.81, 1.14, 1.24}}, kGatedPace{11.1, 1, {1.75}};
+  constexpr Pace kFewPace{3.49, 1, {0.25}, 1.29}, kStreamPace{3.49, 2, {0.44, 0.88}, 0.5},
+      kStreamLongPace{3.49, 1, {0.79}, 0.5}, kSplitPace{4.43, 2, {0.57, 1.54}, 0.5}, k256Pace{7.27, 1, {2.01}, 0.5},
+      k128Pace{7.27, 2, {1.02, 3.51}, 0.5}, kFlatPace{7.27, 2, {0.72, 1.47}, 0.5},
+      k64Pace{7.27, 4, {0.37, 0.89, 1.07, 1.74}, 0.5}, kGatedPace{11.5, 1, {1.78}, 0.5};
   Plan best{kTile256, 1, gated};
   double best_us = 1e30;
   auto consider = [&](int variant, int splits, int64_t tiles, int steps, const Pace& pace, bool own) {
     const bool sums = !own && (gated || splits > 1);
     double us = rounds_us(tiles * splits * (own ? 1 : parts), steps, pace);
-    if (sums) us += (gated ? 2.64 : 1.01) + 8.0 * parts * splits * M * static_cast<double>(N) / 4.62e6;
+    if (sums) us += (gated ? 2.72 : 1.61) + 8.0 * parts * splits * M * static_cast<double>(N) / 5.51e6;
     if (us < best_us) best_us = us, best = Plan{variant, splits, sums};
   };
-  const int waves = stream_waves(nkb);
-  consider(kStream32, 1, tiles_of(N, stream_rows(N, parts)) * tiles_of(M, 32), (nkb + waves - 1) / waves,
-           nkb > 26 ? kStreamLongPace : kStreamPace, false);
-  consider(kSplit, 1, tiles_of(N, 32) * tiles_of(M, 32), (nkb + 3) / 4, kSplitPace, false);
-  for (int k = 1; k <= 8 && (k == 1 || 2 * k <= nkb + 1); ++k) {
-    const int steps = (nkb + k - 1) / k;
+  const int64_t units = tiles_of(N, stream_rows(N, parts));
+  for (int k = 1; k <= kMaxSplits && (k == 1 || 2 * k <= nkb + 1); ++k) {
+    const int steps = (nkb + k - 1) / k, waves = stream_waves(steps), stream_steps = (steps + waves - 1) / waves;
+    if (M <= 16) {
+      if (k == 1 || units * k * parts <= 256)
+        consider(M <= 8 ? kStream8 : kStream16, k, units, stream_steps, kFewPace, false);
+      continue;
+    }
+    consider(kStream32, k, units * tiles_of(M, 32), stream_steps, waves > 4 ? kStreamLongPace : kStreamPace, false);
+    consider(kSplit, k, tiles_of(N, 32) * tiles_of(M, 32), (steps + 3) / 4, kSplitPace, false);
     consider(kTile256, k, tiles_of(N, 256) * tiles_of(M, 128), steps, k256Pace, false);
     consider(kTile128, k, tiles_of(N, 128) * tiles_of(M, 128), steps, k128Pace, false);
     consider(kTileFlat, k, tiles_of(N, 128) * tiles_of(M, 64), steps, kFlatPace, false);
     consider(kTile64, k, tiles_of(N, 64) * tiles_of(M, 64), steps, k64Pace, false);
   }
-  if (gated) consider(kTileGated, 1, tiles_of(N, 128) * tiles_of(M, 128), nkb, kGatedPace, true);
+  if (gated && M > 16) consider(kTileGated, 1, tiles_of(N, 128) * tiles_of(M, 128), nkb, kGatedPace, true);
   return best;
 }
 
@@ -812,7 +832,7 @@ extern "C" int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, i
   p.sums = plan.sums ? static_cast<float*>(workspace) : nullptr, p.sums_ld = (N + 3) / 4 * 4, p.splits = plan.splits;
   auto s = reinterpret_cast<hipStream_t>(stream);
   const int rc = launch_variant(p, plan.variant, 1, s);
-  return rc != ZKV_OK || !plan.sums ? rc : launch_join(p, s);
+  return rc != ZKV_OK || !plan.sums ? rc : launch_join(p, false, s);
 }
 
 extern "C" int zkv_fp8_linear_call(const zkv_fp8_linear_args* a, zkv_stream_t stream) {
@@ -847,7 +867,7 @@ extern "C" int zkv_fp8_gated_linear(const uint8_t* x, int64_t x_ld, const float*
   p.sums = plan.sums ? static_cast<float*>(workspace) : nullptr, p.sums_ld = (F + 3) / 4 * 4, p.splits = plan.splits;
   auto s = reinterpret_cast<hipStream_t>(stream);
   const int rc = launch_variant(p, plan.variant, 2, s);
-  return rc != ZKV_OK || !plan.sums ? rc : launch_gated_join(p, s);
+  return rc != ZKV_OK || !plan.sums ? rc : launch_join(p, true, s);
 }
 
 extern "C" int zkv_fp8_gated_linear_call(const zkv_fp8_gated_linear_args* a, zkv_stream_t stream) {
