@@ -703,7 +703,7 @@ int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, c
 /* --------------------------------------------------------------------------
  * Linear layers in 8 bits: rows of e4m3 codes [M, 128 B] with an fp32 scale per
  * 128 channels, weights of codes [rows, 128 B] with a scale per 128 x 128; a code
- * stands for code * scale.  B = ceil(K / 128); codes behind K are 0.  The scale
+ * stands for code * scale.  B = ceil(K / 128); codes behind K are 0 (NaN in a NaN block).  The scale
  * of a block is its largest magnitude / 448, at least 2^-100 (NaN, as its codes,
  * where it holds an infinity or a NaN).  Scales of rows lie at m * s_m + b * s_b,
  * those of a weight [blocks of rows, B] contiguous.  Types: 0 bf16, 1 fp16, 2

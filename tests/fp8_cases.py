@@ -20,7 +20,8 @@ def padded(x: torch.Tensor) -> torch.Tensor:
 def scales_of(x: torch.Tensor) -> torch.Tensor:
     """The scale of each row's blocks of 128, in x's type (fp32: the IEEE quotient)."""
     amax = padded(x).view(x.shape[0], -1, B).abs().amax(-1)
-    return torch.maximum(amax / torch.full_like(amax, 448.0), torch.full_like(amax, LEAST))
+    s = torch.maximum(amax / torch.full_like(amax, 448.0), torch.full_like(amax, LEAST))
+    return torch.where(amax.isfinite(), s, torch.full_like(s, float("nan")))      # (an infinity: NaN, as its codes)
 
 
 def coded(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -89,13 +90,18 @@ def check_rows(x, codes, scales):
     assert torch.equal(scales.cpu(), s) and torch.equal(codes.cpu().float(), want.float())
 
 
+def _near(got, want, bound) -> bool:
+    """Within the bound, NaN where NaN is."""
+    return bool((((got - want).abs() <= bound) | (got.isnan() & want.isnan())).all())
+
+
 def check_norm(x, weight, eps, residual, codes, scales, total=None):
     h = x.double() + (0 if residual is None else residual.double())
     y = h * (h.square().mean(-1, keepdim=True) + eps).rsqrt() * weight.double()
     s = scales_of(y)
-    assert ((scales.double() - s).abs() <= NORM_REL * s).all()
-    y = padded(y)
-    assert ((values(codes, scales) - y).abs() <= code_bound(y, s, NORM_REL)).all()
+    assert _near(scales.double(), s, NORM_REL * s)
+    y = torch.where(s.isnan().repeat_interleave(B, 1), float("nan"), padded(y))     # (an infinity: its whole block)
+    assert _near(values(codes, scales), y, code_bound(y, s, NORM_REL))
     if residual is not None:
         assert torch.equal(total, (x.float() + residual.float()).to(x.dtype))
 
