@@ -248,6 +248,9 @@ __global__ __launch_bounds__(64 * kWaves) void fp8_stream_kernel(const LinearArg
       wait_vmcnt<kDmas + 1>();
     else
       wait_vmcnt<0>();
+    // (to the compiler neither the wait nor the DMAs' arrival touches memory: the reads stay
+    // behind it)
+    asm volatile("" ::: "memory");
     const uint8_t* src = mine + stage * kRegion;
     u32x4_t a[kNT][2], b[kMT][2];
     float ws[kNT], xs[kMT];
