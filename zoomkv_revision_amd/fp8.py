@@ -121,9 +121,33 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _runs(t: torch.Tensor) -> tuple[int, int, int]:
+    """A contiguous or 2-D tensor as runs of bytes of one length: (the length, how
+    many, the bytes from one to the next).  Where no dim is contiguous, a run spans
+    what lies between its elements too."""
+    size = t.element_size()
+    if t.is_contiguous():
+        return t.numel() * size, 1, 1
+    (inner, n), (outer, count) = sorted((s, n) if n > 1 else (0, 1) for s, n in zip(t.stride(), t.shape))
+    length = (inner * (n - 1) + 1) * size
+    if outer * size > length:
+        return length, count, outer * size
+    return length + outer * (count - 1) * size, 1, 1
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share memory.  Runs that lie equally far apart (columns of
+    one buffer) and one run among others are told apart; else by the extents."""
     (a0, a1), (b0, b1) = _extent(a), _extent(b)
-    return a0 < b1 and b0 < a1
+    if a0 >= b1 or b0 >= a1:
+        return False
+    (a_len, a_n, a_step), (b_len, b_n, b_step) = _runs(a), _runs(b)
+    if a_n > 1 and b_n > 1 and a_step != b_step:
+        return True
+    # run j of b lies over run i of a where -b_len < b0 - a0 + (j - i) step < a_len
+    step, apart = a_step if a_n > 1 else b_step, b0 - a0
+    least, most = (-b_len - apart) // step + 1, -((apart - a_len) // step) - 1
+    return max(least, 1 - a_n) <= min(most, b_n - 1)
 
 
 def _check_apart(name: str, out: torch.Tensor, *others) -> None:
