@@ -62,3 +62,18 @@ def test_columns_that_meet_are_refused():
     three = torch.zeros(M, 3 * K, dtype=BF)
     with pytest.raises(ValueError, match="residual itself or lie apart"):
         fp8.rms_norm_quant(**_norm(x=three[:, :K], residual=three[:, K:2 * K], sum_out=three[:, 2 * K - 1:3 * K - 1]))
+
+
+def test_codes_over_scales_are_refused():
+    flat = torch.zeros(M * 256 + 16, dtype=torch.uint8)
+    codes = flat[:M * 256].view(E4M3).view(M, 256)
+    over = lambda rows, cols: flat[-4 * rows * cols - 16:-16].view(torch.float32).view(rows, cols)
+    beside = torch.zeros(M, 272, dtype=torch.uint8)
+    for call in (lambda: fp8.quantize_rows(**_rows(codes=codes, scales=over(M, 2))),
+                 lambda: fp8.rms_norm_quant(**_norm(codes=codes, scales=over(M, 2))),
+                 lambda: fp8.quantize_rows(**_rows(codes=beside[:, :256].view(E4M3),
+                                                   scales=beside.view(torch.float32)[:, 63:65])),
+                 lambda: fp8.gated_linear(**_gated(out_codes=flat[-16 - M * 128:-16].view(E4M3).view(M, 128),
+                                                     out_scales=over(M, 1)))):
+        with pytest.raises(ValueError, match="apart from the inputs and the other outputs"):
+            call()

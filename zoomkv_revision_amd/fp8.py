@@ -196,6 +196,7 @@ def _rows_args(x, weight, eps, residual, sum_out, codes, scales):
     _same_device(x, weight=weight, residual=residual, sum_out=sum_out, codes=codes, scales=scales)
     for name, t in (("codes", codes), ("scales", scales)):
         _check_apart(name, t, x, weight, residual, sum_out)
+    _check_apart("scales", scales, codes)
     if sum_out is not None:
         _check_apart("sum_out", sum_out, weight)
     require_gpu(x)
@@ -487,7 +488,7 @@ def _gated_args(codes, scales, weight, out_codes, out_scales, workspace):
     s_m, s_b = _check_scales("out_scales", out_scales, M, F, apart=True)
     inputs = codes, scales, weight.codes, weight.scales
     _check_apart("out_codes", out_codes, *inputs)
-    _check_apart("out_scales", out_scales, *inputs)
+    _check_apart("out_scales", out_scales, *inputs, out_codes)
     _same_device(codes, out_codes=out_codes, out_scales=out_scales)
     ws = _workspace(lib().zkv_fp8_gated_workspace_size(M, F, K), workspace, codes)
     _check_apart("workspace", ws, *inputs, out_codes, out_scales)
