@@ -77,3 +77,31 @@ def test_codes_over_scales_are_refused():
                                                      out_scales=over(M, 1)))):
         with pytest.raises(ValueError, match="apart from the inputs and the other outputs"):
             call()
+
+
+def test_scales_that_share_places_are_refused():
+    """By enumeration over strides; single rows and blocks have none to share."""
+    buf = torch.zeros(4096)
+    for rows in (1, 2, 4, 5):
+        for nb in (1, 2, 3):
+            for s0 in range(7):
+                for s1 in range(7):
+                    t = buf.as_strided((rows, nb), (s0, s1))
+                    places = {i * s0 + j * s1 for i in range(rows) for j in range(nb)}
+                    check = lambda: fp8._check_scales("scales", t, rows, 128 * nb, apart=True)
+                    if len(places) == rows * nb:
+                        check()
+                    else:
+                        with pytest.raises(ValueError, match="a place for every scale"):
+                            check()
+
+
+def test_calls_refuse_scales_that_share_places():
+    wide = torch.zeros(256, 256, dtype=BF)
+    over = torch.zeros(512).as_strided((256, 2), (1, 1))
+    with pytest.raises(ValueError, match="a place for every scale"):
+        fp8.quantize_rows(wide, scales=over)
+    gate = fp8.Fp8Weight(torch.zeros(512, 256, dtype=torch.uint8).view(E4M3), torch.ones(4, 2), parts=2)
+    codes = torch.zeros(256, 256, dtype=torch.uint8).view(E4M3)
+    with pytest.raises(ValueError, match="a place for every scale"):
+        fp8.gated_linear(codes, torch.ones(256, 2), gate, out_scales=over)

@@ -30,6 +30,7 @@ The reference's projections are bf16 (Z/model_hub/qwen.py:439-604).
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 
 import torch
@@ -98,8 +99,12 @@ def _check_scales(name: str, scales: torch.Tensor, rows: int, K: int, apart: boo
     if scales.dtype != torch.float32 or tuple(scales.shape) != (rows, blocks(K)):
         raise ValueError(f"{name} must be float32 [{rows}, {blocks(K)}]; got {scales.dtype} {list(scales.shape)}")
     s = _strides(scales)
-    if apart and any(x < 1 for x, n in zip(s, scales.shape) if n > 1):
-        raise ValueError(f"{name} must have a place for every scale; got strides {scales.stride()}")
+    if apart and scales.numel() > 1:
+        # two of them share a place if i rows and j blocks are as far apart for some i, j
+        # in the shape, the least of which are the other's stride over the common divisor
+        common = math.gcd(*s)
+        if common < 1 or s[1] // common < rows and s[0] // common < blocks(K):
+            raise ValueError(f"{name} must have a place for every scale; got strides {scales.stride()}")
     return s
 
 
