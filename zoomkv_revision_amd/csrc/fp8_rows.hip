@@ -201,6 +201,7 @@ __global__ __launch_bounds__(256) void fp8_weight_kernel(const WeightParams p) {
 }
 
 constexpr int kNormMaxK = 65536;  // 1024 threads of 8 chunks
+constexpr int kLaunchRows = 1 << 21;
 
 int blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
@@ -220,6 +221,18 @@ extern "C" int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type,
   ZKV_REQUIRE(codes_ld >= static_cast<int64_t>(blocks_of(K)) * kFp8Block && codes_ld % 8 == 0 &&
                   (reinterpret_cast<uintptr_t>(codes) & 7) == 0,
               "zkv_fp8_rows: rows of codes hold whole blocks of 128 and start on 8 bytes");
+  // (a launch holds fewer than 2^32 threads, a row takes up to 1024 of them: more rows go in
+  // several launches)
+  const int64_t item = type == kRowF32 ? 4 : 2;
+  for (; M > kLaunchRows; M -= kLaunchRows) {
+    const int rc = zkv_fp8_rows(x, x_ld, kLaunchRows, K, type, norm_w, eps, residual, res_ld, sum_out, sum_ld, codes,
+                                codes_ld, scales, s_m, s_b, stream);
+    if (rc != ZKV_OK) return rc;
+    x = static_cast<const uint8_t*>(x) + kLaunchRows * x_ld * item;
+    if (residual) residual = static_cast<const uint8_t*>(residual) + kLaunchRows * res_ld * item;
+    if (sum_out) sum_out = static_cast<uint8_t*>(sum_out) + kLaunchRows * sum_ld * item;
+    codes += kLaunchRows * codes_ld, scales += kLaunchRows * s_m;
+  }
   const int per = (M + 7) / 8;
   const RowsParams p{x, x_ld, norm_w, residual, res_ld, sum_out, sum_ld, codes, codes_ld, scales,
                      s_m, s_b, eps, M, K, per};
