@@ -696,6 +696,17 @@ int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
   using Shape = TileShape<kGated, kWN, kWM, kI, kJ>;
   const int tiles_n = (p.N + Shape::kCols - 1) / Shape::kCols, tiles_m = (p.M + Shape::kRowsM - 1) / Shape::kRowsM;
   const unsigned grid = (static_cast<unsigned>(tiles_n) * tiles_m * p.splits * parts + 7) / 8 * 8;
+  // A launch holds fewer than 2^32 threads.  (Of all products within the limits on sizes only
+  // gated ones of nearly 2^37 outputs reach that: rows in two halves)
+  if constexpr (kGated) {
+    if (grid >= (int64_t{1} << 32) / (64 * Shape::kWaves)) {
+      LinearArgs a = p, b = p;
+      a.M = tiles_m / 2 * Shape::kRowsM, b.M = p.M - a.M;
+      b.x += a.M * p.x_ld, b.xs += a.M * p.xs_m, b.codes += a.M * p.codes_ld, b.scales += a.M * p.s_m;
+      const int rc = launch_tile<kGated, kWN, kWM, kI, kJ>(a, parts, s);
+      return rc != ZKV_OK ? rc : launch_tile<kGated, kWN, kWM, kI, kJ>(b, parts, s);
+    }
+  }
   fp8_tile_kernel<kGated, kWN, kWM, kI, kJ>
       <<<grid, 64 * Shape::kWaves, 0, s>>>(p, tiles_n, tiles_m, parts);
   return check_launch("fp8_tile_kernel");
