@@ -195,12 +195,18 @@ def _is_paged(cache) -> bool:
 
 class RandomQwen3:
     """Random-init bf16 weights of a Qwen3 decoder (std 0.02, norms at 1), on one
-    GPU; weights="fp8" keeps the layers' projections as 8-bit codes with scales."""
+    GPU; weights="fp8" keeps the layers' projections as 8-bit codes with scales (on
+    the GPU of at most fp8.MAX_K channels)."""
 
     def __init__(self, geo: Qwen3Geometry, device, seed: int = 42, max_position: int = 1 << 17,
                  fused: bool = True, weights: str = "bf16"):
         if weights not in ("bf16", "fp8"):
             raise ValueError(f"weights must be bf16 or fp8; got {weights!r}")
+        if weights == "fp8" and fused and torch.device(device).type == "cuda":
+            from .fp8 import MAX_K
+            for name, n in (("hidden", geo.hidden), ("heads * head_dim", geo.heads * geo.head_dim), ("ffn", geo.ffn)):
+                if -(-n // 128) * 128 > MAX_K:
+                    raise ValueError(f"8-bit projections take at most {MAX_K} channels; got {name} = {n}")
         self.geo = geo
         self.weights = weights
         self.device = torch.device(device)
