@@ -1,5 +1,6 @@
-"""CPU: in the 8-bit products' kernels every read of the LDS behind a wait for DMAs is
-kept there by the source, not by the order that a compiler happens to choose.
+"""CPU: the module that the 8-bit products compile to.  Every read of the LDS behind a
+wait for DMAs is kept there by the source, not by the order that a compiler happens to
+choose; and no kernel is built that no call reaches.
 
 The DMAs are inline assembly and the wait an intrinsic without memory effects, so a
 plain read may move across it unless an assembly statement that clobbers memory
@@ -39,11 +40,22 @@ def test_a_read_without_its_fence_is_found():
     assert unfenced(text % "  tail call void asm sideeffect \"\", \"~{memory}\"() #1\n") == []
 
 
-def test_reads_stay_behind_their_waits(tmp_path):
-    out = tmp_path / "fp8_linear.ll"
+@pytest.fixture(scope="module")
+def module(tmp_path_factory):
+    out = tmp_path_factory.mktemp("ir") / "fp8_linear.ll"
     cmd = [HIPCC, *CFLAGS, "--cuda-device-only", "-emit-llvm", "-S", str(CSRC / "fp8_linear.hip"), "-o", str(out)]
     subprocess.run(cmd, check=True, capture_output=True)
     ir = out.read_text()
-    kernels = set(re.findall(r"^define amdgpu_kernel [^\n]*@(\w+)\(", ir, re.M))
+    return ir, set(re.findall(r"^define amdgpu_kernel [^\n]*@(\w+)\(", ir, re.M))
+
+
+def test_reads_stay_behind_their_waits(module):
+    ir, kernels = module
     assert sum("fp8_stream_kernel" in k for k in kernels) >= 6 and sum("fp8_tile_kernel" in k for k in kernels) == 5
     assert unfenced(ir) == []
+
+
+def test_the_join_of_one_run_is_the_gated_one(module):
+    """A linear product in one run leaves no sums; a gated one leaves its two parts'."""
+    runs = lambda name: sorted(int(n) for k in module[1] for n in re.findall(name + r"ILi(\d+)E", k))
+    assert runs("fp8_gated_join_kernel") == list(range(1, 9)) and runs("15fp8_join_kernel") == list(range(2, 9))

@@ -386,18 +386,27 @@ __global__ __launch_bounds__(256) void fp8_gated_join_kernel(const LinearArgs p)
 
 constexpr int kMaxSplits = 8;
 
+template <int kSplits>
+void launch_join_of(const LinearArgs& p, bool gated, dim3 grid, hipStream_t s) {
+  if (gated)
+    fp8_gated_join_kernel<kSplits><<<grid, 256, 0, s>>>(p);
+  else if constexpr (kSplits > 1)  // (a linear product leaves sums in two runs or more)
+    fp8_join_kernel<kSplits><<<grid, 256, 0, s>>>(p);
+}
+
 int launch_join(const LinearArgs& p, bool gated, hipStream_t s) {
   const dim3 grid = gated ? dim3((p.M + 15) / 16, (p.N + kFp8Block - 1) / kFp8Block) : dim3(p.M, (p.N + 1023) / 1024);
-#define ZKV_JOIN(S)                                                  \
-  case S:                                                            \
-    if (gated) fp8_gated_join_kernel<S><<<grid, 256, 0, s>>>(p);     \
-    else fp8_join_kernel<S><<<grid, 256, 0, s>>>(p);                 \
-    break;
   switch (p.splits) {
-    ZKV_JOIN(1) ZKV_JOIN(2) ZKV_JOIN(3) ZKV_JOIN(4) ZKV_JOIN(5) ZKV_JOIN(6) ZKV_JOIN(7) ZKV_JOIN(8)
+    case 1: launch_join_of<1>(p, gated, grid, s); break;
+    case 2: launch_join_of<2>(p, gated, grid, s); break;
+    case 3: launch_join_of<3>(p, gated, grid, s); break;
+    case 4: launch_join_of<4>(p, gated, grid, s); break;
+    case 5: launch_join_of<5>(p, gated, grid, s); break;
+    case 6: launch_join_of<6>(p, gated, grid, s); break;
+    case 7: launch_join_of<7>(p, gated, grid, s); break;
+    case 8: launch_join_of<8>(p, gated, grid, s); break;
     default: return fail(ZKV_EINVAL, "fp8 linear: %d runs of k", p.splits);
   }
-#undef ZKV_JOIN
   return check_launch("fp8_join_kernel");
 }
 
