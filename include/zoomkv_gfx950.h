@@ -799,6 +799,13 @@ typedef struct {
 } zkv_fp8_gated_linear_args;
 int zkv_fp8_gated_linear_call(const zkv_fp8_gated_linear_args* args, zkv_stream_t stream);
 
+/* How a product of M rows with a weight of `parts` (1: linear, 2: gated) times N rows
+ * runs, for tuning and tests: 16 * kernel + runs of k, -1 for sizes that are refused.
+ * Kernels: units of 16 weight rows for 8 (0), 16 (1) and 32 (2) rows of x, of 32 x 32
+ * (3); tiles of weight rows x rows of x, 256 x 128 (4), 128 x 128 (5), 128 x 64 (6),
+ * 64 x 64 (7), and of 128 whole gated outputs x 128 (8). */
+int zkv_fp8_plan(int M, int N, int K, int parts);
+
 #ifdef __cplusplus
 }
 #endif

@@ -102,6 +102,7 @@ SIGNATURES = {
                                   I32, I32, I32, F32, I32, P, I32, P, P, SZ, P]),
     "zkv_fp8_rows": (I32, [P, I64, I32, I32, I32, P, F32, P, I64, P, I64, P, I64, P, I64, I64, P]),
     "zkv_fp8_weight": (I32, [P, I64, I32, I32, I32, I32, P, I64, P, P]),
+    "zkv_fp8_plan": (I32, [I32, I32, I32, I32]),
     "zkv_fp8_linear_workspace_size": (SZ, [I32, I32, I32]),
     "zkv_fp8_linear": (I32, [P, I64, P, I64, I64, P, I64, P, I32, I32, I32, P, I64, P, I64, I32, P, SZ, P]),
     "zkv_fp8_gated_workspace_size": (SZ, [I32, I32, I32]),

@@ -813,14 +813,20 @@ size_t sums_bytes(const Plan& plan, int parts, int M, int N) {
 
 int blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
-// Checks what both entry points take; null or what is wrong.
-const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, const uint8_t* w, int64_t w_ld,
-                           const float* ws, int M, int N, int K) {
-  if (!x || !xs || !w || !ws) return "null pointer";
+// The sizes that both entry points take; null or what is wrong.
+const char* check_sizes(int M, int N, int K) {
   if (M < 1 || N < 1 || K < 1) return "empty product";
   if (M >= 1 << 20 || N >= 1 << 22 || static_cast<int64_t>(M) * N > int64_t{1} << 37)
     return "below 2^20 rows of x, 2^22 rows of the weight, and at most 2^37 outputs";
   if (K % kFp8Block || K > 128 * kFp8Block) return "K is a multiple of 128, at most 16384";
+  return nullptr;
+}
+
+// And their operands.
+const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, const uint8_t* w, int64_t w_ld,
+                           const float* ws, int M, int N, int K) {
+  if (!x || !xs || !w || !ws) return "null pointer";
+  if (const char* bad = check_sizes(M, N, K)) return bad;
   if (x_ld < K || w_ld < K || !rows_on_16(x, x_ld, 1) || !rows_on_16(w, w_ld, 1))
     return "rows of codes hold K bytes and start on 16";
   if (x_ld >= 1 << 23 || w_ld >= 1 << 23) return "rows of codes lie less than 8 MiB apart";
@@ -831,6 +837,12 @@ const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, cons
 }  // namespace zkv
 
 using namespace zkv;
+
+extern "C" int zkv_fp8_plan(int M, int N, int K, int parts) {
+  if (check_sizes(M, N, K) || parts < 1 || parts > 2) return -1;
+  const Plan plan = plan_product(M, N, K / kFp8Block, parts);
+  return 16 * plan.variant + plan.splits;
+}
 
 extern "C" size_t zkv_fp8_linear_workspace_size(int M, int N, int K) {
   if (M < 1 || N < 1 || K < 1) return 0;
