@@ -712,8 +712,8 @@ int zkv_paged_attention(const void* q, int64_t q_sb, int64_t q_sh, int is_f16, c
 
 /* Rows x [M, K] of `type` (row strides in elements) as codes (rows of whole
  * blocks, on 8 bytes) and scales.  norm_w [K] (nullable): of h * rsqrt(mean(h^2)
- * + eps) * norm_w, h = x [+ residual], K <= 65536; M < 2^27; sum_out (nullable) takes h
- * rounded to `type`, and may be x or residual. */
+ * + eps) * norm_w, h = x [+ residual], K <= 65536; M < 2^27 (a launch per 2^21 rows);
+ * sum_out (nullable) takes h rounded to `type`, and may be x or residual. */
 int zkv_fp8_rows(const void* x, int64_t x_ld, int M, int K, int type, const void* norm_w, float eps,
                  const void* residual, int64_t res_ld, void* sum_out, int64_t sum_ld, uint8_t* codes,
                  int64_t codes_ld, float* scales, int64_t s_m, int64_t s_b, zkv_stream_t stream);

@@ -725,9 +725,11 @@ int launch_tile(const LinearArgs& p, int parts, hipStream_t s) {
 // Which kernel, and in how many runs of k: the shortest by a model of their times, in
 // us: a start, and a time per block of k (per wave, where waves share k) that grows as the
 // CUs fill, which lowers the clock; and where the runs are joined by a second launch,
-// that and the sums' way out and back.  Over 164 sizes its choice took 1.009 times the
-// best of those measured for each (geometric mean; at worst 1.16).  With as many runs as
-// it takes 64 x 1024 x 9728 went from 15.0 to 9.3 us, 64 x 256 x 16384 from 16.7 to 7.9,
+// that and the sums' way out and back.  Against all kernels that it considers its choice took
+// 1.016 times the best over the 162 sizes that its constants were fitted to (geometric mean;
+// at worst 1.27), 1.023 over 80 others (at worst 1.38).  It has no term for the output's
+// bytes: wide outputs over one or two blocks of k take up to 3.6 times what it says
+// (profiles/fp8_linear_choice.md has the sizes).  With as many runs as it takes 64 x 1024 x 9728 went from 15.0 to 9.3 us, 64 x 256 x 16384 from 16.7 to 7.9,
 // gated 16 x 256 x 16384 from 11.3 to 9.4.  Up to 16 rows a tile of the matrix instruction
 // holds them all, and units of 16 weight rows are the smallest.
 // ---------------------------------------------------------------------------
@@ -813,7 +815,9 @@ size_t sums_bytes(const Plan& plan, int parts, int M, int N) {
 
 int blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
 
-// The sizes that both entry points take; null or what is wrong.
+// The sizes that both entry points take; null or what is wrong.  (K: the kernels and the
+// workspace have no limit of their own there; the choice is measured, and the bounds on
+// errors tested, up to 128 blocks.)
 const char* check_sizes(int M, int N, int K) {
   if (M < 1 || N < 1 || K < 1) return "empty product";
   if (M >= 1 << 20 || N >= 1 << 22 || static_cast<int64_t>(M) * N > int64_t{1} << 37)

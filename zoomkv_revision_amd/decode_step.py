@@ -293,8 +293,8 @@ class RandomQwen3:
         return cache.compute(q, ldx)
 
     def layer_decode_fp8(self, ldx: int, hidden: torch.Tensor, cache) -> torch.Tensor:
-        """layer_decode with 8-bit projections: seven launches (eight or nine where
-        a product takes two) around cache.compute."""
+        """layer_decode with 8-bit projections: eight launches around cache.compute, and
+        one more for each of the four products that takes two."""
         from . import fp8
         geo, L = self.geo, self.layers[ldx]
         bs = hidden.shape[0]

@@ -39,7 +39,7 @@ from ._lib import check, device_stream, lib, packed_args, ptr, require_gpu
 from .paged import _launch, _nothing, _Plan, _same_device, _strides
 
 BLOCK = 128
-MAX_K = 16384          # of a product
+MAX_K = 16384          # of a product (what the choice of kernels and the bounds on errors are measured for)
 MAX_NORM_K = 65536     # of a normed row
 E4M3 = torch.float8_e4m3fn
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
