@@ -747,7 +747,8 @@ int zkv_fp8_weight(const void* w, int64_t w_ld, int N, int K, int type, int part
  * be residual).  K is a multiple of 128, at most 16384; M < 2^20, N < 2^22, M * N
  * at most 2^37; rows of codes start on 16
  * bytes, less than 8 MiB apart.  workspace: zkv_fp8_linear_workspace_size(M, N, K)
- * bytes (0 where k is not split) on 16, of any content; calls that overlap on one race. */
+ * bytes (0 where k is not split, and for sizes that are refused) on 16, of any content; calls
+ * that overlap on one race. */
 size_t zkv_fp8_linear_workspace_size(int M, int N, int K);
 int zkv_fp8_linear(const uint8_t* x, int64_t x_ld, const float* xs, int64_t xs_m, int64_t xs_b, const uint8_t* w,
                    int64_t w_ld, const float* ws, int M, int N, int K, const void* residual, int64_t res_ld,

@@ -55,3 +55,14 @@ def test_products_fit_a_launch():
                                    (1, 1 << 22, 128, 2), (1 << 19, 1 << 19, 128, 1), (1, 1, 128, 3), (1, 1, 128, 0)])
 def test_refused_sizes_have_no_plan(sizes):
     assert lib().zkv_fp8_plan(*sizes) == -1
+
+
+@pytest.mark.parametrize("entry", ["zkv_fp8_linear_workspace_size", "zkv_fp8_gated_workspace_size"])
+def test_workspaces_of_sizes_at_and_beyond_the_limits(entry):
+    """K is rounded up to whole blocks; sizes that the calls refuse need none (they passed 32
+    bits in the choice)."""
+    size, top = getattr(lib(), entry), (1 << 31) - 1
+    assert size(64, 64, 16300) == size(64, 64, 16384) > 0 and size(64, 256, 9728 - 50) == size(64, 256, 9728) > 0
+    for sizes in ((top, 64, top), (top, top, 16384), (64, 1 << 22, 16384), (64, 64, top), (64, 64, 16385), (64, 64, 0),
+                  (64, 64, -1), (0, 64, 16384), (1 << 20, 64, 16384)):
+        assert size(*sizes) == 0

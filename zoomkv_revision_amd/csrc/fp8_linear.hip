@@ -826,6 +826,11 @@ const char* check_sizes(int M, int N, int K) {
   return nullptr;
 }
 
+// Whether they take the sizes with K rounded up to whole blocks.
+bool takes_sizes(int M, int N, int K) {
+  return K >= 1 && K <= 128 * kFp8Block && !check_sizes(M, N, blocks_of(K) * kFp8Block);
+}
+
 // And their operands.
 const char* check_operands(const uint8_t* x, int64_t x_ld, const float* xs, const uint8_t* w, int64_t w_ld,
                            const float* ws, int M, int N, int K) {
@@ -849,7 +854,7 @@ extern "C" int zkv_fp8_plan(int M, int N, int K, int parts) {
 }
 
 extern "C" size_t zkv_fp8_linear_workspace_size(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1) return 0;
+  if (!takes_sizes(M, N, K)) return 0;
   return sums_bytes(plan_product(M, N, blocks_of(K), 1), 1, M, N);
 }
 
@@ -881,7 +886,7 @@ extern "C" int zkv_fp8_linear_call(const zkv_fp8_linear_args* a, zkv_stream_t st
 }
 
 extern "C" size_t zkv_fp8_gated_workspace_size(int M, int F, int K) {
-  if (M < 1 || F < 1 || K < 1) return 0;
+  if (!takes_sizes(M, F, K)) return 0;
   return sums_bytes(plan_product(M, F, blocks_of(K), 2), 2, M, F);
 }
 
